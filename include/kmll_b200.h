@@ -357,6 +357,70 @@ int kmll_argmax_f32_packed(kmll_stream_t stream, const float* logits, size_t n,
 int kmll_top_k_f32(kmll_stream_t stream, const float* logits, size_t n, int k, uint32_t* tokens,
                    float* values);
 
+/* Next token of every row of logits [rows, ld] (f32, or bf16 with is_f32 = 0), one given random number u[row] in [0, 1) each; no
+ * counterpart in kmll, whose sampler (crates/inference/src/inference.rs:7069-7125) runs on the host over the k best logits.  With the tokens
+ * in the order of their logits (the lower index first among equals) and w = exp((logit - largest) / temperature), the first n tokens stay:
+ * at most top_k (0 or less: off), the fewest that hold top_p of the weight of those (1 or more: off), none whose w is below min_p (0: off).
+ * The token is the first at which the weight so far passes u times the weight of all n; logprobs (may be null) gets the
+ * logarithm of its share.  temperature, top_k, top_p and min_p are arrays of one value per row, or null (1, off, off, off).  A temperature
+ * of at most FLT_EPSILON (or NaN) takes the first of the largest logits, log-probability 0.  Logits of -infinity or NaN are never taken; where a row
+ * has no others its token is -1 and its log-probability -infinity; +infinity excludes everything finite.  vocab <= 524288.  Weights are
+ * held as multiples of 2^-44 of the largest: results do not change from call to call. */
+int kmll_sample_rows(kmll_stream_t stream, const void* logits, int is_f32, int ld, int rows, int vocab, const double* u, const float* temperature,
+                     const int32_t* top_k, const float* top_p, const float* min_p, int32_t* tokens, float* logprobs);
+
+/* ------------------------------------------------------------------------------------------
+ * Requests of unequal length over one cache of pages in 8 bits (no counterpart in kmll, whose caches are dense f32 and hold one sequence)
+ *
+ * A page holds `block` tokens (16, 32, 64 or 128) of every kv head: int8 codes and one f32 scale per (page, head), value = code * scale.  The
+ * scale is the largest magnitude written to the page so far over 127, the rule of the RS-I8 weights; code = value / scale rounded to the
+ * nearest whole number, ties to even.  When a page's scale grows its older codes become code * old / new, rounded the same way (an entry that is
+ * coded again g times is off by at most (g + 1) / 2 of the last scale).  The first row written to place 0 of a page starts it anew.  Infinities
+ * take the code of the largest magnitude and NaN counts as 0, so that one value does not spoil its page.
+ *   keys   int8 [pages][kv_heads][head_dim / 16][block][16]      values int8 [pages][kv_heads][block / 16][head_dim][16]
+ *   scales f32  [pages][kv_heads] for each of them; head_dim is a multiple of 16 up to 256, codes are 16-byte aligned
+ * Request r of a step has rows query_start[r] .. query_start[r + 1] - 1 of the step's rows, context[r] tokens in the cache with them, and its page i in
+ * block_table[r * table_width + i].  All these arrays lie on the device, so that a captured step serves any lengths.
+ * ---------------------------------------------------------------------------------------- */
+/* The pages of a step.  Request r has lengths[r] tokens in the cache and brings new_tokens[r]; pages that they need come off the top of the
+ * stack free_blocks[0 .. *free_count) of free_capacity entries, request after request, and are written to block_table.  Outputs: context[r] = lengths[r] +
+ * new_tokens[r] (may be `lengths` itself), query_start[requests + 1], and for each of token_capacity rows its position and its slot = page *
+ * block + position % block; rows behind the last token get position 0 and slot -1.  *free_count_out may be *free_count.  *status: 0, or nothing
+ * is taken and no row has a slot (query_start is all 0, context = lengths) because 1 = too few free pages, 2 = a request outgrows its
+ * table row, 3 = a negative count, or more tokens than token_capacity.  At most 8192 requests. */
+int kmll_paged_plan(kmll_stream_t stream, const int32_t* lengths, const int32_t* new_tokens, int requests, int block, int32_t* block_table, int table_width,
+                    const int32_t* free_blocks, int free_capacity, const int32_t* free_count, int token_capacity, int32_t* context, int32_t* query_start,
+                    int32_t* positions, int32_t* slots, int32_t* free_count_out, int32_t* status);
+/* Pages of the requests with ended[r] != 0 go back on the stack (request after request, their table entries become -1) and their context becomes
+ * 0; context_out and free_count_out may be the inputs.  *status: 0, or nothing is changed because 1 = the stack is too small, 3 = a context that is
+ * negative or longer than its table row. */
+int kmll_paged_release(kmll_stream_t stream, const int32_t* context, const int32_t* ended, int requests, int block, int32_t* block_table, int table_width,
+                       int32_t* free_blocks, int free_capacity, const int32_t* free_count, int32_t* context_out, int32_t* free_count_out, int32_t* status);
+/* Rotation of a step's queries and keys, keys and values into the cache: kmll_prepare_incremental_attention for rows of many requests.  Rows are f32 or (is_f32
+ * = 0) bf16, [tokens] at a pitch of ld_* elements; query_rot is [tokens, heads, head_dim] of the same type and may be `query` where its rows lie together.
+ * Entries d and d + n_freqs turn by positions[t] * freqs[d] (computed in 64 bits, so far positions keep their angles), entries from 2 * n_freqs on pass
+ * through; n_freqs = 0: no rotation, positions and freqs may be null.  Codes are those of the 64-bit rotated keys.  heads = 0: keys and values only.
+ * Rows whose slot is outside the cache are left out, their query_rot as it was.  The rows of one page must follow one another in ascending
+ * order, and no two rows may have the same slot. */
+int kmll_prepare_paged_attention(kmll_stream_t stream, const void* query, int ld_query, const void* key, int ld_key, const void* value, int ld_value, int is_f32,
+                                 const float* freqs, int n_freqs, const int32_t* positions, const int32_t* slots, int tokens, int heads, int kv_heads,
+                                 int head_dim, void* query_rot, int8_t* k_codes, float* k_scales, int8_t* v_codes, float* v_scales, int pages, int block);
+/* Rows `slots` of the cache in f32, [count, kv_heads, head_dim] each; rows whose slot is outside the cache are left as they were. */
+int kmll_paged_cache_rows(kmll_stream_t stream, const int8_t* k_codes, const float* k_scales, const int8_t* v_codes, const float* v_scales, int pages, int block,
+                          int kv_heads, int head_dim, const int32_t* slots, int count, float* k, float* v);
+/* Attention of a step's rows over the cache: row i of request r is position context[r] - rows + i and attends the positions up to its own, the
+ * last `window` of them (0: all); query head h reads kv head h / (heads / kv_heads); softmax(scale * q . k) . v, scale > 0.  query and out are [tokens,
+ * heads, head_dim], f32 or (is_f32 = 0) bf16.  A row that attends nothing is 0; rows of no request are left as they were.  Entries of block_table behind a
+ * context are not read, entries outside the cache count as pages that are not attended.  max_query and max_context bound the rows and the context
+ * of a request: they choose kernels and shares, not results.  workspace: kmll_paged_attention_workspace_bytes(...) bytes, 16-byte aligned, zero
+ * before its first use (calls leave its counters zero); calls that overlap need workspaces of their own, so two graphs that may run at the
+ * same time are captured with two.  May be null where that function says 0. */
+size_t kmll_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim, int requests, int tokens, int max_query, int max_context);
+int kmll_paged_attention(kmll_stream_t stream, const void* query, int is_f32, const int32_t* query_start, const int32_t* context, const int32_t* block_table,
+                         int table_width, int requests, int tokens, int max_query, int max_context, int heads, const int8_t* k_codes, const float* k_scales,
+                         const int8_t* v_codes, const float* v_scales, int pages, int block, int kv_heads, int head_dim, float scale, int window,
+                         void* workspace, void* out);
+
 /* ------------------------------------------------------------------------------------------
  * Operators of the layered decoders (kmll_layered_create, kmll_b200_runtime.h); no counterpart in kmll.
  * Weights are bf16 rows at a pitch of `pitch` elements (a multiple of 8, 16-byte aligned rows).

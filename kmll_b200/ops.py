@@ -568,6 +568,181 @@ def top_k_f32(logits, k: int):
     return tokens, values
 
 
+def sample_rows(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, logprobs=None):
+    """Next token of every row of logits [rows, vocab] (f32 or bf16, rows at any pitch) from u [rows] float64 in [0, 1); settings are one
+    value per row on the device, or None.  Returns (tokens int32 [rows], logprobs f32 [rows])."""
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise KmllError(-2, "logits must be [rows, vocab] in float32 or bfloat16 with rows in one piece")
+    rows, vocab = logits.shape
+    dev = _here(logits)
+    tokens = torch.empty(rows, dtype=torch.int32, device=dev) if tokens is None else tokens
+    logprobs = torch.empty(rows, dtype=torch.float32, device=dev) if logprobs is None else logprobs
+    check(load().kmll_sample_rows(_stream(), logits.data_ptr(), 1 if logits.dtype == torch.float32 else 0, logits.stride(0) if rows > 1 else vocab, rows, vocab,
+                                  _array(u, torch.float64, rows, "u"), _array(temperature, torch.float32, rows, "temperature"), _array(top_k, torch.int32, rows, "top_k"),
+                                  _array(top_p, torch.float32, rows, "top_p"), _array(min_p, torch.float32, rows, "min_p"), _array(tokens, torch.int32, rows, "tokens"),
+                                  _array(logprobs, torch.float32, rows, "logprobs")))
+    return tokens, logprobs
+
+
+# ---- requests of unequal length over one cache of pages in 8 bits ---------------------------------------------------------------
+def _here(t: torch.Tensor) -> torch.device:
+    """The device of a tensor that lies on the current GPU, whose current stream the call uses."""
+    if not t.is_cuda:
+        raise KmllError(-2, "operand must be a CUDA tensor (there is no CPU path)")
+    if t.get_device() != torch.cuda.current_device():
+        raise KmllError(-2, f"operand lies on GPU {t.get_device()}, the current one is {torch.cuda.current_device()}")
+    return t.device
+
+
+def _array(t, dtype, least: int, name: str) -> int | None:
+    """Pointer of a contiguous array of at least `least` entries; None stays None."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.numel() < least:
+        raise KmllError(-2, f"{name} must hold {least} entries of {dtype}, got {t.numel()} of {t.dtype}")
+    _here(t)
+    return _p(t)
+
+
+@dataclass
+class DevicePagedI8Cache:
+    """Keys and values of many requests in pages of int8 codes with a scale per (page, kv head); layouts in include/kmll_b200.h."""
+    k_codes: torch.Tensor   # int8 [pages, kv_heads, head_dim / 16, block, 16]
+    v_codes: torch.Tensor   # int8 [pages, kv_heads, block / 16, head_dim, 16]
+    k_scales: torch.Tensor  # float32 [pages, kv_heads]
+    v_scales: torch.Tensor  # float32 [pages, kv_heads]
+    pages: int
+    block: int
+    kv_heads: int
+    head_dim: int
+
+    @staticmethod
+    def create(pages: int, block: int, kv_heads: int, head_dim: int, device="cuda") -> "DevicePagedI8Cache":
+        if block not in (16, 32, 64, 128) or head_dim % 16 or not 16 <= head_dim <= 256 or pages < 1 or kv_heads < 1:
+            raise KmllError(-2, f"no cache of {pages} pages of {block} tokens, {kv_heads} heads of {head_dim}")
+        return DevicePagedI8Cache(torch.zeros((pages, kv_heads, head_dim // 16, block, 16), dtype=torch.int8, device=device),
+                                  torch.zeros((pages, kv_heads, block // 16, head_dim, 16), dtype=torch.int8, device=device),
+                                  torch.zeros((pages, kv_heads), dtype=torch.float32, device=device), torch.zeros((pages, kv_heads), dtype=torch.float32, device=device),
+                                  pages, block, kv_heads, head_dim)
+
+    @staticmethod
+    def from_parts(k_codes, v_codes, k_scales, v_scales) -> "DevicePagedI8Cache":
+        if k_codes.dim() != 5 or v_codes.dim() != 5 or k_codes.shape[4] != 16 or v_codes.shape[4] != 16:
+            raise KmllError(-2, "paged codes must be [pages, kv_heads, head_dim / 16, block, 16] and [pages, kv_heads, block / 16, head_dim, 16]")
+        pages, kv_heads, units, block, _ = k_codes.shape
+        if tuple(v_codes.shape) != (pages, kv_heads, block // 16, 16 * units, 16) or block not in (16, 32, 64, 128):
+            raise KmllError(-2, f"paged codes of keys {tuple(k_codes.shape)} and values {tuple(v_codes.shape)} do not belong together")
+        if tuple(k_scales.shape) != (pages, kv_heads) or tuple(v_scales.shape) != (pages, kv_heads):
+            raise KmllError(-2, "paged scales must be [pages, kv_heads]")
+        if k_codes.dtype != torch.int8 or v_codes.dtype != torch.int8 or k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32:
+            raise KmllError(-2, "paged codes must be int8, their scales float32")
+        return DevicePagedI8Cache(k_codes, v_codes, k_scales, v_scales, pages, block, kv_heads, 16 * units)
+
+    def _pointers(self):
+        _here(self.k_codes)
+        return _p(self.k_codes), _p(self.k_scales), _p(self.v_codes), _p(self.v_scales), self.pages, self.block
+
+    @property
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.k_codes, self.v_codes, self.k_scales, self.v_scales))
+
+
+def paged_plan(lengths, new_tokens, block: int, block_table, free_blocks, free_count, context, query_start, positions, slots, free_count_out, status):
+    """The pages of a step: kmll_paged_plan.  int32 arrays on the device; positions and slots as long as the step's rows may be, block_table [requests,
+    width] (updated), free_blocks a stack of free_count[0] pages."""
+    requests, width = block_table.shape
+    rows = positions.numel()
+    i32 = torch.int32
+    if slots.numel() != rows:
+        raise KmllError(-2, "positions and slots must be of one length")
+    check(load().kmll_paged_plan(_stream(), _array(lengths, i32, requests, "lengths"), _array(new_tokens, i32, requests, "new_tokens"), requests, block,
+                                 _array(block_table, i32, 0, "block_table"), width, _array(free_blocks, i32, 0, "free_blocks"), free_blocks.numel(),
+                                 _array(free_count, i32, 1, "free_count"), rows, _array(context, i32, requests, "context"),
+                                 _array(query_start, i32, requests + 1, "query_start"), _array(positions, i32, rows, "positions"), _array(slots, i32, rows, "slots"),
+                                 _array(free_count_out, i32, 1, "free_count_out"), _array(status, i32, 1, "status")))
+
+
+def paged_release(context, ended, block: int, block_table, free_blocks, free_count, context_out, free_count_out, status):
+    """Pages of the requests with ended != 0 go back on the stack: kmll_paged_release."""
+    requests, width = block_table.shape
+    i32 = torch.int32
+    check(load().kmll_paged_release(_stream(), _array(context, i32, requests, "context"), _array(ended, i32, requests, "ended"), requests, block,
+                                    _array(block_table, i32, 0, "block_table"), width, _array(free_blocks, i32, 0, "free_blocks"), free_blocks.numel(),
+                                    _array(free_count, i32, 1, "free_count"), _array(context_out, i32, requests, "context_out"),
+                                    _array(free_count_out, i32, 1, "free_count_out"), _array(status, i32, 1, "status")))
+
+
+def _head_rows(t, heads, head_dim, dtype, name):
+    """(pointer, pitch in elements) of rows [tokens, heads, head_dim] (or [tokens, heads * head_dim]) whose heads lie together."""
+    if t.dtype != dtype or t.numel() != t.shape[0] * heads * head_dim:
+        raise KmllError(-2, f"{name} must be [tokens, {heads}, {head_dim}] in {dtype}, got {tuple(t.shape)} in {t.dtype}")
+    _here(t)
+    whole = t.stride(-1) == 1 and (t.dim() == 2 or t.stride(1) == head_dim or heads == 1)
+    if t.numel() and not (t.is_contiguous() or (t.dim() in (2, 3) and whole)):
+        raise KmllError(-2, f"the heads of a row of {name} must lie together")
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else heads * head_dim
+
+
+def prepare_paged_attention(query, key, value, freqs, positions, slots, cache: DevicePagedI8Cache, query_rot=None):
+    """Rotation of a step's queries and keys, keys and values into the cache: prepare_incremental_attention (ops/inference.rs:1291-1362) for rows
+    of many requests.  query [tokens, heads, head_dim], key and value [tokens, kv_heads, head_dim], f32 or bf16; freqs None: no
+    rotation.  Returns the turned queries."""
+    tokens, heads = query.shape[0], query.numel() // max(1, query.shape[0] * cache.head_dim)
+    dtype = query.dtype
+    if dtype not in (torch.float32, torch.bfloat16) or key.shape[0] != tokens or value.shape[0] != tokens:
+        raise KmllError(-2, "query, key and value must be rows of the same tokens in float32 or bfloat16")
+    q, k, v = _head_rows(query, heads, cache.head_dim, dtype, "query"), _head_rows(key, cache.kv_heads, cache.head_dim, dtype, "key"), \
+        _head_rows(value, cache.kv_heads, cache.head_dim, dtype, "value")
+    query_rot = torch.empty(query.shape, dtype=dtype, device=query.device) if query_rot is None else query_rot
+    if query_rot.numel() != query.numel() or query_rot.dtype != dtype:
+        raise KmllError(-2, "query_rot must be as large as query, of its type")
+    n_freqs = 0 if freqs is None else freqs.numel()
+    check(load().kmll_prepare_paged_attention(_stream(), *q, *k, *v, 1 if dtype == torch.float32 else 0, _array(freqs, torch.float32, 0, "freqs"), n_freqs,
+                                              None if freqs is None else _array(positions, torch.int32, tokens, "positions"), _array(slots, torch.int32, tokens, "slots"),
+                                              tokens, heads, cache.kv_heads, cache.head_dim, _p(query_rot), *cache._pointers()))
+    return query_rot
+
+
+def paged_cache_rows(cache: DevicePagedI8Cache, slots, k=None, v=None):
+    """Rows of the cache in f32: (keys, values), [count, kv_heads, head_dim] each."""
+    shape = (slots.numel(), cache.kv_heads, cache.head_dim)
+    dev = _here(cache.k_codes)
+    k = torch.empty(shape, dtype=torch.float32, device=dev) if k is None else k
+    v = torch.empty(shape, dtype=torch.float32, device=dev) if v is None else v
+    need = shape[0] * shape[1] * shape[2]
+    check(load().kmll_paged_cache_rows(_stream(), *cache._pointers(), cache.kv_heads, cache.head_dim, _array(slots, torch.int32, 0, "slots"), shape[0],
+                                       _array(k, torch.float32, need, "k"), _array(v, torch.float32, need, "v")))
+    return k, v
+
+
+def paged_attention_workspace(cache: DevicePagedI8Cache, heads: int, requests: int, tokens: int, max_query: int, max_context: int):
+    """Scratch of paged_attention for steps up to these sizes (zeroed; None where none is needed); one for calls that may overlap each."""
+    n = int(load().kmll_paged_attention_workspace_bytes(heads, cache.kv_heads, cache.head_dim, requests, tokens, max_query, max_context))
+    return torch.zeros(n, dtype=torch.uint8, device=cache.k_codes.device) if n > 0 else None
+
+
+def paged_attention(query, query_start, context, block_table, cache: DevicePagedI8Cache, max_query: int, max_context: int, scale: float, window: int = 0, workspace=None,
+                    out=None):
+    """Attention of a step's rows, query [tokens, heads, head_dim] f32 or bf16, over the pages of their requests: kmll_paged_attention."""
+    tokens, heads = query.shape[0], query.numel() // max(1, query.shape[0] * cache.head_dim)
+    dtype = query.dtype
+    if dtype not in (torch.float32, torch.bfloat16) or query.numel() != tokens * heads * cache.head_dim:
+        raise KmllError(-2, f"query must be [tokens, heads, {cache.head_dim}] in float32 or bfloat16")
+    dev = _here(query)
+    out = torch.empty((tokens, heads * cache.head_dim), dtype=dtype, device=dev) if out is None else out
+    if out.numel() != query.numel() or out.dtype != dtype:
+        raise KmllError(-2, "out must be as large as query, of its type")
+    requests, width = block_table.shape
+    need = int(load().kmll_paged_attention_workspace_bytes(heads, cache.kv_heads, cache.head_dim, requests, tokens, max_query, max_context))
+    if workspace is None and need > 0:
+        workspace = torch.zeros(need, dtype=torch.uint8, device=dev)
+    check(load().kmll_paged_attention(_stream(), _p(query), 1 if dtype == torch.float32 else 0, _array(query_start, torch.int32, requests + 1, "query_start"),
+                                      _array(context, torch.int32, requests, "context"), _array(block_table, torch.int32, 0, "block_table"), width, requests, tokens,
+                                      max_query, max_context, heads, *cache._pointers(), cache.kv_heads, cache.head_dim, scale, window,
+                                      _array(workspace, torch.uint8, need, "workspace"), _p(out)))
+    return out
+
+
 # ---- operators of the layered decoders (bf16 weights [rows, cols], cols a multiple of 8) ------------------------------------
 def _pitch(w: torch.Tensor) -> int:
     if w.dtype != torch.bfloat16 or w.dim() != 2 or w.shape[1] % 8:
