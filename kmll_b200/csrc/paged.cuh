@@ -7,4 +7,49 @@ namespace kmll {
 
 int check_paged_cache(const char* who, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, int pages, int block, int kv_heads, int head_dim);
 
+struct PagedArgs {
+    const void* query;
+    const int32_t *query_start, *context, *table;
+    int width, requests, tokens, heads, kv_heads, head_dim, block, pages;
+    const int8_t *k_codes, *v_codes;
+    const float *k_scales, *v_scales;
+    float scale2;  // log2(e) times the score scale
+    int window;
+    void* out;
+    int skip_rows;  // requests with at most this many rows (tokens times query heads of a kv head) belong to another kernel
+};
+
+template <typename T>
+__device__ inline float row_entry(const void* p, size_t i);
+template <>
+__device__ inline float row_entry<float>(const void* p, size_t i) { return static_cast<const float*>(p)[i]; }
+template <>
+__device__ inline float row_entry<uint16_t>(const void* p, size_t i) { return bf16_bits_to_f32(static_cast<const uint16_t*>(p)[i]); }
+__device__ inline void store_row(float* p, float v) { *p = v; }
+__device__ inline void store_row(uint16_t* p, float v) { *p = f32_to_bf16_bits(v); }
+
+// A request's rows and the positions they attend together.
+struct PagedRequest {
+    int first, rows;  // rows of the step, tokens
+    int pos0;         // position of the first row (negative: rows that attend nothing)
+    int lo, hi;       // positions lo .. hi - 1
+    __device__ static PagedRequest of(const PagedArgs& a, int r) {
+        PagedRequest q;
+        q.first = a.query_start[r];
+        q.rows = min(a.query_start[r + 1], a.tokens) - q.first;
+        if (q.first < 0 || q.rows < 0) q.rows = 0;
+        const int context = a.context[r];
+        q.pos0 = context - q.rows;
+        q.hi = max(0, min(context, a.width * a.block));
+        q.lo = a.window > 0 ? min(q.hi, max(0, q.pos0 - a.window + 1)) : 0;
+        return q;
+    }
+};
+
+// paged_decode.cu: requests of at most kPagedDecodeRows rows, heads of 64 or 128
+constexpr int kPagedDecodeRows = 16;
+bool paged_decode_serves(int head_dim);
+size_t paged_decode_workspace_bytes(int requests, int kv_heads, int head_dim, int max_rows);
+int paged_decode_launch(cudaStream_t stream, const PagedArgs& a, bool f32, int max_rows, int max_context, void* workspace);
+
 }  // namespace kmll

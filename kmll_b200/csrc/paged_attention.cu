@@ -7,25 +7,6 @@
 namespace kmll {
 namespace {
 
-struct PagedArgs {
-    const void* query;
-    const int32_t *query_start, *context, *table;
-    int width, requests, tokens, heads, kv_heads, head_dim, block, pages;
-    const int8_t *k_codes, *v_codes;
-    const float *k_scales, *v_scales;
-    float scale2;  // log2(e) times the score scale
-    int window;
-    void* out;
-};
-
-template <typename T>
-__device__ inline float row_entry(const void* p, size_t i);
-template <>
-__device__ inline float row_entry<float>(const void* p, size_t i) { return static_cast<const float*>(p)[i]; }
-template <>
-__device__ inline float row_entry<uint16_t>(const void* p, size_t i) { return bf16_bits_to_f32(static_cast<const uint16_t*>(p)[i]); }
-__device__ inline void store_row(float* p, float v) { *p = v; }
-__device__ inline void store_row(uint16_t* p, float v) { *p = f32_to_bf16_bits(v); }
 __device__ inline int code_at(uint4 u, int i) {
     const uint32_t w = i < 4 ? u.x : i < 8 ? u.y : i < 12 ? u.z : u.w;
     return (int)(int8_t)(w >> (8 * (i & 3)));
@@ -45,10 +26,9 @@ __global__ void __launch_bounds__(128) paged_rows_kernel(const PagedArgs a) {
         if (a.query_start[mid] <= t) lo = mid;
         else hi = mid;
     }
-    const int first = a.query_start[lo], behind = a.query_start[lo + 1];
-    if (t < first || t >= behind) return;
-    const int context = min(a.context[lo], a.width * a.block), pos = min(a.context[lo] - (behind - first) + (t - first), context - 1);
-    const int start = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    const PagedRequest rq = PagedRequest::of(a, lo);
+    if (t < rq.first || t >= rq.first + rq.rows || (long long)rq.rows * group <= a.skip_rows) return;
+    const int pos = min(rq.pos0 + (t - rq.first), rq.hi - 1), start = a.window > 0 ? max(0, rq.pos0 + (t - rq.first) - a.window + 1) : 0;
     const int32_t* const table = a.table + (size_t)lo * a.width;
     for (int g = warp; g < group; g += 4) {
         const size_t row = ((size_t)t * a.heads + (size_t)h * group + g) * hd;
@@ -108,7 +88,8 @@ __global__ void __launch_bounds__(128) paged_rows_kernel(const PagedArgs a) {
 using namespace kmll;
 
 extern "C" size_t kmll_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim, int requests, int tokens, int max_query, int max_context) {
-    return 0;
+    if (heads <= 0 || kv_heads <= 0 || requests <= 0 || tokens <= 0 || max_query <= 0 || !paged_decode_serves(head_dim)) return 0;
+    return paged_decode_workspace_bytes(requests, kv_heads, head_dim, (long long)max_query * (heads / kv_heads) <= 8 ? 8 : kPagedDecodeRows);
 }
 
 extern "C" int kmll_paged_attention(kmll_stream_t stream, const void* query, int is_f32, const int32_t* query_start, const int32_t* context, const int32_t* block_table,
@@ -127,8 +108,16 @@ extern "C" int kmll_paged_attention(kmll_stream_t stream, const void* query, int
     KMLL_REQUIRE_PTR(context);
     KMLL_REQUIRE_PTR(block_table);
     KMLL_REQUIRE_PTR(out);
-    const PagedArgs a = {query, query_start, context, block_table, table_width, requests, tokens, heads, kv_heads, head_dim, block, pages, k_codes, v_codes,
-                         k_scales, v_scales, scale * 1.4426950408889634f, window, out};
+    PagedArgs a = {query, query_start, context, block_table, table_width, requests, tokens, heads, kv_heads, head_dim, block, pages, k_codes, v_codes,
+                   k_scales, v_scales, scale * 1.4426950408889634f, window, out, 0};
+    const long long max_rows = (long long)max_query * (heads / kv_heads);
+    if (paged_decode_serves(head_dim) && (reinterpret_cast<uintptr_t>(query) & 15u) == 0) {
+        KMLL_REQUIRE_PTR(workspace);
+        KMLL_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "paged attention: the workspace must be 16-byte aligned");
+        KMLL_TRY_RC(paged_decode_launch(as_stream(stream), a, is_f32 != 0, max_rows <= 8 ? 8 : kPagedDecodeRows, max_context, workspace));
+        if (max_rows <= kPagedDecodeRows) return check_launch("paged attention");
+        a.skip_rows = kPagedDecodeRows;
+    }
     const cudaError_t e = is_f32 ? launch(paged_rows_kernel<float>, dim3(tokens, kv_heads), dim3(128), 0, as_stream(stream), true, a)
                                  : launch(paged_rows_kernel<uint16_t>, dim3(tokens, kv_heads), dim3(128), 0, as_stream(stream), true, a);
     if (e != cudaSuccess) return fail(KMLL_ERR_CUDA, "paged attention: %s", cudaGetErrorString(e));

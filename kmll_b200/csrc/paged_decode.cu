@@ -1,0 +1,528 @@
+// Attention of single tokens (and of a few rows) over the paged 8-bit cache: the codes go to the tensor cores as they lie.
+//
+//   S^T[key][row] = K[key] . q[row]: A = 16 keys x 32 codes by ldmatrix, B = q as a 24-bit integer (bf16 rows: 16 bits) below the largest
+//   entry of its row, in bytes; mma.m16n8k32 s8 x u8 / s8 -> s32, one MMA per byte, exact; S = k_scale * q_scale * (D0 + 2^8 D1 + 2^16 D2)
+//   O^T[dim][row] += V^T[dim][key] P^T[key][row]: A = 16 columns x 32 keys (values lie with the keys of a column together), B =
+//   softmax weights times the page's value scale, as 24-bit (bf16: 16-bit) fractions of the largest scale in the tile, in bytes
+// Nothing is converted on the way from memory to the tensor cores, and both contractions are exact; what is rounded are q and the weights,
+// to 2^-24 of the largest of their row.  (f32 rows cost three MMAs where bf16 heads and remainders would cost two of twice the size,
+// behind a conversion of every code.)
+//
+// A warp is a pipeline of its own over tiles of 32 keys (two stages of keys and values, cp.async in 16-byte groups), with its own running
+// maximum and sum; four warps take the tiles of a stretch in turn and meet at its end.  The work of a call is one axis, requests x kv heads x
+// tiles, cut into equal shares for the blocks, whatever the contexts; where a share ends within a head, the blocks that have parts of it leave
+// maximum, sum and O in the workspace and the last to arrive joins them in the order of the blocks: results do not change from call to call.
+// Bound: HBM (2 * head_dim bytes per key and kv head).
+#include <type_traits>
+
+#include "internal.cuh"
+#include "mma_bf16.cuh"
+#include "paged.cuh"
+
+namespace kmll {
+namespace {
+
+constexpr int kPdWarps = 4;
+constexpr int kPdThreads = kPdWarps * 32;
+constexpr int kPdKeys = 32;      // keys of a tile
+constexpr int kPdBlocks = 444;   // three blocks on each of 148 multiprocessors
+constexpr int kPdStages = 2;
+
+struct PdMeta {  // of a stage: the two groups of 16 keys may lie in two pages
+    float k_scale[2], v_scale[2];
+    int there[2], unused[2];
+};
+
+template <int HD>
+struct PdShape {
+    static constexpr int kTile = HD * kPdKeys;              // bytes of the keys or of the values of a tile
+    static constexpr int kStage = 2 * kTile;
+    static constexpr int kWarp = kPdStages * kStage;
+    static constexpr int kOffMeta = kPdWarps * kWarp;
+    static constexpr int kSmem = kOffMeta + kPdWarps * kPdStages * (int)sizeof(PdMeta);
+};
+
+__device__ inline void mma_s8u8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ inline void mma_s8s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ inline void cp_async4_zfill_to(uint32_t smem_addr, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_addr), "l"(src), "r"(bytes) : "memory");
+}
+template <int N>
+__device__ inline void cp_async_wait_group() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ inline void cp_async_commit_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+template <typename T>
+__device__ inline void load4(const void* p, size_t i, float (&v)[4]);
+template <>
+__device__ inline void load4<float>(const void* p, size_t i, float (&v)[4]) {
+    const float4 x = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+}
+template <>
+__device__ inline void load4<uint16_t>(const void* p, size_t i, float (&v)[4]) {
+    const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+    v[0] = __uint_as_float(x.x << 16); v[1] = __uint_as_float(x.x & 0xffff0000u);
+    v[2] = __uint_as_float(x.y << 16); v[3] = __uint_as_float(x.y & 0xffff0000u);
+}
+
+struct PdWork {
+    int* arrived;     // [requests * kv_heads], zero between calls
+    float* partials;  // [blocks][2][8 * NC rows][2 + HD]
+};
+
+// Tiles of a request that this kernel serves (one where its rows attend nothing: they are written as zeros).
+__device__ inline int pd_tiles(const PagedRequest& q, int group, int limit) {
+    if (q.rows == 0 || (long long)q.rows * group > limit) return 0;
+    return max(1, (q.hi + kPdKeys - 1) / kPdKeys - q.lo / kPdKeys);
+}
+
+// NB: bytes of q and of the weights; NC: columns of eight rows.
+template <int HD, typename T, int NB, int NC>
+__global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kernel(const PagedArgs a, const PdWork work) {
+    using S = PdShape<HD>;
+    constexpr int KS = HD / 32, DT = HD / 16, ROWS = 8 * NC, PITCH = HD + 4;
+    extern __shared__ __align__(128) unsigned char pd_smem[];
+    __shared__ long long s_before[kPdWarps + 1];
+    __shared__ long long s_start;
+    __shared__ int s_request, s_last;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, group = a.heads / a.kv_heads;
+    pdl_wait();
+    // ---- the share of this block
+    const int per = (a.requests + kPdThreads - 1) / kPdThreads;
+    long long mine = 0;
+    for (int i = 0; i < per; ++i) {
+        const int r = tid * per + i;
+        if (r < a.requests) mine += pd_tiles(PagedRequest::of(a, r), group, ROWS);
+    }
+    long long before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += v;
+    }
+    if (lane == 31) s_before[warp] = before;
+    __syncthreads();
+    before -= mine;
+    long long total = 0;
+    for (int w = 0; w < kPdWarps; ++w) {
+        if (w == warp) before += total;
+        total += s_before[w];
+    }
+    total *= a.kv_heads;
+    before *= a.kv_heads;
+    mine *= a.kv_heads;
+    const long long share = max((long long)kPdWarps, (total + gridDim.x - 1) / gridDim.x);
+    const long long w0 = (long long)blockIdx.x * share, w1 = min(total, w0 + share);
+    if (w0 >= w1) return;
+    if (w0 >= before && w0 < before + mine) {
+        long long at = before;
+        for (int i = 0; i < per; ++i) {
+            const int r = tid * per + i;
+            if (r >= a.requests) break;
+            const long long n = (long long)pd_tiles(PagedRequest::of(a, r), group, ROWS) * a.kv_heads;
+            if (w0 < at + n) {
+                s_request = r;
+                s_start = at;
+                break;
+            }
+            at += n;
+        }
+    }
+    __syncthreads();
+    int r = s_request;
+    long long start = s_start;  // of the request on the axis
+    unsigned char* const ring = pd_smem + warp * S::kWarp;
+    PdMeta* const meta = reinterpret_cast<PdMeta*>(pd_smem + S::kOffMeta) + warp * kPdStages;
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring), meta_at = (uint32_t)__cvta_generic_to_shared(meta);
+    const int half = lane >> 4;  // group of 16 keys whose copies this lane makes
+    // place of a key among the 16 of its group: the keys of the MMA's rows 0-7 and 8-15 are such that the weights come out of the
+    // transpose with four keys in a row in one lane, which is how the values have them
+    const int key16 = lane & 15, place16 = 8 * ((key16 >> 1) & 1) + 2 * (key16 >> 2) + (key16 & 1);
+
+    for (long long w = w0; w < w1;) {
+        const PagedRequest rq = PagedRequest::of(a, r);
+        const int tiles = pd_tiles(rq, group, ROWS);
+        if (tiles == 0 || w >= start + (long long)tiles * a.kv_heads) {
+            start += (long long)tiles * a.kv_heads;
+            ++r;
+            continue;
+        }
+        const int h = (int)((w - start) / tiles), ta = (int)((w - start) - (long long)h * tiles);
+        const int tb = (int)min((long long)tiles, ta + (w1 - w));
+        const int key0 = rq.lo / kPdKeys * kPdKeys;  // of tile 0
+        const int32_t* const table = a.table + (size_t)r * a.width;
+        const int mine_n = tb - ta > warp ? (tb - ta - warp + kPdWarps - 1) / kPdWarps : 0;
+        auto page_of = [&](int i) {  // of this lane's group of 16 keys in the warp's i-th tile; -1: nothing there
+            const int key = key0 + (ta + warp + i * kPdWarps) * kPdKeys + half * 16;
+            if (i >= mine_n || key >= rq.hi) return -1;
+            const int p = table[key / a.block];
+            return p >= 0 && p < a.pages ? p : -1;
+        };
+        auto in_page = [&](int i) { return (key0 + (ta + warp + i * kPdWarps) * kPdKeys + half * 16) % a.block; };
+        auto copy_keys = [&](int i, int page) {
+            if (i < mine_n) {
+                const int st = i % kPdStages, at = in_page(i);
+                const size_t ph = (size_t)max(page, 0) * a.kv_heads + h;
+                const uint32_t bytes = page >= 0 ? 16u : 0u;
+                const int8_t* const src = a.k_codes + ph * a.block * HD + (at + key16) * 16;
+                const uint32_t dst = ring_at + st * S::kStage + (half * 16 + place16) * 16;
+#pragma unroll
+                for (int c = 0; c < HD / 16; ++c) cp_async16_zfill_to(dst + c * (kPdKeys * 16), src + (size_t)c * a.block * 16, bytes);
+                if (key16 == 0) {
+                    const uint32_t m = meta_at + st * (uint32_t)sizeof(PdMeta) + half * 4;
+                    cp_async4_zfill_to(m, a.k_scales + ph, page >= 0 ? 4u : 0u);
+                    cp_async4_zfill_to(m + 8, a.v_scales + ph, page >= 0 ? 4u : 0u);
+                    meta[st].there[half] = page >= 0;
+                }
+            }
+            cp_async_commit_group();
+        };
+        auto copy_values = [&](int i, int page) {
+            if (i < mine_n) {
+                const int st = i % kPdStages, at = in_page(i);
+                const size_t ph = (size_t)max(page, 0) * a.kv_heads + h;
+                const uint32_t bytes = page >= 0 ? 16u : 0u;
+                const int8_t* const src = a.v_codes + ph * a.block * HD + ((size_t)(at >> 4) * HD + key16) * 16;
+                const uint32_t dst = ring_at + st * S::kStage + S::kTile + (half * HD + key16) * 16;
+#pragma unroll
+                for (int d = 0; d < HD / 16; ++d) cp_async16_zfill_to(dst + d * 256, src + d * 256, bytes);
+            }
+            cp_async_commit_group();
+        };
+        int pages[kPdStages];
+#pragma unroll
+        for (int i = 0; i < kPdStages; ++i) pages[i] = page_of(i);
+#pragma unroll
+        for (int i = 0; i < kPdStages; ++i) {
+            copy_keys(i, pages[i]);
+            copy_values(i, pages[i]);
+        }
+        int next_page = page_of(kPdStages);
+
+        // ---- q of eight rows a column: bytes of round(q * 2^sh), the largest entry of a row between 2^(8 NB - 2) and 2^(8 NB - 1)
+        const int n_rows = rq.rows * group;
+        uint32_t qb[NC][NB][KS][2];
+        float q_unit[NC][2];   // of this lane's two score columns: 2^-sh * scale
+        int last[NC][2], first_key[NC][2];
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) {
+            const int row = nc * 8 + g;
+            const bool live = row < n_rows;
+            const size_t at = ((size_t)(rq.first + (live ? row / group : 0)) * a.heads + (size_t)h * group + (live ? row % group : 0)) * HD;
+            float q[KS][2][4], top = 0.0f;
+            bool finite = true;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    load4<T>(a.query, at + ks * 32 + e * 16 + t * 4, q[ks][e]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        top = fmaxf(top, fabsf(q[ks][e][i]));
+                        finite = finite && fabsf(q[ks][e][i]) < INFINITY;
+                    }
+                }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int bits = finite ? 1 : 0;
+            finite = (bits & __shfl_xor_sync(0xffffffffu, bits, 1)) != 0;
+            finite = ((finite ? 1 : 0) & __shfl_xor_sync(0xffffffffu, finite ? 1 : 0, 2)) != 0;
+            int e2 = 0;
+            if (top > 0.0f && top < INFINITY) frexpf(top, &e2);  // top in [2^(e2 - 1), 2^e2)
+            const int sh = max(-120, min(120, 8 * NB - 1 - e2));
+            const float up = ldexpf(1.0f, sh);
+            const int most = (1 << (8 * NB - 1)) - 1;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    uint32_t x[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = live ? (uint32_t)max(-most, min(most, __float2int_rn(q[ks][e][i] * up))) : 0u;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const uint32_t pick = (uint32_t)(b | ((b + 4) << 4));
+                        qb[nc][b][ks][e] = __byte_perm(__byte_perm(x[0], x[1], pick), __byte_perm(x[2], x[3], pick), 0x5410);
+                    }
+                }
+            // (a row with an infinity or NaN has no scores)
+            const float unit = finite ? ldexpf(a.scale2, -sh) : __int_as_float(0x7fffffff);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                q_unit[nc][e] = __shfl_sync(0xffffffffu, unit, 8 * t + 4 * e);
+                const int col = nc * 8 + 2 * t + e;
+                last[nc][e] = col < n_rows ? min(rq.pos0 + col / group, rq.hi - 1) : -1;
+                first_key[nc][e] = a.window > 0 ? last[nc][e] < 0 ? 0 : rq.pos0 + col / group - a.window + 1 : 0;
+            }
+        }
+        const int sure_end = min(rq.pos0 + 1, rq.hi), sure_from = a.window > 0 ? rq.pos0 + rq.rows - a.window : 0;  // keys that every row attends
+
+        float m[NC][2], l[NC][2], acc[NC][DT][4];
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) {
+            m[nc][0] = m[nc][1] = -INFINITY;
+            l[nc][0] = l[nc][1] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[nc][d][0] = acc[nc][d][1] = acc[nc][d][2] = acc[nc][d][3] = 0.0f;
+        }
+        for (int i = 0; i < mine_n; ++i) {
+            const int st = i % kPdStages;
+            const unsigned char* const keys = ring + st * S::kStage;
+            const unsigned char* const vals = keys + S::kTile;
+            cp_async_wait_group<2 * kPdStages - 1>();
+            __syncwarp();
+            const PdMeta mt = meta[st];
+            // ---- scores of 2 x 16 keys
+            float s[NC][2][4];
+#pragma unroll
+            for (int half16 = 0; half16 < 2; ++half16) {
+                int d[NC][NB][4];
+#pragma unroll
+                for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) d[nc][b][0] = d[nc][b][1] = d[nc][b][2] = d[nc][b][3] = 0;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    uint32_t f[4];
+                    ldmatrix_x4(f, keys + ((2 * ks + (lane >> 4)) * kPdKeys + half16 * 16 + (lane & 15)) * 16);
+#pragma unroll
+                    for (int nc = 0; nc < NC; ++nc) {
+#pragma unroll
+                        for (int b = 0; b < NB - 1; ++b) mma_s8u8(d[nc][b], f, qb[nc][b][ks][0], qb[nc][b][ks][1]);
+                        mma_s8s8(d[nc][NB - 1], f, qb[nc][NB - 1][ks][0], qb[nc][NB - 1][ks][1]);
+                    }
+                }
+#pragma unroll
+                for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float v = (float)(d[nc][0][e] + (d[nc][1][e] << 8));
+                        if (NB == 3) v = fmaf((float)d[nc][NB - 1][e], 65536.0f, v);
+                        s[nc][half16][e] = v * (mt.k_scale[half16] * q_unit[nc][e & 1]);
+                    }
+            }
+            // (the places of the keys are free again)
+            __syncwarp();
+            const int page_next = next_page;
+            // The scales of a stage come with its keys, but its value scales are read above: both are in registers now.
+            copy_keys(i + kPdStages, page_next);
+            next_page = page_of(i + kPdStages + 1);
+            const int tile_key = key0 + (ta + warp + i * kPdWarps) * kPdKeys;
+            if (tile_key + kPdKeys > sure_end || tile_key < sure_from || !(mt.there[0] && mt.there[1])) {
+#pragma unroll
+                for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+                    for (int half16 = 0; half16 < 2; ++half16)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int key = tile_key + half16 * 16 + 4 * (g >> 1) + (g & 1) + 2 * (e >> 1);
+                            if (key > last[nc][e & 1] || key < first_key[nc][e & 1] || !mt.there[half16]) s[nc][half16][e] = -INFINITY;
+                        }
+            }
+            // ---- running maximum and sum of this lane's two columns; weights as whole numbers
+            const float vmax = fmaxf(mt.v_scale[0], mt.v_scale[1]);
+            constexpr float kWhole = NB == 3 ? 16777215.0f : 65535.0f;
+            const float v_rel[2] = {vmax > 0.0f ? mt.v_scale[0] / vmax * kWhole : 0.0f, vmax > 0.0f ? mt.v_scale[1] / vmax * kWhole : 0.0f};
+            uint32_t pb[NC][NB][2];
+#pragma unroll
+            for (int nc = 0; nc < NC; ++nc) {
+                float turn[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float top = fmaxf(fmaxf(s[nc][0][e], s[nc][0][e + 2]), fmaxf(s[nc][1][e], s[nc][1][e + 2]));
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    top = fmaxf(top, m[nc][e]);
+                    const float base = top == -INFINITY ? 0.0f : top;
+                    turn[e] = ex2_approx(m[nc][e] - base);
+                    m[nc][e] = top;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int half16 = 0; half16 < 2; ++half16)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            float& x = s[nc][half16][e + 2 * k];
+                            x = ex2_approx(x - base);
+                            sum += x;
+                        }
+                    l[nc][e] = fmaf(l[nc][e], turn[e], sum);
+                }
+                if (__any_sync(0xffffffffu, turn[0] != 1.0f || turn[1] != 1.0f)) {
+#pragma unroll
+                    for (int d = 0; d < DT; ++d)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[nc][d][e] *= turn[e & 1];
+                }
+#pragma unroll
+                for (int half16 = 0; half16 < 2; ++half16) {
+                    uint32_t x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = __float2uint_rn(s[nc][half16][e] * v_rel[half16]);
+                    const uint32_t r0 = movmatrix_trans(__byte_perm(x[0], x[1], 0x5410)), r1 = movmatrix_trans(__byte_perm(x[2], x[3], 0x5410));
+                    pb[nc][0][half16] = __byte_perm(r0, r1, 0x6420);
+                    pb[nc][1][half16] = __byte_perm(r0, r1, 0x7531);
+                    if (NB == 3) {
+                        const uint32_t r2 = movmatrix_trans(__byte_perm(x[0], x[1], 0x7632)), r3 = movmatrix_trans(__byte_perm(x[2], x[3], 0x7632));
+                        pb[nc][NB - 1][half16] = __byte_perm(r2, r3, 0x6420);
+                    }
+                }
+            }
+            cp_async_wait_group<2 * kPdStages - 1>();
+            __syncwarp();
+            const float v_unit = vmax / kWhole;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                uint32_t f[4];
+                ldmatrix_x4(f, vals + ((lane >> 4) * HD + dt * 16 + (lane & 15)) * 16);
+#pragma unroll
+                for (int nc = 0; nc < NC; ++nc) {
+                    int d[NB][4];
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        d[b][0] = d[b][1] = d[b][2] = d[b][3] = 0;
+                        mma_s8u8(d[b], f, pb[nc][b][0], pb[nc][b][1]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float v = (float)(d[0][e] + (d[1][e] << 8));
+                        if (NB == 3) v = fmaf((float)d[NB - 1][e], 65536.0f, v);
+                        acc[nc][dt][e] = fmaf(v, v_unit, acc[nc][dt][e]);
+                    }
+                }
+            }
+            __syncwarp();
+            copy_values(i + kPdStages, page_next);
+        }
+        cp_async_wait_group<0>();
+        __syncthreads();
+        // ---- the four warps' shares of the stretch
+        float* const stage = reinterpret_cast<float*>(ring);        // [ROWS][PITCH], then maximum and sum of each row
+        static_assert(ROWS * (PITCH + 2) * 4 <= S::kWarp, "the sums of a warp fit over its ring");
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float sum = l[nc][e];
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                const int row = nc * 8 + 2 * t + e;
+                if (g == 0) {
+                    stage[ROWS * PITCH + 2 * row] = m[nc][e];
+                    stage[ROWS * PITCH + 2 * row + 1] = sum;
+                }
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    stage[row * PITCH + d * 16 + g] = acc[nc][d][e];
+                    stage[row * PITCH + d * 16 + g + 8] = acc[nc][d][e + 2];
+                }
+            }
+        __syncthreads();
+        const long long seq0 = start + (long long)h * tiles;
+        const bool whole = ta == 0 && tb == tiles;
+        float* const part = work.partials + ((size_t)blockIdx.x * 2 + (w == w0 ? 0 : 1)) * ROWS * (HD + 2);
+        for (int i = tid; i < n_rows * (HD / 4); i += kPdThreads) {
+            const int row = i / (HD / 4), c = i % (HD / 4) * 4;
+            float mw[kPdWarps], top = -INFINITY, sum = 0.0f;
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int k = 0; k < kPdWarps; ++k) {
+                mw[k] = reinterpret_cast<const float*>(pd_smem + k * S::kWarp)[ROWS * PITCH + 2 * row];
+                top = fmaxf(top, mw[k]);
+            }
+            const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (int k = 0; k < kPdWarps; ++k) {
+                const float* const from = reinterpret_cast<const float*>(pd_smem + k * S::kWarp);
+                const float f = ex2_approx(mw[k] - base);
+                const float4 x = *reinterpret_cast<const float4*>(from + row * PITCH + c);
+                sum = fmaf(from[ROWS * PITCH + 2 * row + 1], f, sum);
+                y.x = fmaf(x.x, f, y.x); y.y = fmaf(x.y, f, y.y); y.z = fmaf(x.z, f, y.z); y.w = fmaf(x.w, f, y.w);
+            }
+            if (whole) {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // (a row that attends nothing is zero)
+                T* const to = static_cast<T*>(a.out) + ((size_t)(rq.first + row / group) * a.heads + (size_t)h * group + row % group) * HD + c;
+                store_row(to, y.x * inv);
+                store_row(to + 1, y.y * inv);
+                store_row(to + 2, y.z * inv);
+                store_row(to + 3, y.w * inv);
+            } else {
+                float* const to = part + row * (HD + 2);
+                if (c == 0) { to[0] = top; to[1] = sum; }
+                to[2 + c] = y.x; to[3 + c] = y.y; to[4 + c] = y.z; to[5 + c] = y.w;
+            }
+        }
+        if (!whole) {
+            __threadfence();
+            __syncthreads();
+            const int c0 = (int)(seq0 / share), c1 = (int)((seq0 + tiles - 1) / share);
+            if (tid == 0) s_last = atomicAdd(work.arrived + (size_t)r * a.kv_heads + h, 1) == c1 - c0;
+            __syncthreads();
+            if (s_last) {
+                __threadfence();
+                if (tid == 0) work.arrived[(size_t)r * a.kv_heads + h] = 0;
+                // the first block's part is its last stretch unless the head begins with its share
+                auto part_of = [&](int c) { return work.partials + ((size_t)c * 2 + (c == c0 && seq0 != (long long)c0 * share ? 1 : 0)) * ROWS * (HD + 2); };
+                for (int i = tid; i < n_rows * (HD / 2); i += kPdThreads) {
+                    const int row = i / (HD / 2), c = i % (HD / 2) * 2;
+                    float top = -INFINITY, sum = 0.0f, y0 = 0.0f, y1 = 0.0f;
+                    for (int k = c0; k <= c1; ++k) {
+                        const float* const from = part_of(k) + row * (HD + 2);
+                        const float2 st = __ldcg(reinterpret_cast<const float2*>(from)), x = __ldcg(reinterpret_cast<const float2*>(from + 2 + c));
+                        const float now = fmaxf(top, st.x), base = now == -INFINITY ? 0.0f : now, f = ex2_approx(top - base), e = ex2_approx(st.x - base);
+                        top = now;
+                        sum = fmaf(sum, f, st.y * e);
+                        y0 = fmaf(y0, f, x.x * e);
+                        y1 = fmaf(y1, f, x.y * e);
+                    }
+                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    T* const to = static_cast<T*>(a.out) + ((size_t)(rq.first + row / group) * a.heads + (size_t)h * group + row % group) * HD + c;
+                    store_row(to, y0 * inv);
+                    store_row(to + 1, y1 * inv);
+                }
+            }
+        }
+        __syncthreads();  // (the ring is free again)
+        w += tb - ta;
+    }
+}
+
+size_t pd_counter_bytes(int requests, int kv_heads) { return ((size_t)requests * kv_heads * 4 + 255) / 256 * 256; }
+
+}  // namespace
+
+bool paged_decode_serves(int head_dim) { return head_dim == 64 || head_dim == 128; }
+
+size_t paged_decode_workspace_bytes(int requests, int kv_heads, int head_dim, int max_rows) {
+    return pd_counter_bytes(requests, kv_heads) + (size_t)kPdBlocks * 2 * (max_rows <= 8 ? 8 : 16) * (head_dim + 2) * 4;
+}
+
+int paged_decode_launch(cudaStream_t stream, const PagedArgs& a, bool f32, int max_rows, int max_context, void* workspace) {
+    PdWork work;
+    work.arrived = static_cast<int*>(workspace);
+    work.partials = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + pd_counter_bytes(a.requests, a.kv_heads));
+    // no more blocks than there can be shares of one tile a warp
+    const long long most = (long long)a.requests * a.kv_heads * (max_context / kPdKeys + 2), blocks = (most + kPdWarps - 1) / kPdWarps;
+    const dim3 grid((unsigned)(blocks < kPdBlocks ? blocks : kPdBlocks));
+    auto go = [&](auto kern, int smem) {
+        const cudaError_t e = allow_all_dynamic_smem(kern);
+        return e != cudaSuccess ? e : launch(kern, grid, dim3(kPdThreads), (size_t)smem, stream, true, a, work);
+    };
+    auto pick = [&](auto hd) {
+        constexpr int HD = decltype(hd)::value;
+        if (max_rows <= 8) return f32 ? go(paged_decode_kernel<HD, float, 3, 1>, PdShape<HD>::kSmem) : go(paged_decode_kernel<HD, uint16_t, 2, 1>, PdShape<HD>::kSmem);
+        return f32 ? go(paged_decode_kernel<HD, float, 3, 2>, PdShape<HD>::kSmem) : go(paged_decode_kernel<HD, uint16_t, 2, 2>, PdShape<HD>::kSmem);
+    };
+    const cudaError_t e = a.head_dim == 128 ? pick(std::integral_constant<int, 128>()) : pick(std::integral_constant<int, 64>());
+    if (e != cudaSuccess) return fail(KMLL_ERR_CUDA, "paged attention: %s", cudaGetErrorString(e));
+    return KMLL_OK;
+}
+
+}  // namespace kmll
