@@ -29,6 +29,7 @@
 #include <mutex>
 
 #include "internal.cuh"
+#include "paged.cuh"
 #include "tcgen05.cuh"
 
 namespace kmll {
@@ -1502,7 +1503,8 @@ int kmll_device_status(int* status_out) {
     KMLL_REQUIRE_PTR(status_out);
     cudaError_t e = cudaMemcpyFromSymbol(status_out, g_device_status, sizeof(int));
     if (e != cudaSuccess) return fail(KMLL_ERR_CUDA, "device_status: %s", cudaGetErrorString(e));
-    return *status_out != 0 ? KMLL_OK : prompt_attention_status(status_out);
+    if (*status_out == 0) KMLL_TRY_RC(prompt_attention_status(status_out));
+    return *status_out != 0 ? KMLL_OK : paged_prompt_status(status_out);
 }
 
 int kmll_linear_i8(kmll_stream_t s, const float* x, const int8_t* w, const float* scales, int rows, int cols, float* y) {

@@ -52,4 +52,9 @@ bool paged_decode_serves(int head_dim);
 size_t paged_decode_workspace_bytes(int requests, int kv_heads, int head_dim, int max_rows);
 int paged_decode_launch(cudaStream_t stream, const PagedArgs& a, bool f32, int max_rows, int max_context, void* workspace);
 
+// paged_prompt.cu: requests of more than a.skip_rows rows, heads of 64 or 128
+bool paged_prompt_serves(const PagedArgs& a);
+int paged_prompt_launch(cudaStream_t stream, const PagedArgs& a, bool f32);
+int paged_prompt_status(int* status_out);  // 1 after a wait inside a kernel of that file ran out, 0 otherwise
+
 }  // namespace kmll

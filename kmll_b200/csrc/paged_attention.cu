@@ -118,6 +118,10 @@ extern "C" int kmll_paged_attention(kmll_stream_t stream, const void* query, int
         if (max_rows <= kPagedDecodeRows) return check_launch("paged attention");
         a.skip_rows = kPagedDecodeRows;
     }
+    if (paged_prompt_serves(a)) {
+        KMLL_TRY_RC(paged_prompt_launch(as_stream(stream), a, is_f32 != 0));
+        return check_launch("paged attention");
+    }
     const cudaError_t e = is_f32 ? launch(paged_rows_kernel<float>, dim3(tokens, kv_heads), dim3(128), 0, as_stream(stream), true, a)
                                  : launch(paged_rows_kernel<uint16_t>, dim3(tokens, kv_heads), dim3(128), 0, as_stream(stream), true, a);
     if (e != cudaSuccess) return fail(KMLL_ERR_CUDA, "paged attention: %s", cudaGetErrorString(e));
