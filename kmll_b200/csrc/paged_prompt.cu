@@ -16,6 +16,7 @@
 // O is rescaled only when a row's maximum has grown by more than 2^8.  Every wait is bounded; a time-out raises the status word, and the block frees
 // its tensor memory and returns (no copies are under way: the fetches are loads).
 #include <climits>
+#include <type_traits>
 
 #include "internal.cuh"
 #include "mma_bf16.cuh"
@@ -44,7 +45,7 @@ struct PpShape {
     static constexpr int kQPlane = kPpRows * HD * 2, kK = kPpKeys * HD * 2, kVBox = HD * 128, kV = 2 * kVBox;
     static constexpr int kOffK = NP * kQPlane, kOffV = kOffK + 2 * kK, kOffScales = kOffV + 2 * kV;
     static constexpr int kOffStat = kOffScales + 4 * (int)sizeof(PpScales), kOffUnit = kOffStat + 2 * kPpRows * 8;
-    static constexpr int kOffBars = kOffUnit + kPpRows * 4;
+    static constexpr int kOffBars = kOffUnit + kPpRows * 8;
     static constexpr int kSmemBytes = kOffBars + 256 + 1024;
     static constexpr int kStagePitch = HD / 2 + 4;
     static_assert(kSmemBytes <= 227 * 1024 && 8 * 32 * kStagePitch * 4 <= kOffScales, "shape");
@@ -76,6 +77,26 @@ __device__ inline uint32_t pp_rest(float x0, float x1, uint32_t hi) {
     return pp_round(x0 - y.x, x1 - y.y);
 }
 
+template <int E>
+__device__ inline void load_entries(const float* p, float (&x)[E]) {
+    if constexpr (E == 4) {
+        const float4 u = *reinterpret_cast<const float4*>(p);
+        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+    } else {
+        const float2 u = *reinterpret_cast<const float2*>(p);
+        x[0] = u.x; x[1] = u.y;
+    }
+}
+template <int E>
+__device__ inline void load_entries(const uint16_t* p, float (&x)[E]) {
+#pragma unroll
+    for (int k = 0; k < E / 2; ++k) {
+        const uint32_t u = reinterpret_cast<const uint32_t*>(p)[k];
+        x[2 * k] = __uint_as_float(u << 16);
+        x[2 * k + 1] = __uint_as_float(u & 0xffff0000u);
+    }
+}
+
 template <int HD, typename T>
 __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const PagedArgs a) {
     constexpr int NP = sizeof(T) == 4 ? 2 : 1;
@@ -92,7 +113,8 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
     int* const s_unit = reinterpret_cast<int*>(tmem_slot + 1);  // request, tile of 128 rows
     PpScales* const scales = reinterpret_cast<PpScales*>(smem + S::kOffScales);
     float* const units = reinterpret_cast<float*>(smem + S::kOffUnit);
-    const int tid = threadIdx.x, lane = tid & 31, warp = uniform_warp_index(), group = a.heads / a.kv_heads, h = blockIdx.y;
+    int* const row_of = reinterpret_cast<int*>(units + kPpRows);  // rows of the block among the step's (token, head) rows
+    const int tid = threadIdx.x, lane = tid & 31, warp = uniform_warp_index(), group = a.heads / a.kv_heads, h = blockIdx.y, block_log = 31 - __clz(a.block), in_block = a.block - 1;
     if (tid == 0) {
         for (int b = 0; b < 2; ++b) {
             mbar_init(&s_full[b], 1);
@@ -148,54 +170,50 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
         const int last_own = rq.pos0 + (row0 + live - 1) / group;  // (a context longer than its table row is cut at the table's end)
         const int low = a.window > 0 ? max(0, first_pos - a.window + 1) : 0, first = low & ~15;
         const int tiles = last_pos >= low ? (last_pos - first) / kPpKeys + 1 : 0;
-        auto row_at = [&](int r) { return ((size_t)(rq.first + (row0 + r) / group) * a.heads + (size_t)h * group + (row0 + r) % group) * HD; };
-        // ---- Q: a thread of the first four warps has a row, for its largest entry; then all write planes
-        if (tid < kPpRows) {
+        // ---- Q: a warp has a row at a time, HD / 32 entries a lane; its largest entry gives the power of two
+        constexpr int E = HD / 32, kWarps = kPpThreads / 32, kOwn = (kPpRows + kWarps - 1) / kWarps;
+        float x[kOwn][E];
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            const int r = warp + i * kWarps;
+#pragma unroll
+            for (int k = 0; k < E; ++k) x[i][k] = 0.0f;
+            if (r >= kPpRows) continue;
+            const int token = (row0 + r) / group, place = (rq.first + token) * a.heads + h * group + (row0 + r - token * group);
+            if (lane == 0) row_of[r] = place;
+            if (r < live) load_entries<E>(static_cast<const T*>(a.query) + (size_t)place * HD + lane * E, x[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            const int r = warp + i * kWarps;
+            if (r >= kPpRows) continue;
             float top = 0.0f;
             bool finite = true;
-            if (tid < live) {
-                const T* const q = static_cast<const T*>(a.query) + row_at(tid);
-                for (int i = 0; i < HD; i += 16 / (int)sizeof(T)) {
-                    const uint4 u = *reinterpret_cast<const uint4*>(q + i);
-                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float x = __uint_as_float(sizeof(T) == 4 ? w[k] : w[k] << 16), y = __uint_as_float(sizeof(T) == 4 ? w[k] : w[k] & 0xffff0000u);
-                        top = fmaxf(top, fmaxf(fabsf(x), fabsf(y)));
-                        finite = finite && fabsf(x) < INFINITY && fabsf(y) < INFINITY;
-                    }
-                }
+            for (int k = 0; k < E; ++k) {
+                top = fmaxf(top, fabsf(x[i][k]));
+                finite = finite && fabsf(x[i][k]) < INFINITY;
             }
+            top = warp_max(top);
             int e2 = 0;
             if (top > 0.0f && top < INFINITY) frexpf(top, &e2);
-            const int sh = max(-120, min(120, 11 - e2));  // the largest entry between 2^10 and 2^11
-            units[tid] = finite ? ldexpf(1.0f, sh) : __int_as_float(0x7fffffff);
-        }
-        __syncthreads();
-        for (int i = tid; i < kPpRows * (HD / 8); i += kPpThreads) {
-            const int r = i / (HD / 8), c8 = i % (HD / 8);
-            uint4 hi = make_uint4(0u, 0u, 0u, 0u), lo = hi;
-            if (r < live) {
-                const T* const q = static_cast<const T*>(a.query) + row_at(r) + c8 * 8;
-                const float up = units[r];
-                float x[8];
-                if constexpr (sizeof(T) == 4) {
-                    const float4 u = reinterpret_cast<const float4*>(q)[0], v = reinterpret_cast<const float4*>(q)[1];
-                    x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
-                } else {
-                    const uint4 u = *reinterpret_cast<const uint4*>(q);
-                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            const float up = ldexpf(1.0f, max(-120, min(120, 11 - e2)));  // the largest entry between 2^10 and 2^11
+            if (lane == 0) units[r] = up;
+            if (!__all_sync(0xffffffffu, finite) && lane == 0) units[r] = __int_as_float(0x7fffffff);
+            unsigned char* const at = smem + (lane * E >> 6) * kPpBox + r * 128 + ((((lane * E >> 3) & 7) ^ (r & 7)) << 4) + (lane * E & 7) * 2;
+            uint32_t hi[E / 2], lo[E / 2];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) { x[2 * k] = __uint_as_float(w[k] << 16); x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u); }
-                }
-#pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] *= up;
-                hi = make_uint4(pp_round(x[0], x[1]), pp_round(x[2], x[3]), pp_round(x[4], x[5]), pp_round(x[6], x[7]));
-                if (NP == 2) lo = make_uint4(pp_rest(x[0], x[1], hi.x), pp_rest(x[2], x[3], hi.y), pp_rest(x[4], x[5], hi.z), pp_rest(x[6], x[7], hi.w));
+            for (int k = 0; k < E / 2; ++k) {
+                hi[k] = pp_round(x[i][2 * k] * up, x[i][2 * k + 1] * up);
+                lo[k] = pp_rest(x[i][2 * k] * up, x[i][2 * k + 1] * up, hi[k]);
             }
-            unsigned char* const at = smem + (c8 >> 3) * kPpBox + r * 128 + (((c8 & 7) ^ (r & 7)) << 4);
-            *reinterpret_cast<uint4*>(at) = hi;
-            if (NP == 2) *reinterpret_cast<uint4*>(at + S::kQPlane) = lo;
+            if constexpr (E == 4) {
+                *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
+                if (NP == 2) *reinterpret_cast<uint2*>(at + S::kQPlane) = make_uint2(lo[0], lo[1]);
+            } else {
+                *reinterpret_cast<uint32_t*>(at) = hi[0];
+                if (NP == 2) *reinterpret_cast<uint32_t*>(at + S::kQPlane) = lo[0];
+            }
         }
         fence_proxy_async_smem();
         __syncthreads();
@@ -203,33 +221,31 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
 
         if (warp >= 8 && warp < 12) {
             // ---- codes to operands
-            const int tt = tid - 256;  // 0 .. 127: the key; the column (heads of 64: two groups of keys at once)
+            const int tt = tid - 256;  // 0 .. 127: the key; of the values the group of 16 keys tt / 16, columns tt % 16, + 16, ..
             const int32_t* const table = a.table + (size_t)request * a.width;
-            constexpr int U = HD / 16, VG = 128 / HD;  // 16-byte groups of a key; groups of keys per round of the values
+            constexpr int U = HD / 16;  // 16-byte groups of a key; columns of a group of values per thread
             uint4 kc[U], vc[U];
-            auto page_of = [&](int j) {  // lanes 0-7 (and again): page of group lane & 7 of tile j, -1: nothing there
+            auto entry_of = [&](int j) {  // lanes 0-7 (and again): table entry of group lane & 7 of tile j; looked at a tile later, when it has come
                 const int key = first + j * kPpKeys + (lane & 7) * 16;
-                if (j >= tiles || key >= rq.hi) return -1;
-                const int p = table[key / a.block];
-                return p >= 0 && p < a.pages ? p : -1;
+                int p = -1;
+                if (j < tiles && key < rq.hi) p = table[key >> block_log];
+                return p;
             };
-            auto fetch_keys = [&](int j, int page) {
-                const int p = __shfl_sync(0xffffffffu, page, tt >> 4), at = (first + j * kPpKeys + tt) % a.block;
-                const uint4* const src = reinterpret_cast<const uint4*>(a.k_codes + ((size_t)max(p, 0) * a.kv_heads + h) * a.block * HD) + at;
+            auto page_of = [&](int entry) { return entry >= 0 && entry < a.pages ? entry : -1; };  // -1: nothing there
+            // (volatile loads: they stay where they are written, a tile ahead of their use; where nothing is there any codes do, no row sees them)
+            // One page per thread and tile: more shuffles between the loads would share their scoreboards and wait for them.
+            auto fetch_keys = [&](int j, int p) {
+                const uint4* const src = reinterpret_cast<const uint4*>(a.k_codes + ((size_t)max(p, 0) * a.kv_heads + h) * a.block * HD) + ((first + j * kPpKeys + tt) & in_block);
 #pragma unroll
-                for (int c = 0; c < U; ++c) kc[c] = p >= 0 ? __ldg(src + (size_t)c * a.block) : make_uint4(0u, 0u, 0u, 0u);
+                for (int c = 0; c < U; ++c) kc[c] = ld_stream_u4(src + (size_t)c * a.block);
             };
-            auto fetch_values = [&](int j, int page) {
-                const int d = tt % HD;
+            auto fetch_values = [&](int j, int p) {
+                const uint4* const src = reinterpret_cast<const uint4*>(a.v_codes + ((size_t)max(p, 0) * a.kv_heads + h) * a.block * HD) +
+                                         (size_t)(((first + j * kPpKeys + (tt & ~15)) & in_block) >> 4) * HD + (tt & 15);
 #pragma unroll
-                for (int c = 0; c < U; ++c) {
-                    const int tg = c * VG + tt / HD;
-                    const int p = __shfl_sync(0xffffffffu, page, tg), at = (first + j * kPpKeys + tg * 16) % a.block / 16;
-                    vc[c] = p >= 0 ? __ldg(reinterpret_cast<const uint4*>(a.v_codes + ((size_t)p * a.kv_heads + h) * a.block * HD) + (size_t)at * HD + d)
-                                   : make_uint4(0u, 0u, 0u, 0u);
-                }
+                for (int c = 0; c < U; ++c) vc[c] = ld_stream_u4(src + c * 16);
             };
-            int page = page_of(0), next = page_of(1);
+            int page = page_of(entry_of(0)), entry = entry_of(1);
             float ks = 0.0f, vs = 0.0f;  // lanes 0-7 of warp 8: scales of the tile in kc
             auto fetch_scales = [&](int p) {
                 if (warp == 8 && lane < 8) {
@@ -239,8 +255,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
             };
             if (tiles > 0) {
                 fetch_scales(page);
-                fetch_keys(0, page);
-                fetch_values(0, page);
+                const int p = __shfl_sync(0xffffffffu, page, tt >> 4);
+                fetch_keys(0, p);
+                fetch_values(0, p);
             }
             for (int j = 0; j < tiles; ++j) {
                 const int st = j & 1, before = j - 2;
@@ -264,24 +281,22 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&k_full[st]);
+                const int next = page_of(entry), p_next = __shfl_sync(0xffffffffu, next, tt >> 4);
                 if (j + 1 < tiles) {
                     fetch_scales(next);
-                    fetch_keys(j + 1, next);
+                    fetch_keys(j + 1, p_next);
                 }
                 ok = before < 0 || warp_wait(&pv_done[st], (uint32_t)(before >> 1) & 1u);
                 if (!ok) break;
-                unsigned char* const vrow = smem + S::kOffV + st * S::kV + (tt % HD) * 128;
+                unsigned char* const vrow = smem + S::kOffV + st * S::kV + (tt >> 6) * S::kVBox + (tt & 15) * 128;
 #pragma unroll
-                for (int c = 0; c < U; ++c) {
-                    const int tg = c * VG + tt / HD;
-                    pp_put(vrow + (tg >> 2) * S::kVBox, (tg & 3) * 2, tt & 7, vc[c]);
-                }
+                for (int c = 0; c < U; ++c) pp_put(vrow + c * 2048, ((tt >> 4) & 3) * 2, tt & 7, vc[c]);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&v_full[st]);
-                if (j + 1 < tiles) fetch_values(j + 1, next);
+                if (j + 1 < tiles) fetch_values(j + 1, p_next);
                 page = next;
-                next = page_of(j + 2);
+                entry = entry_of(j + 2);
             }
         } else if (warp == 12) {
             constexpr uint32_t idesc_s = gemm_idesc_f16(128, kPpKeys), idesc_o = gemm_idesc_f16(128, HD);
@@ -339,27 +354,33 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                 tcgen05_fence_after();
                 const PpScales& sc = scales[j & 3];
                 const bool masked = t0 + kPpKeys - 1 > first_pos || t0 < low || (a.window > 0 && t0 < last_own - a.window + 1) || sc.there != 0xffu;
+                // keys of chunk c that the row attends, a bit each
+                auto seen_of = [&](int c) {
+                    const int k0 = t0 + c * 32, from = max(lo - k0, 0), to = min(pos - k0, 31);
+                    const uint32_t pair = sc.there >> (2 * c);
+                    const uint32_t there = (pair & 1u ? 0xffffu : 0u) | (pair & 2u ? 0xffff0000u : 0u);
+                    return from <= to ? (0xffffffffu << from) & (0xffffffffu >> (31 - to)) & there : 0u;
+                };
                 float top = -INFINITY;
+                auto largest = [&](auto is_masked) {
+#pragma unroll 1
+                    for (int c = 0; c < kPpKeys / 32; ++c) {
+                        uint32_t d[32];
+                        tmem_load_x32(ts + c * 32, d);
+                        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                        const uint32_t seen = is_masked.value ? seen_of(c) : 0u;
 #pragma unroll
-                for (int c = 0; c < kPpKeys / 32; ++c) {
-                    uint32_t d[32];
-                    tmem_load_x32(ts + c * 32, d);
-                    float mx[2] = {-INFINITY, -INFINITY};
-                    if (masked) {
+                        for (int i = 0; i < 32; ++i)
+                            mx[(i >> 4) * 2 + (i & 1)] = fmaxf(mx[(i >> 4) * 2 + (i & 1)], is_masked.value && (seen & (1u << i)) == 0u ? -INFINITY : __uint_as_float(d[i]));
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int key = t0 + c * 32 + i;
-                            const bool seen = key <= pos && key >= lo && ((sc.there >> (2 * c + (i >> 4))) & 1u) != 0u;
-                            mx[i >> 4] = fmaxf(mx[i >> 4], seen ? __uint_as_float(d[i]) : -INFINITY);
+                        for (int k = 0; k < 2; ++k) {
+                            const float x = fmaxf(mx[2 * k], mx[2 * k + 1]);
+                            if (x > -INFINITY) top = fmaxf(top, fmaf(x, sc.k[2 * c + k] * unit, sc.log_v[2 * c + k]));
                         }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) mx[i >> 4] = fmaxf(mx[i >> 4], __uint_as_float(d[i]));
                     }
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-                        if (mx[k] > -INFINITY) top = fmaxf(top, fmaf(mx[k], sc.k[2 * c + k] * unit, sc.log_v[2 * c + k]));
-                }
+                };
+                if (masked) largest(std::true_type());
+                else largest(std::false_type());
                 const bool grow = top > m_ref + 8.0f;  // (a row with nothing attended so far has -inf)
                 if (__any_sync(0xffffffffu, grow)) {
                     const float corr = grow ? ex2_approx(m_ref - top) : 1.0f;
@@ -380,33 +401,35 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                     }
                 }
                 const float m = m_ref == -INFINITY ? 0.0f : m_ref;
+                auto weights = [&](auto is_masked) {
+#pragma unroll 1
+                    for (int c = 0; c < kPpKeys / 32; ++c) {
+                        uint32_t d[32], planes[NP * 16];
+                        tmem_load_x32(ts + c * 32, d);
+                        const uint32_t seen = is_masked.value ? seen_of(c) : 0u;
+                        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        const float f[2] = {sc.k[2 * c] * unit, sc.k[2 * c + 1] * unit}, off[2] = {sc.log_v[2 * c] - m, sc.log_v[2 * c + 1] - m};
 #pragma unroll
-                for (int c = 0; c < kPpKeys / 32; ++c) {
-                    uint32_t d[32], planes[NP * 16];
-                    tmem_load_x32(ts + c * 32, d);
-                    float sum[2] = {0.0f, 0.0f};
-                    const float f[2] = {sc.k[2 * c] * unit, sc.k[2 * c + 1] * unit}, off[2] = {sc.log_v[2 * c] - m, sc.log_v[2 * c + 1] - m};
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int k = i >> 3;
-                        float p0 = ex2_approx(fmaf(__uint_as_float(d[2 * i]), f[k], off[k])), p1 = ex2_approx(fmaf(__uint_as_float(d[2 * i + 1]), f[k], off[k]));
-                        if (masked) {
-                            const int key = t0 + c * 32 + 2 * i;
-                            const bool there = ((sc.there >> (2 * c + k)) & 1u) != 0u;
-                            p0 = there && key <= pos && key >= lo ? p0 : 0.0f;
-                            p1 = there && key + 1 <= pos && key + 1 >= lo ? p1 : 0.0f;
+                        for (int i = 0; i < 16; ++i) {
+                            const int k = i >> 3;
+                            float p0 = ex2_approx(fmaf(__uint_as_float(d[2 * i]), f[k], off[k])), p1 = ex2_approx(fmaf(__uint_as_float(d[2 * i + 1]), f[k], off[k]));
+                            if (is_masked.value) {
+                                p0 = (seen & (1u << (2 * i))) != 0u ? p0 : 0.0f;
+                                p1 = (seen & (2u << (2 * i))) != 0u ? p1 : 0.0f;
+                            }
+                            sum[2 * k] += p0;
+                            sum[2 * k + 1] += p1;
+                            planes[i] = pp_round(p0, p1);
+                            if constexpr (NP == 2) planes[16 + i] = pp_rest(p0, p1, planes[i]);
                         }
-                        sum[k] += p0;
-                        sum[k] += p1;
-                        const uint32_t hi = pp_round(p0, p1);
-                        planes[i] = hi;
-                        if constexpr (NP == 2) planes[16 + i] = pp_rest(p0, p1, hi);
+                        l = fmaf(sum[0] + sum[1], sc.inv_v[2 * c], l);
+                        l = fmaf(sum[2] + sum[3], sc.inv_v[2 * c + 1], l);
+                        if constexpr (NP == 2) tmem_store_x32(ts + c * 32, planes);
+                        else tmem_store_x16(ts + c * 32, planes);
                     }
-                    l = fmaf(sum[0], sc.inv_v[2 * c], l);
-                    l = fmaf(sum[1], sc.inv_v[2 * c + 1], l);
-                    if constexpr (NP == 2) tmem_store_x32(ts + c * 32, planes);
-                    else tmem_store_x16(ts + c * 32, planes);
-                }
+                };
+                if (masked) weights(std::true_type());
+                else weights(std::false_type());
                 tmem_store_wait();
                 tcgen05_fence_before();
                 __syncwarp();
@@ -446,7 +469,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
             for (int i = lane; i < 32 * (HD / 8); i += 32) {
                 const int rr = i / (HD / 8), c4 = i - rr * (HD / 8), row = (warp & 3) * 32 + rr;
                 if (!ok || row >= live) continue;
-                T* const out = static_cast<T*>(a.out) + row_at(row) + stream * (HD / 2) + c4 * 4;
+                T* const out = static_cast<T*>(a.out) + (size_t)row_of[row] * HD + stream * (HD / 2) + c4 * 4;
                 const float4 y = *reinterpret_cast<const float4*>(stage + rr * S::kStagePitch + c4 * 4);
                 if constexpr (sizeof(T) == 4) {
                     *reinterpret_cast<float4*>(out) = y;
@@ -473,7 +496,7 @@ bool paged_prompt_serves(const PagedArgs& a) {
 int paged_prompt_launch(cudaStream_t stream, const PagedArgs& a, bool f32) {
     const int group = a.heads / a.kv_heads;
     const long long tiles = ((long long)a.tokens * group + kPpRows - 1) / kPpRows + a.requests;  // each request ends in a tile of its own
-    KMLL_REQUIRE(tiles <= INT_MAX, "paged attention: too many rows");
+    KMLL_REQUIRE(tiles <= INT_MAX && (long long)a.tokens * a.heads <= INT_MAX, "paged attention: too many rows");
     auto go = [&](auto kern, int smem) {
         const cudaError_t e = allow_all_dynamic_smem(kern);
         return e != cudaSuccess ? e : launch(kern, dim3((unsigned)tiles, a.kv_heads), dim3(kPpThreads), (size_t)smem, stream, true, a);
