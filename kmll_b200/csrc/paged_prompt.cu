@@ -1,20 +1,21 @@
-// Attention of portions of prompts over the paged 8-bit cache on tcgen05: one block = 128 rows of a request and kv head.
+// Attention of portions of prompts over the paged 8-bit cache on tcgen05: one block = up to 256 rows of a request and kv head.
 //
 // A row is a (token, query head) pair: all query heads of a kv head are in the same block, so codes are turned into operands once for all of
-// them, and short portions still fill the 128 rows.  Codes are exact in binary16, which is what both contractions run on:
+// them, and short portions still fill the 128 rows of an MMA.  Codes are exact in binary16, which is what both contractions run on:
 //   S = Q K^T    Q as x * 2^sh = x0 + x1, two binary16 planes (f32 rows: 2^-22 of the row's largest entry) or one (bf16 rows: exact down to 2^-24 of
 //                it); times k_scale of the key's page and 2^-sh
 //   O += P V     the value scale of a key's page goes into the exponent, P = 2^(s + log2 v_scale - m): no multiplication, and the sum of the
 //                weights takes 1 / v_scale once per group of 16 keys.  P is two planes (f32 rows) or one (bf16 rows: 2^-12, below the rounding of
 //                the result).  A maximum is one of s + log2 v_scale; page scales of a head may differ by 2^100.
-// Roles of the 13 warps:
-//   warps 0-3, 4-7  softmax of the even and of the odd key tiles (128 keys), a thread per row: scores by tcgen05.ld, once for the maximum, once
-//                   for the weights, which go back in the place of the scores they came from.  Two independent streams (maximum, sum, O), merged at the end
-//   warps 8-11      fetch the codes of a tile into registers while the tile before is at work, and write them as binary16 operands (128-byte
-//                   swizzle, both K-major: values lie with the keys of a column together)
-//   warp 12         issues S = Q K^T and O += P V
-// O is rescaled only when a row's maximum has grown by more than 2^8.  Every wait is bounded; a time-out raises the status word, and the block frees
-// its tensor memory and returns (no copies are under way: the fetches are loads).
+// Two streams of work share the keys that are brought in: two tiles of 128 rows, or (where there are 128 rows at most) the even and the odd
+// key tiles of one, each with a maximum, a sum and an O of its own, merged at the end.  Roles of the 28 warps:
+//   warps 0-7, 8-15  softmax of a stream, two threads per row with 64 keys of a tile each: scores by tcgen05.ld, their maximum (both threads'), then
+//                    the weights, which go back in the place of the scores.  (One thread per row: 3400 cycles a tile, all of it latency.)
+//   warps 16-23      fetch the codes of a tile of 128 keys into registers while the tile before is at work, and write them as binary16 operands
+//                    (128-byte swizzle, both K-major: values lie with the keys of a column together)
+//   warp 24          issues S = Q K^T and O += P V
+// O is rescaled only when a row's maximum has grown by more than 2^8.  Every wait is bounded; a time-out raises the status word, and
+// the block frees its tensor memory and returns (no copies are under way: the fetches are loads).
 #include <climits>
 #include <type_traits>
 
@@ -30,7 +31,10 @@ __device__ int g_paged_prompt_status = 0;
 namespace {
 
 constexpr int kPpRows = 128, kPpKeys = 128, kPpGroups = kPpKeys / 16;
-constexpr int kPpThreads = 13 * 32;
+constexpr int kPpConvert = 16, kPpIssue = 24;  // first warps of the roles behind the softmax
+constexpr int kPpThreads = 28 * 32;
+// Registers a thread: 72 at the launch (896 threads), then by warpgroup: 4 * 128 * 88 + 2 * 128 * 64 + 128 * 24 = 896 * 72.
+constexpr int kPpRegsLaunch = 72;
 constexpr int kPpBox = 128 * 128;      // 128 rows of 64 binary16 entries
 constexpr uint32_t kPpTmemO = 256;     // scores at 0 and 128, the streams' O behind them
 
@@ -42,13 +46,15 @@ struct PpScales {  // of a tile, per group of 16 keys
 // NP: planes of Q and of P
 template <int HD, int NP>
 struct PpShape {
-    static constexpr int kQPlane = kPpRows * HD * 2, kK = kPpKeys * HD * 2, kVBox = HD * 128, kV = 2 * kVBox;
-    static constexpr int kOffK = NP * kQPlane, kOffV = kOffK + 2 * kK, kOffScales = kOffV + 2 * kV;
-    static constexpr int kOffStat = kOffScales + 4 * (int)sizeof(PpScales), kOffUnit = kOffStat + 2 * kPpRows * 8;
-    static constexpr int kOffBars = kOffUnit + kPpRows * 8;
+    static constexpr int kQPlane = kPpRows * HD * 2, kQTile = NP * kQPlane, kK = kPpKeys * HD * 2, kVBox = HD * 128, kV = 2 * kVBox;
+    static constexpr int kOffK = 2 * kQTile, kStages = kOffK + 2 * (kK + kV) <= 216 * 1024 ? 2 : 1;
+    static constexpr int kOffV = kOffK + kStages * kK, kOffScales = kOffV + kStages * kV;
+    static constexpr int kOffStat = kOffScales + 4 * (int)sizeof(PpScales), kOffTop = kOffStat + 4 * kPpRows * 8;
+    static constexpr int kOffUnit = kOffTop + 2 * 4 * kPpRows * 4;
+    static constexpr int kOffBars = kOffUnit + 2 * kPpRows * 8;
     static constexpr int kSmemBytes = kOffBars + 256 + 1024;
-    static constexpr int kStagePitch = HD / 2 + 4;
-    static_assert(kSmemBytes <= 227 * 1024 && 8 * 32 * kStagePitch * 4 <= kOffScales, "shape");
+    static constexpr int kStagePitch = HD / 2 + 4;  // rows of O on their way out, over the operands
+    static_assert(kSmemBytes <= 227 * 1024 && 16 * 32 * kStagePitch * 4 <= kOffScales, "shape");
 };
 
 // two codes as binary16: 0x6400 + b is 1024 + b
@@ -97,37 +103,67 @@ __device__ inline void load_entries(const uint16_t* p, float (&x)[E]) {
     }
 }
 
+// pairs of f32 in one instruction
+__device__ inline uint64_t pp_pair(float x, float y) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+    return d;
+}
+__device__ inline float2 pp_unpair(uint64_t d) {
+    float2 v;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(d));
+    return v;
+}
+__device__ inline uint64_t pp_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ inline uint64_t pp_add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
 template <int HD, typename T>
 __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const PagedArgs a) {
     constexpr int NP = sizeof(T) == 4 ? 2 : 1;
     using S = PpShape<HD, NP>;
+    constexpr int kStages = S::kStages;
     extern __shared__ unsigned char pp_smem_raw[];
     unsigned char* const smem = pp_smem_raw + ((1024u - (smem_u32(pp_smem_raw) & 1023u)) & 1023u);
-    uint64_t* const s_full = reinterpret_cast<uint64_t*>(smem + S::kOffBars);  // [2] the scores of a tile are there
+    uint64_t* const s_full = reinterpret_cast<uint64_t*>(smem + S::kOffBars);  // [2] the scores of a stream's tile are there
     uint64_t* const p_ready = s_full + 2;    // [2] its weights are there (and O is rescaled)
-    uint64_t* const pv_done = p_ready + 2;   // [2] O has taken the tile
-    uint64_t* const k_full = pv_done + 2;    // [2]
-    uint64_t* const v_full = k_full + 2;     // [2]
-    uint64_t* const sc_full = v_full + 2;    // [4] the scales of a tile are there
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(sc_full + 4);
-    int* const s_unit = reinterpret_cast<int*>(tmem_slot + 1);  // request, tile of 128 rows
+    uint64_t* const pv_done = p_ready + 2;   // [2] its O has taken the tile
+    uint64_t* const k_full = pv_done + 2;    // [kStages]
+    uint64_t* const v_full = k_full + 2;     // [kStages]
+    uint64_t* const k_free = v_full + 2;     // [kStages] the scores that need the stage are done
+    uint64_t* const v_free = k_free + 2;     // [kStages]
+    uint64_t* const sc_full = v_free + 2;    // [4] the scales of a tile are there
+    uint64_t* const pair = sc_full + 4;      // [8] both threads of a row have left their maxima
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(pair + 8);
+    int* const s_unit = reinterpret_cast<int*>(tmem_slot + 1);  // request, unit of 256 rows
     PpScales* const scales = reinterpret_cast<PpScales*>(smem + S::kOffScales);
     float* const units = reinterpret_cast<float*>(smem + S::kOffUnit);
-    int* const row_of = reinterpret_cast<int*>(units + kPpRows);  // rows of the block among the step's (token, head) rows
-    const int tid = threadIdx.x, lane = tid & 31, warp = uniform_warp_index(), group = a.heads / a.kv_heads, h = blockIdx.y, block_log = 31 - __clz(a.block), in_block = a.block - 1;
+    int* const row_of = reinterpret_cast<int*>(units + 2 * kPpRows);  // rows of the block among the step's (token, head) rows
+    const int tid = threadIdx.x, lane = tid & 31, warp = uniform_warp_index(), group = a.heads / a.kv_heads, h = blockIdx.x;
+    const int block_log = 31 - __clz(a.block), in_block = a.block - 1;
     if (tid == 0) {
         for (int b = 0; b < 2; ++b) {
             mbar_init(&s_full[b], 1);
-            mbar_init(&p_ready[b], 4);
+            mbar_init(&p_ready[b], 8);
             mbar_init(&pv_done[b], 1);
-            mbar_init(&k_full[b], 4);
-            mbar_init(&v_full[b], 4);
+            mbar_init(&k_full[b], 8);
+            mbar_init(&v_full[b], 8);
+            mbar_init(&k_free[b], 1);
+            mbar_init(&v_free[b], 1);
         }
         for (int b = 0; b < 4; ++b) mbar_init(&sc_full[b], 1);
+        for (int b = 0; b < 8; ++b) mbar_init(&pair[b], 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         s_unit[0] = -1;
     }
-    if (warp == 12) {
+    if (warp == kPpIssue) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -135,7 +171,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
     __syncthreads();  // (columns first, then the dependents: tcgen05.cuh)
     tcgen05_fence_after();
     pdl_wait();
-    // ---- the block's request and rows: tiles of 128 rows, request after request, the last rows of a request (which see most) first
+    // ---- the block's request and rows: units of 256 rows, request after request, the last rows of a request (which see most) first
     if (warp == 0) {
         int before = 0;
         for (int r0 = 0; r0 < a.requests; r0 += 32) {
@@ -143,7 +179,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
             int n = 0;
             if (r < a.requests) {
                 const long long rows = (long long)PagedRequest::of(a, r).rows * group;
-                n = rows > a.skip_rows ? (int)((rows + kPpRows - 1) / kPpRows) : 0;
+                n = rows > a.skip_rows ? (int)((rows + 2 * kPpRows - 1) / (2 * kPpRows)) : 0;
             }
             int up = n;
 #pragma unroll
@@ -151,13 +187,13 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                 const int v = __shfl_up_sync(0xffffffffu, up, o);
                 if (lane >= o) up += v;
             }
-            const int at = (int)blockIdx.x - before - (up - n);
+            const int at = (int)blockIdx.y - before - (up - n);
             if (n > 0 && at >= 0 && at < n) {
                 s_unit[0] = r;
                 s_unit[1] = n - 1 - at;
             }
             before += __shfl_sync(0xffffffffu, up, 31);
-            if ((int)blockIdx.x < before) break;
+            if ((int)blockIdx.y < before) break;
         }
     }
     __syncthreads();
@@ -165,65 +201,74 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
     bool ok = true;
     if (request >= 0) {
         const PagedRequest rq = PagedRequest::of(a, request);
-        const int row0 = s_unit[1] * kPpRows, live = min(kPpRows, rq.rows * group - row0);
-        const int first_pos = rq.pos0 + row0 / group, last_pos = min(rq.pos0 + (row0 + live - 1) / group, rq.hi - 1);
-        const int last_own = rq.pos0 + (row0 + live - 1) / group;  // (a context longer than its table row is cut at the table's end)
-        const int low = a.window > 0 ? max(0, first_pos - a.window + 1) : 0, first = low & ~15;
-        const int tiles = last_pos >= low ? (last_pos - first) / kPpKeys + 1 : 0;
+        const int row0 = s_unit[1] * 2 * kPpRows, live = min(2 * kPpRows, rq.rows * group - row0);
+        const bool two = live > kPpRows;  // two tiles of rows; else two shares of the keys
+        // positions of rows r .. e - 1 of the block (a context longer than its table row is cut at the table's end)
+        auto own_pos = [&](int r) { return rq.pos0 + (row0 + r) / group; };
+        const int low = a.window > 0 ? max(0, own_pos(0) - a.window + 1) : 0, first = low & ~15;
+        auto tiles_to = [&](int r) {  // key tiles that row r's position needs
+            const int last = min(own_pos(r), rq.hi - 1);
+            return last >= low ? (last - first) / kPpKeys + 1 : 0;
+        };
+        const int tiles = tiles_to(live - 1);
+        const int tiles0 = two ? tiles_to(kPpRows - 1) : tiles;  // of the first stream where the streams are tiles of rows
         // ---- Q: a warp has a row at a time, HD / 32 entries a lane; its largest entry gives the power of two
-        constexpr int E = HD / 32, kWarps = kPpThreads / 32, kOwn = (kPpRows + kWarps - 1) / kWarps;
-        float x[kOwn][E];
+        constexpr int E = HD / 32, kWarps = kPpThreads / 32, kBatch = 5;
+        for (int r0 = warp; r0 < (two ? 2 : 1) * kPpRows; r0 += kWarps * kBatch) {
+            float x[kBatch][E];
 #pragma unroll
-        for (int i = 0; i < kOwn; ++i) {
-            const int r = warp + i * kWarps;
+            for (int i = 0; i < kBatch; ++i) {
+                const int r = r0 + i * kWarps;
 #pragma unroll
-            for (int k = 0; k < E; ++k) x[i][k] = 0.0f;
-            if (r >= kPpRows) continue;
-            const int token = (row0 + r) / group, place = (rq.first + token) * a.heads + h * group + (row0 + r - token * group);
-            if (lane == 0) row_of[r] = place;
-            if (r < live) load_entries<E>(static_cast<const T*>(a.query) + (size_t)place * HD + lane * E, x[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < kOwn; ++i) {
-            const int r = warp + i * kWarps;
-            if (r >= kPpRows) continue;
-            float top = 0.0f;
-            bool finite = true;
-#pragma unroll
-            for (int k = 0; k < E; ++k) {
-                top = fmaxf(top, fabsf(x[i][k]));
-                finite = finite && fabsf(x[i][k]) < INFINITY;
+                for (int k = 0; k < E; ++k) x[i][k] = 0.0f;
+                if (r >= 2 * kPpRows) continue;
+                const int token = (row0 + r) / group, place = (rq.first + token) * a.heads + h * group + (row0 + r - token * group);
+                if (lane == 0) row_of[r] = place;
+                if (r < live) load_entries<E>(static_cast<const T*>(a.query) + (size_t)place * HD + lane * E, x[i]);
             }
-            top = warp_max(top);
-            int e2 = 0;
-            if (top > 0.0f && top < INFINITY) frexpf(top, &e2);
-            const float up = ldexpf(1.0f, max(-120, min(120, 11 - e2)));  // the largest entry between 2^10 and 2^11
-            if (lane == 0) units[r] = up;
-            if (!__all_sync(0xffffffffu, finite) && lane == 0) units[r] = __int_as_float(0x7fffffff);
-            unsigned char* const at = smem + (lane * E >> 6) * kPpBox + r * 128 + ((((lane * E >> 3) & 7) ^ (r & 7)) << 4) + (lane * E & 7) * 2;
-            uint32_t hi[E / 2], lo[E / 2];
 #pragma unroll
-            for (int k = 0; k < E / 2; ++k) {
-                hi[k] = pp_round(x[i][2 * k] * up, x[i][2 * k + 1] * up);
-                lo[k] = pp_rest(x[i][2 * k] * up, x[i][2 * k + 1] * up, hi[k]);
-            }
-            if constexpr (E == 4) {
-                *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
-                if (NP == 2) *reinterpret_cast<uint2*>(at + S::kQPlane) = make_uint2(lo[0], lo[1]);
-            } else {
-                *reinterpret_cast<uint32_t*>(at) = hi[0];
-                if (NP == 2) *reinterpret_cast<uint32_t*>(at + S::kQPlane) = lo[0];
+            for (int i = 0; i < kBatch; ++i) {
+                const int r = r0 + i * kWarps;
+                if (r >= 2 * kPpRows) continue;
+                float top = 0.0f;
+                bool finite = true;
+#pragma unroll
+                for (int k = 0; k < E; ++k) {
+                    top = fmaxf(top, fabsf(x[i][k]));
+                    finite = finite && fabsf(x[i][k]) < INFINITY;
+                }
+                top = warp_max(top);
+                finite = __all_sync(0xffffffffu, finite) != 0;
+                int e2 = 0;
+                if (top > 0.0f && top < INFINITY) frexpf(top, &e2);
+                const float up = ldexpf(1.0f, max(-120, min(120, 11 - e2)));  // the largest entry between 2^10 and 2^11
+                if (lane == 0) units[r] = finite ? up : __int_as_float(0x7fffffff);
+                unsigned char* const at = smem + (r >> 7) * S::kQTile + (lane * E >> 6) * kPpBox + (r & 127) * 128 + ((((lane * E >> 3) & 7) ^ (r & 7)) << 4) + (lane * E & 7) * 2;
+                uint32_t hi[E / 2], lo[E / 2];
+#pragma unroll
+                for (int k = 0; k < E / 2; ++k) {
+                    hi[k] = pp_round(x[i][2 * k] * up, x[i][2 * k + 1] * up);
+                    lo[k] = pp_rest(x[i][2 * k] * up, x[i][2 * k + 1] * up, hi[k]);
+                }
+                if constexpr (E == 4) {
+                    *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
+                    if (NP == 2) *reinterpret_cast<uint2*>(at + S::kQPlane) = make_uint2(lo[0], lo[1]);
+                } else {
+                    *reinterpret_cast<uint32_t*>(at) = hi[0];
+                    if (NP == 2) *reinterpret_cast<uint32_t*>(at + S::kQPlane) = lo[0];
+                }
             }
         }
         fence_proxy_async_smem();
         __syncthreads();
         const uint32_t base = smem_u32(smem);
 
-        if (warp >= 8 && warp < 12) {
+        if (warp >= kPpConvert && warp < kPpIssue) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
             // ---- codes to operands
-            const int tt = tid - 256;  // 0 .. 127: the key; of the values the group of 16 keys tt / 16, columns tt % 16, + 16, ..
+            const int tt = tid - 32 * kPpConvert & 127, side = tid - 32 * kPpConvert >> 7;  // the key; of the values the group of 16 keys tt / 16, columns tt % 16, + 16, ..; half of either
             const int32_t* const table = a.table + (size_t)request * a.width;
-            constexpr int U = HD / 16;  // 16-byte groups of a key; columns of a group of values per thread
+            constexpr int U = HD / 32;  // 16-byte groups of half a key; columns of a group of values per thread
             uint4 kc[U], vc[U];
             auto entry_of = [&](int j) {  // lanes 0-7 (and again): table entry of group lane & 7 of tile j; looked at a tile later, when it has come
                 const int key = first + j * kPpKeys + (lane & 7) * 16;
@@ -235,20 +280,20 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
             // (volatile loads: they stay where they are written, a tile ahead of their use; where nothing is there any codes do, no row sees them)
             // One page per thread and tile: more shuffles between the loads would share their scoreboards and wait for them.
             auto fetch_keys = [&](int j, int p) {
-                const uint4* const src = reinterpret_cast<const uint4*>(a.k_codes + ((size_t)max(p, 0) * a.kv_heads + h) * a.block * HD) + ((first + j * kPpKeys + tt) & in_block);
+                const uint4* const src = reinterpret_cast<const uint4*>(a.k_codes + ((size_t)max(p, 0) * a.kv_heads + h) * a.block * HD) + ((first + j * kPpKeys + tt) & in_block) + (size_t)side * U * a.block;
 #pragma unroll
                 for (int c = 0; c < U; ++c) kc[c] = ld_stream_u4(src + (size_t)c * a.block);
             };
             auto fetch_values = [&](int j, int p) {
                 const uint4* const src = reinterpret_cast<const uint4*>(a.v_codes + ((size_t)max(p, 0) * a.kv_heads + h) * a.block * HD) +
-                                         (size_t)(((first + j * kPpKeys + (tt & ~15)) & in_block) >> 4) * HD + (tt & 15);
+                                         (size_t)(((first + j * kPpKeys + (tt & ~15)) & in_block) >> 4) * HD + side * (HD / 2) + (tt & 15);
 #pragma unroll
                 for (int c = 0; c < U; ++c) vc[c] = ld_stream_u4(src + c * 16);
             };
             int page = page_of(entry_of(0)), entry = entry_of(1);
-            float ks = 0.0f, vs = 0.0f;  // lanes 0-7 of warp 8: scales of the tile in kc
+            float ks = 0.0f, vs = 0.0f;  // lanes 0-7 of the first warp: scales of the tile in kc
             auto fetch_scales = [&](int p) {
-                if (warp == 8 && lane < 8) {
+                if (warp == kPpConvert && lane < 8) {
                     ks = p >= 0 ? a.k_scales[(size_t)p * a.kv_heads + h] : 0.0f;
                     vs = p >= 0 ? a.v_scales[(size_t)p * a.kv_heads + h] : 0.0f;
                 }
@@ -260,10 +305,11 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                 fetch_values(0, p);
             }
             for (int j = 0; j < tiles; ++j) {
-                const int st = j & 1, before = j - 2;
-                ok = before < 0 || warp_wait(&s_full[st], (uint32_t)(before >> 1) & 1u);
+                const int st = j % kStages, before = j - kStages;  // the use of the stage before
+                ok = before < 0 || warp_wait(&k_free[st], (uint32_t)(before / kStages) & 1u);
                 if (!ok) break;
-                if (warp == 8) {
+                if (warp == kPpConvert) {
+                    // (every softmax warp has read the scales of tile j - 4: it wrote the weights of that tile before the scores of tile j - 2 began)
                     PpScales& sc = scales[j & 3];
                     if (lane < 8) {
                         sc.k[lane] = ks;
@@ -277,7 +323,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                 }
                 unsigned char* const krow = smem + S::kOffK + st * S::kK + tt * 128;
 #pragma unroll
-                for (int c = 0; c < U; ++c) pp_put(krow + (c >> 2) * kPpBox, (c & 3) * 2, tt & 7, kc[c]);
+                for (int c = 0; c < U; ++c) pp_put(krow + ((side * U + c) >> 2) * kPpBox, ((side * U + c) & 3) * 2, tt & 7, kc[c]);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&k_full[st]);
@@ -286,9 +332,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                     fetch_scales(next);
                     fetch_keys(j + 1, p_next);
                 }
-                ok = before < 0 || warp_wait(&pv_done[st], (uint32_t)(before >> 1) & 1u);
+                ok = before < 0 || warp_wait(&v_free[st], (uint32_t)(before / kStages) & 1u);
                 if (!ok) break;
-                unsigned char* const vrow = smem + S::kOffV + st * S::kV + (tt >> 6) * S::kVBox + (tt & 15) * 128;
+                unsigned char* const vrow = smem + S::kOffV + st * S::kV + (tt >> 6) * S::kVBox + (side * (HD / 2) + (tt & 15)) * 128;
 #pragma unroll
                 for (int c = 0; c < U; ++c) pp_put(vrow + c * 2048, ((tt >> 4) & 3) * 2, tt & 7, vc[c]);
                 fence_proxy_async_smem();
@@ -298,178 +344,233 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                 page = next;
                 entry = entry_of(j + 2);
             }
-        } else if (warp == 12) {
+        } else if (warp == kPpIssue) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
             constexpr uint32_t idesc_s = gemm_idesc_f16(128, kPpKeys), idesc_o = gemm_idesc_f16(128, HD);
             const uint64_t dq = gemm_smem_desc(base), dk = gemm_smem_desc(base + S::kOffK), dv = gemm_smem_desc(base + S::kOffV);
             const uint32_t lead = elect_lead();
-            auto scores = [&](int j) {
-                const int st = j & 1;
-                if (!warp_wait(&k_full[st], (uint32_t)(j >> 1) & 1u)) return false;
+            // scores of tile j for stream s; `last`: nobody else needs the keys
+            auto scores = [&](int j, int s, bool last) {
+                const int st = j % kStages;
+                if (!warp_wait(&k_full[st], (uint32_t)(j / kStages) & 1u)) return false;
                 tcgen05_fence_after();
-                const uint64_t dkj = dk + (uint64_t)(st * (S::kK >> 4));
+                const uint64_t dkj = dk + (uint64_t)(st * (S::kK >> 4)), dqs = dq + (uint64_t)(two ? s * (S::kQTile >> 4) : 0);
                 uint32_t acc = 0u;
 #pragma unroll
                 for (int p = NP - 1; p >= 0; --p)  // the small products first
 #pragma unroll
                     for (int ks = 0; ks < HD / 16; ++ks) {
                         const int at = (ks >> 2) * kPpBox + (ks & 3) * 32;
-                        lead_mma_f16(lead, (uint32_t)st * 128u, dq + (uint64_t)((p * S::kQPlane + at) >> 4), dkj + (uint64_t)(at >> 4), idesc_s, acc);
+                        lead_mma_f16(lead, (uint32_t)s * 128u, dqs + (uint64_t)((p * S::kQPlane + at) >> 4), dkj + (uint64_t)(at >> 4), idesc_s, acc);
                         acc = 1u;
                     }
-                lead_commit(lead, &s_full[st]);
+                lead_commit(lead, &s_full[s]);
+                if (last) lead_commit(lead, &k_free[st]);
                 return true;
             };
-            if (tiles > 0) ok = scores(0) && (tiles < 2 || scores(1));
-            for (int j = 0; j < tiles && ok; ++j) {
-                const int st = j & 1;
-                ok = warp_wait(&v_full[st], (uint32_t)(j >> 1) & 1u) && warp_wait(&p_ready[st], (uint32_t)(j >> 1) & 1u);
-                if (!ok) break;
+            // O of stream s takes its n-th tile, tile j
+            auto values = [&](int j, int s, int n, bool last) {
+                const int st = j % kStages;
+                if (!(warp_wait(&v_full[st], (uint32_t)(j / kStages) & 1u) && warp_wait(&p_ready[s], (uint32_t)n & 1u))) return false;
                 tcgen05_fence_after();
                 const uint64_t dvj = dv + (uint64_t)(st * (S::kV >> 4));
-                uint32_t acc = j >= 2 ? 1u : 0u;
+                uint32_t acc = n > 0 ? 1u : 0u;
 #pragma unroll
                 for (int p = NP - 1; p >= 0; --p)
 #pragma unroll
                     for (int ks = 0; ks < kPpKeys / 16; ++ks) {  // weights of 32 keys: 16 columns of the first plane, 16 of the second
-                        lead_mma_f16_ts(lead, kPpTmemO + (uint32_t)st * 128u, (uint32_t)(st * 128 + (ks >> 1) * 32 + p * 16 + (ks & 1) * 8),
+                        lead_mma_f16_ts(lead, kPpTmemO + (uint32_t)s * 128u, (uint32_t)(s * 128 + (ks >> 1) * 32 + p * 16 + (ks & 1) * 8),
                                         dvj + (uint64_t)(((ks >> 2) * S::kVBox + (ks & 3) * 32) >> 4), idesc_o, acc);
                         acc = 1u;
                     }
-                lead_commit(lead, &pv_done[st]);
-                if (j + 2 < tiles) ok = scores(j + 2);
+                lead_commit(lead, &pv_done[s]);
+                if (last) lead_commit(lead, &v_free[st]);
+                return true;
+            };
+            if (two) {
+                // (the second stream has every tile, the first the tiles up to its own rows' positions)
+                if (tiles > 0) ok = (tiles0 < 1 || scores(0, 0, false)) && scores(0, 1, true);
+                for (int j = 0; j < tiles && ok; ++j) {
+                    if (j < tiles0) ok = values(j, 0, j, false);
+                    if (ok && j + 1 < tiles0) ok = scores(j + 1, 0, false);
+                    if (ok) ok = values(j, 1, j, true);
+                    if (ok && j + 1 < tiles) ok = scores(j + 1, 1, true);
+                }
+            } else {
+                if (tiles > 0) ok = scores(0, 0, true) && (kStages < 2 || tiles < 2 || scores(1, 1, true));
+                for (int j = 0; j < tiles && ok; ++j) {
+                    if (kStages < 2 && j + 1 < tiles) ok = scores(j + 1, (j + 1) & 1, true);
+                    if (ok) ok = values(j, j & 1, j >> 1, true);
+                    if (ok && kStages >= 2 && j + 2 < tiles) ok = scores(j + 2, j & 1, true);
+                }
             }
-        } else {
-            // ---- softmax of the tiles j = stream, stream + 2, ..
-            const int stream = warp >> 2, r = (warp & 3) * 32 + lane, own = rq.pos0 + (row0 + r) / group;
-            const int pos = min(own, rq.hi - 1), lo = a.window > 0 ? own - a.window + 1 : 0;
-            const float unit = a.scale2 / units[r];  // (a row with an infinity or NaN has no scores)
+        } else if (warp < kPpConvert) {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
+            // ---- softmax: the stream's tiles j = j0, j0 + step, ..
+            const int stream = warp >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane, in_unit = two ? stream * kPpRows + r : r;
+            uint64_t* const pair_bar = pair + stream * 4 + (warp & 3);  // of the two warps that have the same rows
+            float* const tops = reinterpret_cast<float*>(smem + S::kOffTop) + stream * 2 * kPpRows + r;  // [tile parity][stream][half][row]
+            const int step = two ? 1 : 2, end = two && stream == 0 ? tiles0 : tiles;
+            const int own = own_pos(in_unit), pos = min(own, rq.hi - 1), lo = a.window > 0 ? own - a.window + 1 : 0;
+            const int row_a = two ? stream * kPpRows : 0, row_b = min(live, row_a + kPpRows) - 1, first_pos = own_pos(row_a), last_own = own_pos(max(row_b, row_a));
+            const float unit = a.scale2 / units[in_unit];  // (a row with an infinity or NaN has no scores)
             const uint32_t rows = (uint32_t)((warp & 3) * 32) << 16;
             const uint32_t ts = rows + (uint32_t)stream * 128u, to = rows + kPpTmemO + (uint32_t)stream * 128u;
             float m_ref = -INFINITY, l = 0.0f;
             int n = 0;  // tiles of this stream so far
-            for (int j = stream; j < tiles; j += 2, ++n) {
+            for (int j = two ? 0 : stream; j < end; j += step, ++n) {
                 const int t0 = first + j * kPpKeys;
                 ok = warp_wait(&sc_full[j & 3], (uint32_t)(j >> 2) & 1u) && warp_wait(&s_full[stream], (uint32_t)n & 1u);
                 if (!ok) break;
                 tcgen05_fence_after();
                 const PpScales& sc = scales[j & 3];
-                const bool masked = t0 + kPpKeys - 1 > first_pos || t0 < low || (a.window > 0 && t0 < last_own - a.window + 1) || sc.there != 0xffu;
+                const uint32_t there_bits = sc.there;
+                const bool masked = t0 + kPpKeys - 1 > first_pos || t0 < low || (a.window > 0 && t0 < last_own - a.window + 1) || there_bits != 0xffu;
                 // keys of chunk c that the row attends, a bit each
                 auto seen_of = [&](int c) {
-                    const int k0 = t0 + c * 32, from = max(lo - k0, 0), to = min(pos - k0, 31);
-                    const uint32_t pair = sc.there >> (2 * c);
+                    const int k0 = t0 + c * 32, from = max(lo - k0, 0), to_key = min(pos - k0, 31);
+                    const uint32_t pair = there_bits >> (2 * c);
                     const uint32_t there = (pair & 1u ? 0xffffu : 0u) | (pair & 2u ? 0xffff0000u : 0u);
-                    return from <= to ? (0xffffffffu << from) & (0xffffffffu >> (31 - to)) & there : 0u;
+                    return from <= to_key ? (0xffffffffu << from) & (0xffffffffu >> (31 - to_key)) & there : 0u;
                 };
-                float top = -INFINITY;
-                auto largest = [&](auto is_masked) {
-#pragma unroll 1
-                    for (int c = 0; c < kPpKeys / 32; ++c) {
-                        uint32_t d[32];
-                        tmem_load_x32(ts + c * 32, d);
-                        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                        const uint32_t seen = is_masked.value ? seen_of(c) : 0u;
+                // the largest s + log2 v_scale of 32 scores
+                auto largest = [&](auto is_masked, int c, uint32_t (&d)[32]) {
+                    const uint32_t seen = is_masked.value ? seen_of(c) : 0u;
+                    if (is_masked.value) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            mx[(i >> 4) * 2 + (i & 1)] = fmaxf(mx[(i >> 4) * 2 + (i & 1)], is_masked.value && (seen & (1u << i)) == 0u ? -INFINITY : __uint_as_float(d[i]));
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const float x = fmaxf(mx[2 * k], mx[2 * k + 1]);
-                            if (x > -INFINITY) top = fmaxf(top, fmaf(x, sc.k[2 * c + k] * unit, sc.log_v[2 * c + k]));
-                        }
+                        for (int i = 0; i < 32; ++i) d[i] = (seen & (1u << i)) != 0u ? d[i] : 0xff800000u;
                     }
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) {
+                            mx[0] = fmaxf(fmaxf(mx[0], __uint_as_float(d[16 * k + i])), __uint_as_float(d[16 * k + i + 1]));
+                            mx[1] = fmaxf(fmaxf(mx[1], __uint_as_float(d[16 * k + i + 2])), __uint_as_float(d[16 * k + i + 3]));
+                        }
+                        const float x = fmaxf(mx[0], mx[1]);
+                        if (x > -INFINITY) top = fmaxf(top, fmaf(x, sc.k[2 * c + k] * unit, sc.log_v[2 * c + k]));
+                    }
+                    return top;
                 };
-                if (masked) largest(std::true_type());
-                else largest(std::false_type());
-                const bool grow = top > m_ref + 8.0f;  // (a row with nothing attended so far has -inf)
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float corr = grow ? ex2_approx(m_ref - top) : 1.0f;
-                    if (grow) m_ref = top;
-                    l *= corr;
-                    if (n > 0) {
-                        ok = warp_wait(&pv_done[stream], (uint32_t)(n - 1) & 1u);
-                        if (!ok) break;
-                        tcgen05_fence_after();
+                auto weights = [&](auto is_masked, int c, const uint32_t (&d)[32], float m) {
+                    const uint32_t seen = is_masked.value ? seen_of(c) : 0u;
 #pragma unroll
-                        for (int c = 0; c < HD / 32; ++c) {
-                            uint32_t d[32];
-                            tmem_load_x32(to + c * 32, d);
+                    for (int k = 0; k < 2; ++k) {
+                        const float f = sc.k[2 * c + k] * unit, off = sc.log_v[2 * c + k] - m;
+                        const uint64_t ff = pp_pair(f, f), oo = pp_pair(off, off);
+                        uint64_t sum = 0ull;
+                        uint32_t hi[8], rest[NP == 2 ? 8 : 1];
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) d[i] = __float_as_uint(__uint_as_float(d[i]) * corr);
-                            tmem_store_x32(to + c * 32, d);
-                        }
-                    }
-                }
-                const float m = m_ref == -INFINITY ? 0.0f : m_ref;
-                auto weights = [&](auto is_masked) {
-#pragma unroll 1
-                    for (int c = 0; c < kPpKeys / 32; ++c) {
-                        uint32_t d[32], planes[NP * 16];
-                        tmem_load_x32(ts + c * 32, d);
-                        const uint32_t seen = is_masked.value ? seen_of(c) : 0u;
-                        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        const float f[2] = {sc.k[2 * c] * unit, sc.k[2 * c + 1] * unit}, off[2] = {sc.log_v[2 * c] - m, sc.log_v[2 * c + 1] - m};
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int k = i >> 3;
-                            float p0 = ex2_approx(fmaf(__uint_as_float(d[2 * i]), f[k], off[k])), p1 = ex2_approx(fmaf(__uint_as_float(d[2 * i + 1]), f[k], off[k]));
-                            if (is_masked.value) {
-                                p0 = (seen & (1u << (2 * i))) != 0u ? p0 : 0.0f;
-                                p1 = (seen & (2u << (2 * i))) != 0u ? p1 : 0.0f;
+                        for (int i = 0; i < 8; ++i) {
+                            const int at = 8 * k + i;
+                            const float2 e = pp_unpair(pp_fma2(pp_pair(__uint_as_float(d[2 * at]), __uint_as_float(d[2 * at + 1])), ff, oo));
+                            float p0 = ex2_approx(e.x), p1 = ex2_approx(e.y);
+                            if (is_masked.value) {  // (a scale of 0 makes 0 * -infinity of what is masked)
+                                p0 = (seen & (1u << (2 * at))) != 0u ? p0 : 0.0f;
+                                p1 = (seen & (2u << (2 * at))) != 0u ? p1 : 0.0f;
                             }
-                            sum[2 * k] += p0;
-                            sum[2 * k + 1] += p1;
-                            planes[i] = pp_round(p0, p1);
-                            if constexpr (NP == 2) planes[16 + i] = pp_rest(p0, p1, planes[i]);
+                            const uint64_t pp = pp_pair(p0, p1);
+                            sum = pp_add2(sum, pp);
+                            hi[i] = pp_round(p0, p1);
+                            if constexpr (NP == 2) {
+                                const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
+                                const float2 x = pp_unpair(pp_fma2(pp_pair(y.x, y.y), pp_pair(-1.0f, -1.0f), pp));
+                                rest[i] = pp_round(x.x, x.y);
+                            }
                         }
-                        l = fmaf(sum[0] + sum[1], sc.inv_v[2 * c], l);
-                        l = fmaf(sum[2] + sum[3], sc.inv_v[2 * c + 1], l);
-                        if constexpr (NP == 2) tmem_store_x32(ts + c * 32, planes);
-                        else tmem_store_x16(ts + c * 32, planes);
+                        const float2 both = pp_unpair(sum);
+                        l = fmaf(both.x + both.y, sc.inv_v[2 * c + k], l);
+                        tmem_store_x8(ts + c * 32 + k * 8, hi);
+                        if constexpr (NP == 2) tmem_store_x8(ts + c * 32 + 16 + k * 8, rest);
                     }
                 };
-                if (masked) weights(std::true_type());
-                else weights(std::false_type());
+                auto tile = [&](auto is_masked) {
+                    uint32_t d[32];
+                    tmem_load_x32(ts + half * 64, d);
+                    float top = largest(is_masked, 2 * half, d);
+                    tmem_load_x32(ts + half * 64 + 32, d);
+                    top = fmaxf(top, largest(is_masked, 2 * half + 1, d));
+                    // (two buffers: a thread writes the next value of this one behind a barrier that its partner reaches after it has read)
+                    float* const at = tops + (n & 1) * 4 * kPpRows;
+                    at[half * kPpRows] = top;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(pair_bar);
+                    ok = warp_wait(pair_bar, (uint32_t)n & 1u);
+                    if (!ok) return;
+                    top = fmaxf(top, at[(half ^ 1) * kPpRows]);
+                    const bool grow = top > m_ref + 8.0f;  // (a row with nothing attended so far has -inf)
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float corr = grow ? ex2_approx(m_ref - top) : 1.0f;
+                        if (grow) m_ref = top;
+                        l *= corr;
+                        if (n > 0) {  // half of the columns of O each
+                            ok = warp_wait(&pv_done[stream], (uint32_t)(n - 1) & 1u);
+                            if (!ok) return;
+                            tcgen05_fence_after();
+#pragma unroll 1
+                            for (int i = half * (HD / 32); i < (half + 1) * (HD / 32); ++i) {
+                                uint32_t o[16];
+                                tmem_load_x16(to + i * 16, o);
+#pragma unroll
+                                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * corr);
+                                tmem_store_x16(to + i * 16, o);
+                            }
+                        }
+                    }
+                    const float m = m_ref == -INFINITY ? 0.0f : m_ref;
+                    weights(is_masked, 2 * half + 1, d, m);
+                    tmem_load_x32(ts + half * 64, d);
+                    weights(is_masked, 2 * half, d, m);
+                };
+                if (masked) tile(std::true_type());
+                else tile(std::false_type());
+                if (!ok) break;
                 tmem_store_wait();
                 tcgen05_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_ready[stream]);
             }
             if (ok && n > 0) ok = warp_wait(&pv_done[stream], (uint32_t)(n - 1) & 1u);
-            // ---- both streams of a row, then half of its columns per stream's warps
-            float2* const stat = reinterpret_cast<float2*>(smem + S::kOffStat);
-            stat[stream * kPpRows + r] = make_float2(m_ref, l);
+            // ---- the sum of both threads of a row; where the streams are shares of the keys, maximum and sum over both
+            float2* const stat = reinterpret_cast<float2*>(smem + S::kOffStat);  // [stream][half][row]
+            stat[(stream * 2 + half) * kPpRows + r] = make_float2(m_ref, l);
             tcgen05_fence_before();
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+            asm volatile("bar.sync 1, 512;" ::: "memory");
             tcgen05_fence_after();
-            const float2 st0 = stat[r], st1 = stat[kPpRows + r];
-            const float m = fmaxf(st0.x, st1.x), mm = m == -INFINITY ? 0.0f : m;
-            const float w0 = ex2_approx(st0.x - mm), w1 = ex2_approx(st1.x - mm), sum = st0.y * w0 + st1.y * w1, inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            const float f0 = w0 * inv, f1 = w1 * inv;
+            const float m0 = stat[r].x, m1 = stat[2 * kPpRows + r].x, l0 = stat[r].y + stat[kPpRows + r].y, l1 = stat[2 * kPpRows + r].y + stat[3 * kPpRows + r].y;
+            const float m = fmaxf(m0, m1), mm = m == -INFINITY ? 0.0f : m;
+            const float w0 = ex2_approx(m0 - mm), w1 = ex2_approx(m1 - mm), sum = two ? (stream == 0 ? l0 : l1) : l0 * w0 + l1 * w1, inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const float f0 = two ? inv : w0 * inv, f1 = w1 * inv;
+            const bool any0 = two ? n > 0 : tiles > 0, any1 = !two && tiles > 1;
+            // half of the columns each: of the stream's rows, or (one tile of rows) a quarter for each of the four warps
+            const int columns = two ? HD / 2 : HD / 4, from = two ? half * columns : (stream * 2 + half) * columns;
             // the last MMAs are done and nobody loads: the rows leave over the operands' shared memory, so that a warp writes whole runs
             float* const stage = reinterpret_cast<float*>(smem) + warp * 32 * S::kStagePitch;
+#pragma unroll 1
+            for (int c = 0; c < columns; c += 16) {
+                uint32_t d[16], e[16];
+                const uint32_t col = rows + kPpTmemO + (uint32_t)((two ? stream * 128 : 0) + from + c);
+                if (any0) tmem_load_x16(col, d);
+                if (any1) tmem_load_x16(col + 128u, e);
 #pragma unroll
-            for (int c = 0; c < HD / 64; ++c) {
-                uint32_t d[32], e[32];
-                const uint32_t col = rows + kPpTmemO + (uint32_t)(stream * (HD / 2) + c * 32);
-                if (tiles > 0) tmem_load_x32(col, d);
-                if (tiles > 1) tmem_load_x32(col + 128u, e);
-#pragma unroll
-                for (int i = 0; i < 32; i += 4) {
+                for (int i = 0; i < 16; i += 4) {
                     float y[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        y[k] = tiles > 0 ? __uint_as_float(d[i + k]) * f0 : 0.0f;
-                        if (tiles > 1) y[k] = fmaf(__uint_as_float(e[i + k]), f1, y[k]);
+                        y[k] = any0 ? __uint_as_float(d[i + k]) * f0 : 0.0f;
+                        if (any1) y[k] = fmaf(__uint_as_float(e[i + k]), f1, y[k]);
                     }
-                    *reinterpret_cast<float4*>(stage + lane * S::kStagePitch + c * 32 + i) = make_float4(y[0], y[1], y[2], y[3]);
+                    *reinterpret_cast<float4*>(stage + lane * S::kStagePitch + c + i) = make_float4(y[0], y[1], y[2], y[3]);
                 }
             }
             __syncwarp();
-            for (int i = lane; i < 32 * (HD / 8); i += 32) {
-                const int rr = i / (HD / 8), c4 = i - rr * (HD / 8), row = (warp & 3) * 32 + rr;
+            const int quads = columns / 4;
+            for (int i = lane; i < 32 * quads; i += 32) {
+                const int rr = i / quads, c4 = i % quads, row = (two ? stream * kPpRows : 0) + (warp & 3) * 32 + rr;
                 if (!ok || row >= live) continue;
-                T* const out = static_cast<T*>(a.out) + (size_t)row_of[row] * HD + stream * (HD / 2) + c4 * 4;
+                T* const out = static_cast<T*>(a.out) + (size_t)row_of[row] * HD + from + c4 * 4;
                 const float4 y = *reinterpret_cast<const float4*>(stage + rr * S::kStagePitch + c4 * 4);
                 if constexpr (sizeof(T) == 4) {
                     *reinterpret_cast<float4*>(out) = y;
@@ -480,11 +581,12 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
             }
         }
     }
+    if (request >= 0 && warp > kPpIssue) asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
     if (!ok) atomicCAS(&g_paged_prompt_status, 0, 1);
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
-    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(512u) : "memory");
+    if (warp == kPpIssue) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(512u) : "memory");
 }
 
 }  // namespace
@@ -495,11 +597,14 @@ bool paged_prompt_serves(const PagedArgs& a) {
 
 int paged_prompt_launch(cudaStream_t stream, const PagedArgs& a, bool f32) {
     const int group = a.heads / a.kv_heads;
-    const long long tiles = ((long long)a.tokens * group + kPpRows - 1) / kPpRows + a.requests;  // each request ends in a tile of its own
-    KMLL_REQUIRE(tiles <= INT_MAX && (long long)a.tokens * a.heads <= INT_MAX, "paged attention: too many rows");
+    const long long tiles = ((long long)a.tokens * group + 2 * kPpRows - 1) / (2 * kPpRows) + a.requests;  // each request ends in a unit of its own
+    KMLL_REQUIRE(tiles <= 65535 && (long long)a.tokens * a.heads <= INT_MAX, "paged attention: too many rows");
     auto go = [&](auto kern, int smem) {
-        const cudaError_t e = allow_all_dynamic_smem(kern);
-        return e != cudaSuccess ? e : launch(kern, dim3((unsigned)tiles, a.kv_heads), dim3(kPpThreads), (size_t)smem, stream, true, a);
+        cudaFuncAttributes fa;
+        cudaError_t e = cudaFuncGetAttributes(&fa, kern);
+        if (e == cudaSuccess && fa.numRegs < kPpRegsLaunch) e = cudaErrorInvalidDeviceFunction;  // (the warpgroups would wait for registers that the block does not have)
+        if (e == cudaSuccess) e = allow_all_dynamic_smem(kern);
+        return e != cudaSuccess ? e : launch(kern, dim3(a.kv_heads, (unsigned)tiles), dim3(kPpThreads), (size_t)smem, stream, true, a);
     };
     cudaError_t e;
     if (a.head_dim == 128) e = f32 ? go(paged_prompt_kernel<128, float>, PpShape<128, 2>::kSmemBytes) : go(paged_prompt_kernel<128, uint16_t>, PpShape<128, 1>::kSmemBytes);
