@@ -205,7 +205,6 @@ __device__ inline double2 sin_cos(double x) {
 
 struct PrepareArgs {
     const void *query, *key, *value;
-    int f32;
     size_t ldq, ldk, ldv;
     const float* freqs;
     int n_freqs;
@@ -214,7 +213,11 @@ struct PrepareArgs {
     void* query_rot;
     int8_t *k_codes, *v_codes;
     float *k_scales, *v_scales;
-    int pages, block, group;  // group: tokens whose runs a block of threads takes
+    int pages, block;
+    int group, groups;      // tokens whose runs a block of threads takes, and how many such blocks for a set of heads
+    int head_sets;          // of kHeadSet kv heads
+    int q_tokens;           // query rows' tokens of a block of threads
+    int table_tokens;       // tokens whose angles fit into shared memory
 };
 
 template <typename T>
@@ -223,6 +226,15 @@ template <>
 __device__ inline float load_as_f32<float>(const float* p) { return *p; }
 template <>
 __device__ inline float load_as_f32<uint16_t>(const uint16_t* p) { return bf16_bits_to_f32(*p); }
+__device__ inline float2 load_pair(const float* p) { return *reinterpret_cast<const float2*>(p); }
+__device__ inline float2 load_pair(const uint16_t* p) {
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+__device__ inline void store_one(float* p, float v) { *p = v; }
+__device__ inline void store_one(uint16_t* p, float v) { *p = f32_to_bf16_bits(v); }
+__device__ inline void store_pair(float* p, float x, float y) { *reinterpret_cast<float2*>(p) = make_float2(x, y); }
+__device__ inline void store_pair(uint16_t* p, float x, float y) { *reinterpret_cast<uint32_t*>(p) = f32_to_bf16_bits(x) | ((uint32_t)f32_to_bf16_bits(y) << 16); }
 
 // The nearest whole number to v * inv = v / scale, ties to even as the quotient itself has them: where the product is within its rounding
 // error of a tie the quotient decides.
@@ -233,122 +245,182 @@ __device__ inline int code_of(double v, double scale, double inv) {
     return (int)fmin(fmax(c, -127.0), 127.0);
 }
 // A value that is not finite must not spoil its page: an infinity takes the largest code, NaN counts as 0.
-__device__ inline bool is_finite(double v) { return fabs(v) < 1e300; }
+__device__ inline double finite_size(double v) { return fabs(v) < 1e300 ? fabs(v) : 0.0; }
 
-constexpr int kPrepareThreads = 128;
+constexpr int kPrepareThreads = 256;
+constexpr int kHeadSet = 4, kHeadThreads = kPrepareThreads / kHeadSet;  // kv heads of a block of threads; threads of one
 
-// Blocks (x, y): y < kv_heads keys, y < 2 * kv_heads values of one head, above that query heads.  A run is a stretch of tokens with ascending
-// slots in one page; the thread block whose tokens hold the first of a run takes all of it, so that a page's scale is known in one place.
-template <typename T>
+// Blocks of threads along x: keys (groups of tokens x sets of heads), values (the same), query rows.  A run is a stretch of tokens with ascending
+// slots in one page; the block whose tokens hold the first of a run takes all of it, so that a page's scale is known in one place.  A head has 64
+// threads, a thread the same entries of every token; the first walk over the run finds the largest magnitude, the second (out of L1 / L2) codes.
+// The angles of a token are computed once per block into shared memory, not for every head.  VEC: entries lie so that two load together.
+template <typename T, int VEC>
 __global__ void __launch_bounds__(kPrepareThreads) prepare_paged_kernel(const PrepareArgs a) {
-    __shared__ float scratch[33];
-    const int tid = threadIdx.x, t0 = blockIdx.x * a.group, t1 = min(a.tokens, t0 + a.group), hd = a.head_dim, half = a.n_freqs;
-    const int y = blockIdx.y;
+    extern __shared__ __align__(16) double2 table[];  // [token][n_freqs] sine, cosine
+    __shared__ int s_slots[2 * 128 + 1];
+    __shared__ int s_run;
+    __shared__ float s_top[kPrepareThreads / 32];
+    const int tid = threadIdx.x, hd = a.head_dim, half = a.n_freqs, limit = a.pages * a.block;
+    const int kv_blocks = a.groups * a.head_sets;
     pdl_wait();
-    const int limit = a.pages * a.block;
-    if (y >= 2 * a.kv_heads) {
-        const int h = y - 2 * a.kv_heads, items = half + (hd - 2 * half);
-        for (int i = tid; i < (t1 - t0) * items; i += kPrepareThreads) {
-            const int t = t0 + i / items, d = i % items;
-            const int slot = a.slots[t];
+    if ((int)blockIdx.x >= 2 * kv_blocks) {
+        // ---- query rows: a warp has a row at a time
+        const int t0 = ((int)blockIdx.x - 2 * kv_blocks) * a.q_tokens, n = min(a.q_tokens, a.tokens - t0), lane = tid & 31, warp = tid >> 5;
+        for (int i = tid; i < n * half; i += kPrepareThreads) table[i] = sin_cos((double)a.positions[t0 + i / half] * (double)a.freqs[i % half]);
+        __syncthreads();
+        for (int t = 0; t < n; ++t) {
+            const int slot = a.slots[t0 + t];
             if (slot < 0 || slot >= limit) continue;
-            const T* src = static_cast<const T*>(a.query) + (size_t)t * a.ldq + (size_t)h * hd;
-            T* dst = static_cast<T*>(a.query_rot) + ((size_t)t * a.heads + h) * hd;
-            if (d >= half) {
-                dst[d + half] = src[d + half];
-                continue;
-            }
-            const double2 sc = sin_cos((double)a.positions[t] * (double)a.freqs[d]);
-            const double u = load_as_f32(src + d), v = load_as_f32(src + d + half);
-            const float p = (float)(u * sc.y - v * sc.x), q = (float)(u * sc.x + v * sc.y);
-            if constexpr (sizeof(T) == 4) {
-                dst[d] = p;
-                dst[d + half] = q;
-            } else {
-                dst[d] = f32_to_bf16_bits(p);
-                dst[d + half] = f32_to_bf16_bits(q);
+            const double2* const turn = table + t * half;
+            const T* const src = static_cast<const T*>(a.query) + (size_t)(t0 + t) * a.ldq;
+            T* const dst = static_cast<T*>(a.query_rot) + (size_t)(t0 + t) * a.heads * hd;
+#pragma unroll 2
+            for (int h = warp; h < a.heads; h += kPrepareThreads / 32) {
+                for (int d = lane * VEC; d < half; d += 32 * VEC) {
+                    const T* const at = src + h * hd + d;
+                    T* const to = dst + h * hd + d;
+                    if constexpr (VEC == 2) {
+                        const float2 u = load_pair(at), v = load_pair(at + half);
+                        const double2 s0 = turn[d], s1 = turn[d + 1];
+                        store_pair(to, (float)(u.x * s0.y - v.x * s0.x), (float)(u.y * s1.y - v.y * s1.x));
+                        store_pair(to + half, (float)(u.x * s0.x + v.x * s0.y), (float)(u.y * s1.x + v.y * s1.y));
+                    } else {
+                        const double u = load_as_f32(at), v = load_as_f32(at + half);
+                        const double2 s0 = turn[d];
+                        store_one(to, (float)(u * s0.y - v * s0.x));
+                        store_one(to + half, (float)(u * s0.x + v * s0.y));
+                    }
+                }
+                for (int d = 2 * half + lane; d < hd; d += 32) dst[h * hd + d] = src[h * hd + d];
             }
         }
         return;
     }
-    const bool keys = y < a.kv_heads;
-    const int h = keys ? y : y - a.kv_heads;
-    const T* const in = static_cast<const T*>(keys ? a.key : a.value) + (size_t)h * hd;
+    const bool keys = (int)blockIdx.x < kv_blocks;
+    const int item = keys ? blockIdx.x : blockIdx.x - kv_blocks, set = item % a.head_sets, t0 = item / a.head_sets * a.group, t1 = min(a.tokens, t0 + a.group);
+    const int sub = tid / kHeadThreads, lt = tid % kHeadThreads, h = set * kHeadSet + sub;
+    const bool live = h < a.kv_heads;
+    const T* const in = static_cast<const T*>(keys ? a.key : a.value) + (size_t)(live ? h : 0) * hd;
     const size_t ld = keys ? a.ldk : a.ldv;
     const int turned = keys ? half : 0;
-    // entries d and (for d < turned) d + turned of token t
-    auto pair = [&](int t, int d, double& u, double& v) {
-        const T* src = in + (size_t)t * ld;
-        if (d >= turned) {
-            u = load_as_f32(src + d + turned);
-            v = 0.0;
-            return;
-        }
-        const double2 sc = sin_cos((double)a.positions[t] * (double)a.freqs[d]);
-        const double p = load_as_f32(src + d), q = load_as_f32(src + d + turned);
-        u = p * sc.y - q * sc.x;
-        v = p * sc.x + q * sc.y;
-    };
-    const int items = hd - turned;
+    // slots of the tokens t0 - 1 .. (every run that begins here ends among them)
+    for (int i = tid; i <= a.group + a.block; i += kPrepareThreads) {
+        const int t = t0 - 1 + i;
+        s_slots[i] = t >= 0 && t < a.tokens ? a.slots[t] : INT_MIN;
+    }
+    __syncthreads();
     for (int t = t0; t < t1; ++t) {
-        const int slot = a.slots[t];
+        const int* const slots = s_slots + (t - t0 + 1);
+        const int slot = slots[0];
         if (slot < 0 || slot >= limit) continue;
         const int at = slot % a.block, page = slot / a.block;
-        if (at != 0 && t > 0 && a.slots[t - 1] == slot - 1) continue;
-        int n = 1;
-        while (at + n < a.block && t + n < a.tokens && a.slots[t + n] == slot + n) ++n;
+        if (at != 0 && t > 0 && slots[-1] == slot - 1) continue;
+        // ---- length of the run: up to the first token that does not follow
+        if (tid == 0) s_run = min(a.block - at, a.tokens - t);
+        __syncthreads();
+        for (int i = tid; i < a.block - at; i += kPrepareThreads)
+            if (slots[i] != slot + i) atomicMin(&s_run, i);
+        __syncthreads();
+        const int n = s_run;
+        const bool kept = n <= a.table_tokens;  // the angles of the whole run stay in shared memory
+        auto angles = [&](int i0, int i1) {
+            __syncthreads();
+            for (int i = tid; i < (i1 - i0) * turned; i += kPrepareThreads) table[i] = sin_cos((double)a.positions[t + i0 + i / turned] * (double)a.freqs[i % turned]);
+            __syncthreads();
+        };
+        // calls f(token of the run, entry, value) for this thread's entries, 64-bit turned values
+        auto walk = [&](bool again, auto f) {
+            for (int i0 = 0; i0 < n; i0 += a.table_tokens) {
+                const int i1 = min(n, i0 + a.table_tokens);
+                if (turned > 0 && !(again && kept)) angles(i0, i1);
+                if (!live) continue;
+                for (int d = lt; d < turned; d += kHeadThreads) {
+                    const T* src = in + (size_t)(t + i0) * ld + d;
+                    const double2* turn = table + d;
+#pragma unroll 8
+                    for (int i = i0; i < i1; ++i, src += ld, turn += turned) {
+                        const double p = load_as_f32(src), q = load_as_f32(src + turned);
+                        const double2 sc = *turn;
+                        f(i, d, p * sc.y - q * sc.x);
+                        f(i, d + turned, p * sc.x + q * sc.y);
+                    }
+                }
+                for (int d = 2 * turned + lt; d < hd; d += kHeadThreads) {
+                    const T* src = in + (size_t)(t + i0) * ld + d;
+#pragma unroll 8
+                    for (int i = i0; i < i1; ++i, src += ld) f(i, d, (double)load_as_f32(src));
+                }
+            }
+        };
         double largest = 0.0;
-        for (int i = tid; i < n * items; i += kPrepareThreads) {
-            double u, v;
-            pair(t + i / items, i % items, u, v);
-            if (is_finite(u)) largest = fmax(largest, fabs(u));
-            if (is_finite(v)) largest = fmax(largest, fabs(v));
-        }
-        const float top = block_max((float)(largest / 127.0), scratch);
-        float* const scale_at = (keys ? a.k_scales : a.v_scales) + (size_t)page * a.kv_heads + h;
-        int8_t* const codes = (keys ? a.k_codes : a.v_codes) + ((size_t)page * a.kv_heads + h) * a.block * hd;
-        auto place = [&](int token, int d) { return keys ? ((d >> 4) * a.block + token) * 16 + (d & 15) : ((token >> 4) * hd + d) * 16 + (token & 15); };
-        const float before = at == 0 ? 0.0f : *scale_at, scale = fmaxf(top, before);
-        const double s = scale, inv = scale > 0.0f ? 1.0 / s : 0.0;
+        walk(false, [&](int, int, double v) { largest = fmax(largest, finite_size(v)); });
+        const float mine = warp_max((float)(largest / 127.0));
+        if ((tid & 31) == 0) s_top[tid >> 5] = mine;
+        float* const scale_at = (keys ? a.k_scales : a.v_scales) + (size_t)page * a.kv_heads + (live ? h : 0);
+        const float before = at == 0 ? 0.0f : *scale_at;
         __syncthreads();  // (all have read the scale)
-        if (tid == 0) *scale_at = scale;
-        if (scale > before && at > 0) {
-            for (int i = tid; i < at * hd; i += kPrepareThreads) {
-                int8_t* const c = codes + place(i / hd, i % hd);
-                *c = (int8_t)code_of((double)*c * (double)before, s, inv);
-            }
-        }
-        for (int i = tid; i < n * items; i += kPrepareThreads) {
-            double u, v;
-            const int d = i % items, token = at + i / items;
-            pair(t + i / items, d, u, v);
-            if (!(u == u)) u = 0.0;
-            if (!(v == v)) v = 0.0;
-            if (d < turned) {
-                codes[place(token, d)] = (int8_t)code_of(u, s, inv);
-                codes[place(token, d + turned)] = (int8_t)code_of(v, s, inv);
-            } else {
-                codes[place(token, d + turned)] = (int8_t)code_of(u, s, inv);
-            }
-        }
+        const float scale = fmaxf(before, fmaxf(s_top[2 * sub], s_top[2 * sub + 1]));
+        static_assert(kHeadThreads == 64, "two warps a head");
+        const double s = scale, inv = scale > 0.0f ? 1.0 / s : 0.0;
+        int8_t* const codes = (keys ? a.k_codes : a.v_codes) + ((size_t)page * a.kv_heads + (live ? h : 0)) * a.block * hd;
+        auto place = [&](int token, int d) { return keys ? ((d >> 4) * a.block + token) * 16 + (d & 15) : ((token >> 4) * hd + d) * 16 + (token & 15); };
+        if (live && lt == 0) *scale_at = scale;
+        if (live && scale > before && at > 0)
+            for (int d = lt; d < hd; d += kHeadThreads)
+                for (int i = 0; i < at; ++i) {
+                    int8_t* const c = codes + place(i, d);
+                    *c = (int8_t)code_of((double)*c * (double)before, s, inv);
+                }
+        walk(true, [&](int i, int d, double v) { codes[place(at + i, d)] = (int8_t)code_of(v == v ? v : 0.0, s, inv); });
         __syncthreads();
     }
 }
 
-// Rows of the cache as f32; slots outside of it leave their row as it is.
-__global__ void paged_cache_rows_kernel(const int8_t* k_codes, const float* k_scales, const int8_t* v_codes, const float* v_scales, int pages, int block, int kv_heads,
-                                        int head_dim, const int32_t* slots, int count, float* k, float* v) {
+// Rows of the cache as f32; slots outside of it leave their row as it is.  A block of threads has 16 entries of the list: of keys a thread reads 16
+// bytes (16 entries of a token), of values the 16 tokens of a column, again only where the list moves on to another group of 16.
+__global__ void __launch_bounds__(256) paged_cache_rows_kernel(const int8_t* k_codes, const float* k_scales, const int8_t* v_codes, const float* v_scales, int pages, int block,
+                                                               int kv_heads, int head_dim, const int32_t* slots, int count, float* k, float* v) {
+    __shared__ int s_slots[16];
+    const int tid = threadIdx.x, r0 = blockIdx.x * 16, n = min(16, count - r0), row_len = kv_heads * head_dim, units = head_dim / 16, limit = pages * block;
+    const int block_log = 31 - __clz(block);
     pdl_wait();
-    const int row_len = kv_heads * head_dim;
-    for (int r = blockIdx.x; r < count; r += gridDim.x) {
-        const int slot = slots[r];
-        if (slot < 0 || slot >= pages * block) continue;
-        const int page = slot / block, at = slot % block;
-        for (int i = threadIdx.x; i < row_len; i += blockDim.x) {
-            const int h = i / head_dim, d = i % head_dim;
-            const size_t ph = (size_t)page * kv_heads + h, base = ph * block * head_dim;
-            k[(size_t)r * row_len + i] = (float)k_codes[base + ((d >> 4) * block + at) * 16 + (d & 15)] * k_scales[ph];
-            v[(size_t)r * row_len + i] = (float)v_codes[base + ((at >> 4) * head_dim + d) * 16 + (at & 15)] * v_scales[ph];
+    if (tid < 16) s_slots[tid] = tid < n ? slots[r0 + tid] : -1;
+    __syncthreads();
+    const bool aligned = (reinterpret_cast<uintptr_t>(k) & 15u) == 0;
+    for (int i = tid; i < n * kv_heads * units; i += 256) {
+        const int r = i / (kv_heads * units), hc = i - r * kv_heads * units, h = hc / units, c = hc - h * units, slot = s_slots[r];
+        if (slot < 0 || slot >= limit) continue;
+        const size_t ph = (size_t)(slot >> block_log) * kv_heads + h;
+        const uint4 u = *reinterpret_cast<const uint4*>(k_codes + ph * block * head_dim + ((size_t)c * block + (slot & (block - 1))) * 16);
+        const float s = k_scales[ph];
+        float* const to = k + (size_t)(r0 + r) * row_len + h * head_dim + c * 16;
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const float4 y = make_float4((float)(int8_t)w[b] * s, (float)(int8_t)(w[b] >> 8) * s, (float)(int8_t)(w[b] >> 16) * s, (float)(int8_t)(w[b] >> 24) * s);
+            if (aligned) {
+                reinterpret_cast<float4*>(to)[b] = y;
+            } else {
+                to[4 * b] = y.x; to[4 * b + 1] = y.y; to[4 * b + 2] = y.z; to[4 * b + 3] = y.w;
+            }
+        }
+    }
+    for (int i = tid; i < row_len; i += 256) {
+        const int h = i / head_dim, d = i - h * head_dim;
+        uint4 u = make_uint4(0u, 0u, 0u, 0u);
+        float s = 0.0f;
+        int held = -1;
+        for (int r = 0; r < n; ++r) {
+            const int slot = s_slots[r];
+            if (slot < 0 || slot >= limit) continue;
+            if (slot >> 4 != held) {
+                held = slot >> 4;
+                const size_t ph = (size_t)(slot >> block_log) * kv_heads + h;
+                u = *reinterpret_cast<const uint4*>(v_codes + ph * block * head_dim + ((size_t)((slot & (block - 1)) >> 4) * head_dim + d) * 16);
+                s = v_scales[ph];
+            }
+            const uint32_t e = slot & 15, w = e < 4 ? u.x : e < 8 ? u.y : e < 12 ? u.z : u.w;
+            v[(size_t)(r0 + r) * row_len + i] = (float)(int8_t)(w >> (8 * (e & 3))) * s;
         }
     }
 }
@@ -445,12 +517,26 @@ extern "C" int kmll_prepare_paged_attention(kmll_stream_t stream, const void* qu
         KMLL_REQUIRE_PTR(freqs);
         KMLL_REQUIRE_PTR(positions);
     }
-    PrepareArgs a = {query, key, value, is_f32, (size_t)ld_query, (size_t)ld_key, (size_t)ld_value, freqs, n_freqs, positions, slots, tokens, heads, kv_heads, head_dim,
-                     query_rot, k_codes, v_codes, k_scales, v_scales, pages, block, 1};
-    if (tokens > 512) a.group = block;
-    const dim3 grid((tokens + a.group - 1) / a.group, 2 * kv_heads + heads);
-    const cudaError_t e = is_f32 ? launch(prepare_paged_kernel<float>, grid, dim3(kPrepareThreads), 0, as_stream(stream), true, a)
-                                 : launch(prepare_paged_kernel<uint16_t>, grid, dim3(kPrepareThreads), 0, as_stream(stream), true, a);
+    PrepareArgs a = {query, key, value, (size_t)ld_query, (size_t)ld_key, (size_t)ld_value, freqs, n_freqs, positions, slots, tokens, heads, kv_heads, head_dim,
+                     query_rot, k_codes, v_codes, k_scales, v_scales, pages, block};
+    // few tokens: each may begin a run; many: they come in pages, and one block of threads per page has no runs that begin elsewhere to step over
+    a.group = tokens <= 512 ? 1 : block;
+    a.groups = (tokens + a.group - 1) / a.group;
+    a.head_sets = (kv_heads + kHeadSet - 1) / kHeadSet;
+    a.q_tokens = tokens <= 512 ? 1 : 8;
+    const int per_token = n_freqs * (int)sizeof(double2);
+    a.table_tokens = per_token > 0 ? min(block, 96 * 1024 / per_token) : block;
+    const size_t table_bytes = (size_t)per_token * (tokens <= 512 && a.table_tokens > tokens ? tokens : a.table_tokens);
+    const long long blocks = 2ll * a.groups * a.head_sets + (heads > 0 ? (tokens + a.q_tokens - 1) / a.q_tokens : 0);
+    KMLL_REQUIRE(blocks <= INT_MAX, "prepare paged attention: too many rows");
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(query) | reinterpret_cast<uintptr_t>(query_rot);
+    const bool pairs = n_freqs % 2 == 0 && ld_query % 2 == 0 && bits % (is_f32 ? 8 : 4) == 0;
+    auto go = [&](auto kern) {
+        const cudaError_t e = allow_all_dynamic_smem(kern);
+        return e != cudaSuccess ? e : launch(kern, dim3((unsigned)blocks), dim3(kPrepareThreads), table_bytes, as_stream(stream), true, a);
+    };
+    const cudaError_t e = is_f32 ? pairs ? go(prepare_paged_kernel<float, 2>) : go(prepare_paged_kernel<float, 1>)
+                                 : pairs ? go(prepare_paged_kernel<uint16_t, 2>) : go(prepare_paged_kernel<uint16_t, 1>);
     if (e != cudaSuccess) return fail(KMLL_ERR_CUDA, "prepare paged attention: %s", cudaGetErrorString(e));
     return check_launch("prepare paged attention");
 }
@@ -463,7 +549,7 @@ extern "C" int kmll_paged_cache_rows(kmll_stream_t stream, const int8_t* k_codes
     KMLL_REQUIRE_PTR(slots);
     KMLL_REQUIRE_PTR(k);
     KMLL_REQUIRE_PTR(v);
-    const cudaError_t e = launch(paged_cache_rows_kernel, dim3(min(count, 8192)), dim3(256), 0, as_stream(stream), true, k_codes, k_scales, v_codes, v_scales, pages, block,
+    const cudaError_t e = launch(paged_cache_rows_kernel, dim3((count + 15) / 16), dim3(256), 0, as_stream(stream), true, k_codes, k_scales, v_codes, v_scales, pages, block,
                                  kv_heads, head_dim, slots, count, k, v);
     if (e != cudaSuccess) return fail(KMLL_ERR_CUDA, "paged cache rows: %s", cudaGetErrorString(e));
     return check_launch("paged cache rows");

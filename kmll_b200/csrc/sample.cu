@@ -2,10 +2,16 @@
 //
 // With the tokens in the order of their logits (the lower index first among equals) every filter keeps the first so many of them, so a set is told by
 // its weight alone, and the choice itself is one more search of the same kind: the first token at which the weight so far reaches a
-// target.  Nothing is sorted.  Weights exp((logit - largest) / temperature) are whole numbers of 2^-44: sums do not depend on an order, and
-// what is lost is below 2^-45 of the largest weight per token.  One pass fills a histogram of the weights over 2048 bins of equal
-// ratio; a search finds its bin there, collects the bin's tokens and ranks them (or splits the bin again while it holds too many).
+// target.  No row is sorted.  Weights exp((logit - largest) / temperature) are whole numbers of 2^-44: sums do not depend on an order, and
+// what is lost is below 2^-45 of the largest weight per token.
+//   1  the largest logit
+//   2  a histogram over 4096 bins of equal ratio, the highest logits first: with top-k of the tokens (no weights are needed), otherwise of the weights
+//   3  with top-k: the tokens of all bins up to the one in which the k-th lies are collected; one block ranks them by counting, sums their
+//      weights, cuts and chooses at once.  Otherwise each border (top-p, then the choice) is a search: its bin's tokens are
+//      collected and ranked; a bin of more than 1024 (flat rows, equal logits) is split until they are fewer.  A large k, or equals around the
+//      k-th, is a search by count.
 // A cluster of blocks has one row: every block a share of the tokens, block 0 the sums.
+// Bound: latency of the steps for few rows; for many the weights of step 2 (64-bit exponentials and shared-memory atomics, one per token).
 #include <cooperative_groups.h>
 
 #include <cfloat>
@@ -17,14 +23,14 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kSampleThreads = 1024;
-constexpr int kBins = 2048;
-constexpr int kList = 2048;          // tokens that are ranked at once
+constexpr int kBins = 4096, kSubBins = 1024;
+constexpr int kList = 1024;          // tokens that are ranked at once
 constexpr int kUnit = 44;            // weights are multiples of 2^-kUnit
-constexpr double kBinsPerFactor2 = (double)kBins / (kUnit + 1.5);
+constexpr float kBinsPerFactor2 = (float)kBins / (kUnit + 1.5f);  // tokens behind the last bin weigh less than half a unit
 
 struct SampleArgs {
     const void* logits;
-    int f32, vocab;
+    int vocab;
     size_t ld;
     const double* u;
     const float* temperature;
@@ -34,17 +40,25 @@ struct SampleArgs {
     float* logprobs;
 };
 
+struct SampleBins {  // of a row, in its block 0: tokens and weight of a bin, and of all bins in front of it
+    uint32_t *count, *count_before;
+    unsigned long long *weight, *before;
+};
 struct SampleShared {
-    uint32_t count[kBins], low[kBins], high[kBins];  // tokens; weight of the bin in two words
-    uint32_t sub_count[kBins], sub_low[kBins], sub_high[kBins];
-    unsigned long long before[kBins];                // block 0: weight in front of the bin
-    uint32_t count_before[kBins];
-    unsigned long long list[kList], sorted[kList];
+    uint32_t count[kBins], low[kBins], high[kBins];  // this block's: tokens; weight of the bin in two words
+    // block 0, of the row
+    uint32_t all_count[kBins], count_before[kBins];
+    unsigned long long all_weight[kBins], before[kBins];
+    uint32_t sub_count[kSubBins], sub_count_before[kSubBins];
+    unsigned long long sub_weight[kSubBins], sub_before[kSubBins];
+    unsigned long long list[kList], sorted[kList], sums[kList];
+    double powers[32];                               // 2^(j / 32)
     unsigned long long warp_sum[32];
+    uint32_t warp_count[32];
     unsigned long long least_sum;                    // weight at or above the min-p border
-    float top;
-    // block 0: what a search has found
-    int bin;
+    unsigned long long key_range[2];                 // of a bin's tokens in this block
+    float scratch[33], top;
+    int bin, overflow;
     uint32_t listed;
     unsigned long long base, low_key, high_key, found_key, found_sum;
 };
@@ -61,73 +75,163 @@ __device__ inline float key_logit(unsigned long long key) {
 __device__ inline uint32_t key_index(unsigned long long key) { return 0xffffffffu - (uint32_t)key; }
 
 struct Weigher {
-    double top, inv;  // largest logit, 1 / temperature
-    __device__ double exponent(float l) const { return l == top ? 0.0 : ((double)l - top) * inv; }
-    __device__ unsigned long long weight(double x) const { return (unsigned long long)rint(exp(x) * (double)(1ull << kUnit)); }
-    __device__ int bin(double x) const { return (int)fmin(-x * (1.4426950408889634 * kBinsPerFactor2), (double)kBins); }  // kBins: weighs nothing
+    float top, per_bin;  // largest logit; bins per unit of logit
+    double inv;          // 1 / temperature
+    const double* powers;
+    __device__ double exponent(float l) const { return l == top ? 0.0 : ((double)l - (double)top) * inv; }
+    // e^x = 2^(j / 32) * 2^n * e^r with 32 n + j the nearest whole number to 32 x / ln 2: Taylor's series in |r| <= ln 2 / 64, whose first term left
+    // out is below 2^-52
+    __device__ unsigned long long weight(double x) const {
+        constexpr double kLn2 = 0.693147180559945309;
+        const double y = fmax(x, -100.0) * (32.0 / kLn2), k = rint(y), r = (y - k) * (kLn2 / 32.0);
+        double p = 1.0 / 720.0;
+        p = fma(p, r, 1.0 / 120.0);
+        p = fma(p, r, 1.0 / 24.0);
+        p = fma(p, r, 1.0 / 6.0);
+        p = fma(p, r, 0.5);
+        p = fma(p, r, 1.0);
+        p = fma(p, r, 1.0);
+        const int i = (int)k;
+        const double e = p * powers[i & 31];
+        return (unsigned long long)rint(__hiloint2double(__double2hiint(e) + (kUnit + (i >> 5)) * (1 << 20), __double2loint(e)));
+    }
+    // monotone in the logit; kBins: weighs nothing
+    __device__ int bin(float l) const { return l == top ? 0 : (int)fminf((top - l) * per_bin, (float)kBins); }
 };
 __device__ inline void add_weight(uint32_t* low, uint32_t* high, unsigned long long w) {
     const uint32_t lo = (uint32_t)w, old = atomicAdd(low, lo), more = (uint32_t)(w >> 32) + (old + lo < old ? 1u : 0u);
     if (more != 0u) atomicAdd(high, more);
 }
 
-template <typename T>
-__device__ inline float logit_at(const T* row, int i);
-template <>
-__device__ inline float logit_at<float>(const float* row, int i) { return row[i]; }
-template <>
-__device__ inline float logit_at<uint16_t>(const uint16_t* row, int i) { return bf16_bits_to_f32(row[i]); }
+// Calls f(index, logit) for the block's share of a row, in 16-byte pieces.
+template <typename T, typename F>
+__device__ inline void each_logit(const T* row, int vocab, int rank, int blocks, F f) {
+    constexpr int N = 16 / (int)sizeof(T);
+    const int shift = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T)), pieces = (vocab + shift + N - 1) / N, share = (pieces + blocks - 1) / blocks;
+    const int end = min(pieces, (rank + 1) * share);
+#pragma unroll 2
+    for (int c = rank * share + (int)threadIdx.x; c < end; c += kSampleThreads) {
+        const int i0 = c * N - shift;
+        float x[N];
+        if (i0 >= 0 && i0 + N <= vocab) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + i0));
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] = __uint_as_float(sizeof(T) == 4 ? w[e & 3] : e & 1 ? w[e >> 1 & 3] & 0xffff0000u : w[e >> 1 & 3] << 16);
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const int i = i0 + e;
+                x[e] = i < 0 || i >= vocab ? -INFINITY : sizeof(T) == 4 ? reinterpret_cast<const float*>(row)[i] : __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(row)[i] << 16);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) f(i0 + e, x[e]);
+    }
+}
 
-// Sums in front of each of the kBins entries, from counts and two-word weights; all threads of block 0.
-__device__ inline void scan_bins(SampleShared& s, const uint32_t* count, const uint32_t* low, const uint32_t* high) {
-    static_assert(kBins == 2 * kSampleThreads, "two bins a thread");
+// Sums in front of each entry; all threads of block 0.
+template <int N>
+__device__ inline void scan_bins(SampleShared& s, const SampleBins& b) {
+    constexpr int E = N / kSampleThreads;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    unsigned long long w0 = ((unsigned long long)high[2 * tid] << 32) + low[2 * tid], w1 = ((unsigned long long)high[2 * tid + 1] << 32) + low[2 * tid + 1];
-    uint32_t c0 = count[2 * tid], c1 = count[2 * tid + 1];
-    unsigned long long w = w0 + w1;
-    uint32_t c = c0 + c1;
+    unsigned long long w = 0;
+    uint32_t c = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) { w += b.weight[E * tid + i]; c += b.count[E * tid + i]; }
+    const unsigned long long own_w = w;
+    const uint32_t own_c = c;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long a = __shfl_up_sync(0xffffffffu, w, o);
-        const uint32_t b = __shfl_up_sync(0xffffffffu, c, o);
-        if (lane >= o) { w += a; c += b; }
+        const unsigned long long x = __shfl_up_sync(0xffffffffu, w, o);
+        const uint32_t y = __shfl_up_sync(0xffffffffu, c, o);
+        if (lane >= o) { w += x; c += y; }
     }
-    __shared__ uint32_t warp_count[32];
-    if (lane == 31) { s.warp_sum[warp] = w; warp_count[warp] = c; }
+    if (lane == 31) { s.warp_sum[warp] = w; s.warp_count[warp] = c; }
     __syncthreads();
-    unsigned long long wb = 0;
-    uint32_t cb = 0;
-    for (int i = 0; i < warp; ++i) { wb += s.warp_sum[i]; cb += warp_count[i]; }
-    s.before[2 * tid] = wb + w - w0 - w1;
-    s.before[2 * tid + 1] = wb + w - w1;
-    s.count_before[2 * tid] = cb + c - c0 - c1;
-    s.count_before[2 * tid + 1] = cb + c - c1;
+    w -= own_w;
+    c -= own_c;
+    for (int i = 0; i < warp; ++i) { w += s.warp_sum[i]; c += s.warp_count[i]; }
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        b.before[E * tid + i] = w;
+        b.count_before[E * tid + i] = c;
+        w += b.weight[E * tid + i];
+        c += b.count[E * tid + i];
+    }
     __syncthreads();
 }
 
-// CL blocks per row.
+// The listed tokens in order (s.sorted), with the weight up to and with each (s.sums, counted from `sum`); all threads of block 0.
+__device__ inline void rank_list(SampleShared& s, const Weigher& weigh, uint32_t listed, unsigned long long sum) {
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    static_assert(kList == kSampleThreads, "a token a thread");
+    if (tid < listed) {
+        const unsigned long long key = s.list[tid];
+        uint32_t place = 0;
+#pragma unroll 8
+        for (uint32_t j = 0; j < listed; ++j) place += s.list[j] > key ? 1u : 0u;
+        s.sorted[place] = key;
+    }
+    __syncthreads();
+    unsigned long long w = tid < listed ? weigh.weight(weigh.exponent(key_logit(s.sorted[tid]))) : 0ull;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long v = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += v;
+    }
+    if (lane == 31) s.warp_sum[warp] = w;
+    __syncthreads();
+    for (uint32_t i = 0; i < warp; ++i) sum += s.warp_sum[i];
+    s.sums[tid] = sum + w;
+    __syncthreads();
+}
+// Number of the first ranked token at which the weight so far reaches `target` (the last one where none does); all threads of block 0 get it.
+__device__ inline uint32_t reach(SampleShared& s, uint32_t listed, unsigned long long target) {
+    if (threadIdx.x == 0) s.bin = (int)listed - 1;
+    __syncthreads();
+    const uint32_t i = threadIdx.x;
+    if (i < listed && s.sums[i] >= target && (i == 0 || s.sums[i - 1] < target)) s.bin = (int)i;
+    __syncthreads();
+    const uint32_t at = (uint32_t)s.bin;
+    __syncthreads();
+    return at;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kSampleThreads, 1) sample_rows_kernel(const SampleArgs a) {
-    extern __shared__ unsigned char sample_smem[];
+    extern __shared__ __align__(16) unsigned char sample_smem[];
     SampleShared& s = *reinterpret_cast<SampleShared*>(sample_smem);
     cg::cluster_group cluster = cg::this_cluster();
-    const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31;
     const int row = blockIdx.x / blocks;
     SampleShared& s0 = *cluster.map_shared_rank(&s, 0);
+    for (int i = tid; i < kBins; i += kSampleThreads) {
+        s.count[i] = s.low[i] = s.high[i] = s.all_count[i] = 0u;
+        s.all_weight[i] = 0ull;
+    }
+    const SampleBins bins = {s.all_count, s.count_before, s.all_weight, s.before}, subs = {s.sub_count, s.sub_count_before, s.sub_weight, s.sub_before};
+    if (tid < 32) s.powers[tid] = exp2((double)tid / 32.0);
+    if (tid == 0) {
+        s.least_sum = 0ull;
+        s.listed = 0u;
+        s.overflow = 0;
+    }
     pdl_wait();
     const T* const logits = static_cast<const T*>(a.logits) + (size_t)row * a.ld;
-    const int share = (a.vocab + blocks - 1) / blocks, i0 = rank * share, i1 = min(a.vocab, i0 + share);
+    auto each = [&](auto f) { each_logit(logits, a.vocab, rank, blocks, f); };
+    const float temperature = a.temperature != nullptr ? a.temperature[row] : 1.0f, least_p = a.min_p != nullptr ? a.min_p[row] : 0.0f;
+    const float top_p = a.top_p != nullptr ? a.top_p[row] : 1.0f;
+    const int k = a.top_k != nullptr ? a.top_k[row] : 0;
+    const double u = a.u[row];
     // ---- the largest logit (NaN and -infinity are tokens that are never taken)
     float top = -INFINITY;
-    for (int i = i0 + tid; i < i1; i += kSampleThreads) top = fmaxf(top, logit_at(logits, i));
-    __shared__ float scratch[33];
-    top = block_max(top, scratch);
+    each([&](int, float l) { top = fmaxf(top, l); });
+    top = block_max(top, s.scratch);
     if (tid == 0) s.top = top;
-    for (int i = tid; i < kBins; i += kSampleThreads) s.count[i] = s.low[i] = s.high[i] = 0u;
-    if (tid == 0) s.least_sum = 0ull;
     cluster.sync();
     for (int b = 0; b < blocks; ++b) top = fmaxf(top, cluster.map_shared_rank(&s, b)->top);
-    float temperature = a.temperature != nullptr ? a.temperature[row] : 1.0f;
+    top += 0.0f;  // (-0 is 0)
     if (top == -INFINITY) {  // nothing to choose from
         if (rank == 0 && tid == 0) {
             a.tokens[row] = -1;
@@ -137,208 +241,220 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_rows_kernel(const Sa
         return;
     }
     const bool greedy = !(temperature > FLT_EPSILON);
-    const Weigher weigh = {(double)top, greedy ? (double)INFINITY : 1.0 / (double)temperature};
-    const float least_p = a.min_p != nullptr ? a.min_p[row] : 0.0f;
+    const Weigher weigh = {top, greedy ? INFINITY : kBinsPerFactor2 * 1.442695041f / temperature, greedy ? (double)INFINITY : 1.0 / (double)temperature, s.powers};
     const double least = least_p > 0.0f ? log((double)fminf(least_p, 1.0f)) : -INFINITY;
-    // ---- weights into the bins
-    unsigned long long least_sum = 0ull;
-    for (int i = i0 + tid; i < i1; i += kSampleThreads) {
-        const float l = logit_at(logits, i);
-        if (!(l > -INFINITY)) continue;
-        const double x = weigh.exponent(l);
-        const int b = weigh.bin(x);
-        if (b >= kBins) continue;
-        const unsigned long long w = weigh.weight(x);
-        atomicAdd(&s.count[b], 1u);
-        add_weight(&s.low[b], &s.high[b], w);
-        if (x >= least) least_sum += w;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) least_sum += __shfl_xor_sync(0xffffffffu, least_sum, o);
-    if (lane == 0) atomicAdd(&s.least_sum, least_sum);
-    cluster.sync();
-    if (rank == 0) {
-        for (int b = 1; b < blocks; ++b) {
-            const SampleShared& o = *cluster.map_shared_rank(&s, b);
-            for (int i = tid; i < kBins; i += kSampleThreads) {
-                s.count[i] += o.count[i];
-                const unsigned long long w = (((unsigned long long)s.high[i] << 32) | s.low[i]) + (((unsigned long long)o.high[i] << 32) + o.low[i]);
-                s.low[i] = (uint32_t)w;
-                s.high[i] = (uint32_t)(w >> 32);
-            }
-            if (tid == 0) s.least_sum += o.least_sum;
-        }
+    const bool k_on = k > 0 && k < a.vocab, by_k = greedy || (k_on && k <= kList), large_k = !greedy && k_on && k > kList;
+    const int want_k = greedy ? 1 : k;
+
+    // this block's bins into those of the row, and back to zero
+    auto merge = [&](uint32_t* counts, unsigned long long* weights, int n) {
         __syncthreads();
+        for (int i = tid; i < n; i += kSampleThreads) {
+            const uint32_t c = s.count[i];
+            const unsigned long long w = ((unsigned long long)s.high[i] << 32) | s.low[i];
+            if (c != 0u) atomicAdd(&counts[i], c);
+            if (w != 0ull) atomicAdd(&weights[i], w);
+            s.count[i] = s.low[i] = s.high[i] = 0u;
+        }
+        cluster.sync();
+    };
+    // tokens that `take` names into the list of block 0 (which is empty)
+    auto collect = [&](auto take) {
+        each([&](int i, float l) {
+            if (!(l > -INFINITY) || !take(i, l)) return;
+            const uint32_t at = atomicAdd(&s0.listed, 1u);
+            if (at < (uint32_t)kList) s0.list[at] = token_key(l, (uint32_t)i);
+            else s0.overflow = 1;
+        });
+        cluster.sync();
+    };
+    // weight at or above the min-p border, and weights into the bins
+    auto weigh_all = [&](bool counts) {
+        unsigned long long least_sum = 0ull;
+        each([&](int, float l) {
+            if (!(l > -INFINITY)) return;
+            const int b = weigh.bin(l);
+            if (b >= kBins) return;
+            const double x = weigh.exponent(l);
+            const unsigned long long w = weigh.weight(x);
+            if (counts) atomicAdd(&s.count[b], 1u);
+            add_weight(&s.low[b], &s.high[b], w);
+            if (x >= least) least_sum += w;
+        });
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) least_sum += __shfl_xor_sync(0xffffffffu, least_sum, o);
+        if (lane == 0 && least_sum != 0ull) atomicAdd(&s0.least_sum, least_sum);
+        merge(s0.all_count, s0.all_weight, kBins);
+    };
+    auto target_of_u = [&](unsigned long long kept) {
+        const double at = floor((u > 0.0 ? u : 0.0) * (double)kept);
+        return at >= (double)kept ? kept : (unsigned long long)at + 1ull;
+    };
+    auto target_of_p = [&](unsigned long long whole) {
+        const double want = ceil((double)fmaxf(top_p, 0.0f) * (double)whole);
+        return min(whole, max(1ull, (unsigned long long)want));
+    };
+    auto answer = [&](unsigned long long key, unsigned long long kept) {
+        if (tid == 0) {
+            a.tokens[row] = (int32_t)key_index(key);
+            if (a.logprobs != nullptr) a.logprobs[row] = greedy ? 0.0f : (float)(weigh.exponent(key_logit(key)) - log((double)kept / (double)(1ull << kUnit)));
+        }
+    };
+
+    if (by_k) {
+        each([&](int, float l) {
+            if (!(l > -INFINITY)) return;
+            const int b = weigh.bin(l);
+            if (b < kBins) atomicAdd(&s.count[b], 1u);
+        });
+        merge(s0.all_count, s0.all_weight, kBins);
+        if (rank == 0) {
+            scan_bins<kBins>(s, bins);
+            const uint32_t tokens = s.count_before[kBins - 1] + s.all_count[kBins - 1], target = min((uint32_t)want_k, tokens);
+            for (int b = tid; b < kBins; b += kSampleThreads)
+                if (s.count_before[b] < target && s.count_before[b] + s.all_count[b] >= target) s.bin = b;
+        }
+        cluster.sync();
+        const int last = s0.bin;
+        collect([&](int, float l) { return weigh.bin(l) <= last; });
+        if (s0.overflow == 0) {
+            if (rank == 0) {
+                const uint32_t listed = s.listed, n = min(listed, (uint32_t)want_k);
+                rank_list(s, weigh, listed, 0ull);
+                unsigned long long kept = s.sums[n - 1];
+                if (top_p < 1.0f) kept = s.sums[reach(s, n, target_of_p(kept))];
+                if (least > -INFINITY) {
+                    const int heavy = __syncthreads_count((uint32_t)tid < n && weigh.exponent(key_logit(s.sorted[tid])) >= least);
+                    kept = min(kept, s.sums[heavy - 1]);
+                }
+                answer(s.sorted[reach(s, n, target_of_u(kept))], kept);
+            }
+            cluster.sync();
+            return;
+        }
+        cluster.sync();
     }
-    // ---- search: the first token, in order, at which the tokens (by_count) or the weight so far reach `target`
+    if (!greedy) weigh_all(large_k);
+    // the first token, in order, at which the tokens (by_count) or the weight so far reach `target`: its key (found_key), and the weight up to and with
+    // it (found_sum)
     auto search = [&](bool by_count, unsigned long long target) {
         if (rank == 0) {
-            scan_bins(s, s.count, s.low, s.high);
+            scan_bins<kBins>(s, bins);
             for (int b = tid; b < kBins; b += kSampleThreads) {
-                const unsigned long long before = by_count ? s.count_before[b] : s.before[b];
-                const unsigned long long after = before + (by_count ? s.count[b] : (((unsigned long long)s.high[b] << 32) | s.low[b]));
+                const unsigned long long before = by_count ? s.count_before[b] : s.before[b], after = before + (by_count ? s.all_count[b] : s.all_weight[b]);
                 if (before < target && after >= target) {
                     s.bin = b;
-                    s.listed = s.count[b];
                     s.base = before;
                     s.found_sum = s.before[b];
                 }
             }
-            __syncthreads();
-            // logits of the bin: the bin is monotone in the logit, so halving between keys finds both ends
-            if (tid < 2) {
-                const int b = s.bin;
-                const uint32_t highest = (uint32_t)(token_key((float)weigh.top, 0) >> 32);
-                uint32_t lo = 0x007fffffu, hi = highest;  // (below every finite logit; in bin 0)
-                // tid 0: the lowest key with bin <= b; tid 1: the highest key with bin >= b
-                while (hi - lo > 1) {
-                    const uint32_t mid = lo + (hi - lo) / 2;
-                    const float l = key_logit((unsigned long long)mid << 32);
-                    const int at = weigh.bin(weigh.exponent(l));
-                    if (tid == 0 ? at <= b : at < b) hi = mid;
-                    else lo = mid;
-                }
-                if (tid == 0) s.low_key = (unsigned long long)hi << 32;
-                else s.high_key = ((unsigned long long)(b == 0 ? highest : lo) << 32) | 0xffffffffull;
-            }
+            if (tid == 0) { s.listed = 0u; s.overflow = 0; }
         }
+        if (tid == 0) { s.key_range[0] = ~0ull; s.key_range[1] = 0ull; }
         cluster.sync();
-        // split while there are too many to rank
-        while (s0.listed > (uint32_t)kList) {
-            const unsigned long long low_key = s0.low_key, high_key = s0.high_key;
-            int shift = 0;
-            while (((high_key - low_key) >> shift) >= (unsigned long long)kBins) ++shift;
-            for (int i = tid; i < kBins; i += kSampleThreads) s.sub_count[i] = s.sub_low[i] = s.sub_high[i] = 0u;
-            __syncthreads();
-            for (int i = i0 + tid; i < i1; i += kSampleThreads) {
-                const float l = logit_at(logits, i);
-                if (!(l > -INFINITY)) continue;
+        const int bin = s0.bin;
+        collect([&](int, float l) { return weigh.bin(l) == bin; });
+        if (s0.overflow != 0) {
+            unsigned long long low_key = ~0ull, high_key = 0ull;
+            each([&](int i, float l) {
+                if (!(l > -INFINITY) || weigh.bin(l) != bin) return;
                 const unsigned long long key = token_key(l, (uint32_t)i);
-                if (key < low_key || key > high_key) continue;
-                const int b = (int)((high_key - key) >> shift);
-                atomicAdd(&s.sub_count[b], 1u);
-                add_weight(&s.sub_low[b], &s.sub_high[b], weigh.weight(weigh.exponent(l)));
+                low_key = min(low_key, key);
+                high_key = max(high_key, key);
+            });
+            if (high_key != 0ull) {
+                atomicMin(&s.key_range[0], low_key);
+                atomicMax(&s.key_range[1], high_key);
             }
             cluster.sync();
-            if (rank == 0) {
-                for (int b = 1; b < blocks; ++b) {
-                    const SampleShared& o = *cluster.map_shared_rank(&s, b);
-                    for (int i = tid; i < kBins; i += kSampleThreads) {
-                        s.sub_count[i] += o.sub_count[i];
-                        const unsigned long long w = (((unsigned long long)s.sub_high[i] << 32) | s.sub_low[i]) + (((unsigned long long)o.sub_high[i] << 32) + o.sub_low[i]);
-                        s.sub_low[i] = (uint32_t)w;
-                        s.sub_high[i] = (uint32_t)(w >> 32);
-                    }
-                }
-                __syncthreads();
-                scan_bins(s, s.sub_count, s.sub_low, s.sub_high);
-                const unsigned long long base = s.base, sum = s.found_sum;
-                __syncthreads();
-                for (int b = tid; b < kBins; b += kSampleThreads) {
-                    const unsigned long long before = base + (by_count ? s.count_before[b] : s.before[b]);
-                    const unsigned long long after = before + (by_count ? s.sub_count[b] : (((unsigned long long)s.sub_high[b] << 32) | s.sub_low[b]));
+            low_key = ~0ull;
+            high_key = 0ull;
+            for (int b = 0; b < blocks; ++b) {
+                const SampleShared& o = *cluster.map_shared_rank(&s, b);
+                low_key = min(low_key, o.key_range[0]);
+                high_key = max(high_key, o.key_range[1]);
+            }
+            // split: every round leaves one of kSubBins parts of the range, one key at the last
+            bool more = true;
+            while (more) {
+                int shift = 0;
+                while (((high_key - low_key) >> shift) >= (unsigned long long)kSubBins) ++shift;
+                if (rank == 0)
+                    for (int i = tid; i < kSubBins; i += kSampleThreads) { s.sub_count[i] = 0u; s.sub_weight[i] = 0ull; }
+                cluster.sync();
+                each([&](int i, float l) {
+                    if (!(l > -INFINITY)) return;
+                    const unsigned long long key = token_key(l, (uint32_t)i);
+                    if (key < low_key || key > high_key) return;
+                    const int b = (int)((high_key - key) >> shift);
+                    atomicAdd(&s.count[b], 1u);
+                    add_weight(&s.low[b], &s.high[b], weigh.weight(weigh.exponent(l)));
+                });
+                merge(s0.sub_count, s0.sub_weight, kSubBins);
+                if (rank == 0) {
+                    scan_bins<kSubBins>(s, subs);
+                    const unsigned long long base = s.base, sum = s.found_sum;
+                    __syncthreads();
+                    const unsigned long long before = base + (by_count ? s.sub_count_before[tid] : s.sub_before[tid]);
+                    const unsigned long long after = before + (by_count ? s.sub_count[tid] : s.sub_weight[tid]);
                     if (before < target && after >= target) {
-                        s.listed = s.sub_count[b];
+                        s.listed = s.sub_count[tid];
                         s.base = before;
-                        s.found_sum = sum + s.before[b];
-                        s.high_key = high_key - ((unsigned long long)b << shift);
-                        const unsigned long long reach = ((unsigned long long)(b + 1) << shift) - 1;
-                        s.low_key = reach > high_key - low_key ? low_key : high_key - reach;
+                        s.found_sum = sum + s.sub_before[tid];
+                        s.high_key = high_key - ((unsigned long long)tid << shift);
+                        const unsigned long long far = ((unsigned long long)(tid + 1) << shift) - 1;
+                        s.low_key = far > high_key - low_key ? low_key : high_key - far;
                     }
                 }
+                cluster.sync();
+                more = s0.listed > (uint32_t)kList;
+                low_key = s0.low_key;
+                high_key = s0.high_key;
+                cluster.sync();
             }
+            if (rank == 0 && tid == 0) { s.listed = 0u; s.overflow = 0; }
             cluster.sync();
+            collect([&](int i, float l) {
+                const unsigned long long key = token_key(l, (uint32_t)i);
+                return key >= low_key && key <= high_key;
+            });
         }
-        const uint32_t listed = s0.listed;
-        const unsigned long long low_key = s0.low_key, high_key = s0.high_key;
-        cluster.sync();
-        if (rank == 0 && tid == 0) s.listed = 0u;
-        cluster.sync();
-        for (int i = i0 + tid; i < i1; i += kSampleThreads) {
-            const float l = logit_at(logits, i);
-            if (!(l > -INFINITY)) continue;
-            const unsigned long long key = token_key(l, (uint32_t)i);
-            if (key >= low_key && key <= high_key) {
-                const uint32_t at = atomicAdd(&s0.listed, 1u);
-                if (at < (uint32_t)kList) s0.list[at] = key;
-            }
-        }
-        cluster.sync();
         if (rank == 0) {
-            for (uint32_t i = tid; i < listed; i += kSampleThreads) {
-                const unsigned long long key = s.list[i];
-                uint32_t place = 0;
-                for (uint32_t j = 0; j < listed; ++j) place += s.list[j] > key ? 1u : 0u;
-                s.sorted[place] = key;
+            const uint32_t listed = s.listed;
+            const unsigned long long base = s.base;
+            rank_list(s, weigh, listed, s.found_sum);
+            const uint32_t at = by_count ? min((uint32_t)(target - base), listed) - 1u : reach(s, listed, target);
+            if (tid == 0) {
+                s.found_key = s.sorted[at];
+                s.found_sum = s.sums[at];
             }
-            __syncthreads();
-            if (warp == 0) {
-                if (lane == 0) s.found_key = s.sorted[listed - 1];
-                __syncwarp();
-                unsigned long long sum = s.found_sum, reached = s.base;
-                for (uint32_t j0 = 0; j0 < listed; j0 += 32) {
-                    const uint32_t j = j0 + lane;
-                    const unsigned long long key = j < listed ? s.sorted[j] : 0ull;
-                    const unsigned long long w = j < listed ? weigh.weight(weigh.exponent(key_logit(key))) : 0ull;
-                    unsigned long long ws = w;
-#pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const unsigned long long v = __shfl_up_sync(0xffffffffu, ws, o);
-                        if (lane >= o) ws += v;
-                    }
-                    const unsigned long long at = reached + (by_count ? (unsigned long long)(lane + 1) : ws);
-                    const uint32_t hit = __ballot_sync(0xffffffffu, j < listed && at >= target);
-                    if (hit != 0u) {
-                        if (lane == __ffs(hit) - 1) {
-                            s.found_key = key;
-                            s.found_sum = sum + ws;
-                        }
-                        break;
-                    }
-                    const unsigned long long all = __shfl_sync(0xffffffffu, ws, 31);
-                    sum += all;
-                    reached += by_count ? 32ull : all;
-                }
-            }
-            __syncthreads();
         }
         cluster.sync();
     };
     if (greedy) {  // the first of the largest
         search(true, 1ull);
-        if (rank == 0 && tid == 0) {
-            a.tokens[row] = (int32_t)key_index(s.found_key);
-            if (a.logprobs != nullptr) a.logprobs[row] = 0.0f;
-        }
+        if (rank == 0) answer(s.found_key, 1ull);
         cluster.sync();
         return;
     }
-    if (rank == 0) scan_bins(s, s.count, s.low, s.high);
+    if (rank == 0) scan_bins<kBins>(s, bins);
     cluster.sync();
-    const int k = a.top_k != nullptr ? a.top_k[row] : 0;
-    const float top_p = a.top_p != nullptr ? a.top_p[row] : 1.0f;
-    const unsigned long long whole = s0.before[kBins - 1] + (((unsigned long long)s0.high[kBins - 1] << 32) | s0.low[kBins - 1]);
-    const unsigned long long tokens = s0.count_before[kBins - 1] + s0.count[kBins - 1], least_mass = s0.least_sum;
+    unsigned long long kept = s0.before[kBins - 1] + s0.all_weight[kBins - 1];
+    const unsigned long long tokens = s0.count_before[kBins - 1] + s0.all_count[kBins - 1], least_sum = s0.least_sum;
     cluster.sync();
-    unsigned long long kept = whole;
-    if (k > 0 && (unsigned long long)k < tokens) {
+    if (k_on && (unsigned long long)k < tokens) {  // (tokens are counted with top-k only)
         search(true, (unsigned long long)k);
         kept = s0.found_sum;
         cluster.sync();
     }
     if (top_p < 1.0f) {
-        const double want = ceil((double)fmaxf(top_p, 0.0f) * (double)kept);
-        search(false, min(kept, max(1ull, (unsigned long long)want)));
+        search(false, target_of_p(kept));
         kept = s0.found_sum;
         cluster.sync();
     }
-    kept = min(kept, least_mass);
-    const double u = a.u[row], at = floor((u > 0.0 ? u : 0.0) * (double)kept);
-    search(false, at >= (double)kept ? kept : (unsigned long long)at + 1ull);
-    if (rank == 0 && tid == 0) {
-        a.tokens[row] = (int32_t)key_index(s.found_key);
-        if (a.logprobs != nullptr) a.logprobs[row] = (float)(weigh.exponent(key_logit(s.found_key)) - log((double)kept / (double)(1ull << kUnit)));
-    }
+    kept = min(kept, least_sum);
+    search(false, target_of_u(kept));
+    if (rank == 0) answer(s.found_key, kept);
     cluster.sync();
 }
 
@@ -356,7 +472,8 @@ extern "C" int kmll_sample_rows(kmll_stream_t stream, const void* logits, int is
     KMLL_REQUIRE_PTR(logits);
     KMLL_REQUIRE_PTR(u);
     KMLL_REQUIRE_PTR(tokens);
-    const SampleArgs a = {logits, is_f32, vocab, (size_t)ld, u, temperature, top_k, top_p, min_p, tokens, logprobs};
+    KMLL_REQUIRE(reinterpret_cast<uintptr_t>(logits) % (is_f32 ? 4 : 2) == 0, "sample rows: logits are not aligned to their type");
+    const SampleArgs a = {logits, vocab, (size_t)ld, u, temperature, top_k, top_p, min_p, tokens, logprobs};
     const int cluster = rows <= 18 ? 8 : rows <= 37 ? 4 : rows <= 74 ? 2 : 1;
     auto go = [&](auto kern) {
         cudaError_t e = allow_all_dynamic_smem(kern);
