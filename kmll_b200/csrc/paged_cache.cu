@@ -226,35 +226,67 @@ template <>
 __device__ inline float load_as_f32<float>(const float* p) { return *p; }
 template <>
 __device__ inline float load_as_f32<uint16_t>(const uint16_t* p) { return bf16_bits_to_f32(*p); }
-__device__ inline float2 load_pair(const float* p) { return *reinterpret_cast<const float2*>(p); }
-__device__ inline float2 load_pair(const uint16_t* p) {
-    const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
-    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+// V entries that lie together (4: aligned to all of them)
+template <int V>
+__device__ inline void load_some(const float* p, float (&x)[V]) {
+    if constexpr (V == 4) {
+        const float4 u = *reinterpret_cast<const float4*>(p);
+        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+    } else {
+        x[0] = *p;
+    }
 }
-__device__ inline void store_one(float* p, float v) { *p = v; }
-__device__ inline void store_one(uint16_t* p, float v) { *p = f32_to_bf16_bits(v); }
-__device__ inline void store_pair(float* p, float x, float y) { *reinterpret_cast<float2*>(p) = make_float2(x, y); }
-__device__ inline void store_pair(uint16_t* p, float x, float y) { *reinterpret_cast<uint32_t*>(p) = f32_to_bf16_bits(x) | ((uint32_t)f32_to_bf16_bits(y) << 16); }
+template <int V>
+__device__ inline void load_some(const uint16_t* p, float (&x)[V]) {
+    if constexpr (V == 4) {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        x[0] = __uint_as_float(u.x << 16); x[1] = __uint_as_float(u.x & 0xffff0000u);
+        x[2] = __uint_as_float(u.y << 16); x[3] = __uint_as_float(u.y & 0xffff0000u);
+    } else {
+        x[0] = bf16_bits_to_f32(*p);
+    }
+}
+template <int V>
+__device__ inline void store_some(float* p, const float (&x)[V]) {
+    if constexpr (V == 4) *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    else *p = x[0];
+}
+template <int V>
+__device__ inline void store_some(uint16_t* p, const float (&x)[V]) {
+    if constexpr (V == 4) {
+        *reinterpret_cast<uint2*>(p) = make_uint2(f32_to_bf16_bits(x[0]) | ((uint32_t)f32_to_bf16_bits(x[1]) << 16), f32_to_bf16_bits(x[2]) | ((uint32_t)f32_to_bf16_bits(x[3]) << 16));
+    } else {
+        *p = f32_to_bf16_bits(x[0]);
+    }
+}
 
 // The nearest whole number to v * inv = v / scale, ties to even as the quotient itself has them: where the product is within its rounding
-// error of a tie the quotient decides.
+// error of a tie the quotient decides.  Adding 1.5 * 2^52 rounds to a whole number and leaves it in the low word.
 __device__ inline int code_of(double v, double scale, double inv) {
-    if (inv == 0.0) return 0;  // (a page of zeros)
-    const double t = v * inv, n = rint(t);
-    const double c = fabs(fabs(t - n) - 0.5) < 1e-9 ? rint(v / scale) : n;
-    return (int)fmin(fmax(c, -127.0), 127.0);
+    constexpr double kWhole = 6755399441055744.0;
+    double t = v * inv;
+    if (!(fabs(t) < 200.0)) return t > 0.0 && inv > 0.0 ? 127 : t < 0.0 && inv > 0.0 ? -127 : 0;  // (infinities; NaN, and a page of zeros: inv is 0)
+    if (fabs(fabs(t - ((t + kWhole) - kWhole)) - 0.5) < 1e-9) t = v / scale;
+    return min(max(__double2loint(t + kWhole), -127), 127);
+}
+// The same from an f32 value: 32 bits tell wherever no tie is near.
+__device__ inline int code_of(float v, double scale, double inv, float inv32) {
+    const float t = v * inv32, n = rintf(t);
+    if (fabsf(t) < 126.0f && fabsf(fabsf(t - n) - 0.5f) > 1e-4f) return (int)n;
+    return code_of((double)v, scale, inv);
 }
 // A value that is not finite must not spoil its page: an infinity takes the largest code, NaN counts as 0.
 __device__ inline double finite_size(double v) { return fabs(v) < 1e300 ? fabs(v) : 0.0; }
 
 constexpr int kPrepareThreads = 256;
-constexpr int kHeadSet = 4, kHeadThreads = kPrepareThreads / kHeadSet;  // kv heads of a block of threads; threads of one
+constexpr int kHeadSet = 2, kHeadThreads = kPrepareThreads / kHeadSet;  // kv heads of a block of threads; threads of one
 
 // Blocks of threads along x: keys (groups of tokens x sets of heads), values (the same), query rows.  A run is a stretch of tokens with ascending
-// slots in one page; the block whose tokens hold the first of a run takes all of it, so that a page's scale is known in one place.  A head has 64
-// threads, a thread the same entries of every token; the first walk over the run finds the largest magnitude, the second (out of L1 / L2) codes.
-// The angles of a token are computed once per block into shared memory, not for every head.  VEC: entries lie so that two load together.
-template <typename T, int VEC>
+// slots in one page; the block whose tokens hold the first of a run takes all of it, so that a page's scale is known in one place.  A head has 128
+// threads; the first walk over the run finds the largest magnitude, the second (out of L1 / L2) codes.  The angles of a token are computed
+// once per block into shared memory, not for every head.  Codes leave as words: four entries of a key, the sixteen tokens of a value's column.
+// V: entries that a thread loads together.
+template <typename T, int V>
 __global__ void __launch_bounds__(kPrepareThreads) prepare_paged_kernel(const PrepareArgs a) {
     extern __shared__ __align__(16) double2 table[];  // [token][n_freqs] sine, cosine
     __shared__ int s_slots[2 * 128 + 1];
@@ -264,34 +296,36 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_paged_kernel(const Pr
     const int kv_blocks = a.groups * a.head_sets;
     pdl_wait();
     if ((int)blockIdx.x >= 2 * kv_blocks) {
-        // ---- query rows: a warp has a row at a time
-        const int t0 = ((int)blockIdx.x - 2 * kv_blocks) * a.q_tokens, n = min(a.q_tokens, a.tokens - t0), lane = tid & 31, warp = tid >> 5;
+        // ---- query rows of q_tokens tokens: (head, V entries) over the threads, all tokens of a place in turn
+        const int t0 = ((int)blockIdx.x - 2 * kv_blocks) * a.q_tokens, n = min(a.q_tokens, a.tokens - t0), Q = half / V, rest = (hd - 2 * half) / V;
+        if (tid < n) s_slots[tid] = a.slots[t0 + tid];
         for (int i = tid; i < n * half; i += kPrepareThreads) table[i] = sin_cos((double)a.positions[t0 + i / half] * (double)a.freqs[i % half]);
         __syncthreads();
-        for (int t = 0; t < n; ++t) {
-            const int slot = a.slots[t0 + t];
-            if (slot < 0 || slot >= limit) continue;
-            const double2* const turn = table + t * half;
-            const T* const src = static_cast<const T*>(a.query) + (size_t)(t0 + t) * a.ldq;
-            T* const dst = static_cast<T*>(a.query_rot) + (size_t)(t0 + t) * a.heads * hd;
-#pragma unroll 2
-            for (int h = warp; h < a.heads; h += kPrepareThreads / 32) {
-                for (int d = lane * VEC; d < half; d += 32 * VEC) {
-                    const T* const at = src + h * hd + d;
-                    T* const to = dst + h * hd + d;
-                    if constexpr (VEC == 2) {
-                        const float2 u = load_pair(at), v = load_pair(at + half);
-                        const double2 s0 = turn[d], s1 = turn[d + 1];
-                        store_pair(to, (float)(u.x * s0.y - v.x * s0.x), (float)(u.y * s1.y - v.y * s1.x));
-                        store_pair(to + half, (float)(u.x * s0.x + v.x * s0.y), (float)(u.y * s1.x + v.y * s1.y));
-                    } else {
-                        const double u = load_as_f32(at), v = load_as_f32(at + half);
-                        const double2 s0 = turn[d];
-                        store_one(to, (float)(u * s0.y - v * s0.x));
-                        store_one(to + half, (float)(u * s0.x + v * s0.y));
-                    }
+        for (int i = tid; i < a.heads * (Q + rest); i += kPrepareThreads) {
+            const int h = i / (Q + rest), d = (i - h * (Q + rest)) * V;
+            const T* src = static_cast<const T*>(a.query) + (size_t)t0 * a.ldq + h * hd + d;
+            T* dst = static_cast<T*>(a.query_rot) + ((size_t)t0 * a.heads + h) * hd + d;
+#pragma unroll 4
+            for (int t = 0; t < n; ++t, src += a.ldq, dst += (size_t)a.heads * hd) {
+                if (s_slots[t] < 0 || s_slots[t] >= limit) continue;
+                float u[V], v[V];
+                if (d >= half) {  // (entries from 2 * n_freqs on)
+                    load_some<V>(src + half, u);
+                    store_some<V>(dst + half, u);
+                    continue;
                 }
-                for (int d = 2 * half + lane; d < hd; d += 32) dst[h * hd + d] = src[h * hd + d];
+                load_some<V>(src, u);
+                load_some<V>(src + half, v);
+                const double2* const turn = table + t * half + d;
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const double2 s = turn[e];
+                    const double x = u[e], y = v[e];
+                    u[e] = (float)(x * s.y - y * s.x);
+                    v[e] = (float)(x * s.x + y * s.y);
+                }
+                store_some<V>(dst, u);
+                store_some<V>(dst + half, v);
             }
         }
         return;
@@ -328,67 +362,141 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_paged_kernel(const Pr
             for (int i = tid; i < (i1 - i0) * turned; i += kPrepareThreads) table[i] = sin_cos((double)a.positions[t + i0 + i / turned] * (double)a.freqs[i % turned]);
             __syncthreads();
         };
-        // calls f(token of the run, entry, value) for this thread's entries, 64-bit turned values
-        auto walk = [&](bool again, auto f) {
-            for (int i0 = 0; i0 < n; i0 += a.table_tokens) {
-                const int i1 = min(n, i0 + a.table_tokens);
-                if (turned > 0 && !(again && kept)) angles(i0, i1);
+        // calls f(token of the run, entry, V values in 64 bits) for this thread's turned entries, and g(.., V values in 32 bits) for the others
+        auto walk = [&](bool again, auto f, auto g) {
+            for (int i0 = 0; i0 < n && turned > 0; i0 += a.table_tokens) {
+                const int i1 = min(n, i0 + a.table_tokens), Q = turned / V;
+                if (!(again && kept)) angles(i0, i1);
                 if (!live) continue;
-                for (int d = lt; d < turned; d += kHeadThreads) {
-                    const T* src = in + (size_t)(t + i0) * ld + d;
-                    const double2* turn = table + d;
-#pragma unroll 8
-                    for (int i = i0; i < i1; ++i, src += ld, turn += turned) {
-                        const double p = load_as_f32(src), q = load_as_f32(src + turned);
-                        const double2 sc = *turn;
-                        f(i, d, p * sc.y - q * sc.x);
-                        f(i, d + turned, p * sc.x + q * sc.y);
+#pragma unroll 2
+                for (int j = lt; j < (i1 - i0) * Q; j += kHeadThreads) {
+                    const int i = j / Q, d = (j - i * Q) * V;
+                    const T* const src = in + (size_t)(t + i0 + i) * ld + d;
+                    float x[V], y[V];
+                    load_some<V>(src, x);
+                    load_some<V>(src + turned, y);
+                    const double2* const turn = table + i * turned + d;
+                    double p[V], q[V];
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        const double2 sc = turn[e];
+                        p[e] = x[e] * sc.y - y[e] * sc.x;
+                        q[e] = x[e] * sc.x + y[e] * sc.y;
                     }
+                    f(i0 + i, d, p);
+                    f(i0 + i, d + turned, q);
                 }
-                for (int d = 2 * turned + lt; d < hd; d += kHeadThreads) {
-                    const T* src = in + (size_t)(t + i0) * ld + d;
-#pragma unroll 8
-                    for (int i = i0; i < i1; ++i, src += ld) f(i, d, (double)load_as_f32(src));
-                }
+            }
+            const int R = (hd - 2 * turned) / V;
+            if (!live || R == 0) return;
+#pragma unroll 4
+            for (int j = lt; j < n * R; j += kHeadThreads) {
+                const int i = j / R, d = 2 * turned + (j - i * R) * V;
+                float x[V];
+                load_some<V>(in + (size_t)(t + i) * ld + d, x);
+                g(i, d, x);
             }
         };
         double largest = 0.0;
-        walk(false, [&](int, int, double v) { largest = fmax(largest, finite_size(v)); });
-        const float mine = warp_max((float)(largest / 127.0));
+        float largest32 = 0.0f;
+        walk(false, [&](int, int, const double (&v)[V]) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) largest = fmax(largest, finite_size(v[e]));
+        }, [&](int, int, const float (&v)[V]) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) largest32 = fmaxf(largest32, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.0f);
+        });
+        const float mine = warp_max((float)(fmax(largest, (double)largest32) / 127.0));
         if ((tid & 31) == 0) s_top[tid >> 5] = mine;
         float* const scale_at = (keys ? a.k_scales : a.v_scales) + (size_t)page * a.kv_heads + (live ? h : 0);
         const float before = at == 0 ? 0.0f : *scale_at;
         __syncthreads();  // (all have read the scale)
-        const float scale = fmaxf(before, fmaxf(s_top[2 * sub], s_top[2 * sub + 1]));
-        static_assert(kHeadThreads == 64, "two warps a head");
+        float scale = before;
+#pragma unroll
+        for (int w = 0; w < kHeadThreads / 32; ++w) scale = fmaxf(scale, s_top[sub * (kHeadThreads / 32) + w]);
         const double s = scale, inv = scale > 0.0f ? 1.0 / s : 0.0;
+        const float inv32 = (float)inv;
         int8_t* const codes = (keys ? a.k_codes : a.v_codes) + ((size_t)page * a.kv_heads + (live ? h : 0)) * a.block * hd;
-        auto place = [&](int token, int d) { return keys ? ((d >> 4) * a.block + token) * 16 + (d & 15) : ((token >> 4) * hd + d) * 16 + (token & 15); };
         if (live && lt == 0) *scale_at = scale;
-        if (live && scale > before && at > 0)
-            for (int d = lt; d < hd; d += kHeadThreads)
-                for (int i = 0; i < at; ++i) {
-                    int8_t* const c = codes + place(i, d);
-                    *c = (int8_t)code_of((double)*c * (double)before, s, inv);
+        if (live && scale > before && at > 0) {
+            // the tokens in front of the run are coded again, four codes a word: whole words of a key; of a value's column those in front of the run
+            if (keys) {
+                for (int j = lt; j < at * (hd / 4); j += kHeadThreads) {
+                    const int i = j / (hd / 4), d = (j - i * (hd / 4)) * 4;
+                    char4* const c = reinterpret_cast<char4*>(codes + ((d >> 4) * a.block + i) * 16 + (d & 15));
+                    const char4 x = *c;
+                    *c = make_char4((signed char)code_of(x.x * (double)before, s, inv), (signed char)code_of(x.y * (double)before, s, inv),
+                                    (signed char)code_of(x.z * (double)before, s, inv), (signed char)code_of(x.w * (double)before, s, inv));
                 }
-        walk(true, [&](int i, int d, double v) { codes[place(at + i, d)] = (int8_t)code_of(v == v ? v : 0.0, s, inv); });
+            } else {
+                for (int j = lt; j < hd * ((at + 3) / 4); j += kHeadThreads) {
+                    const int i = j / hd * 4, d = j % hd;
+                    signed char* const c = reinterpret_cast<signed char*>(codes + ((i >> 4) * hd + d) * 16 + (i & 15));
+                    char4 x = *reinterpret_cast<char4*>(c);
+                    x.x = (signed char)code_of(x.x * (double)before, s, inv);
+                    if (i + 1 < at) x.y = (signed char)code_of(x.y * (double)before, s, inv);
+                    if (i + 2 < at) x.z = (signed char)code_of(x.z * (double)before, s, inv);
+                    if (i + 3 < at) x.w = (signed char)code_of(x.w * (double)before, s, inv);
+                    *reinterpret_cast<char4*>(c) = x;
+                }
+                __threadfence_block();
+            }
+        }
+        __syncthreads();  // (a word that holds codes of both is written above first)
+        if (keys) {
+            auto put = [&](int i, int d, const int (&c)[V]) {
+                int8_t* const to = codes + ((d >> 4) * a.block + at + i) * 16 + (d & 15);
+                if constexpr (V == 4) *reinterpret_cast<char4*>(to) = make_char4((signed char)c[0], (signed char)c[1], (signed char)c[2], (signed char)c[3]);
+                else *to = (int8_t)c[0];
+            };
+            walk(true, [&](int i, int d, const double (&v)[V]) {
+                int c[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) c[e] = code_of(v[e], s, inv);
+                put(i, d, c);
+            }, [&](int i, int d, const float (&v)[V]) {
+                int c[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) c[e] = code_of(v[e], s, inv, inv32);
+                put(i, d, c);
+            });
+        } else if (live) {
+            // groups of 16 tokens of a column: one 16-byte store where the run has all of them
+            const int g0 = at >> 4, g1 = (at + n - 1) >> 4;
+            for (int j = lt; j < (g1 - g0 + 1) * hd; j += kHeadThreads) {
+                const int g = g0 + j / hd, d = j % hd, i0 = g * 16 - at;  // token of the run at the group's first place
+                int8_t* const to = codes + ((size_t)g * hd + d) * 16;
+                if (i0 >= 0 && i0 + 16 <= n) {
+                    const T* src = in + (size_t)(t + i0) * ld + d;
+                    float x[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[e] = load_as_f32(src + (size_t)e * ld);
+                    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) w[e >> 2] |= (uint32_t)(code_of(x[e], s, inv, inv32) & 255) << (8 * (e & 3));
+                    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+                } else {
+                    for (int i = max(i0, 0); i < min(i0 + 16, n); ++i) to[i - i0] = (int8_t)code_of(load_as_f32(in + (size_t)(t + i) * ld + d), s, inv, inv32);
+                }
+            }
+        }
         __syncthreads();
     }
 }
 
-// Rows of the cache as f32; slots outside of it leave their row as it is.  A block of threads has 16 entries of the list: of keys a thread reads 16
-// bytes (16 entries of a token), of values the 16 tokens of a column, again only where the list moves on to another group of 16.
-__global__ void __launch_bounds__(256) paged_cache_rows_kernel(const int8_t* k_codes, const float* k_scales, const int8_t* v_codes, const float* v_scales, int pages, int block,
+// Rows of the cache as f32; slots outside of it leave their row as it is.  A block of threads has 16 entries of the list and one head: of keys a
+// thread reads 16 bytes (16 entries of a token), of values the 16 tokens of a column, again only where the list moves on to another group of 16.
+__global__ void __launch_bounds__(128) paged_cache_rows_kernel(const int8_t* k_codes, const float* k_scales, const int8_t* v_codes, const float* v_scales, int pages, int block,
                                                                int kv_heads, int head_dim, const int32_t* slots, int count, float* k, float* v) {
     __shared__ int s_slots[16];
-    const int tid = threadIdx.x, r0 = blockIdx.x * 16, n = min(16, count - r0), row_len = kv_heads * head_dim, units = head_dim / 16, limit = pages * block;
+    const int tid = threadIdx.x, r0 = blockIdx.x * 16, h = blockIdx.y, n = min(16, count - r0), row_len = kv_heads * head_dim, units = head_dim / 16, limit = pages * block;
     const int block_log = 31 - __clz(block);
     pdl_wait();
     if (tid < 16) s_slots[tid] = tid < n ? slots[r0 + tid] : -1;
     __syncthreads();
     const bool aligned = (reinterpret_cast<uintptr_t>(k) & 15u) == 0;
-    for (int i = tid; i < n * kv_heads * units; i += 256) {
-        const int r = i / (kv_heads * units), hc = i - r * kv_heads * units, h = hc / units, c = hc - h * units, slot = s_slots[r];
+    for (int i = tid; i < 16 * units; i += 128) {
+        const int r = i & 15, c = i >> 4, slot = s_slots[r];
         if (slot < 0 || slot >= limit) continue;
         const size_t ph = (size_t)(slot >> block_log) * kv_heads + h;
         const uint4 u = *reinterpret_cast<const uint4*>(k_codes + ph * block * head_dim + ((size_t)c * block + (slot & (block - 1))) * 16);
@@ -405,8 +513,7 @@ __global__ void __launch_bounds__(256) paged_cache_rows_kernel(const int8_t* k_c
             }
         }
     }
-    for (int i = tid; i < row_len; i += 256) {
-        const int h = i / head_dim, d = i - h * head_dim;
+    for (int d = tid; d < head_dim; d += 128) {
         uint4 u = make_uint4(0u, 0u, 0u, 0u);
         float s = 0.0f;
         int held = -1;
@@ -420,7 +527,7 @@ __global__ void __launch_bounds__(256) paged_cache_rows_kernel(const int8_t* k_c
                 s = v_scales[ph];
             }
             const uint32_t e = slot & 15, w = e < 4 ? u.x : e < 8 ? u.y : e < 12 ? u.z : u.w;
-            v[(size_t)(r0 + r) * row_len + i] = (float)(int8_t)(w >> (8 * (e & 3))) * s;
+            v[(size_t)(r0 + r) * row_len + h * head_dim + d] = (float)(int8_t)(w >> (8 * (e & 3))) * s;
         }
     }
 }
@@ -529,14 +636,14 @@ extern "C" int kmll_prepare_paged_attention(kmll_stream_t stream, const void* qu
     const size_t table_bytes = (size_t)per_token * (tokens <= 512 && a.table_tokens > tokens ? tokens : a.table_tokens);
     const long long blocks = 2ll * a.groups * a.head_sets + (heads > 0 ? (tokens + a.q_tokens - 1) / a.q_tokens : 0);
     KMLL_REQUIRE(blocks <= INT_MAX, "prepare paged attention: too many rows");
-    const uintptr_t bits = reinterpret_cast<uintptr_t>(query) | reinterpret_cast<uintptr_t>(query_rot);
-    const bool pairs = n_freqs % 2 == 0 && ld_query % 2 == 0 && bits % (is_f32 ? 8 : 4) == 0;
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(query) | reinterpret_cast<uintptr_t>(query_rot) | reinterpret_cast<uintptr_t>(key) | reinterpret_cast<uintptr_t>(value);
+    const bool fours = n_freqs % 4 == 0 && (ld_query | ld_key | ld_value) % 4 == 0 && bits % (is_f32 ? 16 : 8) == 0;
     auto go = [&](auto kern) {
         const cudaError_t e = allow_all_dynamic_smem(kern);
         return e != cudaSuccess ? e : launch(kern, dim3((unsigned)blocks), dim3(kPrepareThreads), table_bytes, as_stream(stream), true, a);
     };
-    const cudaError_t e = is_f32 ? pairs ? go(prepare_paged_kernel<float, 2>) : go(prepare_paged_kernel<float, 1>)
-                                 : pairs ? go(prepare_paged_kernel<uint16_t, 2>) : go(prepare_paged_kernel<uint16_t, 1>);
+    const cudaError_t e = is_f32 ? fours ? go(prepare_paged_kernel<float, 4>) : go(prepare_paged_kernel<float, 1>)
+                                 : fours ? go(prepare_paged_kernel<uint16_t, 4>) : go(prepare_paged_kernel<uint16_t, 1>);
     if (e != cudaSuccess) return fail(KMLL_ERR_CUDA, "prepare paged attention: %s", cudaGetErrorString(e));
     return check_launch("prepare paged attention");
 }
@@ -549,7 +656,7 @@ extern "C" int kmll_paged_cache_rows(kmll_stream_t stream, const int8_t* k_codes
     KMLL_REQUIRE_PTR(slots);
     KMLL_REQUIRE_PTR(k);
     KMLL_REQUIRE_PTR(v);
-    const cudaError_t e = launch(paged_cache_rows_kernel, dim3((count + 15) / 16), dim3(256), 0, as_stream(stream), true, k_codes, k_scales, v_codes, v_scales, pages, block,
+    const cudaError_t e = launch(paged_cache_rows_kernel, dim3((count + 15) / 16, kv_heads), dim3(128), 0, as_stream(stream), true, k_codes, k_scales, v_codes, v_scales, pages, block,
                                  kv_heads, head_dim, slots, count, k, v);
     if (e != cudaSuccess) return fail(KMLL_ERR_CUDA, "paged cache rows: %s", cudaGetErrorString(e));
     return check_launch("paged cache rows");
