@@ -6,6 +6,7 @@
 // operand rows of the 8-bit tensor-core instructions as they lie (a contraction runs along the bytes of a group), eight groups are 128
 // bytes without bank conflicts, and a page of a head is one run of block * head_dim bytes.
 #include <climits>
+#include <type_traits>
 
 #include "internal.cuh"
 #include "paged.cuh"
@@ -215,7 +216,7 @@ struct PrepareArgs {
     float *k_scales, *v_scales;
     int pages, block;
     int group, groups;      // tokens whose runs a block of threads takes, and how many such blocks for a set of heads
-    int head_sets;          // of kHeadSet kv heads
+    int head_sets;          // of HS kv heads
     int q_tokens;           // query rows' tokens of a block of threads
     int table_tokens;       // tokens whose angles fit into shared memory
 };
@@ -262,35 +263,72 @@ __device__ inline void store_some(uint16_t* p, const float (&x)[V]) {
 
 // The nearest whole number to v * inv = v / scale, ties to even as the quotient itself has them: where the product is within its rounding
 // error of a tie the quotient decides.  Adding 1.5 * 2^52 rounds to a whole number and leaves it in the low word.
-__device__ inline int code_of(double v, double scale, double inv) {
+__device__ __noinline__ int code_of(double v, double scale, double inv) {
     constexpr double kWhole = 6755399441055744.0;
     double t = v * inv;
     if (!(fabs(t) < 200.0)) return t > 0.0 && inv > 0.0 ? 127 : t < 0.0 && inv > 0.0 ? -127 : 0;  // (infinities; NaN, and a page of zeros: inv is 0)
     if (fabs(fabs(t - ((t + kWhole) - kWhole)) - 0.5) < 1e-9) t = v / scale;
     return min(max(__double2loint(t + kWhole), -127), 127);
 }
-// The same from an f32 value: 32 bits tell wherever no tie is near.
-__device__ inline int code_of(float v, double scale, double inv, float inv32) {
+// The same in 32 bits where they tell: v is an f32 value, or one that was turned in 32 bits (off by less than 2^-18 of the page's largest, that is
+// 1e-3 of a code); -1000 where a tie may be near or v is at the ends.
+__device__ inline int quick_code(float v, float inv32) {
     const float t = v * inv32, n = rintf(t);
-    if (fabsf(t) < 126.0f && fabsf(fabsf(t - n) - 0.5f) > 1e-4f) return (int)n;
-    return code_of((double)v, scale, inv);
+    return fabsf(t) < 126.0f && fabsf(fabsf(t - n) - 0.5f) > 1e-3f ? (int)n : -1000;
 }
+__device__ inline int code_of(float v, double scale, double inv, float inv32) {
+    const int c = quick_code(v, inv32);
+    return c != -1000 ? c : code_of((double)v, scale, inv);
+}
+// Sine and cosine of an angle as sums of two floats each (48 bits): the first ones turn in 32 bits, all of them in 64.
+struct Angle {
+    float sin, cos, sin_rest, cos_rest;
+    __device__ void set(double2 s) {
+        sin = (float)s.x;
+        cos = (float)s.y;
+        sin_rest = (float)(s.x - (double)sin);
+        cos_rest = (float)(s.y - (double)cos);
+    }
+    __device__ double first(float x, float y) const { return x * ((double)cos + cos_rest) - y * ((double)sin + sin_rest); }
+    __device__ double second(float x, float y) const { return x * ((double)sin + sin_rest) + y * ((double)cos + cos_rest); }
+};
 // A value that is not finite must not spoil its page: an infinity takes the largest code, NaN counts as 0.
 __device__ inline double finite_size(double v) { return fabs(v) < 1e300 ? fabs(v) : 0.0; }
 
 constexpr int kPrepareThreads = 256;
-constexpr int kHeadSet = 2, kHeadThreads = kPrepareThreads / kHeadSet;  // kv heads of a block of threads; threads of one
+
+// Angles of `tokens` positions, [token][freq]: a thread has a place, and steps on by whole blocks of threads without dividing.
+__device__ inline void put_angle(double2* to, double2 s) { *to = s; }
+__device__ inline void put_angle(Angle* to, double2 s) { to->set(s); }
+template <typename A>
+__device__ inline void fill_angles(A* table, const int32_t* positions, const float* freqs, int tokens, int n) {
+    if (n == 0) return;
+    int i = threadIdx.x / n, d = threadIdx.x - i * n;
+    const int by_i = kPrepareThreads / n, by_d = kPrepareThreads - by_i * n;
+    while (i < tokens) {
+        put_angle(table + i * n + d, sin_cos((double)positions[i] * (double)freqs[d]));
+        i += by_i;
+        d += by_d;
+        if (d >= n) { d -= n; ++i; }
+    }
+}
 
 // Blocks of threads along x: keys (groups of tokens x sets of heads), values (the same), query rows.  A run is a stretch of tokens with ascending
-// slots in one page; the block whose tokens hold the first of a run takes all of it, so that a page's scale is known in one place.  A head has 128
-// threads; the first walk over the run finds the largest magnitude, the second (out of L1 / L2) codes.  The angles of a token are computed
-// once per block into shared memory, not for every head.  Codes leave as words: four entries of a key, the sixteen tokens of a value's column.
+// slots in one page; the block whose tokens hold the first of a run takes all of it, so that a page's scale is known in one place.  A head has
+// 256 / HS threads; the first walk over the run finds the largest magnitude, the second (out of L1 / L2) codes.  The angles of a token are computed
+// once per block into shared memory, not for every head.  Keys are turned in 32 bits, and in 64 where that could make another code or another
+// largest magnitude: their codes are those of the 64-bit values.  Codes leave as words: four entries of a key, the sixteen tokens of a value's column.
 // V: entries that a thread loads together.
-template <typename T, int V>
+// HS: kv heads of a block of threads.
+template <typename T, int V, int HS>
 __global__ void __launch_bounds__(kPrepareThreads) prepare_paged_kernel(const PrepareArgs a) {
-    extern __shared__ __align__(16) double2 table[];  // [token][n_freqs] sine, cosine
+    extern __shared__ __align__(16) unsigned char prepare_smem[];  // [token][n_freqs] angles
+    double2* const table = reinterpret_cast<double2*>(prepare_smem);
+    Angle* const key_table = reinterpret_cast<Angle*>(prepare_smem);
+    constexpr int kHeadThreads = kPrepareThreads / HS;
     __shared__ int s_slots[2 * 128 + 1];
     __shared__ int s_run;
+    __shared__ uint32_t s_first[4];
     __shared__ float s_top[kPrepareThreads / 32];
     const int tid = threadIdx.x, hd = a.head_dim, half = a.n_freqs, limit = a.pages * a.block;
     const int kv_blocks = a.groups * a.head_sets;
@@ -299,7 +337,7 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_paged_kernel(const Pr
         // ---- query rows of q_tokens tokens: (head, V entries) over the threads, all tokens of a place in turn
         const int t0 = ((int)blockIdx.x - 2 * kv_blocks) * a.q_tokens, n = min(a.q_tokens, a.tokens - t0), Q = half / V, rest = (hd - 2 * half) / V;
         if (tid < n) s_slots[tid] = a.slots[t0 + tid];
-        for (int i = tid; i < n * half; i += kPrepareThreads) table[i] = sin_cos((double)a.positions[t0 + i / half] * (double)a.freqs[i % half]);
+        fill_angles(table, a.positions + t0, a.freqs, n, half);
         __syncthreads();
         for (int i = tid; i < a.heads * (Q + rest); i += kPrepareThreads) {
             const int h = i / (Q + rest), d = (i - h * (Q + rest)) * V;
@@ -332,7 +370,7 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_paged_kernel(const Pr
     }
     const bool keys = (int)blockIdx.x < kv_blocks;
     const int item = keys ? blockIdx.x : blockIdx.x - kv_blocks, set = item % a.head_sets, t0 = item / a.head_sets * a.group, t1 = min(a.tokens, t0 + a.group);
-    const int sub = tid / kHeadThreads, lt = tid % kHeadThreads, h = set * kHeadSet + sub;
+    const int sub = tid / kHeadThreads, lt = tid % kHeadThreads, h = set * HS + sub;
     const bool live = h < a.kv_heads;
     const T* const in = static_cast<const T*>(keys ? a.key : a.value) + (size_t)(live ? h : 0) * hd;
     const size_t ld = keys ? a.ldk : a.ldv;
@@ -343,12 +381,22 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_paged_kernel(const Pr
         s_slots[i] = t >= 0 && t < a.tokens ? a.slots[t] : INT_MIN;
     }
     __syncthreads();
-    for (int t = t0; t < t1; ++t) {
+    const int block_log = 31 - __clz(a.block);
+    if (tid < 128) {  // first tokens of runs, a bit each
+        bool first = false;
+        if (tid < t1 - t0) {
+            const int slot = s_slots[tid + 1];
+            first = slot >= 0 && slot < limit && ((slot & (a.block - 1)) == 0 || t0 + tid == 0 || s_slots[tid] != slot - 1);
+        }
+        const uint32_t bits = __ballot_sync(0xffffffffu, first);
+        if ((tid & 31) == 0) s_first[tid >> 5] = bits;
+    }
+    __syncthreads();
+    for (int word = 0; word < 4; ++word)
+    for (uint32_t bits = s_first[word]; bits != 0u; bits &= bits - 1u) {
+        const int t = t0 + word * 32 + __ffs(bits) - 1;
         const int* const slots = s_slots + (t - t0 + 1);
-        const int slot = slots[0];
-        if (slot < 0 || slot >= limit) continue;
-        const int at = slot % a.block, page = slot / a.block;
-        if (at != 0 && t > 0 && slots[-1] == slot - 1) continue;
+        const int slot = slots[0], at = slot & (a.block - 1), page = slot >> block_log;
         // ---- length of the run: up to the first token that does not follow
         if (tid == 0) s_run = min(a.block - at, a.tokens - t);
         __syncthreads();
@@ -359,10 +407,10 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_paged_kernel(const Pr
         const bool kept = n <= a.table_tokens;  // the angles of the whole run stay in shared memory
         auto angles = [&](int i0, int i1) {
             __syncthreads();
-            for (int i = tid; i < (i1 - i0) * turned; i += kPrepareThreads) table[i] = sin_cos((double)a.positions[t + i0 + i / turned] * (double)a.freqs[i % turned]);
+            fill_angles(key_table, a.positions + t + i0, a.freqs, i1 - i0, turned);
             __syncthreads();
         };
-        // calls f(token of the run, entry, V values in 64 bits) for this thread's turned entries, and g(.., V values in 32 bits) for the others
+        // calls f(token of the run, first entry, angles, the V pairs, the V turned pairs) for this thread's turned entries, and g(token, entry, V values) for the others
         auto walk = [&](bool again, auto f, auto g) {
             for (int i0 = 0; i0 < n && turned > 0; i0 += a.table_tokens) {
                 const int i1 = min(n, i0 + a.table_tokens), Q = turned / V;
@@ -372,19 +420,16 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_paged_kernel(const Pr
                 for (int j = lt; j < (i1 - i0) * Q; j += kHeadThreads) {
                     const int i = j / Q, d = (j - i * Q) * V;
                     const T* const src = in + (size_t)(t + i0 + i) * ld + d;
-                    float x[V], y[V];
+                    float x[V], y[V], p[V], q[V];
                     load_some<V>(src, x);
                     load_some<V>(src + turned, y);
-                    const double2* const turn = table + i * turned + d;
-                    double p[V], q[V];
+                    const Angle* const turn = key_table + i * turned + d;
 #pragma unroll
                     for (int e = 0; e < V; ++e) {
-                        const double2 sc = turn[e];
-                        p[e] = x[e] * sc.y - y[e] * sc.x;
-                        q[e] = x[e] * sc.x + y[e] * sc.y;
+                        p[e] = fmaf(x[e], turn[e].cos, -(y[e] * turn[e].sin));
+                        q[e] = fmaf(x[e], turn[e].sin, y[e] * turn[e].cos);
                     }
-                    f(i0 + i, d, p);
-                    f(i0 + i, d + turned, q);
+                    f(i0 + i, d, turn, x, y, p, q);
                 }
             }
             const int R = (hd - 2 * turned) / V;
@@ -397,16 +442,47 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_paged_kernel(const Pr
                 g(i, d, x);
             }
         };
-        double largest = 0.0;
+        using Some = const float (&)[V];
+        // ---- the largest magnitude, in 32 bits; of the turned keys those that may be it once more in 64
         float largest32 = 0.0f;
-        walk(false, [&](int, int, const double (&v)[V]) {
+        bool beyond = false;  // a pair whose 32-bit rotation overflows (its entries may be infinities themselves)
+        walk(false, [&](int, int, const Angle*, Some, Some, Some p, Some q) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) largest = fmax(largest, finite_size(v[e]));
-        }, [&](int, int, const float (&v)[V]) {
+            for (int e = 0; e < V; ++e) {
+                const float size = fmaxf(fabsf(p[e]), fabsf(q[e]));
+                beyond = beyond || !(fabsf(p[e]) < INFINITY) || !(fabsf(q[e]) < INFINITY);
+                if (size < INFINITY) largest32 = fmaxf(largest32, size);
+            }
+        }, [&](int, int, Some v) {
 #pragma unroll
             for (int e = 0; e < V; ++e) largest32 = fmaxf(largest32, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.0f);
         });
-        const float mine = warp_max((float)(fmax(largest, (double)largest32) / 127.0));
+        double largest = largest32;
+        if (keys && turned > 0) {
+            const float own = largest32;
+            const float mine = warp_max(own);
+            if ((tid & 31) == 0) s_top[tid >> 5] = mine;
+            const bool all = __syncthreads_or(beyond) != 0;
+            float most = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kHeadThreads / 32; ++w) most = fmaxf(most, s_top[sub * (kHeadThreads / 32) + w]);
+            const float near = all ? 0.0f : most * (1.0f - 0x1p-18f);
+            largest = 0.0;
+            // (few threads have such entries; one that has none of its own goes along where the angles are not all there)
+            const bool mine_too = own >= near;
+            walk(true, [&](int, int, const Angle* turn, Some x, Some y, Some p, Some q) {
+                if (!mine_too) return;
+#pragma unroll 1
+                for (int e = 0; e < V; ++e)
+                    if (all || fmaxf(fabsf(p[e]), fabsf(q[e])) >= near) largest = fmax(largest, fmax(finite_size(turn[e].first(x[e], y[e])), finite_size(turn[e].second(x[e], y[e]))));
+            }, [&](int, int, Some v) {
+                if (!mine_too) return;
+#pragma unroll
+                for (int e = 0; e < V; ++e) largest = fmax(largest, finite_size((double)v[e]));
+            });
+            __syncthreads();  // (s_top is written again)
+        }
+        const float mine = warp_max((float)(largest / 127.0));
         if ((tid & 31) == 0) s_top[tid >> 5] = mine;
         float* const scale_at = (keys ? a.k_scales : a.v_scales) + (size_t)page * a.kv_heads + (live ? h : 0);
         const float before = at == 0 ? 0.0f : *scale_at;
@@ -449,12 +525,21 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_paged_kernel(const Pr
                 if constexpr (V == 4) *reinterpret_cast<char4*>(to) = make_char4((signed char)c[0], (signed char)c[1], (signed char)c[2], (signed char)c[3]);
                 else *to = (int8_t)c[0];
             };
-            walk(true, [&](int i, int d, const double (&v)[V]) {
-                int c[V];
+            walk(true, [&](int i, int d, const Angle* turn, Some x, Some y, Some p, Some q) {
+                int c[2][V];
 #pragma unroll
-                for (int e = 0; e < V; ++e) c[e] = code_of(v[e], s, inv);
-                put(i, d, c);
-            }, [&](int i, int d, const float (&v)[V]) {
+                for (int e = 0; e < V; ++e) {
+                    c[0][e] = quick_code(p[e], inv32);
+                    c[1][e] = quick_code(q[e], inv32);
+                }
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    if (c[0][e] == -1000) c[0][e] = code_of(turn[e].first(x[e], y[e]), s, inv);
+                    if (c[1][e] == -1000) c[1][e] = code_of(turn[e].second(x[e], y[e]), s, inv);
+                }
+                put(i, d, c[0]);
+                put(i, d + turned, c[1]);
+            }, [&](int i, int d, Some v) {
                 int c[V];
 #pragma unroll
                 for (int e = 0; e < V; ++e) c[e] = code_of(v[e], s, inv, inv32);
@@ -610,7 +695,7 @@ extern "C" int kmll_prepare_paged_attention(kmll_stream_t stream, const void* qu
     KMLL_TRY_RC(check_paged_cache("prepare paged attention", k_codes, k_scales, v_codes, v_scales, pages, block, kv_heads, head_dim));
     KMLL_REQUIRE(heads >= 0 && heads <= 4096, "prepare paged attention: %d query heads", heads);
     KMLL_REQUIRE(n_freqs >= 0 && 2 * n_freqs <= head_dim, "prepare paged attention: frequency count %d exceeds half the head size %d", n_freqs, head_dim);
-    KMLL_REQUIRE(query_rot != query || ld_query == heads * head_dim || tokens <= 1, "prepare paged attention: rows that do not lie together cannot turn in place");
+    KMLL_REQUIRE(heads == 0 || query_rot != query || ld_query == heads * head_dim || tokens <= 1, "prepare paged attention: rows that do not lie together cannot turn in place");
     KMLL_REQUIRE(ld_query >= heads * head_dim && ld_key >= kv_heads * head_dim && ld_value >= kv_heads * head_dim, "prepare paged attention: rows overlap");
     if (tokens == 0) return KMLL_OK;
     KMLL_REQUIRE_PTR(key);
@@ -629,11 +714,14 @@ extern "C" int kmll_prepare_paged_attention(kmll_stream_t stream, const void* qu
     // few tokens: each may begin a run; many: they come in pages, and one block of threads per page has no runs that begin elsewhere to step over
     a.group = tokens <= 512 ? 1 : block;
     a.groups = (tokens + a.group - 1) / a.group;
-    a.head_sets = (kv_heads + kHeadSet - 1) / kHeadSet;
+    const int head_set = tokens <= 512 ? 4 : 1;  // (a page of tokens is work for 256 threads, single tokens are not)
+    a.head_sets = (kv_heads + head_set - 1) / head_set;
     a.q_tokens = tokens <= 512 ? 1 : 8;
     const int per_token = n_freqs * (int)sizeof(double2);
-    a.table_tokens = per_token > 0 ? min(block, 96 * 1024 / per_token) : block;
-    const size_t table_bytes = (size_t)per_token * (tokens <= 512 && a.table_tokens > tokens ? tokens : a.table_tokens);
+    a.table_tokens = per_token > 0 ? min(block, 128 * 1024 / per_token) : block;
+    const int key_tokens = min(tokens, a.table_tokens);
+    static_assert(sizeof(Angle) == sizeof(double2), "either table");
+    const size_t table_bytes = (size_t)per_token * max(key_tokens, a.q_tokens);
     const long long blocks = 2ll * a.groups * a.head_sets + (heads > 0 ? (tokens + a.q_tokens - 1) / a.q_tokens : 0);
     KMLL_REQUIRE(blocks <= INT_MAX, "prepare paged attention: too many rows");
     const uintptr_t bits = reinterpret_cast<uintptr_t>(query) | reinterpret_cast<uintptr_t>(query_rot) | reinterpret_cast<uintptr_t>(key) | reinterpret_cast<uintptr_t>(value);
@@ -642,8 +730,12 @@ extern "C" int kmll_prepare_paged_attention(kmll_stream_t stream, const void* qu
         const cudaError_t e = allow_all_dynamic_smem(kern);
         return e != cudaSuccess ? e : launch(kern, dim3((unsigned)blocks), dim3(kPrepareThreads), table_bytes, as_stream(stream), true, a);
     };
-    const cudaError_t e = is_f32 ? fours ? go(prepare_paged_kernel<float, 4>) : go(prepare_paged_kernel<float, 1>)
-                                 : fours ? go(prepare_paged_kernel<uint16_t, 4>) : go(prepare_paged_kernel<uint16_t, 1>);
+    auto pick = [&](auto hs) {
+        constexpr int HS = decltype(hs)::value;
+        return is_f32 ? fours ? go(prepare_paged_kernel<float, 4, HS>) : go(prepare_paged_kernel<float, 1, HS>)
+                      : fours ? go(prepare_paged_kernel<uint16_t, 4, HS>) : go(prepare_paged_kernel<uint16_t, 1, HS>);
+    };
+    const cudaError_t e = head_set == 4 ? pick(std::integral_constant<int, 4>()) : pick(std::integral_constant<int, 1>());
     if (e != cudaSuccess) return fail(KMLL_ERR_CUDA, "prepare paged attention: %s", cudaGetErrorString(e));
     return check_launch("prepare paged attention");
 }

@@ -232,6 +232,15 @@ def test_ties_of_codes_go_to_even(cuda):
     assert cache.k_codes[0, 0, 0, 0].tolist() == [64, 0, 1, 1, 0, -1, 32, 32, 63, 0, 0, 2, 0, 0, 0, 0] and cache.k_scales.item() == 2.0
 
 
+def test_keys_and_values_without_queries(cuda):
+    cache, ks = ops.DevicePagedI8Cache.create(2, 16, 2, 32), po.Store(2, 16, 2, 32)
+    x = torch.randn(5, 4, 32, generator=torch.Generator("cuda").manual_seed(2), device="cuda")
+    none = x[:, :0]
+    ops.prepare_paged_attention(none, x[:, :2], x[:, 2:], torch.tensor(freqs_of(16, 32), device="cuda"), ints(range(5)), ints(range(16, 21)), cache, query_rot=none)
+    ks.append(po.rotate(f64(x[:, :2]), range(5), freqs_of(16, 32)), list(range(16, 21)))
+    np.testing.assert_array_equal(cache.k_codes.cpu().numpy(), po.key_layout(ks.codes))
+
+
 def test_rows_outside_the_cache_are_left_as_they_were(cuda):
     cache = ops.DevicePagedI8Cache.create(2, 16, 1, 32)
     x = torch.ones(3, 1, 32, device="cuda")
