@@ -25,8 +25,20 @@ template <>
 __device__ inline float row_entry<float>(const void* p, size_t i) { return static_cast<const float*>(p)[i]; }
 template <>
 __device__ inline float row_entry<uint16_t>(const void* p, size_t i) { return bf16_bits_to_f32(static_cast<const uint16_t*>(p)[i]); }
+// To the nearest bf16, ties to even, and NaN stays NaN (f32_to_bf16_bits, kmll's rule for weights, carries the NaN of the arithmetic units over
+// into the sign).
+__device__ inline uint16_t bf16_of(float v) {
+    uint16_t b;
+    asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(b) : "f"(v));
+    return b;
+}
+__device__ inline uint32_t bf16_pair_of(float x, float y) {
+    uint32_t b;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b) : "f"(y), "f"(x));
+    return b;
+}
 __device__ inline void store_row(float* p, float v) { *p = v; }
-__device__ inline void store_row(uint16_t* p, float v) { *p = f32_to_bf16_bits(v); }
+__device__ inline void store_row(uint16_t* p, float v) { *p = bf16_of(v); }
 
 // A request's rows and the positions they attend together.
 struct PagedRequest {

@@ -255,9 +255,9 @@ __device__ inline void store_some(float* p, const float (&x)[V]) {
 template <int V>
 __device__ inline void store_some(uint16_t* p, const float (&x)[V]) {
     if constexpr (V == 4) {
-        *reinterpret_cast<uint2*>(p) = make_uint2(f32_to_bf16_bits(x[0]) | ((uint32_t)f32_to_bf16_bits(x[1]) << 16), f32_to_bf16_bits(x[2]) | ((uint32_t)f32_to_bf16_bits(x[3]) << 16));
+        *reinterpret_cast<uint2*>(p) = make_uint2(bf16_pair_of(x[0], x[1]), bf16_pair_of(x[2], x[3]));
     } else {
-        *p = f32_to_bf16_bits(x[0]);
+        *p = bf16_of(x[0]);
     }
 }
 
@@ -270,11 +270,11 @@ __device__ __noinline__ int code_of(double v, double scale, double inv) {
     if (fabs(fabs(t - ((t + kWhole) - kWhole)) - 0.5) < 1e-9) t = v / scale;
     return min(max(__double2loint(t + kWhole), -127), 127);
 }
-// The same in 32 bits where they tell: v is an f32 value, or one that was turned in 32 bits (off by less than 2^-18 of the page's largest, that is
-// 1e-3 of a code); -1000 where a tie may be near or v is at the ends.
+// The same in 32 bits where they tell: v is an f32 value (v * inv32 is off by 2e-5 of a code) or one that was turned in 32 bits (off by 4e-7 of the
+// page's largest: 1e-4 of a code with it); -1000 where a tie may be near or v is at the ends.
 __device__ inline int quick_code(float v, float inv32) {
     const float t = v * inv32, n = rintf(t);
-    return fabsf(t) < 126.0f && fabsf(fabsf(t - n) - 0.5f) > 1e-3f ? (int)n : -1000;
+    return fabsf(t) < 126.0f && fabsf(fabsf(t - n) - 0.5f) > 2.5e-4f ? (int)n : -1000;
 }
 __device__ inline int code_of(float v, double scale, double inv, float inv32) {
     const int c = quick_code(v, inv32);
@@ -297,19 +297,33 @@ __device__ inline double finite_size(double v) { return fabs(v) < 1e300 ? fabs(v
 
 constexpr int kPrepareThreads = 256;
 
-// Angles of `tokens` positions, [token][freq]: a thread has a place, and steps on by whole blocks of threads without dividing.
+// Angles of `tokens` positions, [token][freq].  A thread has a frequency and kSteps tokens; where their positions follow one another it computes the first
+// angle and turns on by one frequency at a time (in 64 bits: kSteps roundings).  It steps through its places without dividing.
 __device__ inline void put_angle(double2* to, double2 s) { *to = s; }
 __device__ inline void put_angle(Angle* to, double2 s) { to->set(s); }
-template <typename A>
+template <int kSteps, typename A>
 __device__ inline void fill_angles(A* table, const int32_t* positions, const float* freqs, int tokens, int n) {
     if (n == 0) return;
-    int i = threadIdx.x / n, d = threadIdx.x - i * n;
-    const int by_i = kPrepareThreads / n, by_d = kPrepareThreads - by_i * n;
-    while (i < tokens) {
-        put_angle(table + i * n + d, sin_cos((double)positions[i] * (double)freqs[d]));
-        i += by_i;
+    int c = threadIdx.x / n, d = threadIdx.x - c * n;
+    const int by_c = kPrepareThreads / n, by_d = kPrepareThreads - by_c * n;
+    while (c * kSteps < tokens) {
+        const int i0 = c * kSteps, m = min(kSteps, tokens - i0);
+        const double f = freqs[d];
+        const int first = positions[i0];
+        bool follow = m > 1;
+#pragma unroll
+        for (int i = 1; i < kSteps; ++i) follow = follow && (i >= m || positions[i0 + i] == first + i);
+        double2 s = sin_cos((double)first * f);
+        put_angle(table + i0 * n + d, s);
+        const double2 step = follow ? sin_cos(f) : make_double2(0.0, 1.0);
+        for (int i = 1; i < m; ++i) {
+            if (follow) s = make_double2(s.x * step.y + s.y * step.x, s.y * step.y - s.x * step.x);
+            else s = sin_cos((double)positions[i0 + i] * f);
+            put_angle(table + (i0 + i) * n + d, s);
+        }
+        c += by_c;
         d += by_d;
-        if (d >= n) { d -= n; ++i; }
+        if (d >= n) { d -= n; ++c; }
     }
 }
 
@@ -337,7 +351,7 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_paged_kernel(const Pr
         // ---- query rows of q_tokens tokens: (head, V entries) over the threads, all tokens of a place in turn
         const int t0 = ((int)blockIdx.x - 2 * kv_blocks) * a.q_tokens, n = min(a.q_tokens, a.tokens - t0), Q = half / V, rest = (hd - 2 * half) / V;
         if (tid < n) s_slots[tid] = a.slots[t0 + tid];
-        fill_angles(table, a.positions + t0, a.freqs, n, half);
+        fill_angles<4>(table, a.positions + t0, a.freqs, n, half);
         __syncthreads();
         for (int i = tid; i < a.heads * (Q + rest); i += kPrepareThreads) {
             const int h = i / (Q + rest), d = (i - h * (Q + rest)) * V;
@@ -407,7 +421,7 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_paged_kernel(const Pr
         const bool kept = n <= a.table_tokens;  // the angles of the whole run stay in shared memory
         auto angles = [&](int i0, int i1) {
             __syncthreads();
-            fill_angles(key_table, a.positions + t + i0, a.freqs, i1 - i0, turned);
+            fill_angles<16>(key_table, a.positions + t + i0, a.freqs, i1 - i0, turned);
             __syncthreads();
         };
         // calls f(token of the run, first entry, angles, the V pairs, the V turned pairs) for this thread's turned entries, and g(token, entry, V values) for the others
@@ -443,12 +457,18 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_paged_kernel(const Pr
             }
         };
         using Some = const float (&)[V];
-        // ---- the largest magnitude, in 32 bits; of the turned keys those that may be it once more in 64
+        // ---- the largest magnitude, in 32 bits; of the turned keys those that may be it once more in 64 (of few tokens all at once: a walk less)
+        constexpr bool kAtOnce = HS > 1;
+        double largest = 0.0;
         float largest32 = 0.0f;
         bool beyond = false;  // a pair whose 32-bit rotation overflows (its entries may be infinities themselves)
-        walk(false, [&](int, int, const Angle*, Some, Some, Some p, Some q) {
+        walk(false, [&](int, int, const Angle* turn, Some x, Some y, Some p, Some q) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
+                if constexpr (kAtOnce) {
+                    largest = fmax(largest, fmax(finite_size(turn[e].first(x[e], y[e])), finite_size(turn[e].second(x[e], y[e]))));
+                    continue;
+                }
                 const float size = fmaxf(fabsf(p[e]), fabsf(q[e]));
                 beyond = beyond || !(fabsf(p[e]) < INFINITY) || !(fabsf(q[e]) < INFINITY);
                 if (size < INFINITY) largest32 = fmaxf(largest32, size);
@@ -457,8 +477,9 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_paged_kernel(const Pr
 #pragma unroll
             for (int e = 0; e < V; ++e) largest32 = fmaxf(largest32, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.0f);
         });
-        double largest = largest32;
-        if (keys && turned > 0) {
+        if (kAtOnce || turned == 0) {
+            largest = fmax(largest, (double)largest32);
+        } else {
             const float own = largest32;
             const float mine = warp_max(own);
             if ((tid & 31) == 0) s_top[tid >> 5] = mine;
@@ -467,10 +488,9 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_paged_kernel(const Pr
 #pragma unroll
             for (int w = 0; w < kHeadThreads / 32; ++w) most = fmaxf(most, s_top[sub * (kHeadThreads / 32) + w]);
             const float near = all ? 0.0f : most * (1.0f - 0x1p-18f);
-            largest = 0.0;
             // (few threads have such entries; one that has none of its own goes along where the angles are not all there)
             const bool mine_too = own >= near;
-            walk(true, [&](int, int, const Angle* turn, Some x, Some y, Some p, Some q) {
+            if (!kept || __any_sync(0xffffffffu, mine_too)) walk(true, [&](int, int, const Angle* turn, Some x, Some y, Some p, Some q) {
                 if (!mine_too) return;
 #pragma unroll 1
                 for (int e = 0; e < V; ++e)

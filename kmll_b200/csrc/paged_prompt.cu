@@ -575,8 +575,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                 if constexpr (sizeof(T) == 4) {
                     *reinterpret_cast<float4*>(out) = y;
                 } else {
-                    *reinterpret_cast<uint2*>(out) = make_uint2(f32_to_bf16_bits(y.x) | ((uint32_t)f32_to_bf16_bits(y.y) << 16),
-                                                                f32_to_bf16_bits(y.z) | ((uint32_t)f32_to_bf16_bits(y.w) << 16));
+                    *reinterpret_cast<uint2*>(out) = make_uint2(bf16_pair_of(y.x, y.y), bf16_pair_of(y.z, y.w));
                 }
             }
         }
