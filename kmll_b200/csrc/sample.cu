@@ -14,6 +14,7 @@
 // Bound: latency of the steps for few rows; for many the weights of step 2 (64-bit exponentials and shared-memory atomics, one per token).
 #include <cooperative_groups.h>
 
+#include <atomic>
 #include <cfloat>
 
 #include "internal.cuh"
@@ -52,12 +53,12 @@ struct SampleShared {
     uint32_t sub_count[kSubBins], sub_count_before[kSubBins];
     unsigned long long sub_weight[kSubBins], sub_before[kSubBins];
     unsigned long long list[kList], sorted[kList], sums[kList];
-    double powers[32];                               // 2^(j / 32)
+    double powers[256];                              // 2^(j / 256)
     unsigned long long warp_sum[32];
     uint32_t warp_count[32];
     unsigned long long least_sum;                    // weight at or above the min-p border
     unsigned long long key_range[2];                 // of a bin's tokens in this block
-    float scratch[33], top;
+    float scratch[33], tops[8];                      // largest logit of every block of the cluster
     int bin, overflow;
     uint32_t listed;
     unsigned long long base, low_key, high_key, found_key, found_sum;
@@ -79,21 +80,20 @@ struct Weigher {
     double inv;          // 1 / temperature
     const double* powers;
     __device__ double exponent(float l) const { return l == top ? 0.0 : ((double)l - (double)top) * inv; }
-    // e^x = 2^(j / 32) * 2^n * e^r with 32 n + j the nearest whole number to 32 x / ln 2: Taylor's series in |r| <= ln 2 / 64, whose first term left
-    // out is below 2^-52
+    // e^x = 2^(j / 256) * 2^n * e^r with 256 n + j the nearest whole number to 256 x / ln 2: Taylor's series in |r| <= ln 2 / 512, whose first term left
+    // out is below 2^-54.  Adding 1.5 * 2^52 (2^52) rounds to a whole number and leaves it in the low bits: conversions run at an eighth of the rate.
     __device__ unsigned long long weight(double x) const {
-        constexpr double kLn2 = 0.693147180559945309;
-        const double y = fmax(x, -100.0) * (32.0 / kLn2), k = rint(y), r = (y - k) * (kLn2 / 32.0);
-        double p = 1.0 / 720.0;
-        p = fma(p, r, 1.0 / 120.0);
-        p = fma(p, r, 1.0 / 24.0);
+        constexpr double kLn2 = 0.693147180559945309, kWhole = 6755399441055744.0;
+        const double y = fmax(x, -100.0) * (256.0 / kLn2), m = y + kWhole, r = (y - (m - kWhole)) * (kLn2 / 256.0);
+        const int i = __double2loint(m);
+        double p = 1.0 / 24.0;
         p = fma(p, r, 1.0 / 6.0);
         p = fma(p, r, 0.5);
         p = fma(p, r, 1.0);
         p = fma(p, r, 1.0);
-        const int i = (int)k;
-        const double e = p * powers[i & 31];
-        return (unsigned long long)rint(__hiloint2double(__double2hiint(e) + (kUnit + (i >> 5)) * (1 << 20), __double2loint(e)));
+        const double e = p * powers[i & 255];
+        const double w = __hiloint2double(__double2hiint(e) + (kUnit + (i >> 8)) * (1 << 20), __double2loint(e));
+        return (unsigned long long)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
     }
     // monotone in the logit; kBins: weighs nothing
     __device__ int bin(float l) const { return l == top ? 0 : (int)fminf((top - l) * per_bin, (float)kBins); }
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_rows_kernel(const Sa
         s.all_weight[i] = 0ull;
     }
     const SampleBins bins = {s.all_count, s.count_before, s.all_weight, s.before}, subs = {s.sub_count, s.sub_count_before, s.sub_weight, s.sub_before};
-    if (tid < 32) s.powers[tid] = exp2((double)tid / 32.0);
+    if (tid < 256) s.powers[tid] = exp2((double)tid / 256.0);
     if (tid == 0) {
         s.least_sum = 0ull;
         s.listed = 0u;
@@ -228,9 +228,9 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_rows_kernel(const Sa
     float top = -INFINITY;
     each([&](int, float l) { top = fmaxf(top, l); });
     top = block_max(top, s.scratch);
-    if (tid == 0) s.top = top;
+    if (tid < blocks) cluster.map_shared_rank(&s, tid)->tops[rank] = top;
     cluster.sync();
-    for (int b = 0; b < blocks; ++b) top = fmaxf(top, cluster.map_shared_rank(&s, b)->top);
+    for (int b = 0; b < blocks; ++b) top = fmaxf(top, s.tops[b]);
     top += 0.0f;  // (-0 is 0)
     if (top == -INFINITY) {  // nothing to choose from
         if (rank == 0 && tid == 0) {
@@ -335,11 +335,11 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_rows_kernel(const Sa
         cluster.sync();
     }
     if (!greedy) weigh_all(large_k);
-    // the first token, in order, at which the tokens (by_count) or the weight so far reach `target`: its key (found_key), and the weight up to and with
-    // it (found_sum)
+    // The first token, in order, at which the tokens (by_count) or the weight so far reach `target` (block 0's): block 0 gets its key (found_key), and the
+    // weight up to and with it (found_sum).  The bins' sums are there.
     auto search = [&](bool by_count, unsigned long long target) {
         if (rank == 0) {
-            scan_bins<kBins>(s, bins);
+            __syncthreads();  // (all have read what the search before found)
             for (int b = tid; b < kBins; b += kSampleThreads) {
                 const unsigned long long before = by_count ? s.count_before[b] : s.before[b], after = before + (by_count ? s.all_count[b] : s.all_weight[b]);
                 if (before < target && after >= target) {
@@ -428,34 +428,56 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_rows_kernel(const Sa
                 s.found_key = s.sorted[at];
                 s.found_sum = s.sums[at];
             }
+            __syncthreads();
         }
-        cluster.sync();
     };
+    if (rank == 0) scan_bins<kBins>(s, bins);
     if (greedy) {  // the first of the largest
         search(true, 1ull);
         if (rank == 0) answer(s.found_key, 1ull);
-        cluster.sync();
+        cluster.sync();  // (block 0's shared memory stays while others read it)
         return;
     }
-    if (rank == 0) scan_bins<kBins>(s, bins);
-    cluster.sync();
-    unsigned long long kept = s0.before[kBins - 1] + s0.all_weight[kBins - 1];
-    const unsigned long long tokens = s0.count_before[kBins - 1] + s0.all_count[kBins - 1], least_sum = s0.least_sum;
-    cluster.sync();
-    if (k_on && (unsigned long long)k < tokens) {  // (tokens are counted with top-k only)
-        search(true, (unsigned long long)k);
-        kept = s0.found_sum;
-        cluster.sync();
+    unsigned long long kept = 0ull;  // (block 0's)
+    if (rank == 0) kept = s.before[kBins - 1] + s.all_weight[kBins - 1];
+    if (k_on) {
+        search(true, min((unsigned long long)k, (unsigned long long)s.count_before[kBins - 1] + s.all_count[kBins - 1]));
+        kept = s.found_sum;
     }
     if (top_p < 1.0f) {
         search(false, target_of_p(kept));
-        kept = s0.found_sum;
-        cluster.sync();
+        kept = s.found_sum;
     }
-    kept = min(kept, least_sum);
+    if (rank == 0) kept = min(kept, s.least_sum);
     search(false, target_of_u(kept));
     if (rank == 0) answer(s.found_key, kept);
     cluster.sync();
+}
+
+// Clusters of `c` blocks that the GPU runs at once: asked for once per kernel and size (an occupancy query, no allocation).
+template <typename K>
+int clusters_at_once(K kernel, int c) {
+    static std::atomic<int> known[9];
+    int n = known[c].load(std::memory_order_relaxed);
+    if (n == 0) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(c * 16);
+        cfg.blockDim = dim3(kSampleThreads);
+        cfg.dynamicSmemBytes = sizeof(SampleShared);
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = c;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+            cudaGetLastError();
+            n = 1;
+        }
+        known[c].store(n, std::memory_order_relaxed);
+    }
+    return n;
 }
 
 }  // namespace
@@ -474,9 +496,17 @@ extern "C" int kmll_sample_rows(kmll_stream_t stream, const void* logits, int is
     KMLL_REQUIRE_PTR(tokens);
     KMLL_REQUIRE(reinterpret_cast<uintptr_t>(logits) % (is_f32 ? 4 : 2) == 0, "sample rows: logits are not aligned to their type");
     const SampleArgs a = {logits, vocab, (size_t)ld, u, temperature, top_k, top_p, min_p, tokens, logprobs};
-    const int cluster = rows <= 18 ? 8 : rows <= 37 ? 4 : rows <= 74 ? 2 : 1;
+    // The most blocks per row that still let all rows run at once: a row's steps are short, a second round of clusters costs as much as the first
+    // (16 rows of 151936, greedy: clusters of 8, of which fewer than 16 fit, 29 us, of 4 19, of 2 29; 64 rows of 152064: of 4 41, of 2 30, of 1 51).
     auto go = [&](auto kern) {
         cudaError_t e = allow_all_dynamic_smem(kern);
+        int cluster = 1;
+        for (int c = 8; c > 1 && e == cudaSuccess; c >>= 1) {
+            if (rows > 148 / c) continue;
+            if (rows > clusters_at_once(kern, c)) continue;
+            cluster = c;
+            break;
+        }
         if (e != cudaSuccess) return e;
         return launch_cluster(kern, dim3((unsigned)rows * cluster), cluster, dim3(kSampleThreads), sizeof(SampleShared), as_stream(stream), true, a);
     };
