@@ -7,6 +7,11 @@ namespace kmll {
 
 int check_paged_cache(const char* who, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, int pages, int block, int kv_heads, int head_dim);
 
+// A kernel whose dynamic shared memory varies with the call, and is small as a rule, is opted in when a call needs it (never back: graphs keep what their nodes need).
+constexpr size_t kSmemWithoutOptIn = 46 * 1024;
+template <typename K>
+inline cudaError_t allow_dynamic_smem(K kernel, size_t bytes) { return bytes > kSmemWithoutOptIn ? allow_all_dynamic_smem(kernel) : cudaSuccess; }
+
 struct PagedArgs {
     const void* query;
     const int32_t *query_start, *context, *table;

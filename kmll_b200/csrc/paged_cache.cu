@@ -678,7 +678,7 @@ extern "C" int kmll_paged_plan(kmll_stream_t stream, const int32_t* lengths, con
     const PlanArgs a = {lengths, new_tokens, requests, block, block_table, table_width, free_blocks, free_capacity, free_count, token_capacity, context, query_start,
                         positions, slots, free_count_out, status};
     const int cluster = token_capacity > 2 * kPlanThreads ? 8 : 1;
-    cudaError_t e = allow_all_dynamic_smem(paged_plan_kernel);
+    cudaError_t e = allow_dynamic_smem(paged_plan_kernel, (3 * (size_t)requests + 2) * 4);
     if (e == cudaSuccess)
         e = launch_cluster(paged_plan_kernel, dim3(cluster), cluster, dim3(kPlanThreads), (3 * (size_t)requests + 2) * 4, as_stream(stream), true, a);
     if (e != cudaSuccess) return fail(KMLL_ERR_CUDA, "paged plan: %s", cudaGetErrorString(e));
@@ -700,7 +700,7 @@ extern "C" int kmll_paged_release(kmll_stream_t stream, const int32_t* context, 
         KMLL_REQUIRE_PTR(context_out);
     }
     if (free_capacity > 0) KMLL_REQUIRE_PTR(free_blocks);
-    cudaError_t e = allow_all_dynamic_smem(paged_release_kernel);
+    cudaError_t e = allow_dynamic_smem(paged_release_kernel, 2 * (size_t)requests * 4);
     if (e == cudaSuccess)
         e = launch(paged_release_kernel, dim3(1), dim3(kPlanThreads), 2 * (size_t)requests * 4, as_stream(stream), true, context, ended, requests, block, block_table,
                    table_width, free_blocks, free_capacity, free_count, context_out, free_count_out, status);
@@ -747,7 +747,7 @@ extern "C" int kmll_prepare_paged_attention(kmll_stream_t stream, const void* qu
     const uintptr_t bits = reinterpret_cast<uintptr_t>(query) | reinterpret_cast<uintptr_t>(query_rot) | reinterpret_cast<uintptr_t>(key) | reinterpret_cast<uintptr_t>(value);
     const bool fours = n_freqs % 4 == 0 && (ld_query | ld_key | ld_value) % 4 == 0 && bits % (is_f32 ? 16 : 8) == 0;
     auto go = [&](auto kern) {
-        const cudaError_t e = allow_all_dynamic_smem(kern);
+        const cudaError_t e = allow_dynamic_smem(kern, table_bytes);
         return e != cudaSuccess ? e : launch(kern, dim3((unsigned)blocks), dim3(kPrepareThreads), table_bytes, as_stream(stream), true, a);
     };
     auto pick = [&](auto hs) {

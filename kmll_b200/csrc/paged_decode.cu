@@ -27,6 +27,10 @@ constexpr int kPdThreads = kPdWarps * 32;
 constexpr int kPdKeys = 32;      // keys of a tile
 constexpr int kPdBlocks = 444;   // three blocks on each of 148 multiprocessors
 constexpr int kPdStages = 2;
+// What a stretch costs besides its tiles (queries, first copies, the warps' meeting), in tiles: so much longer is a head on the axis of work, or
+// blocks whose share is many short requests would end last (64 requests of 100 to 8000 tokens, 32 / 8 heads of 128: 0 tiles 96 us,
+// 4 80, 8 72, 20 72; one of 2048: 14.6, 11.0, 11.3, 11.8).
+constexpr int kPdStretch = 8;
 
 struct PdMeta {  // of a stage: the two groups of 16 keys may lie in two pages
     float k_scale[2], v_scale[2];
@@ -83,6 +87,7 @@ __device__ inline int pd_tiles(const PagedRequest& q, int group, int limit) {
     if (q.rows == 0 || (long long)q.rows * group > limit) return 0;
     return max(1, (q.hi + kPdKeys - 1) / kPdKeys - q.lo / kPdKeys);
 }
+__device__ inline long long pd_length(int tiles) { return tiles > 0 ? tiles + kPdStretch : 0; }
 
 // NB: bytes of q and of the weights; NC: columns of eight rows.
 template <int HD, typename T, int NB, int NC>
@@ -100,7 +105,7 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
     long long mine = 0;
     for (int i = 0; i < per; ++i) {
         const int r = tid * per + i;
-        if (r < a.requests) mine += pd_tiles(PagedRequest::of(a, r), group, ROWS);
+        if (r < a.requests) mine += pd_length(pd_tiles(PagedRequest::of(a, r), group, ROWS));
     }
     long long before = mine;
 #pragma unroll
@@ -127,7 +132,7 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
         for (int i = 0; i < per; ++i) {
             const int r = tid * per + i;
             if (r >= a.requests) break;
-            const long long n = (long long)pd_tiles(PagedRequest::of(a, r), group, ROWS) * a.kv_heads;
+            const long long n = pd_length(pd_tiles(PagedRequest::of(a, r), group, ROWS)) * a.kv_heads;
             if (w0 < at + n) {
                 s_request = r;
                 s_start = at;
@@ -149,14 +154,18 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
 
     for (long long w = w0; w < w1;) {
         const PagedRequest rq = PagedRequest::of(a, r);
-        const int tiles = pd_tiles(rq, group, ROWS);
-        if (tiles == 0 || w >= start + (long long)tiles * a.kv_heads) {
-            start += (long long)tiles * a.kv_heads;
+        const int tiles = pd_tiles(rq, group, ROWS), length = (int)pd_length(tiles);
+        if (tiles == 0 || w >= start + (long long)length * a.kv_heads) {
+            start += (long long)length * a.kv_heads;
             ++r;
             continue;
         }
-        const int h = (int)((w - start) / tiles), ta = (int)((w - start) - (long long)h * tiles);
-        const int tb = (int)min((long long)tiles, ta + (w1 - w));
+        const int h = (int)((w - start) / length), ua = (int)((w - start) - (long long)h * length);
+        const int ub = (int)min((long long)length, ua + (w1 - w)), ta = max(0, ua - kPdStretch), tb = max(0, ub - kPdStretch);
+        if (ta == tb) {
+            w += ub - ua;
+            continue;
+        }
         const int key0 = rq.lo / kPdKeys * kPdKeys;  // of tile 0
         const int32_t* const table = a.table + (size_t)r * a.width;
         const int mine_n = tb - ta > warp ? (tb - ta - warp + kPdWarps - 1) / kPdWarps : 0;
@@ -425,9 +434,9 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
                 }
             }
         __syncthreads();
-        const long long seq0 = start + (long long)h * tiles;
         const bool whole = ta == 0 && tb == tiles;
-        float* const part = work.partials + ((size_t)blockIdx.x * 2 + (w == w0 ? 0 : 1)) * ROWS * (HD + 2);
+        // (a block has at most one head that it goes on with, and one that it begins and leaves)
+        float* const part = work.partials + ((size_t)blockIdx.x * 2 + (ta > 0 ? 0 : 1)) * ROWS * (HD + 2);
         for (int i = tid; i < n_rows * (HD / 4); i += kPdThreads) {
             const int row = i / (HD / 4), c = i % (HD / 4) * 4;
             float mw[kPdWarps], top = -INFINITY, sum = 0.0f;
@@ -462,35 +471,53 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
         if (!whole) {
             __threadfence();
             __syncthreads();
-            const int c0 = (int)(seq0 / share), c1 = (int)((seq0 + tiles - 1) / share);
-            if (tid == 0) s_last = atomicAdd(work.arrived + (size_t)r * a.kv_heads + h, 1) == c1 - c0;
+            // blocks that have tiles of this head
+            const long long seq0 = start + (long long)h * length;
+            const int c0 = (int)((seq0 + kPdStretch) / share), n = (int)((seq0 + length - 1) / share) - c0 + 1;
+            if (tid == 0) s_last = atomicAdd(work.arrived + (size_t)r * a.kv_heads + h, 1) == n - 1;
             __syncthreads();
             if (s_last) {
                 __threadfence();
                 if (tid == 0) work.arrived[(size_t)r * a.kv_heads + h] = 0;
-                // the first block's part is its last stretch unless the head begins with its share
-                auto part_of = [&](int c) { return work.partials + ((size_t)c * 2 + (c == c0 && seq0 != (long long)c0 * share ? 1 : 0)) * ROWS * (HD + 2); };
+                auto part_of = [&](int k) { return work.partials + ((size_t)(c0 + k) * 2 + (k == 0 ? 1 : 0)) * ROWS * (HD + 2); };
+                float* const factor = reinterpret_cast<float*>(pd_smem);  // [row][part]: 2^(maximum - largest) / sum
+                static_assert(ROWS * kPdBlocks * 4 <= kPdWarps * S::kWarp, "factors fit over the ring");
+                for (int row = warp; row < n_rows; row += kPdWarps) {
+                    float top = -INFINITY, sum = 0.0f;
+                    for (int k = lane; k < n; k += 32) top = fmaxf(top, __ldcg(part_of(k) + row * (HD + 2)));
+                    top = warp_max(top);
+                    const float base = top == -INFINITY ? 0.0f : top;
+                    for (int k = lane; k < n; k += 32) {
+                        const float2 st = __ldcg(reinterpret_cast<const float2*>(part_of(k) + row * (HD + 2)));
+                        const float f = ex2_approx(st.x - base);
+                        factor[row * n + k] = f;
+                        sum = fmaf(st.y, f, sum);
+                    }
+                    sum = warp_sum(sum);
+                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    for (int k = lane; k < n; k += 32) factor[row * n + k] *= inv;
+                }
+                __syncthreads();
                 for (int i = tid; i < n_rows * (HD / 2); i += kPdThreads) {
                     const int row = i / (HD / 2), c = i % (HD / 2) * 2;
-                    float top = -INFINITY, sum = 0.0f, y0 = 0.0f, y1 = 0.0f;
-                    for (int k = c0; k <= c1; ++k) {
-                        const float* const from = part_of(k) + row * (HD + 2);
-                        const float2 st = __ldcg(reinterpret_cast<const float2*>(from)), x = __ldcg(reinterpret_cast<const float2*>(from + 2 + c));
-                        const float now = fmaxf(top, st.x), base = now == -INFINITY ? 0.0f : now, f = ex2_approx(top - base), e = ex2_approx(st.x - base);
-                        top = now;
-                        sum = fmaf(sum, f, st.y * e);
-                        y0 = fmaf(y0, f, x.x * e);
-                        y1 = fmaf(y1, f, x.y * e);
+                    const float* const from = part_of(0) + row * (HD + 2) + 2 + c;
+                    const float* const f = factor + row * n;
+                    const float2 x0 = __ldcg(reinterpret_cast<const float2*>(from));
+                    float y0 = x0.x * f[0], y1 = x0.y * f[0];
+#pragma unroll 8
+                    for (int k = 1; k < n; ++k) {
+                        const float2 x = __ldcg(reinterpret_cast<const float2*>(from + (size_t)(2 * k - 1) * ROWS * (HD + 2)));
+                        y0 = fmaf(x.x, f[k], y0);
+                        y1 = fmaf(x.y, f[k], y1);
                     }
-                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                     T* const to = static_cast<T*>(a.out) + ((size_t)(rq.first + row / group) * a.heads + (size_t)h * group + row % group) * HD + c;
-                    store_row(to, y0 * inv);
-                    store_row(to + 1, y1 * inv);
+                    store_row(to, y0);
+                    store_row(to + 1, y1);
                 }
             }
         }
         __syncthreads();  // (the ring is free again)
-        w += tb - ta;
+        w += ub - ua;
     }
 }
 
@@ -509,7 +536,7 @@ int paged_decode_launch(cudaStream_t stream, const PagedArgs& a, bool f32, int m
     work.arrived = static_cast<int*>(workspace);
     work.partials = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + pd_counter_bytes(a.requests, a.kv_heads));
     // no more blocks than there can be shares of one tile a warp
-    const long long most = (long long)a.requests * a.kv_heads * (max_context / kPdKeys + 2), blocks = (most + kPdWarps - 1) / kPdWarps;
+    const long long most = (long long)a.requests * a.kv_heads * (max_context / kPdKeys + 2 + kPdStretch), blocks = (most + kPdWarps - 1) / kPdWarps;
     const dim3 grid((unsigned)(blocks < kPdBlocks ? blocks : kPdBlocks));
     auto go = [&](auto kern, int smem) {
         const cudaError_t e = allow_all_dynamic_smem(kern);

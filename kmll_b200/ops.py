@@ -8,6 +8,7 @@ CUDA stream to libkmll_b200.so.  Nothing here computes on the CPU.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -573,38 +574,41 @@ def sample_rows(logits, u, temperature=None, top_k=None, top_p=None, min_p=None,
     value per row on the device, or None.  Returns (tokens int32 [rows], logprobs f32 [rows])."""
     if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise KmllError(-2, "logits must be [rows, vocab] in float32 or bfloat16 with rows in one piece")
+    gpu = _here(logits)
     rows, vocab = logits.shape
-    dev = _here(logits)
-    tokens = torch.empty(rows, dtype=torch.int32, device=dev) if tokens is None else tokens
-    logprobs = torch.empty(rows, dtype=torch.float32, device=dev) if logprobs is None else logprobs
-    check(load().kmll_sample_rows(_stream(), logits.data_ptr(), 1 if logits.dtype == torch.float32 else 0, logits.stride(0) if rows > 1 else vocab, rows, vocab,
-                                  _array(u, torch.float64, rows, "u"), _array(temperature, torch.float32, rows, "temperature"), _array(top_k, torch.int32, rows, "top_k"),
-                                  _array(top_p, torch.float32, rows, "top_p"), _array(min_p, torch.float32, rows, "min_p"), _array(tokens, torch.int32, rows, "tokens"),
-                                  _array(logprobs, torch.float32, rows, "logprobs")))
+    f32, i32 = torch.float32, torch.int32
+    tokens = torch.empty(rows, dtype=i32, device=logits.device) if tokens is None else tokens
+    logprobs = torch.empty(rows, dtype=f32, device=logits.device) if logprobs is None else logprobs
+    check(load().kmll_sample_rows(_stream(), logits.data_ptr(), 1 if logits.dtype is f32 else 0, logits.stride(0) if rows > 1 else vocab, rows, vocab,
+                                  _array(u, torch.float64, rows, "u", gpu), _array(temperature, f32, rows, "temperature", gpu), _array(top_k, i32, rows, "top_k", gpu),
+                                  _array(top_p, f32, rows, "top_p", gpu), _array(min_p, f32, rows, "min_p", gpu), _array(tokens, i32, rows, "tokens", gpu),
+                                  _array(logprobs, f32, rows, "logprobs", gpu)))
     return tokens, logprobs
 
 
 # ---- requests of unequal length over one cache of pages in 8 bits ---------------------------------------------------------------
-def _here(t: torch.Tensor) -> torch.device:
-    """The device of a tensor that lies on the current GPU, whose current stream the call uses."""
-    if not t.is_cuda:
+def _here(t: torch.Tensor) -> int:
+    """Index of the GPU that a tensor lies on: the current one, whose current stream the call uses."""
+    at = t.get_device()
+    if at < 0:
         raise KmllError(-2, "operand must be a CUDA tensor (there is no CPU path)")
-    if t.get_device() != torch.cuda.current_device():
-        raise KmllError(-2, f"operand lies on GPU {t.get_device()}, the current one is {torch.cuda.current_device()}")
-    return t.device
+    if at != torch._C._cuda_getDevice():
+        raise KmllError(-2, f"operand lies on GPU {at}, the current one is {torch._C._cuda_getDevice()}")
+    return at
 
 
-def _array(t, dtype, least: int, name: str) -> int | None:
-    """Pointer of a contiguous array of at least `least` entries; None stays None."""
+def _array(t, dtype, least: int, name: str, gpu: int) -> int | None:
+    """Pointer of a contiguous array of at least `least` entries on that GPU; None stays None."""
     if t is None:
         return None
-    if t.dtype != dtype or t.numel() < least:
-        raise KmllError(-2, f"{name} must hold {least} entries of {dtype}, got {t.numel()} of {t.dtype}")
-    _here(t)
-    return _p(t)
+    if t.dtype is not dtype or t.numel() < least or not t.is_contiguous():
+        raise KmllError(-2, f"{name} must hold {least} entries of {dtype} in one piece, got {tuple(t.shape)} of {t.dtype}")
+    if t.get_device() != gpu:
+        raise KmllError(-2, f"{name} must lie on GPU {gpu}, it is on {t.device}")
+    return t.data_ptr()
 
 
-@dataclass
+@dataclass(frozen=True)
 class DevicePagedI8Cache:
     """Keys and values of many requests in pages of int8 codes with a scale per (page, kv head); layouts in include/kmll_b200.h."""
     k_codes: torch.Tensor   # int8 [pages, kv_heads, head_dim / 16, block, 16]
@@ -615,6 +619,18 @@ class DevicePagedI8Cache:
     block: int
     kv_heads: int
     head_dim: int
+
+    def __post_init__(self):
+        pages, block, kv_heads, head_dim = self.pages, self.block, self.kv_heads, self.head_dim
+        if tuple(self.k_codes.shape) != (pages, kv_heads, head_dim // 16, block, 16) or tuple(self.v_codes.shape) != (pages, kv_heads, block // 16, head_dim, 16):
+            raise KmllError(-2, f"paged codes of keys {tuple(self.k_codes.shape)} and values {tuple(self.v_codes.shape)} do not belong together")
+        if tuple(self.k_scales.shape) != (pages, kv_heads) or tuple(self.v_scales.shape) != (pages, kv_heads):
+            raise KmllError(-2, "paged scales must be [pages, kv_heads]")
+        parts = (self.k_codes, self.v_codes, self.k_scales, self.v_scales)
+        if [t.dtype for t in parts] != [torch.int8, torch.int8, torch.float32, torch.float32]:
+            raise KmllError(-2, "paged codes must be int8, their scales float32")
+        if not all(t.is_contiguous() and t.device == self.k_codes.device for t in parts):
+            raise KmllError(-2, "paged codes and scales must be contiguous, on one device")
 
     @staticmethod
     def create(pages: int, block: int, kv_heads: int, head_dim: int, device="cuda") -> "DevicePagedI8Cache":
@@ -627,20 +643,15 @@ class DevicePagedI8Cache:
 
     @staticmethod
     def from_parts(k_codes, v_codes, k_scales, v_scales) -> "DevicePagedI8Cache":
-        if k_codes.dim() != 5 or v_codes.dim() != 5 or k_codes.shape[4] != 16 or v_codes.shape[4] != 16:
+        if k_codes.dim() != 5 or k_codes.shape[3] not in (16, 32, 64, 128):
             raise KmllError(-2, "paged codes must be [pages, kv_heads, head_dim / 16, block, 16] and [pages, kv_heads, block / 16, head_dim, 16]")
         pages, kv_heads, units, block, _ = k_codes.shape
-        if tuple(v_codes.shape) != (pages, kv_heads, block // 16, 16 * units, 16) or block not in (16, 32, 64, 128):
-            raise KmllError(-2, f"paged codes of keys {tuple(k_codes.shape)} and values {tuple(v_codes.shape)} do not belong together")
-        if tuple(k_scales.shape) != (pages, kv_heads) or tuple(v_scales.shape) != (pages, kv_heads):
-            raise KmllError(-2, "paged scales must be [pages, kv_heads]")
-        if k_codes.dtype != torch.int8 or v_codes.dtype != torch.int8 or k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32:
-            raise KmllError(-2, "paged codes must be int8, their scales float32")
         return DevicePagedI8Cache(k_codes, v_codes, k_scales, v_scales, pages, block, kv_heads, 16 * units)
 
-    def _pointers(self):
-        _here(self.k_codes)
-        return _p(self.k_codes), _p(self.k_scales), _p(self.v_codes), _p(self.v_scales), self.pages, self.block
+    def _pointers(self, gpu: int):
+        if self.k_codes.get_device() != gpu:
+            raise KmllError(-2, f"the cache must lie on GPU {gpu}, it is on {self.k_codes.device}")
+        return self.k_codes.data_ptr(), self.k_scales.data_ptr(), self.v_codes.data_ptr(), self.v_scales.data_ptr(), self.pages, self.block
 
     @property
     def nbytes(self) -> int:
@@ -651,95 +662,100 @@ def paged_plan(lengths, new_tokens, block: int, block_table, free_blocks, free_c
     """The pages of a step: kmll_paged_plan.  int32 arrays on the device; positions and slots as long as the step's rows may be, block_table [requests,
     width] (updated), free_blocks a stack of free_count[0] pages."""
     requests, width = block_table.shape
-    rows = positions.numel()
-    i32 = torch.int32
+    rows, i32, gpu = positions.numel(), torch.int32, _here(block_table)
     if slots.numel() != rows:
         raise KmllError(-2, "positions and slots must be of one length")
-    check(load().kmll_paged_plan(_stream(), _array(lengths, i32, requests, "lengths"), _array(new_tokens, i32, requests, "new_tokens"), requests, block,
-                                 _array(block_table, i32, 0, "block_table"), width, _array(free_blocks, i32, 0, "free_blocks"), free_blocks.numel(),
-                                 _array(free_count, i32, 1, "free_count"), rows, _array(context, i32, requests, "context"),
-                                 _array(query_start, i32, requests + 1, "query_start"), _array(positions, i32, rows, "positions"), _array(slots, i32, rows, "slots"),
-                                 _array(free_count_out, i32, 1, "free_count_out"), _array(status, i32, 1, "status")))
+    check(load().kmll_paged_plan(_stream(), _array(lengths, i32, requests, "lengths", gpu), _array(new_tokens, i32, requests, "new_tokens", gpu), requests, block,
+                                 _array(block_table, i32, 0, "block_table", gpu), width, _array(free_blocks, i32, 0, "free_blocks", gpu), free_blocks.numel(),
+                                 _array(free_count, i32, 1, "free_count", gpu), rows, _array(context, i32, requests, "context", gpu),
+                                 _array(query_start, i32, requests + 1, "query_start", gpu), _array(positions, i32, rows, "positions", gpu),
+                                 _array(slots, i32, rows, "slots", gpu), _array(free_count_out, i32, 1, "free_count_out", gpu), _array(status, i32, 1, "status", gpu)))
 
 
 def paged_release(context, ended, block: int, block_table, free_blocks, free_count, context_out, free_count_out, status):
     """Pages of the requests with ended != 0 go back on the stack: kmll_paged_release."""
     requests, width = block_table.shape
-    i32 = torch.int32
-    check(load().kmll_paged_release(_stream(), _array(context, i32, requests, "context"), _array(ended, i32, requests, "ended"), requests, block,
-                                    _array(block_table, i32, 0, "block_table"), width, _array(free_blocks, i32, 0, "free_blocks"), free_blocks.numel(),
-                                    _array(free_count, i32, 1, "free_count"), _array(context_out, i32, requests, "context_out"),
-                                    _array(free_count_out, i32, 1, "free_count_out"), _array(status, i32, 1, "status")))
+    i32, gpu = torch.int32, _here(block_table)
+    check(load().kmll_paged_release(_stream(), _array(context, i32, requests, "context", gpu), _array(ended, i32, requests, "ended", gpu), requests, block,
+                                    _array(block_table, i32, 0, "block_table", gpu), width, _array(free_blocks, i32, 0, "free_blocks", gpu), free_blocks.numel(),
+                                    _array(free_count, i32, 1, "free_count", gpu), _array(context_out, i32, requests, "context_out", gpu),
+                                    _array(free_count_out, i32, 1, "free_count_out", gpu), _array(status, i32, 1, "status", gpu)))
 
 
-def _head_rows(t, heads, head_dim, dtype, name):
+def _head_rows(t, tokens, heads, head_dim, dtype, name, gpu):
     """(pointer, pitch in elements) of rows [tokens, heads, head_dim] (or [tokens, heads * head_dim]) whose heads lie together."""
-    if t.dtype != dtype or t.numel() != t.shape[0] * heads * head_dim:
-        raise KmllError(-2, f"{name} must be [tokens, {heads}, {head_dim}] in {dtype}, got {tuple(t.shape)} in {t.dtype}")
-    _here(t)
-    whole = t.stride(-1) == 1 and (t.dim() == 2 or t.stride(1) == head_dim or heads == 1)
-    if t.numel() and not (t.is_contiguous() or (t.dim() in (2, 3) and whole)):
+    if t.dtype is not dtype or t.shape[0] != tokens or t.numel() != tokens * heads * head_dim or t.get_device() != gpu:
+        raise KmllError(-2, f"{name} must be [{tokens}, {heads}, {head_dim}] in {dtype} on GPU {gpu}, got {tuple(t.shape)} in {t.dtype} on {t.device}")
+    if t.is_contiguous() or t.numel() == 0:
+        return t.data_ptr(), heads * head_dim
+    if t.dim() not in (2, 3) or t.stride(-1) != 1 or (t.dim() == 3 and t.shape[1] > 1 and (t.stride(1) != t.shape[2] or t.shape[2] != head_dim)):
         raise KmllError(-2, f"the heads of a row of {name} must lie together")
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else heads * head_dim
+    return t.data_ptr(), t.stride(0) if tokens > 1 else heads * head_dim
 
 
 def prepare_paged_attention(query, key, value, freqs, positions, slots, cache: DevicePagedI8Cache, query_rot=None):
     """Rotation of a step's queries and keys, keys and values into the cache: prepare_incremental_attention (ops/inference.rs:1291-1362) for rows
     of many requests.  query [tokens, heads, head_dim], key and value [tokens, kv_heads, head_dim], f32 or bf16; freqs None: no
     rotation.  Returns the turned queries."""
-    tokens, heads = query.shape[0], query.numel() // max(1, query.shape[0] * cache.head_dim)
-    dtype = query.dtype
-    if dtype not in (torch.float32, torch.bfloat16) or key.shape[0] != tokens or value.shape[0] != tokens:
-        raise KmllError(-2, "query, key and value must be rows of the same tokens in float32 or bfloat16")
-    q, k, v = _head_rows(query, heads, cache.head_dim, dtype, "query"), _head_rows(key, cache.kv_heads, cache.head_dim, dtype, "key"), \
-        _head_rows(value, cache.kv_heads, cache.head_dim, dtype, "value")
+    dtype, tokens, kv_heads, head_dim = key.dtype, key.shape[0], cache.kv_heads, cache.head_dim
+    if dtype is not torch.float32 and dtype is not torch.bfloat16:
+        raise KmllError(-2, "query, key and value must be rows in float32 or bfloat16")
+    heads, gpu = query.numel() // max(1, tokens * head_dim), _here(key)
+    q, ldq = _head_rows(query, tokens, heads, head_dim, dtype, "query", gpu)
+    k, ldk = _head_rows(key, tokens, kv_heads, head_dim, dtype, "key", gpu)
+    v, ldv = _head_rows(value, tokens, kv_heads, head_dim, dtype, "value", gpu)
     query_rot = torch.empty(query.shape, dtype=dtype, device=query.device) if query_rot is None else query_rot
-    if query_rot.numel() != query.numel() or query_rot.dtype != dtype:
-        raise KmllError(-2, "query_rot must be as large as query, of its type")
-    n_freqs = 0 if freqs is None else freqs.numel()
-    check(load().kmll_prepare_paged_attention(_stream(), *q, *k, *v, 1 if dtype == torch.float32 else 0, _array(freqs, torch.float32, 0, "freqs"), n_freqs,
-                                              None if freqs is None else _array(positions, torch.int32, tokens, "positions"), _array(slots, torch.int32, tokens, "slots"),
-                                              tokens, heads, cache.kv_heads, cache.head_dim, _p(query_rot), *cache._pointers()))
+    if query_rot.numel() != query.numel():
+        raise KmllError(-2, "query_rot must be as large as query")
+    check(load().kmll_prepare_paged_attention(_stream(), q, ldq, k, ldk, v, ldv, 1 if dtype is torch.float32 else 0, _array(freqs, torch.float32, 0, "freqs", gpu),
+                                              0 if freqs is None else freqs.numel(), None if freqs is None else _array(positions, torch.int32, tokens, "positions", gpu),
+                                              _array(slots, torch.int32, tokens, "slots", gpu), tokens, heads, kv_heads, head_dim,
+                                              _array(query_rot, dtype, 0, "query_rot", gpu) if heads else None, *cache._pointers(gpu)))
     return query_rot
 
 
 def paged_cache_rows(cache: DevicePagedI8Cache, slots, k=None, v=None):
     """Rows of the cache in f32: (keys, values), [count, kv_heads, head_dim] each."""
-    shape = (slots.numel(), cache.kv_heads, cache.head_dim)
-    dev = _here(cache.k_codes)
-    k = torch.empty(shape, dtype=torch.float32, device=dev) if k is None else k
-    v = torch.empty(shape, dtype=torch.float32, device=dev) if v is None else v
-    need = shape[0] * shape[1] * shape[2]
-    check(load().kmll_paged_cache_rows(_stream(), *cache._pointers(), cache.kv_heads, cache.head_dim, _array(slots, torch.int32, 0, "slots"), shape[0],
-                                       _array(k, torch.float32, need, "k"), _array(v, torch.float32, need, "v")))
+    gpu, count = _here(cache.k_codes), slots.numel()
+    shape, need = (count, cache.kv_heads, cache.head_dim), count * cache.kv_heads * cache.head_dim
+    k = torch.empty(shape, dtype=torch.float32, device=cache.k_codes.device) if k is None else k
+    v = torch.empty(shape, dtype=torch.float32, device=cache.k_codes.device) if v is None else v
+    check(load().kmll_paged_cache_rows(_stream(), *cache._pointers(gpu), cache.kv_heads, cache.head_dim, _array(slots, torch.int32, 0, "slots", gpu), count,
+                                       _array(k, torch.float32, need, "k", gpu), _array(v, torch.float32, need, "v", gpu)))
     return k, v
+
+
+@functools.lru_cache(maxsize=4096)
+def _paged_attention_bytes(heads, kv_heads, head_dim, requests, tokens, max_query, max_context) -> int:
+    return int(load().kmll_paged_attention_workspace_bytes(heads, kv_heads, head_dim, requests, tokens, max_query, max_context))
 
 
 def paged_attention_workspace(cache: DevicePagedI8Cache, heads: int, requests: int, tokens: int, max_query: int, max_context: int):
     """Scratch of paged_attention for steps up to these sizes (zeroed; None where none is needed); one for calls that may overlap each."""
-    n = int(load().kmll_paged_attention_workspace_bytes(heads, cache.kv_heads, cache.head_dim, requests, tokens, max_query, max_context))
+    n = _paged_attention_bytes(heads, cache.kv_heads, cache.head_dim, requests, tokens, max_query, max_context)
     return torch.zeros(n, dtype=torch.uint8, device=cache.k_codes.device) if n > 0 else None
 
 
 def paged_attention(query, query_start, context, block_table, cache: DevicePagedI8Cache, max_query: int, max_context: int, scale: float, window: int = 0, workspace=None,
                     out=None):
     """Attention of a step's rows, query [tokens, heads, head_dim] f32 or bf16, over the pages of their requests: kmll_paged_attention."""
-    tokens, heads = query.shape[0], query.numel() // max(1, query.shape[0] * cache.head_dim)
-    dtype = query.dtype
-    if dtype not in (torch.float32, torch.bfloat16) or query.numel() != tokens * heads * cache.head_dim:
-        raise KmllError(-2, f"query must be [tokens, heads, {cache.head_dim}] in float32 or bfloat16")
-    dev = _here(query)
-    out = torch.empty((tokens, heads * cache.head_dim), dtype=dtype, device=dev) if out is None else out
-    if out.numel() != query.numel() or out.dtype != dtype:
-        raise KmllError(-2, "out must be as large as query, of its type")
+    tokens, head_dim, dtype = query.shape[0], cache.head_dim, query.dtype
+    heads = query.numel() // max(1, tokens * head_dim)
+    need = tokens * heads * head_dim
+    if (dtype is not torch.float32 and dtype is not torch.bfloat16) or query.numel() != need:
+        raise KmllError(-2, f"query must be [tokens, heads, {head_dim}] in float32 or bfloat16")
+    out = torch.empty((tokens, heads * head_dim), dtype=dtype, device=query.device) if out is None else out
+    if out.numel() != need:
+        raise KmllError(-2, "out must be as large as query")
     requests, width = block_table.shape
-    need = int(load().kmll_paged_attention_workspace_bytes(heads, cache.kv_heads, cache.head_dim, requests, tokens, max_query, max_context))
-    if workspace is None and need > 0:
-        workspace = torch.zeros(need, dtype=torch.uint8, device=dev)
-    check(load().kmll_paged_attention(_stream(), _p(query), 1 if dtype == torch.float32 else 0, _array(query_start, torch.int32, requests + 1, "query_start"),
-                                      _array(context, torch.int32, requests, "context"), _array(block_table, torch.int32, 0, "block_table"), width, requests, tokens,
-                                      max_query, max_context, heads, *cache._pointers(), cache.kv_heads, cache.head_dim, scale, window,
-                                      _array(workspace, torch.uint8, need, "workspace"), _p(out)))
+    i32, gpu = torch.int32, _here(query)
+    scratch = _paged_attention_bytes(heads, cache.kv_heads, head_dim, requests, tokens, max_query, max_context)
+    if workspace is None and scratch > 0:
+        workspace = torch.zeros(scratch, dtype=torch.uint8, device=query.device)
+    check(load().kmll_paged_attention(_stream(), _array(query, dtype, need, "query", gpu), 1 if dtype is torch.float32 else 0,
+                                      _array(query_start, i32, requests + 1, "query_start", gpu), _array(context, i32, requests, "context", gpu),
+                                      _array(block_table, i32, 0, "block_table", gpu), width, requests, tokens, max_query, max_context, heads, *cache._pointers(gpu),
+                                      cache.kv_heads, head_dim, scale, window, _array(workspace, torch.uint8, scratch, "workspace", gpu), _array(out, dtype, need, "out", gpu)))
     return out
 
 
