@@ -63,15 +63,44 @@ struct PagedRequest {
     }
 };
 
+// The rows that a block of the prompt kernel takes: 256 (token, query head) rows of a request and kv head, and the key tiles they see.
+constexpr int kPpUnit = 256, kPpKeys = 128;
+struct PagedUnit {
+    int row0, live;  // first row of the request's, how many
+    int low, first;  // first position that a row attends, and the first position of tile 0 (whole groups of 16)
+    __device__ static PagedUnit of(const PagedArgs& a, const PagedRequest& q, int group, int unit) {
+        PagedUnit u;
+        u.row0 = unit * kPpUnit;
+        u.live = min(kPpUnit, q.rows * group - u.row0);
+        u.low = a.window > 0 ? max(0, q.pos0 + u.row0 / group - a.window + 1) : 0;
+        u.first = u.low & ~15;
+        return u;
+    }
+    __device__ int tiles_to(const PagedRequest& q, int group, int row) const {  // key tiles that a row's position needs
+        const int last = min(q.pos0 + (row0 + row) / group, q.hi - 1);
+        return last >= low ? (last - first) / kPpKeys + 1 : 0;
+    }
+    __device__ int tiles(const PagedRequest& q, int group) const { return tiles_to(q, group, live - 1); }
+};
+// What the prompt kernel's blocks do, in the order in which they start: entry 0 is the number of entries, then (request, unit, part of how many << 16 | part, place of
+// the unit's parts in the workspace).  A null list: none is wanted.
+struct PagedOrder {
+    int4* list;
+    int capacity;     // entries
+    int split_blocks; // parts (of all kv heads) that the workspace has room for
+};
+
 // paged_decode.cu: requests of at most kPagedDecodeRows rows, heads of 64 or 128
 constexpr int kPagedDecodeRows = 16;
 bool paged_decode_serves(int head_dim);
 size_t paged_decode_workspace_bytes(int requests, int kv_heads, int head_dim, int max_rows);
-int paged_decode_launch(cudaStream_t stream, const PagedArgs& a, bool f32, int max_rows, int max_context, void* workspace);
+int paged_decode_launch(cudaStream_t stream, const PagedArgs& a, bool f32, int max_rows, int max_context, void* workspace, const PagedOrder& order);
 
 // paged_prompt.cu: requests of more than a.skip_rows rows, heads of 64 or 128
 bool paged_prompt_serves(const PagedArgs& a);
-int paged_prompt_launch(cudaStream_t stream, const PagedArgs& a, bool f32);
+size_t paged_prompt_workspace_bytes(int heads, int kv_heads, int head_dim, int requests, int tokens);
+PagedOrder paged_prompt_order(const PagedArgs& a, void* workspace);
+int paged_prompt_launch(cudaStream_t stream, const PagedArgs& a, bool f32, void* workspace);
 int paged_prompt_status(int* status_out);  // 1 after a wait inside a kernel of that file ran out, 0 otherwise
 
 }  // namespace kmll

@@ -89,7 +89,9 @@ using namespace kmll;
 
 extern "C" size_t kmll_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim, int requests, int tokens, int max_query, int max_context) {
     if (heads <= 0 || kv_heads <= 0 || requests <= 0 || tokens <= 0 || max_query <= 0 || !paged_decode_serves(head_dim)) return 0;
-    return paged_decode_workspace_bytes(requests, kv_heads, head_dim, (long long)max_query * (heads / kv_heads) <= 8 ? 8 : kPagedDecodeRows);
+    const long long max_rows = (long long)max_query * (heads / kv_heads);
+    const size_t few = paged_decode_workspace_bytes(requests, kv_heads, head_dim, max_rows <= 8 ? 8 : kPagedDecodeRows);
+    return max_rows <= kPagedDecodeRows ? few : (few + 255) / 256 * 256 + paged_prompt_workspace_bytes(heads, kv_heads, head_dim, requests, tokens);
 }
 
 extern "C" int kmll_paged_attention(kmll_stream_t stream, const void* query, int is_f32, const int32_t* query_start, const int32_t* context, const int32_t* block_table,
@@ -114,13 +116,17 @@ extern "C" int kmll_paged_attention(kmll_stream_t stream, const void* query, int
     if (paged_decode_serves(head_dim) && (reinterpret_cast<uintptr_t>(query) & 15u) == 0) {
         KMLL_REQUIRE_PTR(workspace);
         KMLL_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "paged attention: the workspace must be 16-byte aligned");
-        KMLL_TRY_RC(paged_decode_launch(as_stream(stream), a, is_f32 != 0, max_rows <= 8 ? 8 : kPagedDecodeRows, max_context, workspace));
-        if (max_rows <= kPagedDecodeRows) return check_launch("paged attention");
+        const size_t few = (paged_decode_workspace_bytes(requests, kv_heads, head_dim, max_rows <= 8 ? 8 : kPagedDecodeRows) + 255) / 256 * 256;
+        void* const rest = static_cast<unsigned char*>(workspace) + few;
+        const bool many = max_rows > kPagedDecodeRows && paged_prompt_serves(a);
         a.skip_rows = kPagedDecodeRows;
-    }
-    if (paged_prompt_serves(a)) {
-        KMLL_TRY_RC(paged_prompt_launch(as_stream(stream), a, is_f32 != 0));
-        return check_launch("paged attention");
+        KMLL_TRY_RC(paged_decode_launch(as_stream(stream), a, is_f32 != 0, max_rows <= 8 ? 8 : kPagedDecodeRows, max_context, workspace,
+                                        many ? paged_prompt_order(a, rest) : PagedOrder{nullptr, 0, 0}));
+        if (max_rows <= kPagedDecodeRows) return check_launch("paged attention");
+        if (many) {
+            KMLL_TRY_RC(paged_prompt_launch(as_stream(stream), a, is_f32 != 0, rest));
+            return check_launch("paged attention");
+        }
     }
     const cudaError_t e = is_f32 ? launch(paged_rows_kernel<float>, dim3(tokens, kv_heads), dim3(128), 0, as_stream(stream), true, a)
                                  : launch(paged_rows_kernel<uint16_t>, dim3(tokens, kv_heads), dim3(128), 0, as_stream(stream), true, a);

@@ -13,6 +13,7 @@
 // tiles, cut into equal shares for the blocks, whatever the contexts; where a share ends within a head, the blocks that have parts of it leave
 // maximum, sum and O in the workspace and the last to arrive joins them in the order of the blocks: results do not change from call to call.
 // Bound: HBM (2 * head_dim bytes per key and kv head).
+#include <climits>
 #include <type_traits>
 
 #include "internal.cuh"
@@ -89,9 +90,76 @@ __device__ inline int pd_tiles(const PagedRequest& q, int group, int limit) {
 }
 __device__ inline long long pd_length(int tiles) { return tiles > 0 ? tiles + kPdStretch : 0; }
 
+// ---- the order of the prompt kernel's blocks (one block of this kernel, beside those that attend) ---------------------------------------------
+// A unit of T key tiles costs about T + kPdFixed; 148 run at once.  Units are cut into parts of at most `cut` tiles where that evens out the
+// end: of sixteen cuts the one with the smallest max(longest, all / 148 + half of the longest) is taken.  The longest parts start first.
+constexpr int kPdFixed = 3, kPdCuts = 16;
+__device__ inline void paged_order(const PagedArgs& a, const PagedOrder& o, int group) {
+    __shared__ int s_most, s_bucket[64], s_cut, s_place;
+    __shared__ int s_parts[kPdCuts], s_split[kPdCuts], s_tiles;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // f(request, unit, its tiles) over all units: warps take requests, lanes units
+    auto each = [&](auto f) {
+        for (int r = warp; r < a.requests; r += kPdWarps) {
+            const PagedRequest q = PagedRequest::of(a, r);
+            const long long rows = (long long)q.rows * group;
+            if (rows <= a.skip_rows) continue;
+            for (int u = lane; u < (int)((rows + kPpUnit - 1) / kPpUnit); u += 32) f(r, u, PagedUnit::of(a, q, group, u).tiles(q, group));
+        }
+        __syncthreads();
+    };
+    if (tid < 64) s_bucket[tid] = 0;
+    if (tid < kPdCuts) s_parts[tid] = s_split[tid] = 0;
+    if (tid == 0) s_most = s_tiles = s_place = 0;
+    __syncthreads();
+    each([&](int, int, int tiles) {
+        atomicMax(&s_most, tiles);
+        atomicAdd(&s_tiles, tiles);
+    });
+    const int most = max(s_most, 1);
+    auto cut_of = [&](int i) { return max(4, (most * (kPdCuts - i) + kPdCuts - 1) / kPdCuts); };  // i = 0: whole units
+    each([&](int, int, int tiles) {
+        for (int i = 0; i < kPdCuts; ++i) {
+            const int parts = max(1, (tiles + cut_of(i) - 1) / cut_of(i));
+            atomicAdd(&s_parts[i], parts);
+            if (parts > 1) atomicAdd(&s_split[i], parts);
+        }
+    });
+    if (tid == 0) {
+        float best = INFINITY;
+        for (int i = 0; i < kPdCuts; ++i) {
+            if (i > 0 && ((long long)s_split[i] * a.kv_heads > o.split_blocks || s_parts[i] > o.capacity)) continue;
+            const float longest = (float)(min(cut_of(i), most) + kPdFixed + (s_split[i] > 0 ? kPdFixed : 0));
+            const float all = ((float)s_tiles + (float)s_parts[i] * kPdFixed) * (float)a.kv_heads / 148.0f;
+            const float cost = fmaxf(longest, all + 0.5f * longest);
+            if (cost < best) { best = cost; s_cut = cut_of(i); }
+        }
+    }
+    __syncthreads();
+    const int cut = s_cut;
+    auto parts_of = [&](int tiles) { return cut >= most ? 1 : max(1, (tiles + cut - 1) / cut); };
+    auto bucket_of = [&](int tiles, int parts) { return 63 - min(63, (tiles + parts - 1) / parts * 64 / (min(cut, most) + 1)); };
+    each([&](int, int, int tiles) { atomicAdd(&s_bucket[bucket_of(tiles, parts_of(tiles))], parts_of(tiles)); });
+    if (tid == 0) {
+        int at = 0;
+        for (int b = 0; b < 64; ++b) {
+            const int n = s_bucket[b];
+            s_bucket[b] = at;
+            at += n;
+        }
+        o.list[0] = make_int4(min(at, o.capacity), 0, 0, 0);
+    }
+    __syncthreads();
+    each([&](int r, int u, int tiles) {
+        const int parts = parts_of(tiles), place = parts > 1 ? atomicAdd(&s_place, parts) : 0, at = atomicAdd(&s_bucket[bucket_of(tiles, parts)], parts);
+        for (int p = 0; p < parts; ++p)
+            if (at + p < o.capacity) o.list[1 + at + p] = make_int4(r, u, parts << 16 | p, place);
+    });
+}
+
 // NB: bytes of q and of the weights; NC: columns of eight rows.
 template <int HD, typename T, int NB, int NC>
-__global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kernel(const PagedArgs a, const PdWork work) {
+__global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kernel(const PagedArgs a, const PdWork work, const PagedOrder order) {
     using S = PdShape<HD>;
     constexpr int KS = HD / 32, DT = HD / 16, ROWS = 8 * NC, PITCH = HD + 4;
     extern __shared__ __align__(128) unsigned char pd_smem[];
@@ -100,6 +168,11 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
     __shared__ int s_request, s_last;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, group = a.heads / a.kv_heads;
     pdl_wait();
+    const int blocks = (int)gridDim.x - (order.list != nullptr ? 1 : 0);
+    if ((int)blockIdx.x == blocks) {
+        paged_order(a, order, group);
+        return;
+    }
     // ---- the share of this block
     const int per = (a.requests + kPdThreads - 1) / kPdThreads;
     long long mine = 0;
@@ -124,7 +197,7 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
     total *= a.kv_heads;
     before *= a.kv_heads;
     mine *= a.kv_heads;
-    const long long share = max((long long)kPdWarps, (total + gridDim.x - 1) / gridDim.x);
+    const long long share = max((long long)kPdWarps, (total + blocks - 1) / blocks);
     const long long w0 = (long long)blockIdx.x * share, w1 = min(total, w0 + share);
     if (w0 >= w1) return;
     if (w0 >= before && w0 < before + mine) {
@@ -531,16 +604,16 @@ size_t paged_decode_workspace_bytes(int requests, int kv_heads, int head_dim, in
     return pd_counter_bytes(requests, kv_heads) + (size_t)kPdBlocks * 2 * (max_rows <= 8 ? 8 : 16) * (head_dim + 2) * 4;
 }
 
-int paged_decode_launch(cudaStream_t stream, const PagedArgs& a, bool f32, int max_rows, int max_context, void* workspace) {
+int paged_decode_launch(cudaStream_t stream, const PagedArgs& a, bool f32, int max_rows, int max_context, void* workspace, const PagedOrder& order) {
     PdWork work;
     work.arrived = static_cast<int*>(workspace);
     work.partials = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + pd_counter_bytes(a.requests, a.kv_heads));
     // no more blocks than there can be shares of one tile a warp
     const long long most = (long long)a.requests * a.kv_heads * (max_context / kPdKeys + 2 + kPdStretch), blocks = (most + kPdWarps - 1) / kPdWarps;
-    const dim3 grid((unsigned)(blocks < kPdBlocks ? blocks : kPdBlocks));
+    const dim3 grid((unsigned)(blocks < kPdBlocks ? blocks : kPdBlocks) + (order.list != nullptr ? 1 : 0));
     auto go = [&](auto kern, int smem) {
         const cudaError_t e = allow_all_dynamic_smem(kern);
-        return e != cudaSuccess ? e : launch(kern, grid, dim3(kPdThreads), (size_t)smem, stream, true, a, work);
+        return e != cudaSuccess ? e : launch(kern, grid, dim3(kPdThreads), (size_t)smem, stream, true, a, work, order);
     };
     auto pick = [&](auto hd) {
         constexpr int HD = decltype(hd)::value;

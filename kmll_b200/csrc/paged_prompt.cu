@@ -14,7 +14,8 @@
 //   warps 16-23      fetch the codes of a tile of 128 keys into registers while the tile before is at work, and write them as binary16 operands
 //                    (128-byte swizzle, both K-major: values lie with the keys of a column together)
 //   warp 24          issues S = Q K^T and O += P V
-// O is rescaled only when a row's maximum has grown by more than 2^8.  Every wait is bounded; a time-out raises the status word, and
+// O is rescaled only when a row's maximum has grown by more than 2^8.  Which rows a block takes, and which part of their keys, stands in a list that a block of the
+// kernel for few rows has made (paged_decode.cu): parts leave maximum, sum and O in the workspace, and the last to arrive joins them in order.  Every wait is bounded; a time-out raises the status word, and
 // the block frees its tensor memory and returns (no copies are under way: the fetches are loads).
 #include <climits>
 #include <type_traits>
@@ -30,7 +31,7 @@ __device__ int g_paged_prompt_status = 0;
 
 namespace {
 
-constexpr int kPpRows = 128, kPpKeys = 128, kPpGroups = kPpKeys / 16;
+constexpr int kPpRows = 128, kPpGroups = kPpKeys / 16;
 constexpr int kPpConvert = 16, kPpIssue = 24;  // first warps of the roles behind the softmax
 constexpr int kPpThreads = 28 * 32;
 // Registers a thread: 72 at the launch (896 threads), then by warpgroup: 4 * 128 * 88 + 2 * 128 * 64 + 128 * 24 = 896 * 72.
@@ -125,8 +126,17 @@ __device__ inline uint64_t pp_add2(uint64_t a, uint64_t b) {
     return d;
 }
 
+struct PpWork {
+    const int4* list;
+    int* arrived;      // [parts' places * kv heads], zero between calls
+    float* partials;   // [parts' places * kv heads]: (maximum, sum) of 256 rows, then their O
+};
+template <int HD>
+__host__ __device__ constexpr size_t pp_partial_floats() { return (size_t)kPpUnit * (HD + 2); }
+constexpr int kPpSplitBlocks = 296;  // two for each multiprocessor
+
 template <int HD, typename T>
-__global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const PagedArgs a, const PpWork work) {
     constexpr int NP = sizeof(T) == 4 ? 2 : 1;
     using S = PpShape<HD, NP>;
     constexpr int kStages = S::kStages;
@@ -142,12 +152,15 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
     uint64_t* const sc_full = v_free + 2;    // [4] the scales of a tile are there
     uint64_t* const pair = sc_full + 4;      // [8] both threads of a row have left their maxima
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(pair + 8);
-    int* const s_unit = reinterpret_cast<int*>(tmem_slot + 1);  // request, unit of 256 rows
+    int* const s_last = reinterpret_cast<int*>(tmem_slot + 1);  // all other parts of the unit have arrived
     PpScales* const scales = reinterpret_cast<PpScales*>(smem + S::kOffScales);
     float* const units = reinterpret_cast<float*>(smem + S::kOffUnit);
     int* const row_of = reinterpret_cast<int*>(units + 2 * kPpRows);  // rows of the block among the step's (token, head) rows
     const int tid = threadIdx.x, lane = tid & 31, warp = uniform_warp_index(), group = a.heads / a.kv_heads, h = blockIdx.x;
     const int block_log = 31 - __clz(a.block), in_block = a.block - 1;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if ((int)blockIdx.y >= work.list[0].x) return;
+    const int4 entry = work.list[1 + blockIdx.y];
     if (tid == 0) {
         for (int b = 0; b < 2; ++b) {
             mbar_init(&s_full[b], 1);
@@ -161,7 +174,6 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
         for (int b = 0; b < 4; ++b) mbar_init(&sc_full[b], 1);
         for (int b = 0; b < 8; ++b) mbar_init(&pair[b], 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        s_unit[0] = -1;
     }
     if (warp == kPpIssue) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
@@ -170,48 +182,19 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
     tcgen05_fence_before();
     __syncthreads();  // (columns first, then the dependents: tcgen05.cuh)
     tcgen05_fence_after();
-    pdl_wait();
-    // ---- the block's request and rows: units of 256 rows, request after request, the last rows of a request (which see most) first
-    if (warp == 0) {
-        int before = 0;
-        for (int r0 = 0; r0 < a.requests; r0 += 32) {
-            const int r = r0 + lane;
-            int n = 0;
-            if (r < a.requests) {
-                const long long rows = (long long)PagedRequest::of(a, r).rows * group;
-                n = rows > a.skip_rows ? (int)((rows + 2 * kPpRows - 1) / (2 * kPpRows)) : 0;
-            }
-            int up = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, up, o);
-                if (lane >= o) up += v;
-            }
-            const int at = (int)blockIdx.y - before - (up - n);
-            if (n > 0 && at >= 0 && at < n) {
-                s_unit[0] = r;
-                s_unit[1] = n - 1 - at;
-            }
-            before += __shfl_sync(0xffffffffu, up, 31);
-            if ((int)blockIdx.y < before) break;
-        }
-    }
-    __syncthreads();
-    const int request = s_unit[0];
+    pdl_launch_dependents();
     bool ok = true;
-    if (request >= 0) {
-        const PagedRequest rq = PagedRequest::of(a, request);
-        const int row0 = s_unit[1] * 2 * kPpRows, live = min(2 * kPpRows, rq.rows * group - row0);
+    {
+        const PagedRequest rq = PagedRequest::of(a, entry.x);
+        const PagedUnit un = PagedUnit::of(a, rq, group, entry.y);
+        const int parts = entry.z >> 16, part = entry.z & 0xffff;
+        const int row0 = un.row0, live = un.live, low = un.low;
         const bool two = live > kPpRows;  // two tiles of rows; else two shares of the keys
-        // positions of rows r .. e - 1 of the block (a context longer than its table row is cut at the table's end)
-        auto own_pos = [&](int r) { return rq.pos0 + (row0 + r) / group; };
-        const int low = a.window > 0 ? max(0, own_pos(0) - a.window + 1) : 0, first = low & ~15;
-        auto tiles_to = [&](int r) {  // key tiles that row r's position needs
-            const int last = min(own_pos(r), rq.hi - 1);
-            return last >= low ? (last - first) / kPpKeys + 1 : 0;
-        };
-        const int tiles = tiles_to(live - 1);
-        const int tiles0 = two ? tiles_to(kPpRows - 1) : tiles;  // of the first stream where the streams are tiles of rows
+        auto own_pos = [&](int r) { return rq.pos0 + (row0 + r) / group; };  // (a context longer than its table row is cut at the table's end)
+        // this part's tiles, counted from its first one
+        const int all_tiles = un.tiles(rq, group), size = (all_tiles + parts - 1) / parts, from_tile = min(all_tiles, part * size);
+        const int tiles = min(size, all_tiles - from_tile), first = un.first + from_tile * kPpKeys;
+        const int tiles0 = two ? min(tiles, max(0, un.tiles_to(rq, group, kPpRows - 1) - from_tile)) : tiles;  // of the first stream where the streams are tiles of rows
         // ---- Q: a warp has a row at a time, HD / 32 entries a lane; its largest entry gives the power of two
         constexpr int E = HD / 32, kWarps = kPpThreads / 32, kBatch = 5;
         for (int r0 = warp; r0 < (two ? 2 : 1) * kPpRows; r0 += kWarps * kBatch) {
@@ -267,7 +250,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
             asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
             // ---- codes to operands
             const int tt = tid - 32 * kPpConvert & 127, side = tid - 32 * kPpConvert >> 7;  // the key; of the values the group of 16 keys tt / 16, columns tt % 16, + 16, ..; half of either
-            const int32_t* const table = a.table + (size_t)request * a.width;
+            const int32_t* const table = a.table + (size_t)entry.x * a.width;
             constexpr int U = HD / 32;  // 16-byte groups of half a key; columns of a group of values per thread
             uint4 kc[U], vc[U];
             auto entry_of = [&](int j) {  // lanes 0-7 (and again): table entry of group lane & 7 of tile j; looked at a tile later, when it has come
@@ -461,7 +444,8 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                         const float f = sc.k[2 * c + k] * unit, off = sc.log_v[2 * c + k] - m;
                         const uint64_t ff = pp_pair(f, f), oo = pp_pair(off, off);
                         uint64_t sum = 0ull;
-                        uint32_t hi[8], rest[NP == 2 ? 8 : 1];
+                        uint32_t hi[8];
+                        [[maybe_unused]] uint32_t rest[NP == 2 ? 8 : 1];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             const int at = 8 * k + i;
@@ -542,8 +526,10 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
             const float m0 = stat[r].x, m1 = stat[2 * kPpRows + r].x, l0 = stat[r].y + stat[kPpRows + r].y, l1 = stat[2 * kPpRows + r].y + stat[3 * kPpRows + r].y;
             const float m = fmaxf(m0, m1), mm = m == -INFINITY ? 0.0f : m;
             const float w0 = ex2_approx(m0 - mm), w1 = ex2_approx(m1 - mm), sum = two ? (stream == 0 ? l0 : l1) : l0 * w0 + l1 * w1, inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            const float f0 = two ? inv : w0 * inv, f1 = w1 * inv;
+            const float whole = parts > 1 ? 1.0f : inv, f0 = two ? whole : w0 * whole, f1 = w1 * whole;
             const bool any0 = two ? n > 0 : tiles > 0, any1 = !two && tiles > 1;
+            float* const partial = work.partials + (size_t)((entry.w + part) * a.kv_heads + h) * pp_partial_floats<HD>();
+            if (parts > 1 && half == 0 && (two || stream == 0)) reinterpret_cast<float2*>(partial)[two ? in_unit : r] = make_float2(two ? m_ref : m, sum);
             // half of the columns each: of the stream's rows, or (one tile of rows) a quarter for each of the four warps
             const int columns = two ? HD / 2 : HD / 4, from = two ? half * columns : (stream * 2 + half) * columns;
             // the last MMAs are done and nobody loads: the rows leave over the operands' shared memory, so that a warp writes whole runs
@@ -570,17 +556,53 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
             for (int i = lane; i < 32 * quads; i += 32) {
                 const int rr = i / quads, c4 = i % quads, row = (two ? stream * kPpRows : 0) + (warp & 3) * 32 + rr;
                 if (!ok || row >= live) continue;
-                T* const out = static_cast<T*>(a.out) + (size_t)row_of[row] * HD + from + c4 * 4;
                 const float4 y = *reinterpret_cast<const float4*>(stage + rr * S::kStagePitch + c4 * 4);
+                if (parts > 1) {
+                    *reinterpret_cast<float4*>(partial + 2 * kPpUnit + row * HD + from + c4 * 4) = y;
+                    continue;
+                }
+                T* const out = static_cast<T*>(a.out) + (size_t)row_of[row] * HD + from + c4 * 4;
                 if constexpr (sizeof(T) == 4) {
                     *reinterpret_cast<float4*>(out) = y;
                 } else {
                     *reinterpret_cast<uint2*>(out) = make_uint2(bf16_pair_of(y.x, y.y), bf16_pair_of(y.z, y.w));
                 }
             }
+            if (parts > 1) {
+                __threadfence();
+                asm volatile("bar.sync 1, 512;" ::: "memory");
+                int* const arrived = work.arrived + entry.w * a.kv_heads + h;
+                if (tid == 0) *s_last = atomicAdd(arrived, 1) == parts - 1;
+                asm volatile("bar.sync 1, 512;" ::: "memory");
+                if (*s_last != 0) {
+                    __threadfence();
+                    if (tid == 0) *arrived = 0;
+                    const float* const p0 = work.partials + (size_t)(entry.w * a.kv_heads + h) * pp_partial_floats<HD>();
+                    const size_t pitch = (size_t)a.kv_heads * pp_partial_floats<HD>();
+                    for (int i = tid; i < live * (HD / 4); i += 512) {
+                        const int row = i / (HD / 4), c = i % (HD / 4) * 4;
+                        float top = -INFINITY, all = 0.0f;
+                        for (int k = 0; k < parts; ++k) top = fmaxf(top, __ldcg(p0 + k * pitch + 2 * row));
+                        const float base_top = top == -INFINITY ? 0.0f : top;
+                        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 2
+                        for (int k = 0; k < parts; ++k) {
+                            const float2 st = __ldcg(reinterpret_cast<const float2*>(p0 + k * pitch) + row);
+                            const float4 x = __ldcg(reinterpret_cast<const float4*>(p0 + k * pitch + 2 * kPpUnit + row * HD + c));
+                            const float f = ex2_approx(st.x - base_top);
+                            all = fmaf(st.y, f, all);
+                            y.x = fmaf(x.x, f, y.x); y.y = fmaf(x.y, f, y.y); y.z = fmaf(x.z, f, y.z); y.w = fmaf(x.w, f, y.w);
+                        }
+                        const float over = all == 0.0f ? 0.0f : 1.0f / all;
+                        T* const out = static_cast<T*>(a.out) + (size_t)row_of[row] * HD + c;
+                        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = make_float4(y.x * over, y.y * over, y.z * over, y.w * over);
+                        else *reinterpret_cast<uint2*>(out) = make_uint2(bf16_pair_of(y.x * over, y.y * over), bf16_pair_of(y.z * over, y.w * over));
+                    }
+                }
+            }
         }
     }
-    if (request >= 0 && warp > kPpIssue) asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
+    if (warp > kPpIssue) asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
     if (!ok) atomicCAS(&g_paged_prompt_status, 0, 1);
     tcgen05_fence_before();
     __syncthreads();
@@ -594,16 +616,38 @@ bool paged_prompt_serves(const PagedArgs& a) {
     return (a.head_dim == 64 || a.head_dim == 128) && ((reinterpret_cast<uintptr_t>(a.query) | reinterpret_cast<uintptr_t>(a.out)) & 15u) == 0;
 }
 
-int paged_prompt_launch(cudaStream_t stream, const PagedArgs& a, bool f32) {
-    const int group = a.heads / a.kv_heads;
-    const long long tiles = ((long long)a.tokens * group + 2 * kPpRows - 1) / (2 * kPpRows) + a.requests;  // each request ends in a unit of its own
-    KMLL_REQUIRE(tiles <= 65535 && (long long)a.tokens * a.heads <= INT_MAX, "paged attention: too many rows");
+namespace {
+long long pp_units(int heads, int kv_heads, int requests, int tokens) {  // each request ends in a unit of its own
+    return ((long long)tokens * (heads / kv_heads) + kPpUnit - 1) / kPpUnit + requests;
+}
+int pp_capacity(int heads, int kv_heads, int requests, int tokens) {
+    const long long n = pp_units(heads, kv_heads, requests, tokens) + kPpSplitBlocks / kv_heads;
+    return (int)(n < 65535 ? n : 65535);
+}
+size_t pp_list_bytes(int capacity) { return ((size_t)(1 + capacity) * sizeof(int4) + 255) / 256 * 256; }
+constexpr size_t kPpArrivedBytes = (kPpSplitBlocks * 4 + 255) / 256 * 256;
+}  // namespace
+
+size_t paged_prompt_workspace_bytes(int heads, int kv_heads, int head_dim, int requests, int tokens) {
+    return pp_list_bytes(pp_capacity(heads, kv_heads, requests, tokens)) + kPpArrivedBytes + kPpSplitBlocks * sizeof(float) * (size_t)kPpUnit * (head_dim + 2);
+}
+
+PagedOrder paged_prompt_order(const PagedArgs& a, void* workspace) {
+    return PagedOrder{static_cast<int4*>(workspace), pp_capacity(a.heads, a.kv_heads, a.requests, a.tokens), kPpSplitBlocks};
+}
+
+int paged_prompt_launch(cudaStream_t stream, const PagedArgs& a, bool f32, void* workspace) {
+    if (pp_units(a.heads, a.kv_heads, a.requests, a.tokens) > 65535 || (long long)a.tokens * a.heads > INT_MAX)
+        return fail(KMLL_ERR_CAPACITY, "paged attention: %d tokens of %d heads in one call", a.tokens, a.heads);
+    const int capacity = pp_capacity(a.heads, a.kv_heads, a.requests, a.tokens);
+    unsigned char* const at = static_cast<unsigned char*>(workspace) + pp_list_bytes(capacity);
+    const PpWork work = {static_cast<const int4*>(workspace), reinterpret_cast<int*>(at), reinterpret_cast<float*>(at + kPpArrivedBytes)};
     auto go = [&](auto kern, int smem) {
         cudaFuncAttributes fa;
         cudaError_t e = cudaFuncGetAttributes(&fa, kern);
         if (e == cudaSuccess && fa.numRegs < kPpRegsLaunch) e = cudaErrorInvalidDeviceFunction;  // (the warpgroups would wait for registers that the block does not have)
         if (e == cudaSuccess) e = allow_all_dynamic_smem(kern);
-        return e != cudaSuccess ? e : launch(kern, dim3(a.kv_heads, (unsigned)tiles), dim3(kPpThreads), (size_t)smem, stream, true, a);
+        return e != cudaSuccess ? e : launch(kern, dim3(a.kv_heads, (unsigned)capacity), dim3(kPpThreads), (size_t)smem, stream, true, a, work);
     };
     cudaError_t e;
     if (a.head_dim == 128) e = f32 ? go(paged_prompt_kernel<128, float>, PpShape<128, 2>::kSmemBytes) : go(paged_prompt_kernel<128, uint16_t>, PpShape<128, 1>::kSmemBytes);
