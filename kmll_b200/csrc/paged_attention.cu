@@ -87,10 +87,14 @@ __global__ void __launch_bounds__(128) paged_rows_kernel(const PagedArgs a) {
 
 using namespace kmll;
 
+// Rows up to which a request goes to the kernel for few rows.  Eight take half of the registers of sixteen (three blocks on a multiprocessor for two); sixteen are for
+// calls that have no more, and for heads in groups of more than eight, whose single tokens need them.
+static int few_rows(long long max_rows, int group) { return max_rows <= 8 || (max_rows > kPagedDecodeRows && group <= 8) ? 8 : kPagedDecodeRows; }
+
 extern "C" size_t kmll_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim, int requests, int tokens, int max_query, int max_context) {
     if (heads <= 0 || kv_heads <= 0 || requests <= 0 || tokens <= 0 || max_query <= 0 || !paged_decode_serves(head_dim)) return 0;
     const long long max_rows = (long long)max_query * (heads / kv_heads);
-    const size_t few = paged_decode_workspace_bytes(requests, kv_heads, head_dim, max_rows <= 8 ? 8 : kPagedDecodeRows);
+    const size_t few = paged_decode_workspace_bytes(requests, kv_heads, head_dim, few_rows(max_rows, heads / kv_heads));
     return max_rows <= kPagedDecodeRows ? few : (few + 255) / 256 * 256 + paged_prompt_workspace_bytes(heads, kv_heads, head_dim, requests, tokens);
 }
 
@@ -116,11 +120,12 @@ extern "C" int kmll_paged_attention(kmll_stream_t stream, const void* query, int
     if (paged_decode_serves(head_dim) && (reinterpret_cast<uintptr_t>(query) & 15u) == 0) {
         KMLL_REQUIRE_PTR(workspace);
         KMLL_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "paged attention: the workspace must be 16-byte aligned");
-        const size_t few = (paged_decode_workspace_bytes(requests, kv_heads, head_dim, max_rows <= 8 ? 8 : kPagedDecodeRows) + 255) / 256 * 256;
+        const int limit = few_rows(max_rows, heads / kv_heads);
+        const size_t few = (paged_decode_workspace_bytes(requests, kv_heads, head_dim, limit) + 255) / 256 * 256;
         void* const rest = static_cast<unsigned char*>(workspace) + few;
         const bool many = max_rows > kPagedDecodeRows && paged_prompt_serves(a);
-        a.skip_rows = kPagedDecodeRows;
-        KMLL_TRY_RC(paged_decode_launch(as_stream(stream), a, is_f32 != 0, max_rows <= 8 ? 8 : kPagedDecodeRows, max_context, workspace,
+        a.skip_rows = limit;
+        KMLL_TRY_RC(paged_decode_launch(as_stream(stream), a, is_f32 != 0, limit, max_context, workspace,
                                         many ? paged_prompt_order(a, rest) : PagedOrder{nullptr, 0, 0}));
         if (max_rows <= kPagedDecodeRows) return check_launch("paged attention");
         if (many) {

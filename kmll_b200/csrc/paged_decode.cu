@@ -26,7 +26,7 @@ namespace {
 constexpr int kPdWarps = 4;
 constexpr int kPdThreads = kPdWarps * 32;
 constexpr int kPdKeys = 32;      // keys of a tile
-constexpr int kPdBlocks = 444;   // three blocks on each of 148 multiprocessors
+constexpr int kPdBlocks = 444;   // three blocks on each of 148 multiprocessors (sixteen rows: two)
 constexpr int kPdStages = 2;
 // What a stretch costs besides its tiles (queries, first copies, the warps' meeting), in tiles: so much longer is a head on the axis of work, or
 // blocks whose share is many short requests would end last (64 requests of 100 to 8000 tokens, 32 / 8 heads of 128: 0 tiles 96 us,
@@ -92,69 +92,126 @@ __device__ inline long long pd_length(int tiles) { return tiles > 0 ? tiles + kP
 
 // ---- the order of the prompt kernel's blocks (one block of this kernel, beside those that attend) ---------------------------------------------
 // A unit of T key tiles costs about T + kPdFixed; 148 run at once.  Units are cut into parts of at most `cut` tiles where that evens out the
-// end: of sixteen cuts the one with the smallest max(longest, all / 148 + half of the longest) is taken.  The longest parts start first.
-constexpr int kPdFixed = 3, kPdCuts = 16;
-__device__ inline void paged_order(const PagedArgs& a, const PagedOrder& o, int group) {
-    __shared__ int s_most, s_bucket[64], s_cut, s_place;
-    __shared__ int s_parts[kPdCuts], s_split[kPdCuts], s_tiles;
+// end: of sixteen cuts the one with the smallest max(longest, all / 148 + half of the longest) is taken.  The longest parts start first.  More units
+// than kPdUnits even out by themselves: they go in the order of the requests, the last rows of each first, whole.
+constexpr int kPdFixed = 3, kPdCuts = 16, kPdUnits = 2048;
+struct PdOrderShared {
+    int request[kPdUnits];
+    unsigned short unit[kPdUnits], tiles[kPdUnits];
+    int bucket[64], cost_parts[kPdCuts], cost_split[kPdCuts], warp_sum[kPdWarps], most, all, cut, place;
+};
+__device__ inline void paged_order(const PagedArgs& a, const PagedOrder& o, int group, PdOrderShared& s) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // f(request, unit, its tiles) over all units: warps take requests, lanes units
-    auto each = [&](auto f) {
-        for (int r = warp; r < a.requests; r += kPdWarps) {
-            const PagedRequest q = PagedRequest::of(a, r);
-            const long long rows = (long long)q.rows * group;
-            if (rows <= a.skip_rows) continue;
-            for (int u = lane; u < (int)((rows + kPpUnit - 1) / kPpUnit); u += 32) f(r, u, PagedUnit::of(a, q, group, u).tiles(q, group));
+    if (tid < 64) s.bucket[tid] = 0;
+    if (tid == 0) s.most = s.all = s.place = 0;
+    // ---- units, request after request
+    int units = 0;
+    for (int r0 = 0; r0 < a.requests; r0 += kPdThreads) {
+        const int r = r0 + tid;
+        int n = 0;
+        if (r < a.requests) {
+            const long long rows = (long long)PagedRequest::of(a, r).rows * group;
+            n = rows > a.skip_rows ? (int)((rows + kPpUnit - 1) / kPpUnit) : 0;
+        }
+        int up = n;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, up, d);
+            if (lane >= d) up += v;
         }
         __syncthreads();
-    };
-    if (tid < 64) s_bucket[tid] = 0;
-    if (tid < kPdCuts) s_parts[tid] = s_split[tid] = 0;
-    if (tid == 0) s_most = s_tiles = s_place = 0;
+        if (lane == 31) s.warp_sum[warp] = up;
+        __syncthreads();
+        int base = units + up - n;
+        for (int w = 0; w < kPdWarps; ++w) {
+            if (w < warp) base += s.warp_sum[w];
+            units += s.warp_sum[w];
+        }
+        for (uint32_t bits = __ballot_sync(0xffffffffu, n > 0); bits != 0u; bits &= bits - 1u) {  // a warp fills in its requests one by one
+            const int from = __ffs(bits) - 1, b = __shfl_sync(0xffffffffu, base, from), m = __shfl_sync(0xffffffffu, n, from), rr = __shfl_sync(0xffffffffu, r, from);
+            for (int u = lane; u < m; u += 32) {
+                const int last_first = m - 1 - u;
+                if (b + u < o.capacity) o.list[1 + b + u] = make_int4(rr, last_first, 1 << 16, 0);
+                if (b + u < kPdUnits) {
+                    s.request[b + u] = rr;
+                    s.unit[b + u] = (unsigned short)last_first;
+                }
+            }
+        }
+    }
+    if (tid == 0) o.list[0] = make_int4(min(units, o.capacity), 0, 0, 0);
+    if (units > kPdUnits) return;
     __syncthreads();
-    each([&](int, int, int tiles) {
-        atomicMax(&s_most, tiles);
-        atomicAdd(&s_tiles, tiles);
-    });
-    const int most = max(s_most, 1);
+    // ---- their tiles
+    int most = 0, all = 0;
+    for (int i = tid; i < units; i += kPdThreads) {
+        const PagedRequest q = PagedRequest::of(a, s.request[i]);
+        const int tiles = min(65535, PagedUnit::of(a, q, group, s.unit[i]).tiles(q, group));
+        s.tiles[i] = (unsigned short)tiles;
+        most = max(most, tiles);
+        all += tiles;
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    all = __reduce_add_sync(0xffffffffu, all);
+    if (lane == 0) {
+        atomicMax(&s.most, most);
+        atomicAdd(&s.all, all);
+    }
+    __syncthreads();
+    most = max(s.most, 1);
     auto cut_of = [&](int i) { return max(4, (most * (kPdCuts - i) + kPdCuts - 1) / kPdCuts); };  // i = 0: whole units
-    each([&](int, int, int tiles) {
-        for (int i = 0; i < kPdCuts; ++i) {
-            const int parts = max(1, (tiles + cut_of(i) - 1) / cut_of(i));
-            atomicAdd(&s_parts[i], parts);
-            if (parts > 1) atomicAdd(&s_split[i], parts);
+    for (int i = warp; i < kPdCuts; i += kPdWarps) {
+        const int cut = cut_of(i);
+        int parts = 0, split = 0;
+        for (int j = lane; j < units; j += 32) {
+            const int n = max(1, (s.tiles[j] + cut - 1) / cut);
+            parts += n;
+            split += n > 1 ? n : 0;
         }
-    });
-    if (tid == 0) {
-        float best = INFINITY;
-        for (int i = 0; i < kPdCuts; ++i) {
-            if (i > 0 && ((long long)s_split[i] * a.kv_heads > o.split_blocks || s_parts[i] > o.capacity)) continue;
-            const float longest = (float)(min(cut_of(i), most) + kPdFixed + (s_split[i] > 0 ? kPdFixed : 0));
-            const float all = ((float)s_tiles + (float)s_parts[i] * kPdFixed) * (float)a.kv_heads / 148.0f;
-            const float cost = fmaxf(longest, all + 0.5f * longest);
-            if (cost < best) { best = cost; s_cut = cut_of(i); }
-        }
+        parts = __reduce_add_sync(0xffffffffu, parts);
+        split = __reduce_add_sync(0xffffffffu, split);
+        if (lane == 0) { s.cost_parts[i] = parts; s.cost_split[i] = split; }
     }
     __syncthreads();
-    const int cut = s_cut;
-    auto parts_of = [&](int tiles) { return cut >= most ? 1 : max(1, (tiles + cut - 1) / cut); };
-    auto bucket_of = [&](int tiles, int parts) { return 63 - min(63, (tiles + parts - 1) / parts * 64 / (min(cut, most) + 1)); };
-    each([&](int, int, int tiles) { atomicAdd(&s_bucket[bucket_of(tiles, parts_of(tiles))], parts_of(tiles)); });
-    if (tid == 0) {
-        int at = 0;
-        for (int b = 0; b < 64; ++b) {
-            const int n = s_bucket[b];
-            s_bucket[b] = at;
-            at += n;
+    if (warp == 0) {
+        unsigned long long mine = ~0ull;  // (cost, which): the smallest cost, of equal ones the longest parts
+        if (lane < kPdCuts) {
+            const int parts = s.cost_parts[lane], split = s.cost_split[lane];
+            const float longest = (float)(min(cut_of(lane), most) + kPdFixed + (split > 0 ? kPdFixed : 0));
+            const float cost = fmaxf(longest, ((float)s.all + (float)parts * kPdFixed) * (float)a.kv_heads / 148.0f + 0.5f * longest);
+            if (lane == 0 || ((long long)split * a.kv_heads <= o.split_blocks && parts <= o.capacity)) mine = ((unsigned long long)__float_as_uint(cost) << 32) | lane;
         }
-        o.list[0] = make_int4(min(at, o.capacity), 0, 0, 0);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) {
+            const unsigned long long v = __shfl_xor_sync(0xffffffffu, mine, d);
+            mine = v < mine ? v : mine;
+        }
+        if (lane == 0) s.cut = cut_of((int)(mine & 31u));
     }
     __syncthreads();
-    each([&](int r, int u, int tiles) {
-        const int parts = parts_of(tiles), place = parts > 1 ? atomicAdd(&s_place, parts) : 0, at = atomicAdd(&s_bucket[bucket_of(tiles, parts)], parts);
+    const int cut = min(s.cut, most);
+    auto parts_of = [&](int tiles) { return max(1, (tiles + cut - 1) / cut); };
+    auto bucket_of = [&](int tiles, int parts) { return 63 - min(63, (tiles + parts - 1) / parts * 64 / (cut + 1)); };
+    for (int i = tid; i < units; i += kPdThreads) atomicAdd(&s.bucket[bucket_of(s.tiles[i], parts_of(s.tiles[i]))], parts_of(s.tiles[i]));
+    __syncthreads();
+    if (warp == 0) {
+        const int n0 = s.bucket[2 * lane], n1 = s.bucket[2 * lane + 1];
+        int up = n0 + n1;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, up, d);
+            if (lane >= d) up += v;
+        }
+        s.bucket[2 * lane] = up - n0 - n1;
+        s.bucket[2 * lane + 1] = up - n1;
+        if (lane == 31) o.list[0] = make_int4(min(up, o.capacity), 0, 0, 0);
+    }
+    __syncthreads();
+    for (int i = tid; i < units; i += kPdThreads) {
+        const int tiles = s.tiles[i], parts = parts_of(tiles), place = parts > 1 ? atomicAdd(&s.place, parts) : 0, at = atomicAdd(&s.bucket[bucket_of(tiles, parts)], parts);
         for (int p = 0; p < parts; ++p)
-            if (at + p < o.capacity) o.list[1 + at + p] = make_int4(r, u, parts << 16 | p, place);
-    });
+            if (at + p < o.capacity) o.list[1 + at + p] = make_int4(s.request[i], s.unit[i], parts << 16 | p, place);
+    }
 }
 
 // NB: bytes of q and of the weights; NC: columns of eight rows.
@@ -170,7 +227,8 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
     pdl_wait();
     const int blocks = (int)gridDim.x - (order.list != nullptr ? 1 : 0);
     if ((int)blockIdx.x == blocks) {
-        paged_order(a, order, group);
+        static_assert(sizeof(PdOrderShared) <= S::kSmem, "the order's tables fit into the block's shared memory");
+        paged_order(a, order, group, *reinterpret_cast<PdOrderShared*>(pd_smem));
         return;
     }
     // ---- the share of this block
@@ -610,7 +668,8 @@ int paged_decode_launch(cudaStream_t stream, const PagedArgs& a, bool f32, int m
     work.partials = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + pd_counter_bytes(a.requests, a.kv_heads));
     // no more blocks than there can be shares of one tile a warp
     const long long most = (long long)a.requests * a.kv_heads * (max_context / kPdKeys + 2 + kPdStretch), blocks = (most + kPdWarps - 1) / kPdWarps;
-    const dim3 grid((unsigned)(blocks < kPdBlocks ? blocks : kPdBlocks) + (order.list != nullptr ? 1 : 0));
+    const int at_once = max_rows <= 8 ? kPdBlocks : kPdBlocks / 3 * 2;
+    const dim3 grid((unsigned)(blocks < at_once ? blocks : at_once) + (order.list != nullptr ? 1 : 0));
     auto go = [&](auto kern, int smem) {
         const cudaError_t e = allow_all_dynamic_smem(kern);
         return e != cudaSuccess ? e : launch(kern, grid, dim3(kPdThreads), (size_t)smem, stream, true, a, work, order);

@@ -151,7 +151,8 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
     uint64_t* const v_free = k_free + 2;     // [kStages]
     uint64_t* const sc_full = v_free + 2;    // [4] the scales of a tile are there
     uint64_t* const pair = sc_full + 4;      // [8] both threads of a row have left their maxima
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(pair + 8);
+    uint64_t* const q_full = pair + 8;       // the queries are there
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(q_full + 1);
     int* const s_last = reinterpret_cast<int*>(tmem_slot + 1);  // all other parts of the unit have arrived
     PpScales* const scales = reinterpret_cast<PpScales*>(smem + S::kOffScales);
     float* const units = reinterpret_cast<float*>(smem + S::kOffUnit);
@@ -159,8 +160,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
     const int tid = threadIdx.x, lane = tid & 31, warp = uniform_warp_index(), group = a.heads / a.kv_heads, h = blockIdx.x;
     const int block_log = 31 - __clz(a.block), in_block = a.block - 1;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if ((int)blockIdx.y >= work.list[0].x) return;
-    const int4 entry = work.list[1 + blockIdx.y];
+    const int entries = work.list[0].x;
+    const int4 entry = work.list[1 + blockIdx.y];  // (the list has room for one per block)
+    if ((int)blockIdx.y >= entries) return;
     if (tid == 0) {
         for (int b = 0; b < 2; ++b) {
             mbar_init(&s_full[b], 1);
@@ -173,6 +175,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
         }
         for (int b = 0; b < 4; ++b) mbar_init(&sc_full[b], 1);
         for (int b = 0; b < 8; ++b) mbar_init(&pair[b], 2);
+        mbar_init(q_full, kPpConvert);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kPpIssue) {
@@ -195,55 +198,6 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
         const int all_tiles = un.tiles(rq, group), size = (all_tiles + parts - 1) / parts, from_tile = min(all_tiles, part * size);
         const int tiles = min(size, all_tiles - from_tile), first = un.first + from_tile * kPpKeys;
         const int tiles0 = two ? min(tiles, max(0, un.tiles_to(rq, group, kPpRows - 1) - from_tile)) : tiles;  // of the first stream where the streams are tiles of rows
-        // ---- Q: a warp has a row at a time, HD / 32 entries a lane; its largest entry gives the power of two
-        constexpr int E = HD / 32, kWarps = kPpThreads / 32, kBatch = 5;
-        for (int r0 = warp; r0 < (two ? 2 : 1) * kPpRows; r0 += kWarps * kBatch) {
-            float x[kBatch][E];
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                const int r = r0 + i * kWarps;
-#pragma unroll
-                for (int k = 0; k < E; ++k) x[i][k] = 0.0f;
-                if (r >= 2 * kPpRows) continue;
-                const int token = (row0 + r) / group, place = (rq.first + token) * a.heads + h * group + (row0 + r - token * group);
-                if (lane == 0) row_of[r] = place;
-                if (r < live) load_entries<E>(static_cast<const T*>(a.query) + (size_t)place * HD + lane * E, x[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                const int r = r0 + i * kWarps;
-                if (r >= 2 * kPpRows) continue;
-                float top = 0.0f;
-                bool finite = true;
-#pragma unroll
-                for (int k = 0; k < E; ++k) {
-                    top = fmaxf(top, fabsf(x[i][k]));
-                    finite = finite && fabsf(x[i][k]) < INFINITY;
-                }
-                top = warp_max(top);
-                finite = __all_sync(0xffffffffu, finite) != 0;
-                int e2 = 0;
-                if (top > 0.0f && top < INFINITY) frexpf(top, &e2);
-                const float up = ldexpf(1.0f, max(-120, min(120, 11 - e2)));  // the largest entry between 2^10 and 2^11
-                if (lane == 0) units[r] = finite ? up : __int_as_float(0x7fffffff);
-                unsigned char* const at = smem + (r >> 7) * S::kQTile + (lane * E >> 6) * kPpBox + (r & 127) * 128 + ((((lane * E >> 3) & 7) ^ (r & 7)) << 4) + (lane * E & 7) * 2;
-                uint32_t hi[E / 2], lo[E / 2];
-#pragma unroll
-                for (int k = 0; k < E / 2; ++k) {
-                    hi[k] = pp_round(x[i][2 * k] * up, x[i][2 * k + 1] * up);
-                    lo[k] = pp_rest(x[i][2 * k] * up, x[i][2 * k + 1] * up, hi[k]);
-                }
-                if constexpr (E == 4) {
-                    *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
-                    if (NP == 2) *reinterpret_cast<uint2*>(at + S::kQPlane) = make_uint2(lo[0], lo[1]);
-                } else {
-                    *reinterpret_cast<uint32_t*>(at) = hi[0];
-                    if (NP == 2) *reinterpret_cast<uint32_t*>(at + S::kQPlane) = lo[0];
-                }
-            }
-        }
-        fence_proxy_async_smem();
-        __syncthreads();
         const uint32_t base = smem_u32(smem);
 
         if (warp >= kPpConvert && warp < kPpIssue) {
@@ -370,7 +324,10 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                 if (last) lead_commit(lead, &v_free[st]);
                 return true;
             };
-            if (two) {
+            ok = warp_wait(q_full, 0u);
+            tcgen05_fence_after();
+            if (!ok) {
+            } else if (two) {
                 // (the second stream has every tile, the first the tiles up to its own rows' positions)
                 if (tiles > 0) ok = (tiles0 < 1 || scores(0, 0, false)) && scores(0, 1, true);
                 for (int j = 0; j < tiles && ok; ++j) {
@@ -389,6 +346,54 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
             }
         } else if (warp < kPpConvert) {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
+            // ---- Q first: a warp has a row at a time, HD / 32 entries a lane; its largest entry gives the power of two
+            constexpr int E = HD / 32, kBatch = 8;
+            for (int r0 = warp; r0 < (two ? 2 : 1) * kPpRows; r0 += kPpConvert * kBatch) {
+                float x[kBatch][E];
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    const int r = r0 + i * kPpConvert;
+#pragma unroll
+                    for (int k = 0; k < E; ++k) x[i][k] = 0.0f;
+                    const int token = (row0 + r) / group, place = (rq.first + token) * a.heads + h * group + (row0 + r - token * group);
+                    if (lane == 0) row_of[r] = place;
+                    if (r < live) load_entries<E>(static_cast<const T*>(a.query) + (size_t)place * HD + lane * E, x[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    const int r = r0 + i * kPpConvert;
+                    float top = 0.0f;
+                    bool finite = true;
+#pragma unroll
+                    for (int k = 0; k < E; ++k) {
+                        top = fmaxf(top, fabsf(x[i][k]));
+                        finite = finite && fabsf(x[i][k]) < INFINITY;
+                    }
+                    // the power of two that brings the largest entry between 2^10 and 2^11 (its exponent field is 264 less the entry's)
+                    const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+                    const float up = __uint_as_float((uint32_t)min(254, max(1, 264 - (int)(most >> 23))) << 23);
+                    finite = __all_sync(0xffffffffu, finite) != 0;
+                    if (lane == 0) units[r] = finite ? up : __int_as_float(0x7fffffff);
+                    unsigned char* const at = smem + (r >> 7) * S::kQTile + (lane * E >> 6) * kPpBox + (r & 127) * 128 + ((((lane * E >> 3) & 7) ^ (r & 7)) << 4) + (lane * E & 7) * 2;
+                    uint32_t hi[E / 2], lo[E / 2];
+#pragma unroll
+                    for (int k = 0; k < E / 2; ++k) {
+                        hi[k] = pp_round(x[i][2 * k] * up, x[i][2 * k + 1] * up);
+                        lo[k] = pp_rest(x[i][2 * k] * up, x[i][2 * k + 1] * up, hi[k]);
+                    }
+                    if constexpr (E == 4) {
+                        *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
+                        if (NP == 2) *reinterpret_cast<uint2*>(at + S::kQPlane) = make_uint2(lo[0], lo[1]);
+                    } else {
+                        *reinterpret_cast<uint32_t*>(at) = hi[0];
+                        if (NP == 2) *reinterpret_cast<uint32_t*>(at + S::kQPlane) = lo[0];
+                    }
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+            asm volatile("bar.sync 1, 512;" ::: "memory");  // (units and places of rows are there)
             // ---- softmax: the stream's tiles j = j0, j0 + step, ..
             const int stream = warp >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane, in_unit = two ? stream * kPpRows + r : r;
             uint64_t* const pair_bar = pair + stream * 4 + (warp & 3);  // of the two warps that have the same rows
@@ -552,9 +557,10 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                 }
             }
             __syncwarp();
-            const int quads = columns / 4;
-            for (int i = lane; i < 32 * quads; i += 32) {
-                const int rr = i / quads, c4 = i % quads, row = (two ? stream * kPpRows : 0) + (warp & 3) * 32 + rr;
+            const int quads_log = (HD == 128 ? 5 : 4) - (two ? 1 : 2);  // groups of four columns
+#pragma unroll 4
+            for (int i = lane; i < 32 << quads_log; i += 32) {
+                const int rr = i >> quads_log, c4 = i & ((1 << quads_log) - 1), row = (two ? stream * kPpRows : 0) + (warp & 3) * 32 + rr;
                 if (!ok || row >= live) continue;
                 const float4 y = *reinterpret_cast<const float4*>(stage + rr * S::kStagePitch + c4 * 4);
                 if (parts > 1) {
@@ -579,24 +585,33 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                     if (tid == 0) *arrived = 0;
                     const float* const p0 = work.partials + (size_t)(entry.w * a.kv_heads + h) * pp_partial_floats<HD>();
                     const size_t pitch = (size_t)a.kv_heads * pp_partial_floats<HD>();
-                    for (int i = tid; i < live * (HD / 4); i += 512) {
-                        const int row = i / (HD / 4), c = i % (HD / 4) * 4;
+                    // 2^(maximum - largest) / sum of every part of a row, over the operands
+                    float* const factor = reinterpret_cast<float*>(smem);
+                    if (tid < live) {
                         float top = -INFINITY, all = 0.0f;
-                        for (int k = 0; k < parts; ++k) top = fmaxf(top, __ldcg(p0 + k * pitch + 2 * row));
+                        for (int k = 0; k < parts; ++k) top = fmaxf(top, __ldcg(p0 + k * pitch + 2 * tid));
                         const float base_top = top == -INFINITY ? 0.0f : top;
-                        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 2
                         for (int k = 0; k < parts; ++k) {
-                            const float2 st = __ldcg(reinterpret_cast<const float2*>(p0 + k * pitch) + row);
-                            const float4 x = __ldcg(reinterpret_cast<const float4*>(p0 + k * pitch + 2 * kPpUnit + row * HD + c));
-                            const float f = ex2_approx(st.x - base_top);
-                            all = fmaf(st.y, f, all);
-                            y.x = fmaf(x.x, f, y.x); y.y = fmaf(x.y, f, y.y); y.z = fmaf(x.z, f, y.z); y.w = fmaf(x.w, f, y.w);
+                            const float2 st = __ldcg(reinterpret_cast<const float2*>(p0 + k * pitch) + tid);
+                            all = fmaf(st.y, ex2_approx(st.x - base_top), all);
                         }
                         const float over = all == 0.0f ? 0.0f : 1.0f / all;
+                        for (int k = 0; k < parts; ++k) factor[k * kPpUnit + tid] = ex2_approx(__ldcg(p0 + k * pitch + 2 * tid) - base_top) * over;
+                    }
+                    asm volatile("bar.sync 1, 512;" ::: "memory");
+#pragma unroll 4
+                    for (int i = tid; i < live * (HD / 4); i += 512) {
+                        const int row = i / (HD / 4), c = i % (HD / 4) * 4;
+                        const float* const x0 = p0 + 2 * kPpUnit + row * HD + c;
+                        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        for (int k = 0; k < parts; ++k) {
+                            const float4 x = __ldcg(reinterpret_cast<const float4*>(x0 + k * pitch));
+                            const float f = factor[k * kPpUnit + row];
+                            y.x = fmaf(x.x, f, y.x); y.y = fmaf(x.y, f, y.y); y.z = fmaf(x.z, f, y.z); y.w = fmaf(x.w, f, y.w);
+                        }
                         T* const out = static_cast<T*>(a.out) + (size_t)row_of[row] * HD + c;
-                        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = make_float4(y.x * over, y.y * over, y.z * over, y.w * over);
-                        else *reinterpret_cast<uint2*>(out) = make_uint2(bf16_pair_of(y.x * over, y.y * over), bf16_pair_of(y.z * over, y.w * over));
+                        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = y;
+                        else *reinterpret_cast<uint2*>(out) = make_uint2(bf16_pair_of(y.x, y.y), bf16_pair_of(y.z, y.w));
                     }
                 }
             }
