@@ -80,7 +80,7 @@ __device__ inline void load4<uint16_t>(const void* p, size_t i, float (&v)[4]) {
 
 struct PdWork {
     int* arrived;     // [requests * kv_heads], zero between calls
-    float* partials;  // [blocks][2][8 * NC rows][2 + HD]
+    float* partials;  // [blocks][2]: (maximum, sum) of 8 * NC rows, then their O
 };
 
 // Tiles of a request that this kernel serves (one where its rows attend nothing: they are written as zeros).
@@ -223,6 +223,7 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
     __shared__ long long s_before[kPdWarps + 1];
     __shared__ long long s_start;
     __shared__ int s_request, s_last;
+    __shared__ float s_run[3 * ROWS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, group = a.heads / a.kv_heads;
     pdl_wait();
     const int blocks = (int)gridDim.x - (order.list != nullptr ? 1 : 0);
@@ -337,18 +338,34 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
             }
             cp_async_commit_group();
         };
+        auto entry_of = [&](int i) {  // the same, not yet looked at
+            const int key = key0 + (ta + warp + i * kPdWarps) * kPdKeys + half * 16;
+            return i >= mine_n || key >= rq.hi ? -1 : table[key / a.block];
+        };
         int pages[kPdStages];
 #pragma unroll
-        for (int i = 0; i < kPdStages; ++i) pages[i] = page_of(i);
+        for (int i = 0; i < kPdStages; ++i) pages[i] = entry_of(i);
+        // (queries are on their way before the table's entries are needed)
+        const int n_rows = rq.rows * group;
+        float q[NC][KS][2][4];
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) {
+            const int row = nc * 8 + g;
+            const size_t at = ((size_t)(rq.first + (row < n_rows ? row / group : 0)) * a.heads + (size_t)h * group + (row < n_rows ? row % group : 0)) * HD;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) load4<T>(a.query, at + ks * 32 + e * 16 + t * 4, q[nc][ks][e]);
+        }
 #pragma unroll
         for (int i = 0; i < kPdStages; ++i) {
-            copy_keys(i, pages[i]);
-            copy_values(i, pages[i]);
+            const int page = pages[i] >= 0 && pages[i] < a.pages ? pages[i] : -1;
+            copy_keys(i, page);
+            copy_values(i, page);
         }
         int next_page = page_of(kPdStages);
 
         // ---- q of eight rows a column: bytes of round(q * 2^sh), the largest entry of a row between 2^(8 NB - 2) and 2^(8 NB - 1)
-        const int n_rows = rq.rows * group;
         uint32_t qb[NC][NB][KS][2];
         float q_unit[NC][2];   // of this lane's two score columns: 2^-sh * scale
         int last[NC][2], first_key[NC][2];
@@ -356,18 +373,16 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
         for (int nc = 0; nc < NC; ++nc) {
             const int row = nc * 8 + g;
             const bool live = row < n_rows;
-            const size_t at = ((size_t)(rq.first + (live ? row / group : 0)) * a.heads + (size_t)h * group + (live ? row % group : 0)) * HD;
-            float q[KS][2][4], top = 0.0f;
+            float top = 0.0f;
             bool finite = true;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    load4<T>(a.query, at + ks * 32 + e * 16 + t * 4, q[ks][e]);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        top = fmaxf(top, fabsf(q[ks][e][i]));
-                        finite = finite && fabsf(q[ks][e][i]) < INFINITY;
+                        top = fmaxf(top, fabsf(q[nc][ks][e][i]));
+                        finite = finite && fabsf(q[nc][ks][e][i]) < INFINITY;
                     }
                 }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -386,7 +401,7 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
                 for (int e = 0; e < 2; ++e) {
                     uint32_t x[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[i] = live ? (uint32_t)max(-most, min(most, __float2int_rn(q[ks][e][i] * up))) : 0u;
+                    for (int i = 0; i < 4; ++i) x[i] = live ? (uint32_t)max(-most, min(most, __float2int_rn(q[nc][ks][e][i] * up))) : 0u;
 #pragma unroll
                     for (int b = 0; b < NB; ++b) {
                         const uint32_t pick = (uint32_t)(b | ((b + 4) << 4));
@@ -594,9 +609,8 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
                 store_row(to + 2, y.z * inv);
                 store_row(to + 3, y.w * inv);
             } else {
-                float* const to = part + row * (HD + 2);
-                if (c == 0) { to[0] = top; to[1] = sum; }
-                to[2 + c] = y.x; to[3 + c] = y.y; to[4 + c] = y.z; to[5 + c] = y.w;
+                if (c == 0) reinterpret_cast<float2*>(part)[row] = make_float2(top, sum);
+                *reinterpret_cast<float4*>(part + 2 * ROWS + row * HD + c) = y;
             }
         }
         if (!whole) {
@@ -611,39 +625,68 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
                 __threadfence();
                 if (tid == 0) work.arrived[(size_t)r * a.kv_heads + h] = 0;
                 auto part_of = [&](int k) { return work.partials + ((size_t)(c0 + k) * 2 + (k == 0 ? 1 : 0)) * ROWS * (HD + 2); };
-                float* const factor = reinterpret_cast<float*>(pd_smem);  // [row][part]: 2^(maximum - largest) / sum
-                static_assert(ROWS * kPdBlocks * 4 <= kPdWarps * S::kWarp, "factors fit over the ring");
-                for (int row = warp; row < n_rows; row += kPdWarps) {
-                    float top = -INFINITY, sum = 0.0f;
-                    for (int k = lane; k < n; k += 32) top = fmaxf(top, __ldcg(part_of(k) + row * (HD + 2)));
-                    top = warp_max(top);
-                    const float base = top == -INFINITY ? 0.0f : top;
-                    for (int k = lane; k < n; k += 32) {
-                        const float2 st = __ldcg(reinterpret_cast<const float2*>(part_of(k) + row * (HD + 2)));
-                        const float f = ex2_approx(st.x - base);
-                        factor[row * n + k] = f;
-                        sum = fmaf(st.y, f, sum);
+                // [part][row]: maxima, sums, then 2^(maximum - largest) / sum; as many parts as fit over the ring at once
+                constexpr int kHeld = kPdWarps * S::kWarp / (ROWS * 8);
+                float* const tops = reinterpret_cast<float*>(pd_smem);
+                float* const sums = tops + kHeld * ROWS;
+                float4 y[(ROWS * (HD / 4) + kPdThreads - 1) / kPdThreads];
+#pragma unroll
+                for (float4& v : y) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                float* const run = reinterpret_cast<float*>(s_run);  // running maximum and sum of a row, and what the parts before are worth now
+                if (tid < ROWS) { run[tid] = -INFINITY; run[ROWS + tid] = 0.0f; }
+                for (int k0 = 0; k0 < n; k0 += kHeld) {
+                    const int held = min(kHeld, n - k0);
+                    __syncthreads();
+                    for (int i = tid; i < held * ROWS; i += kPdThreads) {
+                        const float2 st = __ldcg(reinterpret_cast<const float2*>(part_of(k0 + i / ROWS)) + i % ROWS);
+                        tops[i] = st.x;
+                        sums[i] = st.y;
                     }
-                    sum = warp_sum(sum);
-                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                    for (int k = lane; k < n; k += 32) factor[row * n + k] *= inv;
-                }
-                __syncthreads();
-                for (int i = tid; i < n_rows * (HD / 2); i += kPdThreads) {
-                    const int row = i / (HD / 2), c = i % (HD / 2) * 2;
-                    const float* const from = part_of(0) + row * (HD + 2) + 2 + c;
-                    const float* const f = factor + row * n;
-                    const float2 x0 = __ldcg(reinterpret_cast<const float2*>(from));
-                    float y0 = x0.x * f[0], y1 = x0.y * f[0];
+                    __syncthreads();
+                    for (int row = warp; row < n_rows; row += kPdWarps) {
+                        float top = run[row], sum = 0.0f;
+                        const float before_top = top;
+                        for (int k = lane; k < held; k += 32) top = fmaxf(top, tops[k * ROWS + row]);
+                        top = warp_max(top);
+                        const float base = top == -INFINITY ? 0.0f : top;
+                        for (int k = lane; k < held; k += 32) {
+                            const float f = ex2_approx(tops[k * ROWS + row] - base);
+                            tops[k * ROWS + row] = f;
+                            sum = fmaf(sums[k * ROWS + row], f, sum);
+                        }
+                        sum = warp_sum(sum);
+                        if (lane == 0) {
+                            const float turn = ex2_approx(before_top - base);
+                            run[row] = top;
+                            run[ROWS + row] = fmaf(run[ROWS + row], turn, sum);
+                            run[2 * ROWS + row] = turn;
+                        }
+                    }
+                    __syncthreads();
+#pragma unroll
+                    for (int j = 0; j < (int)(sizeof(y) / sizeof(y[0])); ++j) {
+                        const int i = tid + j * kPdThreads, row = i / (HD / 4), c = i % (HD / 4) * 4;
+                        if (i >= n_rows * (HD / 4)) break;
+                        const float turn = run[2 * ROWS + row];
+                        y[j].x *= turn; y[j].y *= turn; y[j].z *= turn; y[j].w *= turn;
 #pragma unroll 8
-                    for (int k = 1; k < n; ++k) {
-                        const float2 x = __ldcg(reinterpret_cast<const float2*>(from + (size_t)(2 * k - 1) * ROWS * (HD + 2)));
-                        y0 = fmaf(x.x, f[k], y0);
-                        y1 = fmaf(x.y, f[k], y1);
+                        for (int k = 0; k < held; ++k) {
+                            const float4 x = __ldcg(reinterpret_cast<const float4*>(part_of(k0 + k) + 2 * ROWS + row * HD + c));
+                            const float f = tops[k * ROWS + row];
+                            y[j].x = fmaf(x.x, f, y[j].x); y[j].y = fmaf(x.y, f, y[j].y); y[j].z = fmaf(x.z, f, y[j].z); y[j].w = fmaf(x.w, f, y[j].w);
+                        }
                     }
+                }
+#pragma unroll
+                for (int j = 0; j < (int)(sizeof(y) / sizeof(y[0])); ++j) {
+                    const int i = tid + j * kPdThreads, row = i / (HD / 4), c = i % (HD / 4) * 4;
+                    if (i >= n_rows * (HD / 4)) break;
+                    const float sum = run[ROWS + row], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                     T* const to = static_cast<T*>(a.out) + ((size_t)(rq.first + row / group) * a.heads + (size_t)h * group + row % group) * HD + c;
-                    store_row(to, y0);
-                    store_row(to + 1, y1);
+                    store_row(to, y[j].x * inv);
+                    store_row(to + 1, y[j].y * inv);
+                    store_row(to + 2, y[j].z * inv);
+                    store_row(to + 3, y[j].w * inv);
                 }
             }
         }
