@@ -247,6 +247,32 @@ class Session:
                 break
         return steps
 
+    def generate_sampled_until(self, max_new_tokens: int, stop_token_id: int | None, sampling: SamplingOptions, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0):
+        """Sampling on the device over the whole vocabulary (ops.sample_rows; no counterpart in kmll): top_k 0, top_p 1 and min_p 0 are off.  The random
+        numbers are those of generate_sampled_top_k_until, so with top_k alone the tokens are its tokens as well, up to the f32 rounding of its
+        weights.  One token and its log-probability leave the device per step, not the logits; a step's `logit` is that log-probability."""
+        self._require_ready()
+        validate_sampling_options(sampling)
+        if not (0.0 <= min_p <= 1.0) or not (0.0 < top_p <= 1.0) or top_k < 0:
+            raise ValueError(f"sampling needs 0 < top_p <= 1, 0 <= min_p <= 1 and top_k >= 0, got {top_p}, {min_p}, {top_k}")
+        rng = XorShift64(sampling.seed)
+        dev = self._logits.device
+        settings = [torch.tensor([v], dtype=d, device=dev) for v, d in ((sampling.temperature, torch.float32), (top_k, torch.int32), (top_p, torch.float32), (min_p, torch.float32))]
+        u, token, logprob = torch.zeros(1, dtype=torch.float64, device=dev), torch.zeros(1, dtype=torch.int32, device=dev), torch.zeros(1, dtype=torch.float32, device=dev)
+        steps = []
+        for step in range(max_new_tokens):
+            check(self.dec._lib.kmll_decoder_next_logits(self.dec._h, self.dec._stream(), self._logits.data_ptr()))
+            u.fill_(rng.next_unit_f64())
+            ops.sample_rows(self._logits.view(1, -1), u, *settings, tokens=token, logprobs=logprob)
+            t = int(token.item())
+            if t < 0:
+                raise ValueError("no logit can be sampled from")
+            self.advance_with_token(t)
+            steps.append(GenerationStep(step, t, float(logprob.item()), []))
+            if stop_token_id is not None and t == stop_token_id:
+                break
+        return steps
+
     def run_generation_request(self, prompt_tokens, options: GenerationOptions) -> dict:
         """run_generation_with_runtime (inference.rs:6442-6480): prefill and decode timed separately, a synchronisation
         at both ends of each."""

@@ -510,3 +510,125 @@ def test_steps_of_a_server(cuda, dtype):
             assert [x == 0 for x in cpu["length"]] == [bool(e) for e in ended]
     held = [p for r in range(requests) for p in cpu["table"][r, :-(-cpu["length"][r] // block)]]
     assert sorted(held + cpu["free"][:cpu["count"]]) == list(range(pages))  # no page is lost or held twice
+
+
+# ---- calls that are easily forgotten ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads, kv, hd, block, cached, new, window", [
+    (24, 2, 64, 32, [50, 7, 0], [1, 2, 30], 0), (12, 1, 128, 16, [400, 90], [1, 25], 64), (8, 1, 128, 64, [77, 500], [1, 2], 0), (8, 2, 64, 16, [30, 3, 260], [3, 70, 4], 0),
+    (71, 1, 64, 64, [200], [1], 0), (8, 8, 128, 32, [10, 0], [16, 17], 0)])
+def test_attention_of_few_rows_beside_many(cuda, dtype, heads, kv, hd, block, cached, new, window):
+    """Requests on either side of the number of rows that parts the kernels."""
+    check_attention(make_attention(sum(cached) + heads, heads, kv, hd, block, cached, new, dtype, spare_rows=1), window)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_portions_whose_keys_are_split(cuda, dtype):
+    """Few units over long contexts: parts of a unit's keys in different blocks, more parts than rows' tiles, and a part without any."""
+    check_attention(make_attention(31, 4, 1, 128, 64, [2600, 0], [20, 9], dtype))
+    check_attention(make_attention(32, 4, 1, 64, 16, [1500], [80], dtype), window=700)
+    check_attention(make_attention(33, 2, 2, 128, 128, [900, 1300], [150, 40], dtype))
+
+
+def test_more_units_than_are_put_in_order(cuda):
+    n = 2100
+    check_attention(make_attention(34, 1, 1, 64, 16, [i % 5 for i in range(n)], [9] * n, torch.bfloat16))
+
+
+def test_pages_behind_two_gigabytes(cuda):
+    """Codes of a page lie more than 2^31 bytes into the cache."""
+    pages, block, kv, hd = 140000, 16, 8, 128
+    cache = ops.DevicePagedI8Cache.create(pages, block, kv, hd)
+    assert cache.k_codes.numel() > 2 ** 31
+    rng = np.random.default_rng(3)
+    here = [pages - 1, 3, pages - 7]
+    slots = np.concatenate([np.arange(p * block, (p + 1) * block) for p in here])[:40]
+    ks, vs = po.Store(3, block, kv, hd), po.Store(3, block, kv, hd)
+    small = np.concatenate([np.arange(i * block, (i + 1) * block) for i in range(3)])[:40]
+    for rows, heads in ((1, 16), (40, 8)):
+        k, v = (torch.tensor(rng.normal(0, 1, (40, kv, hd)), device="cuda", dtype=torch.float32) for _ in range(2))
+        ops.prepare_paged_attention(k[:, :0], k, v, None, None, ints(slots), cache, query_rot=k[:, :0])
+        ks.append(f64(k), small.tolist())
+        vs.append(f64(v), small.tolist())
+        got = ops.paged_cache_rows(cache, ints(slots))
+        np.testing.assert_array_equal(got[0].cpu().numpy(), ks.rows(small))
+        np.testing.assert_array_equal(got[1].cpu().numpy(), vs.rows(small))
+        q = torch.tensor(rng.normal(0, 1, (rows, heads, hd)), device="cuda", dtype=torch.float32)
+        out = ops.paged_attention(q, ints([0, rows]), ints([40]), ints([here]), cache, rows, 40, 0.09)
+        s = dict(q=q, start=[0, rows], context=[40], table=np.array([[0, 1, 2]]), block=block, values=[x.codes * x.scales.astype(np.float64)[:, None, :, None] for x in (ks, vs)])
+        want = po.attention(f64(q), s["start"], s["context"], s["table"], block, *s["values"], 0.09, 0, np.zeros(q.shape))
+        assert (np.abs(f64(out).reshape(want.shape) - want) <= attention_bound(s, want, 0.09, 0)).all()
+
+
+def test_requests_that_share_pages(cuda):
+    """A common beginning: the same pages in two rows of the table."""
+    for new in (1, 20):
+        s = make_attention(41, 8, 2, 128, 16, [100, 100], [new, new], torch.float32)
+        s["table"][1, :6] = s["table"][0, :6]
+        check_attention(s)
+
+
+def test_two_streams_at_once(cuda):
+    """Calls that overlap, each with a workspace of its own; operands are waited for by the caller, as with every operator."""
+    a, b = make_attention(51, 8, 2, 128, 32, [900, 30], [1, 1], torch.float32), make_attention(52, 8, 2, 128, 32, [300], [60], torch.float32)
+    args = [(ints(s["start"]), ints(s["context"]), ints(s["table"]), s["cache"], s["most"], max(s["context"]), 0.09) for s in (a, b)]
+    alone = [ops.paged_attention(s["q"], *x).clone() for s, x in zip((a, b), args)]
+    works = [ops.paged_attention_workspace(s["cache"], 8, len(s["context"]), s["q"].shape[0], s["most"], max(s["context"])) for s in (a, b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[], []]
+    for _ in range(10):
+        for i, s in enumerate((a, b)):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(ops.paged_attention(s["q"], *args[i], workspace=works[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, alone[i]) for i in range(2) for o in outs[i])
+
+
+def test_bf16_results_keep_nan(cuda):
+    for new in (1, 40):
+        s = make_attention(61, 8, 2, 128, 32, [70], [new], torch.bfloat16)
+        s["q"][0, 2, 9] = math.nan
+        out = ops.paged_attention(s["q"], ints(s["start"]), ints(s["context"]), ints(s["table"]), s["cache"], s["most"], max(s["context"]), 0.09).view(-1, 8, 128)
+        assert torch.isnan(out[0, 2]).all() and not torch.isnan(out[0, 3]).any()
+        x = s["q"][:1, :2].clone()
+        x[0, 0, 0] = math.nan
+        turned = ops.prepare_paged_attention(x, x, x, torch.tensor(freqs_of(64, 128), device="cuda"), ints([5]), ints([0]), ops.DevicePagedI8Cache.create(1, 16, 2, 128))
+        assert torch.isnan(turned[0, 0, 0]) and torch.isnan(turned[0, 0, 64]) and not torch.isnan(turned[0, 1]).any()
+
+
+def test_prompt_attention_captured_and_replayed(cuda):
+    """A captured step serves other lengths, single tokens beside portions, and leaves its workspace as it found it."""
+    sets = [make_attention(71 + i, 8, 2, 128, 32, cached, new, torch.float32) for i, (cached, new) in enumerate((([600, 3, 90], [1, 50, 13]), ([0, 900, 0], [62, 1, 1])))]
+    width = 40
+    caches = [s["cache"] for s in sets]
+    cache = caches[0] if caches[0].pages >= caches[1].pages else caches[1]
+    ws = ops.paged_attention_workspace(cache, 8, 3, 64, 64, 1000)
+    q, start, context, table, out = torch.zeros(64, 8, 128, device="cuda"), ints([0] * 4), ints([0] * 3), ints(np.zeros((3, width))), torch.zeros(64, 1024, device="cuda")
+
+    def call():
+        ops.paged_attention(q, start, context, table, cache, 64, 1000, 0.09, workspace=ws, out=out)
+
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for s in (sets[0], sets[1], sets[0]):
+        q.copy_(s["q"])
+        start.copy_(ints(s["start"]))
+        context.copy_(ints(s["context"]))
+        t = np.where(s["table"] < cache.pages, s["table"], 0)
+        table.zero_()
+        table[:, :t.shape[1]] = ints(t)[:, :width]
+        graph.replay()
+        replayed = out.clone()
+        again = ops.paged_attention(q, start, context, table, cache, 64, 1000, 0.09)
+        assert torch.equal(replayed, again)
+
+
+def test_the_device_reports_no_time_out(cuda):
+    import ctypes
+
+    from kmll_b200 import lib
+    status = ctypes.c_int(-1)
+    assert lib.load().kmll_device_status(ctypes.byref(status)) == 0 and status.value == 0

@@ -147,3 +147,31 @@ def test_shares_follow_the_weights(cuda):
     share = torch.softmax(x[0].double(), 0).tolist()
     for t, s in enumerate(share):
         assert abs(int((tokens == t).sum()) - s * n) <= 2
+
+
+def test_session_samples_on_the_device(cuda):
+    """With top-k alone the device takes the tokens of the host sampler (same walk, same random numbers); temperature 0 is arg-max decoding; top-p and
+    min-p runs repeat themselves."""
+    from kmll_b200 import runtime as rt
+    from kmll_b200.session import SamplingOptions, Session
+    cfg = rt.DecoderConfig(dim=256, n_layers=2, n_heads=4, n_kv_heads=2, head_dim=64, hidden_dim=512, vocab_size=640, max_seq_len=96, rope_theta=1e6, norm_eps=1e-5,
+                           format=rt.FORMAT_W4G128)
+    dec = rt.Decoder(cfg)
+    dec.init_random(5, 0.05, False)
+    s, prompt = Session(dec), np.random.default_rng(2).integers(0, 640, 9)
+
+    def run(f):
+        s.prefill(prompt)
+        return [st.token_id for st in f()]
+
+    hot = SamplingOptions(temperature=1.2, seed=11)
+    assert run(lambda: s.generate_sampled_until(14, None, hot, top_k=12)) == run(lambda: s.generate_sampled_top_k_until(14, 12, None, hot))
+    assert run(lambda: s.generate_sampled_until(10, None, SamplingOptions(temperature=0.0))) == run(lambda: s.generate_greedy_until(10))
+    a, b = (run(lambda: s.generate_sampled_until(14, None, hot, top_p=0.8, min_p=0.01)) for _ in range(2))
+    assert a == b and s.tokens()[9:] == b
+    stop = a[5]
+    assert run(lambda: s.generate_sampled_until(14, stop, hot, top_p=0.8, min_p=0.01)) == a[:a.index(stop) + 1]
+    for bad in (dict(top_p=0.0), dict(top_p=1.5), dict(min_p=-0.1), dict(top_k=-1)):
+        with pytest.raises(ValueError):
+            s.generate_sampled_until(1, None, hot, **bad)
+    dec.close()
