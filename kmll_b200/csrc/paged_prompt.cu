@@ -14,7 +14,10 @@
 //   warps 16-23      fetch the codes of a tile of 128 keys into registers while the tile before is at work, and write them as binary16 operands
 //                    (128-byte swizzle, both K-major: values lie with the keys of a column together)
 //   warp 24          issues S = Q K^T and O += P V
-// O is rescaled only when a row's maximum has grown by more than 2^8.  Which rows a block takes, and which part of their keys, stands in a list that a block of the
+// O is rescaled only when a row's maximum has grown by more than 2^8.  The accumulators cut what does not fit into 24 bits, so an O of many tiles comes
+// out short, by 2.4e-7 a tile where every tile adds two planes: of f32 rows it leaves tensor memory every six tiles and is summed in f32, rounded, in the
+// workspace (relative error of a prompt of 2048: 1.4e-6 without, 8.7e-7 so; of 8192 5.4e-6 and 1.1e-6; every four tiles 6.6e-7 and 8.0e-7; 32 heads, 2048 tokens: 72, 84 and
+// 87 us).  bf16 results are rounded to 2^-9 in any case.  Which rows a block takes, and which part of their keys, stands in a list that a block of the
 // kernel for few rows has made (paged_decode.cu): parts leave maximum, sum and O in the workspace, and the last to arrive joins them in order.  Every wait is bounded; a time-out raises the status word, and
 // the block frees its tensor memory and returns (no copies are under way: the fetches are loads).
 #include <climits>
@@ -50,7 +53,7 @@ struct PpShape {
     static constexpr int kQPlane = kPpRows * HD * 2, kQTile = NP * kQPlane, kK = kPpKeys * HD * 2, kVBox = HD * 128, kV = 2 * kVBox;
     static constexpr int kOffK = 2 * kQTile, kStages = kOffK + 2 * (kK + kV) <= 216 * 1024 ? 2 : 1;
     static constexpr int kOffV = kOffK + kStages * kK, kOffScales = kOffV + kStages * kV;
-    static constexpr int kOffStat = kOffScales + 4 * (int)sizeof(PpScales), kOffTop = kOffStat + 4 * kPpRows * 8;
+    static constexpr int kOffStat = kOffScales + 4 * (int)sizeof(PpScales), kOffTop = kOffStat + 4 * kPpRows * 16;
     static constexpr int kOffUnit = kOffTop + 2 * 4 * kPpRows * 4;
     static constexpr int kOffBars = kOffUnit + 2 * kPpRows * 8;
     static constexpr int kSmemBytes = kOffBars + 256 + 1024;
@@ -130,10 +133,13 @@ struct PpWork {
     const int4* list;
     int* arrived;      // [parts' places * kv heads], zero between calls
     float* partials;   // [parts' places * kv heads]: (maximum, sum) of 256 rows, then their O
+    float* sums;       // [multiprocessor][2][HD / 4][128 rows][4]: O of earlier tiles, one block at a time on each multiprocessor
 };
 template <int HD>
 __host__ __device__ constexpr size_t pp_partial_floats() { return (size_t)kPpUnit * (HD + 2); }
 constexpr int kPpSplitBlocks = 296;  // two for each multiprocessor
+constexpr int kPpSums = 160;         // multiprocessors that have a place for sums
+constexpr int kPpDrain = 6;
 
 template <int HD, typename T>
 __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const PagedArgs a, const PpWork work) {
@@ -187,6 +193,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
     tcgen05_fence_after();
     pdl_launch_dependents();
     bool ok = true;
+    uint32_t sm;
+    asm volatile("mov.u32 %0, %%smid;" : "=r"(sm));
+    const bool drains = NP == 2 && sm < (uint32_t)kPpSums;
     {
         const PagedRequest rq = PagedRequest::of(a, entry.x);
         const PagedUnit un = PagedUnit::of(a, rq, group, entry.y);
@@ -311,7 +320,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                 if (!(warp_wait(&v_full[st], (uint32_t)(j / kStages) & 1u) && warp_wait(&p_ready[s], (uint32_t)n & 1u))) return false;
                 tcgen05_fence_after();
                 const uint64_t dvj = dv + (uint64_t)(st * (S::kV >> 4));
-                uint32_t acc = n > 0 ? 1u : 0u;
+                uint32_t acc = (drains ? n % kPpDrain : n) > 0 ? 1u : 0u;
 #pragma unroll
                 for (int p = NP - 1; p >= 0; --p)
 #pragma unroll
@@ -405,6 +414,31 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
             const uint32_t rows = (uint32_t)((warp & 3) * 32) << 16;
             const uint32_t ts = rows + (uint32_t)stream * 128u, to = rows + kPpTmemO + (uint32_t)stream * 128u;
             float m_ref = -INFINITY, l = 0.0f;
+            // O of the tiles so far leaves tensor memory: half of the columns each, relative to the maximum at that time
+            float drained_ref = -INFINITY;
+            bool drained = false;
+            // (four columns of 128 rows lie together, so that a warp writes whole runs)
+            auto sums_of = [&](int s, int column) { return reinterpret_cast<float4*>(work.sums) + ((size_t)sm * 2 + s) * (HD / 4) * kPpRows + (size_t)(column / 4) * kPpRows + r; };
+            auto drain = [&]() {
+                const float turn = drained_ref == -INFINITY ? 0.0f : ex2_approx(drained_ref - m_ref);
+                float4* const run = sums_of(stream, half * (HD / 2));
+#pragma unroll 1
+                for (int i = 0; i < HD / 32; ++i) {
+                    float4 x[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[k] = drained ? run[(i * 4 + k) * kPpRows] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    uint32_t o[16];
+                    tmem_load_x16(to + half * (HD / 2) + i * 16, o);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        float4 v = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+                        v.x = fmaf(x[k].x, turn, v.x); v.y = fmaf(x[k].y, turn, v.y); v.z = fmaf(x[k].z, turn, v.z); v.w = fmaf(x[k].w, turn, v.w);
+                        run[(i * 4 + k) * kPpRows] = v;
+                    }
+                }
+                drained = true;
+                drained_ref = m_ref;
+            };
             int n = 0;  // tiles of this stream so far
             for (int j = two ? 0 : stream; j < end; j += step, ++n) {
                 const int t0 = first + j * kPpKeys;
@@ -476,6 +510,13 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                     }
                 };
                 auto tile = [&](auto is_masked) {
+                    const bool fresh = n == 0 || (drains && n % kPpDrain == 0);  // O begins anew with this tile
+                    if (fresh && n > 0) {
+                        ok = warp_wait(&pv_done[stream], (uint32_t)(n - 1) & 1u);
+                        if (!ok) return;
+                        tcgen05_fence_after();
+                        drain();
+                    }
                     uint32_t d[32];
                     tmem_load_x32(ts + half * 64, d);
                     float top = largest(is_masked, 2 * half, d);
@@ -494,7 +535,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                         const float corr = grow ? ex2_approx(m_ref - top) : 1.0f;
                         if (grow) m_ref = top;
                         l *= corr;
-                        if (n > 0) {  // half of the columns of O each
+                        if (!fresh) {  // half of the columns of O each
                             ok = warp_wait(&pv_done[stream], (uint32_t)(n - 1) & 1u);
                             if (!ok) return;
                             tcgen05_fence_after();
@@ -522,9 +563,10 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                 if (lane == 0) mbar_arrive(&p_ready[stream]);
             }
             if (ok && n > 0) ok = warp_wait(&pv_done[stream], (uint32_t)(n - 1) & 1u);
+            if (drained) __threadfence();
             // ---- the sum of both threads of a row; where the streams are shares of the keys, maximum and sum over both
-            float2* const stat = reinterpret_cast<float2*>(smem + S::kOffStat);  // [stream][half][row]
-            stat[(stream * 2 + half) * kPpRows + r] = make_float2(m_ref, l);
+            float4* const stat = reinterpret_cast<float4*>(smem + S::kOffStat);  // [stream][half][row]
+            stat[(stream * 2 + half) * kPpRows + r] = make_float4(m_ref, l, drained ? ex2_approx(drained_ref == -INFINITY ? -INFINITY : drained_ref - m_ref) : 0.0f, 0.0f);
             tcgen05_fence_before();
             asm volatile("bar.sync 1, 512;" ::: "memory");
             tcgen05_fence_after();
@@ -533,6 +575,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
             const float w0 = ex2_approx(m0 - mm), w1 = ex2_approx(m1 - mm), sum = two ? (stream == 0 ? l0 : l1) : l0 * w0 + l1 * w1, inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             const float whole = parts > 1 ? 1.0f : inv, f0 = two ? whole : w0 * whole, f1 = w1 * whole;
             const bool any0 = two ? n > 0 : tiles > 0, any1 = !two && tiles > 1;
+            // what left tensor memory earlier, relative to the maximum of its stream
+            const bool sums0 = drains && (two ? n : (tiles + 1) / 2) > kPpDrain, sums1 = drains && !two && tiles / 2 > kPpDrain;
+            const float g0 = f0 * stat[(two ? stream * 2 : 0) * kPpRows + r].z, g1 = f1 * stat[2 * kPpRows + r].z;
             float* const partial = work.partials + (size_t)((entry.w + part) * a.kv_heads + h) * pp_partial_floats<HD>();
             if (parts > 1 && half == 0 && (two || stream == 0)) reinterpret_cast<float2*>(partial)[two ? in_unit : r] = make_float2(two ? m_ref : m, sum);
             // half of the columns each: of the stream's rows, or (one tile of rows) a quarter for each of the four warps
@@ -552,6 +597,14 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                     for (int k = 0; k < 4; ++k) {
                         y[k] = any0 ? __uint_as_float(d[i + k]) * f0 : 0.0f;
                         if (any1) y[k] = fmaf(__uint_as_float(e[i + k]), f1, y[k]);
+                    }
+                    if (sums0) {
+                        const float4 x = __ldcg(sums_of(two ? stream : 0, from + c + i));
+                        y[0] = fmaf(x.x, g0, y[0]); y[1] = fmaf(x.y, g0, y[1]); y[2] = fmaf(x.z, g0, y[2]); y[3] = fmaf(x.w, g0, y[3]);
+                    }
+                    if (sums1) {
+                        const float4 x = __ldcg(sums_of(1, from + c + i));
+                        y[0] = fmaf(x.x, g1, y[0]); y[1] = fmaf(x.y, g1, y[1]); y[2] = fmaf(x.z, g1, y[2]); y[3] = fmaf(x.w, g1, y[3]);
                     }
                     *reinterpret_cast<float4*>(stage + lane * S::kStagePitch + c + i) = make_float4(y[0], y[1], y[2], y[3]);
                 }
@@ -640,11 +693,13 @@ int pp_capacity(int heads, int kv_heads, int requests, int tokens) {
     return (int)(n < 65535 ? n : 65535);
 }
 size_t pp_list_bytes(int capacity) { return ((size_t)(1 + capacity) * sizeof(int4) + 255) / 256 * 256; }
+size_t pp_partial_bytes(int head_dim) { return kPpSplitBlocks * sizeof(float) * (size_t)kPpUnit * (head_dim + 2); }
 constexpr size_t kPpArrivedBytes = (kPpSplitBlocks * 4 + 255) / 256 * 256;
 }  // namespace
 
 size_t paged_prompt_workspace_bytes(int heads, int kv_heads, int head_dim, int requests, int tokens) {
-    return pp_list_bytes(pp_capacity(heads, kv_heads, requests, tokens)) + kPpArrivedBytes + kPpSplitBlocks * sizeof(float) * (size_t)kPpUnit * (head_dim + 2);
+    return pp_list_bytes(pp_capacity(heads, kv_heads, requests, tokens)) + kPpArrivedBytes + pp_partial_bytes(head_dim) +
+           kPpSums * sizeof(float) * (size_t)kPpUnit * head_dim;
 }
 
 PagedOrder paged_prompt_order(const PagedArgs& a, void* workspace) {
@@ -656,7 +711,8 @@ int paged_prompt_launch(cudaStream_t stream, const PagedArgs& a, bool f32, void*
         return fail(KMLL_ERR_CAPACITY, "paged attention: %d tokens of %d heads in one call", a.tokens, a.heads);
     const int capacity = pp_capacity(a.heads, a.kv_heads, a.requests, a.tokens);
     unsigned char* const at = static_cast<unsigned char*>(workspace) + pp_list_bytes(capacity);
-    const PpWork work = {static_cast<const int4*>(workspace), reinterpret_cast<int*>(at), reinterpret_cast<float*>(at + kPpArrivedBytes)};
+    const PpWork work = {static_cast<const int4*>(workspace), reinterpret_cast<int*>(at), reinterpret_cast<float*>(at + kPpArrivedBytes),
+                         reinterpret_cast<float*>(at + kPpArrivedBytes + pp_partial_bytes(a.head_dim))};
     auto go = [&](auto kern, int smem) {
         cudaFuncAttributes fa;
         cudaError_t e = cudaFuncGetAttributes(&fa, kern);
