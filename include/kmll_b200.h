@@ -411,10 +411,12 @@ int kmll_paged_cache_rows(kmll_stream_t stream, const int8_t* k_codes, const flo
 /* Attention of a step's rows over the cache: row i of request r is position context[r] - rows + i and attends the positions up to its own, the
  * last `window` of them (0: all); query head h reads kv head h / (heads / kv_heads); softmax(scale * q . k) . v, scale > 0.  query and out are [tokens,
  * heads, head_dim], f32 or (is_f32 = 0) bf16.  A row that attends nothing is 0; rows of no request are left as they were.  Entries of block_table behind a
- * context are not read, entries outside the cache count as pages that are not attended.  max_query and max_context bound the rows and the context
- * of a request: they choose kernels and shares, not results.  workspace: kmll_paged_attention_workspace_bytes(...) bytes, 16-byte aligned, zero
- * before its first use (calls leave its counters zero); calls that overlap need workspaces of their own, so two graphs that may run at the
- * same time are captured with two.  May be null where that function says 0. */
+ * context are not read, entries outside the cache count as pages that are not attended.  max_query is at least the rows of every request (rows of a
+ * request with more are left as they were), max_context about its longest context; beyond that they choose kernels and shares, not results.
+ * workspace: kmll_paged_attention_workspace_bytes(...) bytes, 16-byte aligned, zero before its first use.  Calls leave zero what has to be, so one
+ * workspace serves calls of any sizes that need no more bytes, one after another; calls that overlap need workspaces of their own, and two
+ * graphs that may run at the same time are captured with two.  May be null where that function says 0.  requests * kv_heads <= 65536 for heads of
+ * 64 and 128.  f32 rows: relative error about 1e-6 against 64 bits; value scales of a head more than 2^100 apart lose the smaller ones. */
 size_t kmll_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim, int requests, int tokens, int max_query, int max_context);
 int kmll_paged_attention(kmll_stream_t stream, const void* query, int is_f32, const int32_t* query_start, const int32_t* context, const int32_t* block_table,
                          int table_width, int requests, int tokens, int max_query, int max_context, int heads, const int8_t* k_codes, const float* k_scales,

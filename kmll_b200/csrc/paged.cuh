@@ -92,15 +92,19 @@ struct PagedOrder {
 
 // paged_decode.cu: requests of at most kPagedDecodeRows rows, heads of 64 or 128
 constexpr int kPagedDecodeRows = 16;
+// A workspace begins with what has to be zero between calls, at places that no size of a call moves: a counter per (request, kv head), a counter per part of the
+// prompt kernel.  Scratch follows.
+constexpr int kPagedCounters = 65536, kPpSplitBlocks = 296;  // parts: two for each multiprocessor
+constexpr size_t kPagedZeroBytes = (size_t)kPagedCounters * 4 + (kPpSplitBlocks * 4 + 255) / 256 * 256;
 bool paged_decode_serves(int head_dim);
-size_t paged_decode_workspace_bytes(int requests, int kv_heads, int head_dim, int max_rows);
-int paged_decode_launch(cudaStream_t stream, const PagedArgs& a, bool f32, int max_rows, int max_context, void* workspace, const PagedOrder& order);
+size_t paged_decode_scratch_bytes(int head_dim, int max_rows);
+int paged_decode_launch(cudaStream_t stream, const PagedArgs& a, bool f32, int max_rows, int max_context, int* arrived, void* scratch, const PagedOrder& order);
 
 // paged_prompt.cu: requests of more than a.skip_rows rows, heads of 64 or 128
 bool paged_prompt_serves(const PagedArgs& a);
-size_t paged_prompt_workspace_bytes(int heads, int kv_heads, int head_dim, int requests, int tokens);
-PagedOrder paged_prompt_order(const PagedArgs& a, void* workspace);
-int paged_prompt_launch(cudaStream_t stream, const PagedArgs& a, bool f32, void* workspace);
+size_t paged_prompt_scratch_bytes(int heads, int kv_heads, int head_dim, int requests, int tokens);
+PagedOrder paged_prompt_order(const PagedArgs& a, void* scratch);
+int paged_prompt_launch(cudaStream_t stream, const PagedArgs& a, bool f32, int* arrived, void* scratch);
 int paged_prompt_status(int* status_out);  // 1 after a wait inside a kernel of that file ran out, 0 otherwise
 
 }  // namespace kmll

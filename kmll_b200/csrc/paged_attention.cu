@@ -94,8 +94,8 @@ static int few_rows(long long max_rows, int group) { return max_rows <= 8 || (ma
 extern "C" size_t kmll_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim, int requests, int tokens, int max_query, int max_context) {
     if (heads <= 0 || kv_heads <= 0 || requests <= 0 || tokens <= 0 || max_query <= 0 || !paged_decode_serves(head_dim)) return 0;
     const long long max_rows = (long long)max_query * (heads / kv_heads);
-    const size_t few = paged_decode_workspace_bytes(requests, kv_heads, head_dim, few_rows(max_rows, heads / kv_heads));
-    return max_rows <= kPagedDecodeRows ? few : (few + 255) / 256 * 256 + paged_prompt_workspace_bytes(heads, kv_heads, head_dim, requests, tokens);
+    const size_t few = kPagedZeroBytes + paged_decode_scratch_bytes(head_dim, few_rows(max_rows, heads / kv_heads));
+    return max_rows <= kPagedDecodeRows ? few : (few + 255) / 256 * 256 + paged_prompt_scratch_bytes(heads, kv_heads, head_dim, requests, tokens);
 }
 
 extern "C" int kmll_paged_attention(kmll_stream_t stream, const void* query, int is_f32, const int32_t* query_start, const int32_t* context, const int32_t* block_table,
@@ -121,15 +121,18 @@ extern "C" int kmll_paged_attention(kmll_stream_t stream, const void* query, int
         KMLL_REQUIRE_PTR(workspace);
         KMLL_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "paged attention: the workspace must be 16-byte aligned");
         const int limit = few_rows(max_rows, heads / kv_heads);
-        const size_t few = (paged_decode_workspace_bytes(requests, kv_heads, head_dim, limit) + 255) / 256 * 256;
-        void* const rest = static_cast<unsigned char*>(workspace) + few;
+        if ((long long)requests * kv_heads > kPagedCounters)
+            return fail(KMLL_ERR_CAPACITY, "paged attention: %d requests of %d kv heads, at most %d together", requests, kv_heads, kPagedCounters);
+        int* const counters = static_cast<int*>(workspace);
+        unsigned char* const scratch = static_cast<unsigned char*>(workspace) + kPagedZeroBytes;
+        unsigned char* const rest = static_cast<unsigned char*>(workspace) + (kPagedZeroBytes + paged_decode_scratch_bytes(head_dim, limit) + 255) / 256 * 256;
         const bool many = max_rows > kPagedDecodeRows && paged_prompt_serves(a);
         a.skip_rows = limit;
-        KMLL_TRY_RC(paged_decode_launch(as_stream(stream), a, is_f32 != 0, limit, max_context, workspace,
+        KMLL_TRY_RC(paged_decode_launch(as_stream(stream), a, is_f32 != 0, limit, max_context, counters, scratch,
                                         many ? paged_prompt_order(a, rest) : PagedOrder{nullptr, 0, 0}));
         if (max_rows <= kPagedDecodeRows) return check_launch("paged attention");
         if (many) {
-            KMLL_TRY_RC(paged_prompt_launch(as_stream(stream), a, is_f32 != 0, rest));
+            KMLL_TRY_RC(paged_prompt_launch(as_stream(stream), a, is_f32 != 0, counters + kPagedCounters, rest));
             return check_launch("paged attention");
         }
     }

@@ -695,20 +695,14 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
     }
 }
 
-size_t pd_counter_bytes(int requests, int kv_heads) { return ((size_t)requests * kv_heads * 4 + 255) / 256 * 256; }
-
 }  // namespace
 
 bool paged_decode_serves(int head_dim) { return head_dim == 64 || head_dim == 128; }
 
-size_t paged_decode_workspace_bytes(int requests, int kv_heads, int head_dim, int max_rows) {
-    return pd_counter_bytes(requests, kv_heads) + (size_t)kPdBlocks * 2 * (max_rows <= 8 ? 8 : 16) * (head_dim + 2) * 4;
-}
+size_t paged_decode_scratch_bytes(int head_dim, int max_rows) { return (size_t)kPdBlocks * 2 * (max_rows <= 8 ? 8 : 16) * (head_dim + 2) * 4; }
 
-int paged_decode_launch(cudaStream_t stream, const PagedArgs& a, bool f32, int max_rows, int max_context, void* workspace, const PagedOrder& order) {
-    PdWork work;
-    work.arrived = static_cast<int*>(workspace);
-    work.partials = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + pd_counter_bytes(a.requests, a.kv_heads));
+int paged_decode_launch(cudaStream_t stream, const PagedArgs& a, bool f32, int max_rows, int max_context, int* arrived, void* scratch, const PagedOrder& order) {
+    const PdWork work = {arrived, static_cast<float*>(scratch)};
     // no more blocks than there can be shares of one tile a warp
     const long long most = (long long)a.requests * a.kv_heads * (max_context / kPdKeys + 2 + kPdStretch), blocks = (most + kPdWarps - 1) / kPdWarps;
     const int at_once = max_rows <= 8 ? kPdBlocks : kPdBlocks / 3 * 2;

@@ -137,7 +137,6 @@ struct PpWork {
 };
 template <int HD>
 __host__ __device__ constexpr size_t pp_partial_floats() { return (size_t)kPpUnit * (HD + 2); }
-constexpr int kPpSplitBlocks = 296;  // two for each multiprocessor
 constexpr int kPpSums = 160;         // multiprocessors that have a place for sums
 constexpr int kPpDrain = 6;
 
@@ -259,8 +258,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                     PpScales& sc = scales[j & 3];
                     if (lane < 8) {
                         sc.k[lane] = ks;
-                        sc.log_v[lane] = vs > 0.0f ? log2f(vs) : page >= 0 ? -40.0f : 0.0f;
-                        sc.inv_v[lane] = vs > 0.0f ? 1.0f / vs : page >= 0 ? 0x1p40f : 0.0f;
+                        // (a page of zeros: any scale does, one so small that its weights do not push others out of binary16)
+                        sc.log_v[lane] = vs > 0.0f ? log2f(vs) : page >= 0 ? -80.0f : 0.0f;
+                        sc.inv_v[lane] = vs > 0.0f ? 1.0f / vs : page >= 0 ? 0x1p80f : 0.0f;
                     }
                     const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) & 0xffu;
                     if (lane == 0) sc.there = there;
@@ -694,25 +694,23 @@ int pp_capacity(int heads, int kv_heads, int requests, int tokens) {
 }
 size_t pp_list_bytes(int capacity) { return ((size_t)(1 + capacity) * sizeof(int4) + 255) / 256 * 256; }
 size_t pp_partial_bytes(int head_dim) { return kPpSplitBlocks * sizeof(float) * (size_t)kPpUnit * (head_dim + 2); }
-constexpr size_t kPpArrivedBytes = (kPpSplitBlocks * 4 + 255) / 256 * 256;
 }  // namespace
 
-size_t paged_prompt_workspace_bytes(int heads, int kv_heads, int head_dim, int requests, int tokens) {
-    return pp_list_bytes(pp_capacity(heads, kv_heads, requests, tokens)) + kPpArrivedBytes + pp_partial_bytes(head_dim) +
+size_t paged_prompt_scratch_bytes(int heads, int kv_heads, int head_dim, int requests, int tokens) {
+    return pp_list_bytes(pp_capacity(heads, kv_heads, requests, tokens)) + pp_partial_bytes(head_dim) +
            kPpSums * sizeof(float) * (size_t)kPpUnit * head_dim;
 }
 
-PagedOrder paged_prompt_order(const PagedArgs& a, void* workspace) {
-    return PagedOrder{static_cast<int4*>(workspace), pp_capacity(a.heads, a.kv_heads, a.requests, a.tokens), kPpSplitBlocks};
+PagedOrder paged_prompt_order(const PagedArgs& a, void* scratch) {
+    return PagedOrder{static_cast<int4*>(scratch), pp_capacity(a.heads, a.kv_heads, a.requests, a.tokens), kPpSplitBlocks};
 }
 
-int paged_prompt_launch(cudaStream_t stream, const PagedArgs& a, bool f32, void* workspace) {
+int paged_prompt_launch(cudaStream_t stream, const PagedArgs& a, bool f32, int* arrived, void* scratch) {
     if (pp_units(a.heads, a.kv_heads, a.requests, a.tokens) > 65535 || (long long)a.tokens * a.heads > INT_MAX)
         return fail(KMLL_ERR_CAPACITY, "paged attention: %d tokens of %d heads in one call", a.tokens, a.heads);
     const int capacity = pp_capacity(a.heads, a.kv_heads, a.requests, a.tokens);
-    unsigned char* const at = static_cast<unsigned char*>(workspace) + pp_list_bytes(capacity);
-    const PpWork work = {static_cast<const int4*>(workspace), reinterpret_cast<int*>(at), reinterpret_cast<float*>(at + kPpArrivedBytes),
-                         reinterpret_cast<float*>(at + kPpArrivedBytes + pp_partial_bytes(a.head_dim))};
+    unsigned char* const at = static_cast<unsigned char*>(scratch) + pp_list_bytes(capacity);
+    const PpWork work = {static_cast<const int4*>(scratch), arrived, reinterpret_cast<float*>(at), reinterpret_cast<float*>(at + pp_partial_bytes(a.head_dim))};
     auto go = [&](auto kern, int smem) {
         cudaFuncAttributes fa;
         cudaError_t e = cudaFuncGetAttributes(&fa, kern);

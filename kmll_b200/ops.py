@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import math
 from dataclasses import dataclass
 
 import torch
@@ -742,6 +743,8 @@ def paged_attention(query, query_start, context, block_table, cache: DevicePaged
     tokens, head_dim, dtype = query.shape[0], cache.head_dim, query.dtype
     heads = query.numel() // max(1, tokens * head_dim)
     need = tokens * heads * head_dim
+    if tokens == 0:
+        return torch.empty((0, math.prod(query.shape[1:])), dtype=dtype, device=query.device) if out is None else out
     if (dtype is not torch.float32 and dtype is not torch.bfloat16) or query.numel() != need:
         raise KmllError(-2, f"query must be [tokens, heads, {head_dim}] in float32 or bfloat16")
     out = torch.empty((tokens, heads * head_dim), dtype=dtype, device=query.device) if out is None else out

@@ -632,3 +632,42 @@ def test_the_device_reports_no_time_out(cuda):
     from kmll_b200 import lib
     status = ctypes.c_int(-1)
     assert lib.load().kmll_device_status(ctypes.byref(status)) == 0 and status.value == 0
+
+
+def test_one_workspace_for_calls_of_any_size(cuda):
+    """What has to be zero lies at the same place whatever the sizes: scratch of one call is no counter of the next."""
+    small = make_attention(81, 8, 2, 128, 32, [700], [1], torch.float32)
+    large = make_attention(82, 8, 2, 128, 32, [300 + 17 * i for i in range(40)], [1] * 40, torch.float32)
+    mixed = make_attention(83, 8, 2, 128, 32, [900, 40, 0], [30, 1, 90], torch.float32)
+    ws = ops.paged_attention_workspace(mixed["cache"], 8, 64, 200, 90, 2000)
+    for s in (small, large, mixed, small, mixed, large, large, small):
+        check_attention(s, workspace=ws)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_pages_of_zeros_and_tiny_values(cuda, new):
+    s = make_attention(84, 4, 1, 128, 16, [200, 90], [new, new], torch.float32)
+    k, v = s["values"]
+    cache = s["cache"]
+    cache.v_scales.mul_(1e-20)
+    zero = [int(p) for p in s["table"][:, 1]] + [int(s["table"][0, 4])]
+    cache.v_scales[zero] = 0.0
+    cache.v_codes[zero] = 0
+    cache.k_scales[int(s["table"][0, 2])] = 0.0
+    vc = cache.v_codes.cpu().numpy().transpose(0, 2, 4, 1, 3).reshape(v.shape).astype(np.float64)
+    kc = cache.k_codes.cpu().numpy().transpose(0, 3, 1, 2, 4).reshape(k.shape).astype(np.float64)
+    s["values"] = [kc * cache.k_scales.cpu().numpy().astype(np.float64)[:, None, :, None], vc * cache.v_scales.cpu().numpy().astype(np.float64)[:, None, :, None]]
+    check_attention(s)
+
+
+def test_steps_without_rows(cuda):
+    cache = ops.DevicePagedI8Cache.create(2, 16, 2, 64)
+    none = torch.zeros(0, 4, 64, device="cuda")
+    assert ops.paged_attention(none, ints([0]), ints([]), ints(np.zeros((0, 2))), cache, 0, 0, 0.1).shape == (0, 256)
+    assert ops.prepare_paged_attention(none, none[:, :2], none[:, :2], None, None, ints([]), cache).shape == (0, 4, 64)
+    k, v = ops.paged_cache_rows(cache, ints([]))
+    assert k.shape == v.shape == (0, 2, 64)
+    assert ops.sample_rows(torch.zeros(0, 32, device="cuda"), torch.zeros(0, dtype=torch.float64, device="cuda"))[0].shape == (0,)
+    out = torch.full((3, 256), 7.0, device="cuda")  # rows of no request
+    ops.paged_attention(torch.ones(3, 4, 64, device="cuda"), ints([0, 0, 0]), ints([5, 9]), ints(np.zeros((2, 2))), cache, 4, 16, 0.1, out=out)
+    assert (out == 7.0).all()
