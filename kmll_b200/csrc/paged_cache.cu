@@ -296,6 +296,7 @@ struct Angle {
 __device__ inline double finite_size(double v) { return fabs(v) < 1e300 ? fabs(v) : 0.0; }
 
 constexpr int kPrepareThreads = 256;
+constexpr int kPrepareShort = 4;  // tokens of a run that a warp takes
 
 // Angles of `tokens` positions, [token][freq].  A thread has a frequency and kSteps tokens; where their positions follow one another it computes the first
 // angle and turns on by one frequency at a time (in 64 bits: kSteps roundings).  It steps through its places without dividing.
@@ -327,6 +328,62 @@ __device__ inline void fill_angles(A* table, const int32_t* positions, const flo
     }
 }
 
+// The tokens in front of place `at` of a page are coded again, four codes a word: whole words of a key; of a value's column those in front.
+__device__ __noinline__ void code_again(int8_t* codes, bool keys, int at, float before, double s, double inv, int hd, int block, int lt, int threads) {
+    if (keys) {
+        for (int j = lt; j < at * (hd / 4); j += threads) {
+            const int i = j / (hd / 4), d = (j - i * (hd / 4)) * 4;
+            char4* const c = reinterpret_cast<char4*>(codes + ((d >> 4) * block + i) * 16 + (d & 15));
+            const char4 x = *c;
+            *c = make_char4((signed char)code_of(x.x * (double)before, s, inv), (signed char)code_of(x.y * (double)before, s, inv),
+                            (signed char)code_of(x.z * (double)before, s, inv), (signed char)code_of(x.w * (double)before, s, inv));
+        }
+    } else {
+        for (int j = lt; j < hd * ((at + 3) / 4); j += threads) {
+            const int i = j / hd * 4, d = j % hd;
+            signed char* const c = reinterpret_cast<signed char*>(codes + ((i >> 4) * hd + d) * 16 + (i & 15));
+            char4 x = *reinterpret_cast<char4*>(c);
+            x.x = (signed char)code_of(x.x * (double)before, s, inv);
+            if (i + 1 < at) x.y = (signed char)code_of(x.y * (double)before, s, inv);
+            if (i + 2 < at) x.z = (signed char)code_of(x.z * (double)before, s, inv);
+            if (i + 3 < at) x.w = (signed char)code_of(x.w * (double)before, s, inv);
+            *reinterpret_cast<char4*>(c) = x;
+        }
+    }
+}
+
+// A short run of one head by a warp: `in` is the run's first row, `codes` and `scale_at` the page's of that head.  The same numbers as the walks below make.
+template <typename T>
+__device__ inline void prepare_short(const T* in, size_t ld, bool keys, int turned, const float* freqs, const int32_t* positions, int n, int at, int hd, int block,
+                                           int8_t* codes, float* scale_at) {
+    const int lane = threadIdx.x & 31;
+    const float before = at == 0 ? 0.0f : *scale_at;
+    auto each = [&](auto f) {
+        for (int i = 0; i < n; ++i, in += ld) {
+            for (int d = lane; d < turned; d += 32) {
+                Angle turn;
+                turn.set(sin_cos((double)positions[i] * (double)freqs[d]));
+                const float x = load_as_f32(in + d), y = load_as_f32(in + d + turned);
+                f(i, d, turn.first(x, y));
+                f(i, d + turned, turn.second(x, y));
+            }
+            for (int d = 2 * turned + lane; d < hd; d += 32) f(i, d, (double)load_as_f32(in + d));
+        }
+        in -= (size_t)n * ld;
+    };
+    double largest = 0.0;
+    each([&](int, int, double v) { largest = fmax(largest, finite_size(v)); });
+    const float scale = fmaxf(before, warp_max((float)(largest / 127.0)));
+    const double s = scale, inv = scale > 0.0f ? 1.0 / s : 0.0;
+    if (lane == 0) *scale_at = scale;  // (all have read it: warp_max is behind the load)
+    if (scale > before && at > 0) code_again(codes, keys, at, before, s, inv, hd, block, lane, 32);
+    __syncwarp();  // (a word that holds codes of both is written above first)
+    each([&](int i, int d, double v) {
+        const int j = at + i;
+        codes[keys ? ((d >> 4) * block + j) * 16 + (d & 15) : ((j >> 4) * hd + d) * 16 + (j & 15)] = (int8_t)code_of(v, s, inv);
+    });
+}
+
 // Blocks of threads along x: keys (groups of tokens x sets of heads), values (the same), query rows.  A run is a stretch of tokens with ascending
 // slots in one page; the block whose tokens hold the first of a run takes all of it, so that a page's scale is known in one place.  A head has
 // 256 / HS threads; the first walk over the run finds the largest magnitude, the second (out of L1 / L2) codes.  The angles of a token are computed
@@ -342,7 +399,7 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_paged_kernel(const Pr
     constexpr int kHeadThreads = kPrepareThreads / HS;
     __shared__ int s_slots[2 * 128 + 1];
     __shared__ int s_run;
-    __shared__ uint32_t s_first[4];
+    __shared__ uint32_t s_first[4], s_short[4];
     __shared__ float s_top[kPrepareThreads / 32];
     const int tid = threadIdx.x, hd = a.head_dim, half = a.n_freqs, limit = a.pages * a.block;
     const int kv_blocks = a.groups * a.head_sets;
@@ -397,195 +454,197 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_paged_kernel(const Pr
     __syncthreads();
     const int block_log = 31 - __clz(a.block);
     if (tid < 128) {  // first tokens of runs, a bit each
-        bool first = false;
+        bool first = false, few = false;
         if (tid < t1 - t0) {
             const int slot = s_slots[tid + 1];
             first = slot >= 0 && slot < limit && ((slot & (a.block - 1)) == 0 || t0 + tid == 0 || s_slots[tid] != slot - 1);
+            if constexpr (HS == 1) {
+                const int n = min(a.block - (slot & (a.block - 1)), kPrepareShort + 1);
+                few = first && n <= kPrepareShort;
+                for (int i = 1; i < n; ++i) few = few || (first && s_slots[tid + 1 + i] != slot + i);
+            }
         }
-        const uint32_t bits = __ballot_sync(0xffffffffu, first);
-        if ((tid & 31) == 0) s_first[tid >> 5] = bits;
+        const uint32_t bits = __ballot_sync(0xffffffffu, first && !few), few_bits = __ballot_sync(0xffffffffu, few);
+        if ((tid & 31) == 0) {
+            s_first[tid >> 5] = bits;
+            s_short[tid >> 5] = few_bits;
+        }
     }
     __syncthreads();
-    for (int word = 0; word < 4; ++word)
-    for (uint32_t bits = s_first[word]; bits != 0u; bits &= bits - 1u) {
-        const int t = t0 + word * 32 + __ffs(bits) - 1;
-        const int* const slots = s_slots + (t - t0 + 1);
-        const int slot = slots[0], at = slot & (a.block - 1), page = slot >> block_log;
-        // ---- length of the run: up to the first token that does not follow
-        if (tid == 0) s_run = min(a.block - at, a.tokens - t);
-        __syncthreads();
-        for (int i = tid; i < a.block - at; i += kPrepareThreads)
-            if (slots[i] != slot + i) atomicMin(&s_run, i);
-        __syncthreads();
-        const int n = s_run;
-        const bool kept = n <= a.table_tokens;  // the angles of the whole run stay in shared memory
-        auto angles = [&](int i0, int i1) {
-            __syncthreads();
-            fill_angles<16>(key_table, a.positions + t + i0, a.freqs, i1 - i0, turned);
-            __syncthreads();
-        };
-        // calls f(token of the run, first entry, angles, the V pairs, the V turned pairs) for this thread's turned entries, and g(token, entry, V values) for the others
-        auto walk = [&](bool again, auto f, auto g) {
-            for (int i0 = 0; i0 < n && turned > 0; i0 += a.table_tokens) {
-                const int i1 = min(n, i0 + a.table_tokens), Q = turned / V;
-                if (!(again && kept)) angles(i0, i1);
-                if (!live) continue;
-#pragma unroll 2
-                for (int j = lt; j < (i1 - i0) * Q; j += kHeadThreads) {
-                    const int i = j / Q, d = (j - i * Q) * V;
-                    const T* const src = in + (size_t)(t + i0 + i) * ld + d;
-                    float x[V], y[V], p[V], q[V];
-                    load_some<V>(src, x);
-                    load_some<V>(src + turned, y);
-                    const Angle* const turn = key_table + i * turned + d;
-#pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        p[e] = fmaf(x[e], turn[e].cos, -(y[e] * turn[e].sin));
-                        q[e] = fmaf(x[e], turn[e].sin, y[e] * turn[e].cos);
-                    }
-                    f(i0 + i, d, turn, x, y, p, q);
-                }
-            }
-            const int R = (hd - 2 * turned) / V;
-            if (!live || R == 0) return;
-#pragma unroll 4
-            for (int j = lt; j < n * R; j += kHeadThreads) {
-                const int i = j / R, d = 2 * turned + (j - i * R) * V;
-                float x[V];
-                load_some<V>(in + (size_t)(t + i) * ld + d, x);
-                g(i, d, x);
-            }
-        };
-        using Some = const float (&)[V];
-        // ---- the largest magnitude, in 32 bits; of the turned keys those that may be it once more in 64 (of few tokens all at once: a walk less)
-        constexpr bool kAtOnce = HS > 1;
-        double largest = 0.0;
-        float largest32 = 0.0f;
-        bool beyond = false;  // a pair whose 32-bit rotation overflows (its entries may be infinities themselves)
-        walk(false, [&](int, int, const Angle* turn, Some x, Some y, Some p, Some q) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                if constexpr (kAtOnce) {
-                    largest = fmax(largest, fmax(finite_size(turn[e].first(x[e], y[e])), finite_size(turn[e].second(x[e], y[e]))));
-                    continue;
-                }
-                const float size = fmaxf(fabsf(p[e]), fabsf(q[e]));
-                beyond = beyond || !(fabsf(p[e]) < INFINITY) || !(fabsf(q[e]) < INFINITY);
-                if (size < INFINITY) largest32 = fmaxf(largest32, size);
-            }
-        }, [&](int, int, Some v) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) largest32 = fmaxf(largest32, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.0f);
-        });
-        if (kAtOnce || turned == 0) {
-            largest = fmax(largest, (double)largest32);
-        } else {
-            const float own = largest32;
-            const float mine = warp_max(own);
-            if ((tid & 31) == 0) s_top[tid >> 5] = mine;
-            const bool all = __syncthreads_or(beyond) != 0;
-            float most = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kHeadThreads / 32; ++w) most = fmaxf(most, s_top[sub * (kHeadThreads / 32) + w]);
-            const float near = all ? 0.0f : most * (1.0f - 0x1p-18f);
-            // (few threads have such entries; one that has none of its own goes along where the angles are not all there)
-            const bool mine_too = own >= near;
-            if (!kept || __any_sync(0xffffffffu, mine_too)) walk(true, [&](int, int, const Angle* turn, Some x, Some y, Some p, Some q) {
-                if (!mine_too) return;
-#pragma unroll 1
-                for (int e = 0; e < V; ++e)
-                    if (all || fmaxf(fabsf(p[e]), fabsf(q[e])) >= near) largest = fmax(largest, fmax(finite_size(turn[e].first(x[e], y[e])), finite_size(turn[e].second(x[e], y[e]))));
-            }, [&](int, int, Some v) {
-                if (!mine_too) return;
-#pragma unroll
-                for (int e = 0; e < V; ++e) largest = fmax(largest, finite_size((double)v[e]));
-            });
-            __syncthreads();  // (s_top is written again)
-        }
-        const float mine = warp_max((float)(largest / 127.0));
-        if ((tid & 31) == 0) s_top[tid >> 5] = mine;
-        float* const scale_at = (keys ? a.k_scales : a.v_scales) + (size_t)page * a.kv_heads + (live ? h : 0);
-        const float before = at == 0 ? 0.0f : *scale_at;
-        __syncthreads();  // (all have read the scale)
-        float scale = before;
-#pragma unroll
-        for (int w = 0; w < kHeadThreads / 32; ++w) scale = fmaxf(scale, s_top[sub * (kHeadThreads / 32) + w]);
-        const double s = scale, inv = scale > 0.0f ? 1.0 / s : 0.0;
-        const float inv32 = (float)inv;
-        int8_t* const codes = (keys ? a.k_codes : a.v_codes) + ((size_t)page * a.kv_heads + (live ? h : 0)) * a.block * hd;
-        if (live && lt == 0) *scale_at = scale;
-        if (live && scale > before && at > 0) {
-            // the tokens in front of the run are coded again, four codes a word: whole words of a key; of a value's column those in front of the run
-            if (keys) {
-                for (int j = lt; j < at * (hd / 4); j += kHeadThreads) {
-                    const int i = j / (hd / 4), d = (j - i * (hd / 4)) * 4;
-                    char4* const c = reinterpret_cast<char4*>(codes + ((d >> 4) * a.block + i) * 16 + (d & 15));
-                    const char4 x = *c;
-                    *c = make_char4((signed char)code_of(x.x * (double)before, s, inv), (signed char)code_of(x.y * (double)before, s, inv),
-                                    (signed char)code_of(x.z * (double)before, s, inv), (signed char)code_of(x.w * (double)before, s, inv));
-                }
-            } else {
-                for (int j = lt; j < hd * ((at + 3) / 4); j += kHeadThreads) {
-                    const int i = j / hd * 4, d = j % hd;
-                    signed char* const c = reinterpret_cast<signed char*>(codes + ((i >> 4) * hd + d) * 16 + (i & 15));
-                    char4 x = *reinterpret_cast<char4*>(c);
-                    x.x = (signed char)code_of(x.x * (double)before, s, inv);
-                    if (i + 1 < at) x.y = (signed char)code_of(x.y * (double)before, s, inv);
-                    if (i + 2 < at) x.z = (signed char)code_of(x.z * (double)before, s, inv);
-                    if (i + 3 < at) x.w = (signed char)code_of(x.w * (double)before, s, inv);
-                    *reinterpret_cast<char4*>(c) = x;
-                }
-                __threadfence_block();
+    if constexpr (HS == 1) {  // single tokens of many requests: a warp takes each
+        int turn = 0;
+        for (int word = 0; word < 4; ++word) {
+            for (uint32_t bits = s_short[word]; bits != 0u; bits &= bits - 1u) {
+                if (turn++ % (kPrepareThreads / 32) != tid >> 5) continue;
+                const int t = t0 + word * 32 + __ffs(bits) - 1;
+                const int* const slots = s_slots + (t - t0 + 1);
+                const int slot = slots[0], at = slot & (a.block - 1), most = min(a.block - at, a.tokens - t);
+                const size_t place = (size_t)(slot >> block_log) * a.kv_heads + h;
+                int n = 1;
+                while (n < most && slots[n] == slot + n) ++n;
+                prepare_short(in + (size_t)t * ld, ld, keys, turned, a.freqs, a.positions + t, n, at, hd, a.block, (keys ? a.k_codes : a.v_codes) + place * a.block * hd,
+                              (keys ? a.k_scales : a.v_scales) + place);
             }
         }
-        __syncthreads();  // (a word that holds codes of both is written above first)
-        if (keys) {
-            auto put = [&](int i, int d, const int (&c)[V]) {
-                int8_t* const to = codes + ((d >> 4) * a.block + at + i) * 16 + (d & 15);
-                if constexpr (V == 4) *reinterpret_cast<char4*>(to) = make_char4((signed char)c[0], (signed char)c[1], (signed char)c[2], (signed char)c[3]);
-                else *to = (int8_t)c[0];
+    }
+    for (int word = 0; word < 4; ++word) {
+        for (uint32_t bits = s_first[word]; bits != 0u; bits &= bits - 1u) {
+            const int t = t0 + word * 32 + __ffs(bits) - 1;
+            const int* const slots = s_slots + (t - t0 + 1);
+            const int slot = slots[0], at = slot & (a.block - 1), page = slot >> block_log;
+            // ---- length of the run: up to the first token that does not follow
+            if (tid == 0) s_run = min(a.block - at, a.tokens - t);
+            __syncthreads();
+            for (int i = tid; i < a.block - at; i += kPrepareThreads)
+                if (slots[i] != slot + i) atomicMin(&s_run, i);
+            __syncthreads();
+            const int n = s_run;
+            const bool kept = n <= a.table_tokens;  // the angles of the whole run stay in shared memory
+            auto angles = [&](int i0, int i1) {
+                __syncthreads();
+                fill_angles<16>(key_table, a.positions + t + i0, a.freqs, i1 - i0, turned);
+                __syncthreads();
             };
-            walk(true, [&](int i, int d, const Angle* turn, Some x, Some y, Some p, Some q) {
-                int c[2][V];
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    c[0][e] = quick_code(p[e], inv32);
-                    c[1][e] = quick_code(q[e], inv32);
+            // calls f(token of the run, first entry, angles, the V pairs, the V turned pairs) for this thread's turned entries, and g(token, entry, V values) for the others
+            auto walk = [&](bool again, auto f, auto g) {
+                for (int i0 = 0; i0 < n && turned > 0; i0 += a.table_tokens) {
+                    const int i1 = min(n, i0 + a.table_tokens), Q = turned / V;
+                    if (!(again && kept)) angles(i0, i1);
+                    if (!live) continue;
+    #pragma unroll 2
+                    for (int j = lt; j < (i1 - i0) * Q; j += kHeadThreads) {
+                        const int i = j / Q, d = (j - i * Q) * V;
+                        const T* const src = in + (size_t)(t + i0 + i) * ld + d;
+                        float x[V], y[V], p[V], q[V];
+                        load_some<V>(src, x);
+                        load_some<V>(src + turned, y);
+                        const Angle* const turn = key_table + i * turned + d;
+    #pragma unroll
+                        for (int e = 0; e < V; ++e) {
+                            p[e] = fmaf(x[e], turn[e].cos, -(y[e] * turn[e].sin));
+                            q[e] = fmaf(x[e], turn[e].sin, y[e] * turn[e].cos);
+                        }
+                        f(i0 + i, d, turn, x, y, p, q);
+                    }
                 }
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    if (c[0][e] == -1000) c[0][e] = code_of(turn[e].first(x[e], y[e]), s, inv);
-                    if (c[1][e] == -1000) c[1][e] = code_of(turn[e].second(x[e], y[e]), s, inv);
+                const int R = (hd - 2 * turned) / V;
+                if (!live || R == 0) return;
+    #pragma unroll 4
+                for (int j = lt; j < n * R; j += kHeadThreads) {
+                    const int i = j / R, d = 2 * turned + (j - i * R) * V;
+                    float x[V];
+                    load_some<V>(in + (size_t)(t + i) * ld + d, x);
+                    g(i, d, x);
                 }
-                put(i, d, c[0]);
-                put(i, d + turned, c[1]);
-            }, [&](int i, int d, Some v) {
-                int c[V];
-#pragma unroll
-                for (int e = 0; e < V; ++e) c[e] = code_of(v[e], s, inv, inv32);
-                put(i, d, c);
+            };
+            using Some = const float (&)[V];
+            // ---- the largest magnitude, in 32 bits; of the turned keys those that may be it once more in 64 (of few tokens all at once: a walk less)
+            constexpr bool kAtOnce = HS > 1;
+            double largest = 0.0;
+            float largest32 = 0.0f;
+            bool beyond = false;  // a pair whose 32-bit rotation overflows (its entries may be infinities themselves)
+            walk(false, [&](int, int, const Angle* turn, Some x, Some y, Some p, Some q) {
+    #pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    if constexpr (kAtOnce) {
+                        largest = fmax(largest, fmax(finite_size(turn[e].first(x[e], y[e])), finite_size(turn[e].second(x[e], y[e]))));
+                        continue;
+                    }
+                    const float size = fmaxf(fabsf(p[e]), fabsf(q[e]));
+                    beyond = beyond || !(fabsf(p[e]) < INFINITY) || !(fabsf(q[e]) < INFINITY);
+                    if (size < INFINITY) largest32 = fmaxf(largest32, size);
+                }
+            }, [&](int, int, Some v) {
+    #pragma unroll
+                for (int e = 0; e < V; ++e) largest32 = fmaxf(largest32, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.0f);
             });
-        } else if (live) {
-            // groups of 16 tokens of a column: one 16-byte store where the run has all of them
-            const int g0 = at >> 4, g1 = (at + n - 1) >> 4;
-            for (int j = lt; j < (g1 - g0 + 1) * hd; j += kHeadThreads) {
-                const int g = g0 + j / hd, d = j % hd, i0 = g * 16 - at;  // token of the run at the group's first place
-                int8_t* const to = codes + ((size_t)g * hd + d) * 16;
-                if (i0 >= 0 && i0 + 16 <= n) {
-                    const T* src = in + (size_t)(t + i0) * ld + d;
-                    float x[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) x[e] = load_as_f32(src + (size_t)e * ld);
-                    uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) w[e >> 2] |= (uint32_t)(code_of(x[e], s, inv, inv32) & 255) << (8 * (e & 3));
-                    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-                } else {
-                    for (int i = max(i0, 0); i < min(i0 + 16, n); ++i) to[i - i0] = (int8_t)code_of(load_as_f32(in + (size_t)(t + i) * ld + d), s, inv, inv32);
+            if (kAtOnce || turned == 0) {
+                largest = fmax(largest, (double)largest32);
+            } else {
+                const float own = largest32;
+                const float mine = warp_max(own);
+                if ((tid & 31) == 0) s_top[tid >> 5] = mine;
+                const bool all = __syncthreads_or(beyond) != 0;
+                float most = 0.0f;
+    #pragma unroll
+                for (int w = 0; w < kHeadThreads / 32; ++w) most = fmaxf(most, s_top[sub * (kHeadThreads / 32) + w]);
+                const float near = all ? 0.0f : most * (1.0f - 0x1p-18f);
+                // (few threads have such entries; one that has none of its own goes along where the angles are not all there)
+                const bool mine_too = own >= near;
+                if (!kept || __any_sync(0xffffffffu, mine_too)) walk(true, [&](int, int, const Angle* turn, Some x, Some y, Some p, Some q) {
+                    if (!mine_too) return;
+    #pragma unroll 1
+                    for (int e = 0; e < V; ++e)
+                        if (all || fmaxf(fabsf(p[e]), fabsf(q[e])) >= near) largest = fmax(largest, fmax(finite_size(turn[e].first(x[e], y[e])), finite_size(turn[e].second(x[e], y[e]))));
+                }, [&](int, int, Some v) {
+                    if (!mine_too) return;
+    #pragma unroll
+                    for (int e = 0; e < V; ++e) largest = fmax(largest, finite_size((double)v[e]));
+                });
+                __syncthreads();  // (s_top is written again)
+            }
+            const float mine = warp_max((float)(largest / 127.0));
+            if ((tid & 31) == 0) s_top[tid >> 5] = mine;
+            float* const scale_at = (keys ? a.k_scales : a.v_scales) + (size_t)page * a.kv_heads + (live ? h : 0);
+            const float before = at == 0 ? 0.0f : *scale_at;
+            __syncthreads();  // (all have read the scale)
+            float scale = before;
+    #pragma unroll
+            for (int w = 0; w < kHeadThreads / 32; ++w) scale = fmaxf(scale, s_top[sub * (kHeadThreads / 32) + w]);
+            const double s = scale, inv = scale > 0.0f ? 1.0 / s : 0.0;
+            const float inv32 = (float)inv;
+            int8_t* const codes = (keys ? a.k_codes : a.v_codes) + ((size_t)page * a.kv_heads + (live ? h : 0)) * a.block * hd;
+            if (live && lt == 0) *scale_at = scale;
+            if (live && scale > before && at > 0) code_again(codes, keys, at, before, s, inv, hd, a.block, lt, kHeadThreads);
+            __syncthreads();  // (a word that holds codes of both is written above first)
+            if (keys) {
+                auto put = [&](int i, int d, const int (&c)[V]) {
+                    int8_t* const to = codes + ((d >> 4) * a.block + at + i) * 16 + (d & 15);
+                    if constexpr (V == 4) *reinterpret_cast<char4*>(to) = make_char4((signed char)c[0], (signed char)c[1], (signed char)c[2], (signed char)c[3]);
+                    else *to = (int8_t)c[0];
+                };
+                walk(true, [&](int i, int d, const Angle* turn, Some x, Some y, Some p, Some q) {
+                    int c[2][V];
+    #pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        c[0][e] = quick_code(p[e], inv32);
+                        c[1][e] = quick_code(q[e], inv32);
+                    }
+    #pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        if (c[0][e] == -1000) c[0][e] = code_of(turn[e].first(x[e], y[e]), s, inv);
+                        if (c[1][e] == -1000) c[1][e] = code_of(turn[e].second(x[e], y[e]), s, inv);
+                    }
+                    put(i, d, c[0]);
+                    put(i, d + turned, c[1]);
+                }, [&](int i, int d, Some v) {
+                    int c[V];
+    #pragma unroll
+                    for (int e = 0; e < V; ++e) c[e] = code_of(v[e], s, inv, inv32);
+                    put(i, d, c);
+                });
+            } else if (live) {
+                // groups of 16 tokens of a column: one 16-byte store where the run has all of them
+                const int g0 = at >> 4, g1 = (at + n - 1) >> 4;
+                for (int j = lt; j < (g1 - g0 + 1) * hd; j += kHeadThreads) {
+                    const int g = g0 + j / hd, d = j % hd, i0 = g * 16 - at;  // token of the run at the group's first place
+                    int8_t* const to = codes + ((size_t)g * hd + d) * 16;
+                    if (i0 >= 0 && i0 + 16 <= n) {
+                        const T* src = in + (size_t)(t + i0) * ld + d;
+                        float x[16];
+    #pragma unroll
+                        for (int e = 0; e < 16; ++e) x[e] = load_as_f32(src + (size_t)e * ld);
+                        uint32_t w[4] = {0u, 0u, 0u, 0u};
+    #pragma unroll
+                        for (int e = 0; e < 16; ++e) w[e >> 2] |= (uint32_t)(code_of(x[e], s, inv, inv32) & 255) << (8 * (e & 3));
+                        *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+                    } else {
+                        for (int i = max(i0, 0); i < min(i0 + 16, n); ++i) to[i - i0] = (int8_t)code_of(load_as_f32(in + (size_t)(t + i) * ld + d), s, inv, inv32);
+                    }
                 }
             }
+            __syncthreads();
         }
-        __syncthreads();
     }
 }
 
@@ -731,10 +790,13 @@ extern "C" int kmll_prepare_paged_attention(kmll_stream_t stream, const void* qu
     }
     PrepareArgs a = {query, key, value, (size_t)ld_query, (size_t)ld_key, (size_t)ld_value, freqs, n_freqs, positions, slots, tokens, heads, kv_heads, head_dim,
                      query_rot, k_codes, v_codes, k_scales, v_scales, pages, block};
-    // few tokens: each may begin a run; many: they come in pages, and one block of threads per page has no runs that begin elsewhere to step over
-    a.group = tokens <= 512 ? 1 : block;
+    // Few tokens: each may begin a run, 64 threads a head (64 requests of a token: 5.8 us, in groups of 16 8.4; a prompt of 64: 23 and 14).  More: a block takes
+    // the runs of a group, short ones by warps.  Groups are short while blocks are few (600 tokens of as many requests: 21 us, in groups of a page of 64
+    // 31) and pages from there on (2574 tokens of four prompts: 38 us, in groups of 16 43).
+    constexpr int kFewTokens = 64, kSomeTokens = 1024;
+    a.group = tokens <= kFewTokens ? 1 : tokens <= kSomeTokens ? min(block, 16) : block;
     a.groups = (tokens + a.group - 1) / a.group;
-    const int head_set = tokens <= 512 ? 4 : 1;  // (a page of tokens is work for 256 threads, single tokens are not)
+    const int head_set = tokens <= kFewTokens ? 4 : 1;  // (a page of tokens is work for 256 threads, single tokens are not)
     a.head_sets = (kv_heads + head_set - 1) / head_set;
     a.q_tokens = tokens <= 512 ? 1 : 8;
     const int per_token = n_freqs * (int)sizeof(double2);

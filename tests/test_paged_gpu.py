@@ -208,6 +208,34 @@ def test_prepare_of_long_prompts(cuda, tokens, block):
     assert (np.abs(f64(turned) - want) <= 2.0 ** -23 * np.abs(want) + 1e-30).all()
 
 
+@pytest.mark.parametrize("requests, most, kv, hd, rot, block", [(66, 1, 2, 64, 32, 16), (300, 4, 1, 80, 24, 32), (700, 6, 1, 32, 16, 128), (40, 5, 3, 256, 0, 64)])
+def test_prepare_of_short_runs(cuda, requests, most, kv, hd, rot, block):
+    """Steps of a few tokens each for many requests, among them the first and last places of a page and padded rows, over steps in which scales grow."""
+    rng = np.random.default_rng(requests)
+    heads, pages = 2 * kv, 2 * requests
+    cache, ks, vs = ops.DevicePagedI8Cache.create(pages, block, kv, hd), po.Store(pages, block, kv, hd), po.Store(pages, block, kv, hd)
+    table, lengths, freqs = rng.permutation(pages).reshape(requests, 2), rng.integers(0, 2, requests) * (block - most), freqs_of(rot, hd)
+    for step in range(3):
+        slots, positions = [], []
+        for r in range(requests):
+            for p in range(lengths[r], lengths[r] + int(rng.integers(1, most + 1))):
+                slots.append(int(table[r, p // block]) * block + p % block)
+                positions.append(p + 7 * r)
+                lengths[r] += 1
+            if r % 50 == 7:
+                slots.append(-1)
+                positions.append(0)
+        n = len(slots)
+        q, k, v = (torch.tensor(rng.normal(0, 1 + step, (n, h, hd)), device="cuda", dtype=torch.float32) for h in (heads, kv, kv))
+        turned = ops.prepare_paged_attention(q, k, v, torch.tensor(freqs, device="cuda") if rot else None, ints(positions), ints(slots), cache)
+        ks.append(po.rotate(f64(k), positions, freqs) if rot else f64(k), slots)
+        vs.append(f64(v), slots)
+        want = po.rotate(f64(q), positions, freqs) if rot else f64(q)
+        live = np.array(slots) >= 0
+        assert (np.abs(f64(turned) - want) <= 2.0 ** -23 * np.abs(want) + 1e-30)[live].all()
+        same_cache(cache, ks, vs)
+
+
 def test_values_that_are_not_finite_do_not_spoil_their_page(cuda):
     cache, ks, vs = ops.DevicePagedI8Cache.create(3, 16, 1, 32), po.Store(3, 16, 1, 32), po.Store(3, 16, 1, 32)
     x = torch.randn(6, 1, 32, generator=torch.Generator("cuda").manual_seed(1), device="cuda")
