@@ -416,7 +416,9 @@ int kmll_paged_cache_rows(kmll_stream_t stream, const int8_t* k_codes, const flo
  * workspace: kmll_paged_attention_workspace_bytes(...) bytes, 16-byte aligned, zero before its first use.  Calls leave zero what has to be, so one
  * workspace serves calls of any sizes that need no more bytes, one after another; calls that overlap need workspaces of their own, and two
  * graphs that may run at the same time are captured with two.  May be null where that function says 0.  requests * kv_heads <= 65536 for heads of
- * 64 and 128.  f32 rows: relative error about 1e-6 against 64 bits; value scales of a head more than 2^100 apart lose the smaller ones. */
+ * 64 and 128.  f32 rows: relative error about 1e-6 against 64 bits; prompts take
+ * value scales below 2^-80 for 2^-80, and weights whose value scale is less than 2^-100 of the head's largest are lost.  After a time-out
+ * (kmll_device_status) the workspace has to be zeroed. */
 size_t kmll_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim, int requests, int tokens, int max_query, int max_context);
 int kmll_paged_attention(kmll_stream_t stream, const void* query, int is_f32, const int32_t* query_start, const int32_t* context, const int32_t* block_table,
                          int table_width, int requests, int tokens, int max_query, int max_context, int heads, const int8_t* k_codes, const float* k_scales,

@@ -102,6 +102,7 @@ int paged_decode_launch(cudaStream_t stream, const PagedArgs& a, bool f32, int m
 
 // paged_prompt.cu: requests of more than a.skip_rows rows, heads of 64 or 128
 bool paged_prompt_serves(const PagedArgs& a);
+bool paged_prompt_fits(const PagedArgs& a);  // its blocks and rows in 16 and 31 bits
 size_t paged_prompt_scratch_bytes(int heads, int kv_heads, int head_dim, int requests, int tokens);
 PagedOrder paged_prompt_order(const PagedArgs& a, void* scratch);
 int paged_prompt_launch(cudaStream_t stream, const PagedArgs& a, bool f32, int* arrived, void* scratch);

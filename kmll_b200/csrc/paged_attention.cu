@@ -105,7 +105,7 @@ extern "C" int kmll_paged_attention(kmll_stream_t stream, const void* query, int
     KMLL_TRY_RC(check_paged_cache("paged attention", k_codes, k_scales, v_codes, v_scales, pages, block, kv_heads, head_dim));
     KMLL_REQUIRE(requests >= 0 && tokens >= 0 && max_query >= 0 && max_context >= 0 && table_width >= 0, "paged attention: negative size");
     KMLL_REQUIRE(heads > 0 && heads <= 65535 && heads % kv_heads == 0, "paged attention: %d query heads over %d kv heads", heads, kv_heads);
-    KMLL_REQUIRE((long long)table_width * block <= INT_MAX, "paged attention: a table of %d pages of %d tokens: positions are 32 bits", table_width, block);
+    KMLL_REQUIRE((long long)table_width * block <= INT_MAX - 1024, "paged attention: a table of %d pages of %d tokens: positions are 32 bits", table_width, block);
     KMLL_REQUIRE(scale > 0.0f && scale < INFINITY, "paged attention: scale must be positive and finite");
     KMLL_REQUIRE(window >= 0, "paged attention: negative window");
     if (requests == 0 || tokens == 0 || max_query == 0) return KMLL_OK;
@@ -127,6 +127,7 @@ extern "C" int kmll_paged_attention(kmll_stream_t stream, const void* query, int
         unsigned char* const scratch = static_cast<unsigned char*>(workspace) + kPagedZeroBytes;
         unsigned char* const rest = static_cast<unsigned char*>(workspace) + (kPagedZeroBytes + paged_decode_scratch_bytes(head_dim, limit) + 255) / 256 * 256;
         const bool many = max_rows > kPagedDecodeRows && paged_prompt_serves(a);
+        if (many && !paged_prompt_fits(a)) return fail(KMLL_ERR_CAPACITY, "paged attention: %d tokens of %d heads in one call", tokens, heads);
         a.skip_rows = limit;
         KMLL_TRY_RC(paged_decode_launch(as_stream(stream), a, is_f32 != 0, limit, max_context, counters, scratch,
                                         many ? paged_prompt_order(a, rest) : PagedOrder{nullptr, 0, 0}));

@@ -79,7 +79,7 @@ __device__ inline void load4<uint16_t>(const void* p, size_t i, float (&v)[4]) {
 }
 
 struct PdWork {
-    int* arrived;     // [requests * kv_heads], zero between calls
+    int* arrived;     // [requests * kv_heads] of kPagedCounters, zero between calls
     float* partials;  // [blocks][2]: (maximum, sum) of 8 * NC rows, then their O
 };
 
@@ -301,9 +301,9 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
         const int key0 = rq.lo / kPdKeys * kPdKeys;  // of tile 0
         const int32_t* const table = a.table + (size_t)r * a.width;
         const int mine_n = tb - ta > warp ? (tb - ta - warp + kPdWarps - 1) / kPdWarps : 0;
-        auto page_of = [&](int i) {  // of this lane's group of 16 keys in the warp's i-th tile; -1: nothing there
+        auto page_of = [&](int i) {  // of this lane's group of 16 keys in the warp's i-th tile; -1: nothing there, or nothing attended (the page may be another request's by now)
             const int key = key0 + (ta + warp + i * kPdWarps) * kPdKeys + half * 16;
-            if (i >= mine_n || key >= rq.hi) return -1;
+            if (i >= mine_n || key >= rq.hi || key + 16 <= rq.lo) return -1;
             const int p = table[key / a.block];
             return p >= 0 && p < a.pages ? p : -1;
         };
@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
         };
         auto entry_of = [&](int i) {  // the same, not yet looked at
             const int key = key0 + (ta + warp + i * kPdWarps) * kPdKeys + half * 16;
-            return i >= mine_n || key >= rq.hi ? -1 : table[key / a.block];
+            return i >= mine_n || key >= rq.hi || key + 16 <= rq.lo ? -1 : table[key / a.block];
         };
         int pages[kPdStages];
 #pragma unroll

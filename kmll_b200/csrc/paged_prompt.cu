@@ -258,9 +258,10 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                     PpScales& sc = scales[j & 3];
                     if (lane < 8) {
                         sc.k[lane] = ks;
-                        // (a page of zeros: any scale does, one so small that its weights do not push others out of binary16)
-                        sc.log_v[lane] = vs > 0.0f ? log2f(vs) : page >= 0 ? -80.0f : 0.0f;
-                        sc.inv_v[lane] = vs > 0.0f ? 1.0f / vs : page >= 0 ? 0x1p80f : 0.0f;
+                        // (a page of zeros or of next to nothing: its weights still count in the sum, and do not push others out of binary16)
+                        const float v = fmaxf(vs, 0x1p-80f);
+                        sc.log_v[lane] = page >= 0 ? log2f(v) : 0.0f;
+                        sc.inv_v[lane] = page >= 0 ? 1.0f / v : 0.0f;
                     }
                     const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) & 0xffu;
                     if (lane == 0) sc.there = there;
@@ -680,10 +681,6 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
 
 }  // namespace
 
-bool paged_prompt_serves(const PagedArgs& a) {
-    return (a.head_dim == 64 || a.head_dim == 128) && ((reinterpret_cast<uintptr_t>(a.query) | reinterpret_cast<uintptr_t>(a.out)) & 15u) == 0;
-}
-
 namespace {
 long long pp_units(int heads, int kv_heads, int requests, int tokens) {  // each request ends in a unit of its own
     return ((long long)tokens * (heads / kv_heads) + kPpUnit - 1) / kPpUnit + requests;
@@ -696,6 +693,13 @@ size_t pp_list_bytes(int capacity) { return ((size_t)(1 + capacity) * sizeof(int
 size_t pp_partial_bytes(int head_dim) { return kPpSplitBlocks * sizeof(float) * (size_t)kPpUnit * (head_dim + 2); }
 }  // namespace
 
+bool paged_prompt_serves(const PagedArgs& a) {
+    return (a.head_dim == 64 || a.head_dim == 128) && ((reinterpret_cast<uintptr_t>(a.query) | reinterpret_cast<uintptr_t>(a.out)) & 15u) == 0;
+}
+
+bool paged_prompt_fits(const PagedArgs& a) {
+    return pp_units(a.heads, a.kv_heads, a.requests, a.tokens) <= 65535 && (long long)a.tokens * a.heads <= INT_MAX;
+}
 size_t paged_prompt_scratch_bytes(int heads, int kv_heads, int head_dim, int requests, int tokens) {
     return pp_list_bytes(pp_capacity(heads, kv_heads, requests, tokens)) + pp_partial_bytes(head_dim) +
            kPpSums * sizeof(float) * (size_t)kPpUnit * head_dim;
@@ -706,8 +710,6 @@ PagedOrder paged_prompt_order(const PagedArgs& a, void* scratch) {
 }
 
 int paged_prompt_launch(cudaStream_t stream, const PagedArgs& a, bool f32, int* arrived, void* scratch) {
-    if (pp_units(a.heads, a.kv_heads, a.requests, a.tokens) > 65535 || (long long)a.tokens * a.heads > INT_MAX)
-        return fail(KMLL_ERR_CAPACITY, "paged attention: %d tokens of %d heads in one call", a.tokens, a.heads);
     const int capacity = pp_capacity(a.heads, a.kv_heads, a.requests, a.tokens);
     unsigned char* const at = static_cast<unsigned char*>(scratch) + pp_list_bytes(capacity);
     const PpWork work = {static_cast<const int4*>(scratch), arrived, reinterpret_cast<float*>(at), reinterpret_cast<float*>(at + pp_partial_bytes(a.head_dim))};

@@ -699,3 +699,25 @@ def test_steps_without_rows(cuda):
     out = torch.full((3, 256), 7.0, device="cuda")  # rows of no request
     ops.paged_attention(torch.ones(3, 4, 64, device="cuda"), ints([0, 0, 0]), ints([5, 9]), ints(np.zeros((2, 2))), cache, 4, 16, 0.1, out=out)
     assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("new", [1, 3, 40])
+def test_pages_in_front_of_a_window_are_not_looked_at(cuda, new):
+    """They may be another request's by now, or hold anything: scales that are not finite, and far larger ones."""
+    for trouble in (math.nan, math.inf, 1e20):
+        s = make_attention(85, 4, 1, 128, 16, [400, 130], [new, new], torch.float32)
+        cache, table = s["cache"], s["table"]
+        for r, cached in enumerate((400, 130)):
+            for i in range((cached - 49) // 16):
+                cache.k_scales[int(table[r, i])] = trouble
+                cache.v_scales[int(table[r, i])] = trouble
+        check_attention(s, window=50)
+
+
+def test_value_scales_below_the_smallest_that_prompts_tell_apart(cuda):
+    """Their weights still count: a row whose other keys are of ordinary size keeps its sum."""
+    s = make_attention(86, 4, 1, 128, 16, [200], [40], torch.float32)
+    tiny = [int(s["table"][0, i]) for i in (0, 3, 7)]
+    s["cache"].v_scales[tiny] = 1e-38
+    s["values"][1][tiny] *= 0.0  # (below the tolerance by 20 orders)
+    check_attention(s)
