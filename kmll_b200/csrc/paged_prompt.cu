@@ -10,16 +10,21 @@
 // Two streams of work share the keys that are brought in: two tiles of 128 rows, or (where there are 128 rows at most) the even and the odd
 // key tiles of one, each with a maximum, a sum and an O of its own, merged at the end.  Roles of the 28 warps:
 //   warps 0-7, 8-15  softmax of a stream, two threads per row with 64 keys of a tile each: scores by tcgen05.ld, their maximum (both threads'), then
-//                    the weights, which go back in the place of the scores.  (One thread per row: 3400 cycles a tile, all of it latency.)
+//                    the weights, which go back in the place of the scores
 //   warps 16-23      fetch the codes of a tile of 128 keys into registers while the tile before is at work, and write them as binary16 operands
 //                    (128-byte swizzle, both K-major: values lie with the keys of a column together)
 //   warp 24          issues S = Q K^T and O += P V
-// O is rescaled only when a row's maximum has grown by more than 2^8.  The accumulators cut what does not fit into 24 bits, so an O of many tiles comes
-// out short, by 2.4e-7 a tile where every tile adds two planes: of f32 rows it leaves tensor memory every six tiles and is summed in f32, rounded, in the
-// workspace (relative error of a prompt of 2048: 1.4e-6 without, 8.7e-7 so; of 8192 5.4e-6 and 1.1e-6; every four tiles 6.6e-7 and 8.0e-7; 32 heads, 2048 tokens: 72, 84 and
-// 87 us).  bf16 results are rounded to 2^-9 in any case.  Which rows a block takes, and which part of their keys, stands in a list that a block of the
-// kernel for few rows has made (paged_decode.cu): parts leave maximum, sum and O in the workspace, and the last to arrive joins them in order.  Every wait is bounded; a time-out raises the status word, and
-// the block frees its tensor memory and returns (no copies are under way: the fetches are loads).
+// O is rescaled only when a row's maximum has grown by more than 2^8.  The accumulators cut what does not fit into 24 bits, so an O of many tiles
+// comes out short, by 2.4e-7 a tile where every tile adds two planes: of f32 rows it leaves tensor memory every six tiles and is summed in f32,
+// rounded, in the workspace (relative error of a prompt of 2048: 1.4e-6 without, 8.7e-7 so; of 8192 5.4e-6 and 1.1e-6; every four tiles 6.6e-7
+// and 8.0e-7; 32 query heads over 8, 2048 tokens: 73, 84 and 87 us).  bf16 results are rounded to 2^-9 in any case.
+// Which rows a block takes, and which part of their keys, stands in a list that a block of the kernel for few rows has made (paged_decode.cu):
+// parts leave maximum, sum and O in the workspace, and the last to arrive joins them in order.
+// Every wait is bounded; a time-out raises the status word, and the block frees its tensor memory and returns (no copies are under way: the
+// fetches are loads).
+// Bound: the softmax between the two MMAs of a tile (one thread a row took 3400 cycles a tile, all of it latency), beside the MMAs of f32 rows' two
+// planes.  32 query heads over 8, head size 128, random codes: 2048 tokens 72 us (bf16), 84 to 99 us (f32: more where maxima keep growing), 8192
+// tokens 594 us (bf16, 0.93 PFLOP/s of the causal half) and 965 us (f32); 512 tokens behind 32256 370 us (bf16, 0.74).
 #include <climits>
 #include <type_traits>
 

@@ -11,7 +11,9 @@
 //      collected and ranked; a bin of more than 1024 (flat rows, equal logits) is split until they are fewer.  A large k, or equals around the
 //      k-th, is a search by count.
 // A cluster of blocks has one row: every block a share of the tokens, block 0 the sums.
-// Bound: latency of the steps for few rows; for many the weights of step 2 (64-bit exponentials and shared-memory atomics, one per token).
+// Bound: latency of the steps for few rows; for many the weights of step 2 (64-bit exponentials and shared-memory atomics, one per token).  Greedy,
+// top-k 50, no filter, top-p 0.9 at temperature 0.8: a row of 32000 f32 logits 10, 12, 15 and 19 us; 16 of 151936 22, 23, 36 and 44; 64 of 152064
+// (39 MB, 6 us at the copy bandwidth) 32, 33, 54 and 66.
 #include <cooperative_groups.h>
 
 #include <atomic>
