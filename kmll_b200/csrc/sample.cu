@@ -11,9 +11,10 @@
 //      collected and ranked; a bin of more than 1024 (flat rows, equal logits) is split until they are fewer.  A large k, or equals around the
 //      k-th, is a search by count.
 // A cluster of blocks has one row: every block a share of the tokens, block 0 the sums.
-// Bound: latency of the steps for few rows; for many the weights of step 2 (64-bit exponentials and shared-memory atomics, one per token).  Greedy,
-// top-k 50, no filter, top-p 0.9 at temperature 0.8: a row of 32000 f32 logits 10, 12, 15 and 19 us; 16 of 151936 22, 23, 36 and 44; 64 of 152064
-// (39 MB, 6 us at the copy bandwidth) 32, 33, 54 and 66.
+// Bound: latency of the steps for few rows; for many the weights of step 2 (64-bit exponentials and shared-memory atomics, one per token: half of the time
+// of a row that has them) and instructions per token in the other passes, whose logits come out of L2.  Greedy, top-k 50, no filter, top-p 0.9 at
+// temperature 0.8: a row of 32000 f32 logits 9, 12, 14 and 17 us; 16 of 151936 17, 19, 28 and 34; 64 of 152064 (39 MB, 6 us at the copy bandwidth)
+// 24, 27, 43 and 51; flat rows with top-p, whose bins are split, 84.
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -77,41 +78,45 @@ __device__ inline float key_logit(unsigned long long key) {
 }
 __device__ inline uint32_t key_index(unsigned long long key) { return 0xffffffffu - (uint32_t)key; }
 
+constexpr float kPlace0 = 8388608.0f;  // 2^23: adding it rounds to a whole number, and leaves it in the low bits
 struct Weigher {
     float top, per_bin;  // largest logit; bins per unit of logit
-    double inv;          // 1 / temperature
+    double inv, steps;   // 1 / temperature; steps of 2^(1 / 256) per unit of logit
     const double* powers;
     __device__ double exponent(float l) const { return l == top ? 0.0 : ((double)l - (double)top) * inv; }
-    // e^x = 2^(j / 256) * 2^n * e^r with 256 n + j the nearest whole number to 256 x / ln 2: Taylor's series in |r| <= ln 2 / 512, whose first term left
-    // out is below 2^-54.  Adding 1.5 * 2^52 (2^52) rounds to a whole number and leaves it in the low bits: conversions run at an eighth of the rate.
-    __device__ unsigned long long weight(double x) const {
-        constexpr double kLn2 = 0.693147180559945309, kWhole = 6755399441055744.0;
-        const double y = fmax(x, -100.0) * (256.0 / kLn2), m = y + kWhole, r = (y - (m - kWhole)) * (kLn2 / 256.0);
+    // Of a token that has a bin: 2^(y / 256) = 2^(j / 256) * 2^n * e^(c r) with 256 n + j the nearest whole number to y, c = ln 2 / 256: Taylor's series in
+    // |c r| <= c / 2, whose first term left out is below 2^-54.  Adding 1.5 * 2^52 (2^52) rounds to a whole number and leaves it in the low bits:
+    // conversions run at an eighth of the rate.
+    __device__ unsigned long long weight(float l) const {
+        constexpr double kC = 0.693147180559945309 / 256.0, kWhole = 6755399441055744.0;
+        const double y = l == top ? 0.0 : ((double)l - (double)top) * steps, m = y + kWhole, r = y - (m - kWhole);
         const int i = __double2loint(m);
-        double p = 1.0 / 24.0;
-        p = fma(p, r, 1.0 / 6.0);
-        p = fma(p, r, 0.5);
-        p = fma(p, r, 1.0);
+        double p = kC * kC * kC * kC / 24.0;
+        p = fma(p, r, kC * kC * kC / 6.0);
+        p = fma(p, r, kC * kC / 2.0);
+        p = fma(p, r, kC);
         p = fma(p, r, 1.0);
         const double e = p * powers[i & 255];
         const double w = __hiloint2double(__double2hiint(e) + (kUnit + (i >> 8)) * (1 << 20), __double2loint(e));
         return (unsigned long long)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
     }
-    // monotone in the logit; kBins: weighs nothing
-    __device__ int bin(float l) const { return l == top ? 0 : (int)fminf((top - l) * per_bin, (float)kBins); }
+    // kPlace0 + its bin, monotone in the logit; beyond the last bin (and for -infinity), or NaN (of NaN): weighs nothing
+    __device__ float place(float l) const { return (l == top ? 0.0f : (top - l) * per_bin) + kPlace0; }
 };
+__device__ inline bool has_bin(float place) { return place <= kPlace0 + (float)(kBins - 1); }
+__device__ inline int bin_at(float place) { return (int)(__float_as_uint(place) - 0x4b000000u); }
 __device__ inline void add_weight(uint32_t* low, uint32_t* high, unsigned long long w) {
     const uint32_t lo = (uint32_t)w, old = atomicAdd(low, lo), more = (uint32_t)(w >> 32) + (old + lo < old ? 1u : 0u);
     if (more != 0u) atomicAdd(high, more);
 }
 
-// Calls f(index, logit) for the block's share of a row, in 16-byte pieces.
+// Calls f(index of the first, logits) for the 16-byte pieces of the block's share of a row; what is not the row's is -infinity.
 template <typename T, typename F>
 __device__ inline void each_logit(const T* row, int vocab, int rank, int blocks, F f) {
     constexpr int N = 16 / (int)sizeof(T);
     const int shift = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T)), pieces = (vocab + shift + N - 1) / N, share = (pieces + blocks - 1) / blocks;
     const int end = min(pieces, (rank + 1) * share);
-#pragma unroll 2
+#pragma unroll 1
     for (int c = rank * share + (int)threadIdx.x; c < end; c += kSampleThreads) {
         const int i0 = c * N - shift;
         float x[N];
@@ -127,8 +132,7 @@ __device__ inline void each_logit(const T* row, int vocab, int rank, int blocks,
                 x[e] = i < 0 || i >= vocab ? -INFINITY : sizeof(T) == 4 ? reinterpret_cast<const float*>(row)[i] : __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(row)[i] << 16);
             }
         }
-#pragma unroll
-        for (int e = 0; e < N; ++e) f(i0 + e, x[e]);
+        f(i0, x);
     }
 }
 
@@ -176,7 +180,7 @@ __device__ inline void rank_list(SampleShared& s, const Weigher& weigh, uint32_t
         s.sorted[place] = key;
     }
     __syncthreads();
-    unsigned long long w = tid < listed ? weigh.weight(weigh.exponent(key_logit(s.sorted[tid]))) : 0ull;
+    unsigned long long w = tid < listed ? weigh.weight(key_logit(s.sorted[tid])) : 0ull;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const unsigned long long v = __shfl_up_sync(0xffffffffu, w, o);
@@ -221,7 +225,12 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_rows_kernel(const Sa
     }
     pdl_wait();
     const T* const logits = static_cast<const T*>(a.logits) + (size_t)row * a.ld;
-    auto each = [&](auto f) { each_logit(logits, a.vocab, rank, blocks, f); };
+    auto each = [&](auto f) {
+        each_logit(logits, a.vocab, rank, blocks, [&](int i0, const auto& x) {
+#pragma unroll
+            for (int e = 0; e < (int)(sizeof(x) / 4); ++e) f(i0 + e, x[e]);
+        });
+    };
     const float temperature = a.temperature != nullptr ? a.temperature[row] : 1.0f, least_p = a.min_p != nullptr ? a.min_p[row] : 0.0f;
     const float top_p = a.top_p != nullptr ? a.top_p[row] : 1.0f;
     const int k = a.top_k != nullptr ? a.top_k[row] : 0;
@@ -243,10 +252,18 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_rows_kernel(const Sa
         return;
     }
     const bool greedy = !(temperature > FLT_EPSILON);
-    const Weigher weigh = {top, greedy ? INFINITY : kBinsPerFactor2 * 1.442695041f / temperature, greedy ? (double)INFINITY : 1.0 / (double)temperature, s.powers};
+    const Weigher weigh = {top, greedy ? INFINITY : kBinsPerFactor2 * 1.442695041f / temperature, greedy ? (double)INFINITY : 1.0 / (double)temperature,
+                           greedy ? (double)INFINITY : 256.0 / 0.693147180559945309 / (double)temperature, s.powers};
     const double least = least_p > 0.0f ? log((double)fminf(least_p, 1.0f)) : -INFINITY;
     const bool k_on = k > 0 && k < a.vocab, by_k = greedy || (k_on && k <= kList), large_k = !greedy && k_on && k > kList;
     const int want_k = greedy ? 1 : k;
+    // the smallest logit that min-p leaves: next to where the logarithm says, by the comparison that defines it
+    float least_logit = -INFINITY;
+    if (least > -INFINITY && !greedy) {
+        least_logit = (float)((double)top + least * (double)temperature);
+        for (int i = 0; i < 4 && weigh.exponent(least_logit) >= least; ++i) least_logit = nextafterf(least_logit, -INFINITY);
+        for (int i = 0; i < 8 && !(weigh.exponent(least_logit) >= least); ++i) least_logit = nextafterf(least_logit, INFINITY);
+    }
 
     // this block's bins into those of the row, and back to zero
     auto merge = [&](uint32_t* counts, unsigned long long* weights, int n) {
@@ -260,13 +277,20 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_rows_kernel(const Sa
         }
         cluster.sync();
     };
-    // tokens that `take` names into the list of block 0 (which is empty)
+    // tokens that `take` names into the list of block 0 (which is empty); few pieces have any
     auto collect = [&](auto take) {
-        each([&](int i, float l) {
-            if (!(l > -INFINITY) || !take(i, l)) return;
-            const uint32_t at = atomicAdd(&s0.listed, 1u);
-            if (at < (uint32_t)kList) s0.list[at] = token_key(l, (uint32_t)i);
-            else s0.overflow = 1;
+        each_logit(logits, a.vocab, rank, blocks, [&](int i0, const auto& x) {
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < (int)(sizeof(x) / 4); ++e) any |= take(i0 + e, x[e]);
+            if (!any) return;
+#pragma unroll
+            for (int e = 0; e < (int)(sizeof(x) / 4); ++e) {
+                if (!take(i0 + e, x[e])) continue;
+                const uint32_t at = atomicAdd(&s0.listed, 1u);
+                if (at < (uint32_t)kList) s0.list[at] = token_key(x[e], (uint32_t)(i0 + e));
+                else s0.overflow = 1;
+            }
         });
         cluster.sync();
     };
@@ -274,14 +298,13 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_rows_kernel(const Sa
     auto weigh_all = [&](bool counts) {
         unsigned long long least_sum = 0ull;
         each([&](int, float l) {
-            if (!(l > -INFINITY)) return;
-            const int b = weigh.bin(l);
-            if (b >= kBins) return;
-            const double x = weigh.exponent(l);
-            const unsigned long long w = weigh.weight(x);
+            const float place = weigh.place(l);
+            if (!has_bin(place)) return;
+            const int b = bin_at(place);
+            const unsigned long long w = weigh.weight(l);
             if (counts) atomicAdd(&s.count[b], 1u);
             add_weight(&s.low[b], &s.high[b], w);
-            if (x >= least) least_sum += w;
+            if (l >= least_logit) least_sum += w;
         });
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) least_sum += __shfl_xor_sync(0xffffffffu, least_sum, o);
@@ -305,9 +328,8 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_rows_kernel(const Sa
 
     if (by_k) {
         each([&](int, float l) {
-            if (!(l > -INFINITY)) return;
-            const int b = weigh.bin(l);
-            if (b < kBins) atomicAdd(&s.count[b], 1u);
+            const float place = weigh.place(l);
+            if (has_bin(place)) atomicAdd(&s.count[bin_at(place)], 1u);
         });
         merge(s0.all_count, s0.all_weight, kBins);
         if (rank == 0) {
@@ -317,8 +339,8 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_rows_kernel(const Sa
                 if (s.count_before[b] < target && s.count_before[b] + s.all_count[b] >= target) s.bin = b;
         }
         cluster.sync();
-        const int last = s0.bin;
-        collect([&](int, float l) { return weigh.bin(l) <= last; });
+        const float last = kPlace0 + (float)s0.bin;
+        collect([&](int, float l) { return weigh.place(l) <= last; });
         if (s0.overflow == 0) {
             if (rank == 0) {
                 const uint32_t listed = s.listed, n = min(listed, (uint32_t)want_k);
@@ -354,12 +376,12 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_rows_kernel(const Sa
         }
         if (tid == 0) { s.key_range[0] = ~0ull; s.key_range[1] = 0ull; }
         cluster.sync();
-        const int bin = s0.bin;
-        collect([&](int, float l) { return weigh.bin(l) == bin; });
+        const float bin = kPlace0 + (float)s0.bin;
+        collect([&](int, float l) { return weigh.place(l) == bin; });
         if (s0.overflow != 0) {
             unsigned long long low_key = ~0ull, high_key = 0ull;
             each([&](int i, float l) {
-                if (!(l > -INFINITY) || weigh.bin(l) != bin) return;
+                if (weigh.place(l) != bin) return;
                 const unsigned long long key = token_key(l, (uint32_t)i);
                 low_key = min(low_key, key);
                 high_key = max(high_key, key);
@@ -390,7 +412,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_rows_kernel(const Sa
                     if (key < low_key || key > high_key) return;
                     const int b = (int)((high_key - key) >> shift);
                     atomicAdd(&s.count[b], 1u);
-                    add_weight(&s.low[b], &s.high[b], weigh.weight(weigh.exponent(l)));
+                    add_weight(&s.low[b], &s.high[b], weigh.weight(l));
                 });
                 merge(s0.sub_count, s0.sub_weight, kSubBins);
                 if (rank == 0) {
@@ -418,7 +440,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_rows_kernel(const Sa
             cluster.sync();
             collect([&](int i, float l) {
                 const unsigned long long key = token_key(l, (uint32_t)i);
-                return key >= low_key && key <= high_key;
+                return l > -INFINITY && key >= low_key && key <= high_key;
             });
         }
         if (rank == 0) {
