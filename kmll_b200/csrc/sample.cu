@@ -7,8 +7,8 @@
 //   1  the largest logit
 //   2  a histogram over 4096 bins of equal ratio, the highest logits first: with top-k of the tokens (no weights are needed), otherwise of the weights
 //   3  with top-k: the tokens of all bins up to the one in which the k-th lies are collected; one block ranks them by counting, sums their
-//      weights, cuts and chooses at once.  Otherwise each border (top-p, then the choice) is a search: its bin's tokens are
-//      collected and ranked; a bin of more than 1024 (flat rows, equal logits) is split until they are fewer.  A large k, or equals around the
+//      weights, cuts and chooses at once.  Otherwise each border (top-p, then the choice; both at once where their bins hold few tokens) is a search: its
+//      bin's tokens are collected and ranked; a bin of more than 1024 (flat rows, equal logits) is split until they are fewer.  A large k, or equals around the
 //      k-th, is a search by count.
 // A cluster of blocks has one row: every block a share of the tokens, block 0 the sums.
 // Bound: latency of the steps for few rows; for many the weights of step 2 (64-bit exponentials and shared-memory atomics, one per token: half of the time
@@ -29,6 +29,7 @@ namespace cg = cooperative_groups;
 constexpr int kSampleThreads = 1024;
 constexpr int kBins = 4096, kSubBins = 1024;
 constexpr int kList = 1024;          // tokens that are ranked at once
+constexpr int kBoth = 700;           // tokens up to which two borders are ranked together: ranking costs their square, a search one pass over the row
 constexpr int kUnit = 44;            // weights are multiples of 2^-kUnit
 constexpr float kBinsPerFactor2 = (float)kBins / (kUnit + 1.5f);  // tokens behind the last bin weigh less than half a unit
 
@@ -62,7 +63,7 @@ struct SampleShared {
     unsigned long long least_sum;                    // weight at or above the min-p border
     unsigned long long key_range[2];                 // of a bin's tokens in this block
     float scratch[33], tops[8];                      // largest logit of every block of the cluster
-    int bin, overflow;
+    int bin, overflow, choice[2], many, both;        // many: more tokens than can be listed, by their weight; both: few enough for two borders
     uint32_t listed;
     unsigned long long base, low_key, high_key, found_key, found_sum;
 };
@@ -359,6 +360,8 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_rows_kernel(const Sa
         cluster.sync();
     }
     if (!greedy) weigh_all(large_k);
+    // Tokens that weigh so much around bin b, within a hundredth: those of a bin differ by no more.
+    auto tokens_of = [&](unsigned long long weight, int b) { return (float)weight * exp2f((float)b / kBinsPerFactor2 - (float)kUnit); };
     // The first token, in order, at which the tokens (by_count) or the weight so far reach `target` (block 0's): block 0 gets its key (found_key), and the
     // weight up to and with it (found_sum).  The bins' sums are there.
     auto search = [&](bool by_count, unsigned long long target) {
@@ -370,6 +373,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_rows_kernel(const Sa
                     s.bin = b;
                     s.base = before;
                     s.found_sum = s.before[b];
+                    s.many = by_count ? s.all_count[b] > (uint32_t)kList : tokens_of(s.all_weight[b], b) > (float)kList;
                 }
             }
             if (tid == 0) { s.listed = 0u; s.overflow = 0; }
@@ -377,8 +381,9 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_rows_kernel(const Sa
         if (tid == 0) { s.key_range[0] = ~0ull; s.key_range[1] = 0ull; }
         cluster.sync();
         const float bin = kPlace0 + (float)s0.bin;
-        collect([&](int, float l) { return weigh.place(l) == bin; });
-        if (s0.overflow != 0) {
+        const bool many = s0.many != 0;
+        if (!many) collect([&](int, float l) { return weigh.place(l) == bin; });
+        if (many || s0.overflow != 0) {
             unsigned long long low_key = ~0ull, high_key = 0ull;
             each([&](int i, float l) {
                 if (weigh.place(l) != bin) return;
@@ -464,6 +469,54 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_rows_kernel(const Sa
     }
     unsigned long long kept = 0ull;  // (block 0's)
     if (rank == 0) kept = s.before[kBins - 1] + s.all_weight[kBins - 1];
+    if (top_p < 1.0f && !k_on) {
+        // Both borders at once: what top-p keeps ends within its bin, so the choice lies in one of few bins in front of it (one, as a rule).
+        unsigned long long target = 0ull;
+        if (rank == 0) {
+            auto find = [&](unsigned long long t, int& to) {
+                for (int b = tid; b < kBins; b += kSampleThreads)
+                    if (s.before[b] < t && s.before[b] + s.all_weight[b] >= t) to = b;
+            };
+            target = target_of_p(kept);
+            find(target, s.bin);
+            if (tid == 0) { s.listed = 0u; s.overflow = 0; }
+            __syncthreads();
+            const unsigned long long before = s.before[s.bin];
+            find(target_of_u(min(before + 1ull, s.least_sum)), s.choice[0]);
+            find(target_of_u(min(before + s.all_weight[s.bin], s.least_sum)), s.choice[1]);
+            __syncthreads();
+            if (tid == 0) {
+                const int c0 = s.choice[0], c1 = s.choice[1];
+                const unsigned long long in_front = c1 < s.bin ? s.before[c1] + s.all_weight[c1] : before;  // up to the choice's last bin
+                s.both = tokens_of(s.all_weight[s.bin], s.bin) + tokens_of(in_front - s.before[c0], c1) <= (float)kBoth;
+            }
+        }
+        cluster.sync();
+        if (s0.both != 0) {
+            const float border = kPlace0 + (float)s0.bin, from = kPlace0 + (float)s0.choice[0], to = kPlace0 + (float)s0.choice[1];
+            collect([&](int, float l) {
+                const float place = weigh.place(l);
+                return place == border || (place >= from && place <= to);
+            });
+            if (s0.overflow == 0) {
+                if (rank == 0) {
+                    const uint32_t listed = s.listed;
+                    const unsigned long long before = s.before[s.bin], before_choice = s.before[s.choice[0]];
+                    rank_list(s, weigh, listed, 0ull);
+                    const uint32_t first = (uint32_t)__syncthreads_count((uint32_t)tid < listed && weigh.place(key_logit(s.sorted[tid])) < border);
+                    const unsigned long long own = s.sums[tid], of_first = first > 0u ? s.sums[first - 1u] : 0ull;
+                    __syncthreads();
+                    s.sums[tid] = (uint32_t)tid < first ? before_choice + own : before + (own - of_first);
+                    __syncthreads();
+                    kept = min(s.sums[reach(s, listed, target)], s.least_sum);
+                    answer(s.sorted[reach(s, listed, target_of_u(kept))], kept);
+                }
+                cluster.sync();
+                return;
+            }
+            cluster.sync();
+        }
+    }
     if (k_on) {
         search(true, min((unsigned long long)k, (unsigned long long)s.count_before[kBins - 1] + s.all_count[kBins - 1]));
         kept = s.found_sum;

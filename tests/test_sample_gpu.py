@@ -175,3 +175,17 @@ def test_session_samples_on_the_device(cuda):
         with pytest.raises(ValueError):
             s.generate_sampled_until(1, None, hot, **bad)
     dec.close()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab, spread", [(300, 0.01), (20000, 0.05), (20000, 0.4), (100000, 1.0), (100000, 3.0), (100000, 12.0)])
+def test_both_borders_near_and_far(cuda, dtype, vocab, spread):
+    """Top-p's border and the choice in one bin, in neighbouring ones and far apart, with few and with many tokens in them; min-p on either side of
+    top-p's border.  The six rows of the last u and the four of the last p below 1 have their borders where 1e-7 and 1e-6 of the weight lie behind, on
+    up to 1e5 tokens: these weigh down to 1e-12 of the whole, less than the distance (1e-8) within which borders are not compared."""
+    rng = np.random.default_rng(vocab + int(100 * spread))
+    rows = 24
+    logits = torch.tensor(rng.normal(0, spread, (rows, vocab)), device="cuda").to(dtype)
+    p, u = np.tile([0.02, 0.5, 0.9, 0.999, 0.999999, 0.0], 4), np.repeat([0.0, 0.3, 0.97, 0.9999999], 6)
+    check(logits, u, top_p=p, borders=10)
+    check(logits, u, top_p=p, min_p=np.tile([0.9, 0.3, 0.02, 1e-4], 6), borders=10)
