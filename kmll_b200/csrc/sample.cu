@@ -13,8 +13,8 @@
 // A cluster of blocks has one row: every block a share of the tokens, block 0 the sums.
 // Bound: latency of the steps for few rows; for many the weights of step 2 (64-bit exponentials and shared-memory atomics, one per token: half of the time
 // of a row that has them) and instructions per token in the other passes, whose logits come out of L2.  Greedy, top-k 50, no filter, top-p 0.9 at
-// temperature 0.8: a row of 32000 f32 logits 9, 12, 14 and 17 us; 16 of 151936 17, 19, 28 and 34; 64 of 152064 (39 MB, 6 us at the copy bandwidth)
-// 24, 27, 43 and 51; flat rows with top-p, whose bins are split, 84.
+// temperature 0.8: a row of 32000 f32 logits 10, 12, 15 and 16 us; 16 of 151936 18, 19, 28 and 31; 64 of 152064 (39 MB, 6 us at the copy bandwidth)
+// 25, 28, 43 and 47; flat rows with top-p, whose bins hold more than are ranked together, 86 (both borders one after another always: 51 and 84).
 #include <cooperative_groups.h>
 
 #include <atomic>
