@@ -72,6 +72,14 @@ def test_attention_refusals(handle, over, code, word):
     assert handle.kmll_paged_attention(*attention_args(**over)) == code and word in handle.kmll_last_error()
 
 
+def test_attention_calls_that_do_not_fit_are_refused_before_any_launch(handle):
+    capacity = handle.kmll_paged_attention(*attention_args(requests=40000, heads=4, kv_heads=2))
+    assert capacity < -2 and b"40000 requests" in handle.kmll_last_error()
+    assert handle.kmll_paged_attention(*attention_args(tokens=1 << 24, max_query=1 << 24, heads=4, kv_heads=2)) == capacity and b"tokens" in handle.kmll_last_error()
+    # positions: a tile's end behind the last one still fits into 32 bits
+    assert handle.kmll_paged_attention(*attention_args(table_width=(1 << 31) // 16 - 1)) == -2 and b"32 bits" in handle.kmll_last_error()
+
+
 @pytest.mark.parametrize("at, value, code", [(1, None, -1), (3, 31, -2), (4, -1, -2), (5, 0, -2), (5, (1 << 19) + 1, -2), (6, None, -1), (11, None, -1)])
 def test_sample_refusals(handle, at, value, code):
     args = [None, 16, 1, (1 << 20) if at != 3 else 32, 2, 32, 16, None, None, None, None, 16, None]
