@@ -3,10 +3,13 @@
 //   S^T[key][row] = K[key] . q[row]: A = 16 keys x 32 codes by ldmatrix, B = q as a 24-bit integer (bf16 rows: 16 bits) below the largest
 //   entry of its row, in bytes; mma.m16n8k32 s8 x u8 / s8 -> s32, one MMA per byte, exact; S = k_scale * q_scale * (D0 + 2^8 D1 + 2^16 D2)
 //   O^T[dim][row] += V^T[dim][key] P^T[key][row]: A = 16 columns x 32 keys (values lie with the keys of a column together), B =
-//   softmax weights times the page's value scale, as 24-bit (bf16: 16-bit) fractions of the largest scale in the tile, in bytes
-// Nothing is converted on the way from memory to the tensor cores, and both contractions are exact; what is rounded are q and the weights,
-// to 2^-24 of the largest of their row.  (f32 rows cost three MMAs where bf16 heads and remainders would cost two of twice the size,
-// behind a conversion of every code.)
+//   softmax weights times the page's value scale, as 24-bit (bf16 rows: 16-bit) fractions of the largest of them in the tile of 32 keys, in bytes
+// Nothing is converted on the way from memory to the tensor cores, and both contractions are exact.  What is rounded are q, to 2^-24 (bf16 rows, whose
+// entries have eight bits: 2^-16) of its row's largest entry, and the weights, to 2^-25 (2^-17) of the tile's largest: of the tile's, not of the row's, because
+// the sum of the weights has all of them, and what lies far below one key that dominates a row is most of the result where that key's value is small.
+// For the same reason a tile with weights below 2^-14 (2^-10) of its largest goes twice, the second time with 16 bits of what rounding left.  (64 requests of 8192, 32
+// query heads over 8 of size 128, f32: 186 us either way where scores spread by 1; 208 where they spread by 3 and many tiles go twice, 186 without.)
+// (f32 rows cost three MMAs where bf16 heads and remainders would cost two of twice the size, behind a conversion of every code.)
 //
 // A warp is a pipeline of its own over tiles of 32 keys (two stages of keys and values, cp.async in 16-byte groups), with its own running
 // maximum and sum; four warps take the tiles of a stretch in turn and meet at its end.  The work of a call is one axis, requests x kv heads x
@@ -34,7 +37,6 @@ constexpr int kPdStages = 2;
 // blocks whose share is many short requests would end last (64 requests of 100 to 8000 tokens, 32 / 8 heads of 128: 0 tiles 96 us,
 // 4 80, 8 72, 20 72; one of 2048: 14.6, 11.0, 11.3, 11.8).
 constexpr int kPdStretch = 8;
-
 struct PdMeta {  // of a stage: the two groups of 16 keys may lie in two pages
     float k_scale[2], v_scale[2];
     int there[2], unused[2];
@@ -221,6 +223,9 @@ template <int HD, typename T, int NB, int NC>
 __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kernel(const PagedArgs a, const PdWork work, const PagedOrder order) {
     using S = PdShape<HD>;
     constexpr int KS = HD / 32, DT = HD / 16, ROWS = 8 * NC, PITCH = HD + 4;
+    // A tile's largest weight times its largest value scale becomes kWhole (rounding errors of the factors stay below 2^24, 2^16).  A tile that has a weight below
+    // kNarrow, of which less than ten (six) bits would be left, takes the rest of all of them as well; below kNothing there is no rest.
+    constexpr float kWhole = NB == 3 ? 16776960.0f : 65520.0f, kNarrow = NB == 3 ? 1024.0f : 64.0f, kNothing = 0x1p-16f;
     extern __shared__ __align__(128) unsigned char pd_smem[];
     __shared__ long long s_before[kPdWarps + 1];
     __shared__ long long s_start;
@@ -484,23 +489,27 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
                             if (key > last[nc][e & 1] || key < first_key[nc][e & 1] || !mt.there[half16]) s[nc][half16][e] = -INFINITY;
                         }
             }
-            // ---- running maximum and sum of this lane's two columns; weights as whole numbers
+            // ---- running maximum and sum of this lane's two columns; weights times value scale, the tile's largest weight times its largest scale as kWhole
             const float vmax = fmaxf(mt.v_scale[0], mt.v_scale[1]);
-            constexpr float kWhole = NB == 3 ? 16777215.0f : 65535.0f;
-            const float v_rel[2] = {vmax > 0.0f ? mt.v_scale[0] / vmax * kWhole : 0.0f, vmax > 0.0f ? mt.v_scale[1] / vmax * kWhole : 0.0f};
-            uint32_t pb[NC][NB][2];
+            const float v_rel[2] = {vmax > 0.0f ? mt.v_scale[0] / vmax : 0.0f, vmax > 0.0f ? mt.v_scale[1] / vmax : 0.0f};
+            float v_unit[NC][2];
+            bool wide = false;
 #pragma unroll
             for (int nc = 0; nc < NC; ++nc) {
                 float turn[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float top = fmaxf(fmaxf(s[nc][0][e], s[nc][0][e + 2]), fmaxf(s[nc][1][e], s[nc][1][e + 2]));
+                    float own = fmaxf(fmaxf(s[nc][0][e], s[nc][0][e + 2]), fmaxf(s[nc][1][e], s[nc][1][e + 2]));
 #pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    top = fmaxf(top, m[nc][e]);
+                    for (int o = 4; o < 32; o <<= 1) own = fmaxf(own, __shfl_xor_sync(0xffffffffu, own, o));
+                    const float top = fmaxf(own, m[nc][e]);
                     const float base = top == -INFINITY ? 0.0f : top;
                     turn[e] = ex2_approx(m[nc][e] - base);
                     m[nc][e] = top;
+                    const float largest = ex2_approx(own - base);
+                    const bool any = largest > 0x1p-80f;  // (what is less counts in the sum alone)
+                    const float up = any ? __fdividef(kWhole, largest) : 0.0f;
+                    v_unit[nc][e] = any ? largest * (vmax / kWhole) : 0.0f;
                     float sum = 0.0f;
 #pragma unroll
                     for (int half16 = 0; half16 < 2; ++half16)
@@ -509,6 +518,8 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
                             float& x = s[nc][half16][e + 2 * k];
                             x = ex2_approx(x - base);
                             sum += x;
+                            x *= up * v_rel[half16];
+                            wide = wide || __float_as_uint(x) - __float_as_uint(kNothing) < __float_as_uint(kNarrow) - __float_as_uint(kNothing);
                         }
                     l[nc][e] = fmaf(l[nc][e], turn[e], sum);
                 }
@@ -518,43 +529,54 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
 #pragma unroll
                         for (int e = 0; e < 4; ++e) acc[nc][d][e] *= turn[e & 1];
                 }
+            }
+            // O += V^T times whole numbers, in bytes (of the rest the second one has the sign)
+            auto take = [&](auto rest, auto whole_of, float unit) {
+                constexpr bool kRest = decltype(rest)::value;
+                constexpr int B = kRest ? 2 : NB;
+                uint32_t pb[NC][B][2];
 #pragma unroll
-                for (int half16 = 0; half16 < 2; ++half16) {
-                    uint32_t x[4];
+                for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = __float2uint_rn(s[nc][half16][e] * v_rel[half16]);
-                    const uint32_t r0 = movmatrix_trans(__byte_perm(x[0], x[1], 0x5410)), r1 = movmatrix_trans(__byte_perm(x[2], x[3], 0x5410));
-                    pb[nc][0][half16] = __byte_perm(r0, r1, 0x6420);
-                    pb[nc][1][half16] = __byte_perm(r0, r1, 0x7531);
-                    if (NB == 3) {
-                        const uint32_t r2 = movmatrix_trans(__byte_perm(x[0], x[1], 0x7632)), r3 = movmatrix_trans(__byte_perm(x[2], x[3], 0x7632));
-                        pb[nc][NB - 1][half16] = __byte_perm(r2, r3, 0x6420);
+                    for (int half16 = 0; half16 < 2; ++half16) {
+                        uint32_t x[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = whole_of(s[nc][half16][e]);
+                        const uint32_t r0 = movmatrix_trans(__byte_perm(x[0], x[1], 0x5410)), r1 = movmatrix_trans(__byte_perm(x[2], x[3], 0x5410));
+                        pb[nc][0][half16] = __byte_perm(r0, r1, 0x6420);
+                        pb[nc][1][half16] = __byte_perm(r0, r1, 0x7531);
+                        if constexpr (B == 3) {
+                            const uint32_t r2 = movmatrix_trans(__byte_perm(x[0], x[1], 0x7632)), r3 = movmatrix_trans(__byte_perm(x[2], x[3], 0x7632));
+                            pb[nc][2][half16] = __byte_perm(r2, r3, 0x6420);
+                        }
+                    }
+                cp_async_wait_group<2 * kPdStages - 1>();
+                __syncwarp();
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    uint32_t f[4];
+                    ldmatrix_x4(f, vals + ((lane >> 4) * HD + dt * 16 + (lane & 15)) * 16);
+#pragma unroll
+                    for (int nc = 0; nc < NC; ++nc) {
+                        int d[B][4];
+#pragma unroll
+                        for (int b = 0; b < B; ++b) {
+                            d[b][0] = d[b][1] = d[b][2] = d[b][3] = 0;
+                            if (kRest && b == B - 1) mma_s8s8(d[b], f, pb[nc][b][0], pb[nc][b][1]);
+                            else mma_s8u8(d[b], f, pb[nc][b][0], pb[nc][b][1]);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float v = (float)(d[0][e] + (d[1][e] << 8));
+                            if (B == 3) v = fmaf((float)d[B - 1][e], 65536.0f, v);
+                            acc[nc][dt][e] = fmaf(v, v_unit[nc][e & 1] * unit, acc[nc][dt][e]);
+                        }
                     }
                 }
-            }
-            cp_async_wait_group<2 * kPdStages - 1>();
-            __syncwarp();
-            const float v_unit = vmax / kWhole;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                uint32_t f[4];
-                ldmatrix_x4(f, vals + ((lane >> 4) * HD + dt * 16 + (lane & 15)) * 16);
-#pragma unroll
-                for (int nc = 0; nc < NC; ++nc) {
-                    int d[NB][4];
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        d[b][0] = d[b][1] = d[b][2] = d[b][3] = 0;
-                        mma_s8u8(d[b], f, pb[nc][b][0], pb[nc][b][1]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float v = (float)(d[0][e] + (d[1][e] << 8));
-                        if (NB == 3) v = fmaf((float)d[NB - 1][e], 65536.0f, v);
-                        acc[nc][dt][e] = fmaf(v, v_unit, acc[nc][dt][e]);
-                    }
-                }
-            }
+            };
+            if (__any_sync(0xffffffffu, wide))  // what rounding leaves, in 16 bits more
+                take(std::true_type(), [](float x) { return (uint32_t)min(__float2int_rn((x - rintf(x)) * 65536.0f), 32767); }, 1.0f / 65536.0f);
+            take(std::false_type(), [](float x) { return __float2uint_rn(x); }, 1.0f);
             __syncwarp();
             copy_values(i + kPdStages, page_next);
         }

@@ -721,3 +721,70 @@ def test_value_scales_below_the_smallest_that_prompts_tell_apart(cuda):
     s["cache"].v_scales[tiny] = 1e-38
     s["values"][1][tiny] *= 0.0  # (below the tolerance by 20 orders)
     check_attention(s)
+
+
+# ---- rows with a sink: one key far above all others, whose value is nothing ---------------------------------------------------------
+def make_sink(seed, heads, kv, hd, block, context, new, dtype, nats, mean, spread=1.0):
+    """Key 0 lies `nats` above the others, which score about alike; its value codes are 0, so that the row's result is what the others hold."""
+    s = make_attention(seed, heads, kv, hd, block, [context - new], [new], dtype, spread=spread)
+    rng, cache, table = np.random.default_rng(seed + 1), s["cache"], s["table"][0]
+    pages = cache.pages
+    k, v = np.rint(rng.normal(0, 36, (pages, block, kv, hd))).clip(-127, 127), np.rint(rng.normal(mean, 20, (pages, block, kv, hd))).clip(-127, 127)
+    k[..., 0] = 0
+    k[table[0], 0], v[table[0], 0] = 0, 0
+    k[table[0], 0, :, 0] = 127
+    cache.k_codes.copy_(torch.from_numpy(po.key_layout(k)))
+    cache.v_codes.copy_(torch.from_numpy(po.value_layout(v)))
+    cache.k_scales.fill_(1 / 127)
+    s["q"][..., 0] = nats * math.sqrt(hd)
+    s["v_codes"], s["v_scales"] = v, cache.v_scales.cpu().numpy().astype(np.float64)
+    s["values"] = [k * float(np.float32(1 / 127)), v * s["v_scales"][:, None, :, None]]
+    return s
+
+
+def sink_bound(s, want, prompt):
+    """Elementwise, against what the weights hold: A = sum p_j |v_j| (p of sum 1).  Scores: q is held to 2^-23 of its row's largest entry (prompts: two planes of
+    binary16, 2^-22; one of bf16 rows 2^-22 as well, q being bf16), their sums and the exponent are f32: d, a factor of exp(2 d) of each weight.  Weights: single
+    tokens 2^-25 (bf16: 2^-17) of the largest weight times the largest value scale in a tile of 32 keys, where none is below 2^-14 (2^-10) of that, else 2^-41 (2^-33);
+    (twice that at the end of its 16 bits); prompts 2^-32 of the row's largest weight times value scale, and 2^-21
+    (bf16: 2^-12) of themselves.  ex2 and the sums of a few hundred f32 terms: 2^-18 A
+    (accumulators that cut: 2^-22 a tile of 128 keys)."""
+    q, (k, v) = f64(s["q"]), s["values"]
+    bf16, block, group = s["q"].dtype == torch.bfloat16, s["block"], q.shape[1] // k.shape[2]
+    scale, c, rows, tol = 1 / math.sqrt(q.shape[2]), s["context"][0], s["start"][1], np.zeros_like(want)
+    at = np.arange(c)
+    page = s["table"][0, at // block]
+    for i in range(rows):
+        n = c - rows + i + 1
+        for h in range(q.shape[1]):
+            kk, vv, codes, vs = k[page[:n], at[:n] % block, h // group], v[page[:n], at[:n] % block, h // group], s["v_codes"][page[:n], at[:n] % block, h // group], s["v_scales"][page[:n], h // group]
+            z = kk @ q[i, h] * scale
+            p = np.exp(z - z.max())
+            total, pa = p.sum(), p * vs
+            d = scale * 2.0 ** (-22 if prompt else -23) * np.abs(q[i, h]).max() * np.abs(kk).sum(1).max() + 8 * 2.0 ** -24 * (np.abs(z).max() + 8)
+            if prompt:
+                own = 2.0 ** -32 * pa.max() * np.abs(codes).sum(0) + 2.0 ** (-12 if bf16 else -21) * (p @ np.abs(vv))
+            else:
+                tile = np.arange(0, n, 32)
+                most = (np.maximum.reduceat(p, tile) * np.maximum.reduceat(vs, tile))[at[:n] // 32]
+                own = 1.01 * (np.minimum(2.0 ** (-17 if bf16 else -25) * most, 2.0 ** (-7 if bf16 else -11) * pa) + 2.0 ** (-32 if bf16 else -40) * most) @ np.abs(codes)
+            a = p @ np.abs(vv) / total
+            tol[i, h] = own / total + (np.expm1(2 * d) + 2.0 ** -18 + (n / 128 * 2.0 ** -22 if prompt else 0.0)) * a
+    return tol + np.abs(want) * (2.0 ** -8 if bf16 else 2.0 ** -24)
+
+
+def check_sink(s, prompt):
+    q = s["q"]
+    out = ops.paged_attention(q, ints(s["start"]), ints(s["context"]), ints(s["table"]), s["cache"], s["most"], s["context"][0], 1 / math.sqrt(q.shape[2]))
+    want = po.attention(f64(q), s["start"], s["context"], s["table"], s["block"], *s["values"], 1 / math.sqrt(q.shape[2]), 0, np.zeros(q.shape))
+    off, tol = np.abs(f64(out).reshape(want.shape) - want), sink_bound(s, want, prompt)
+    bad = ~(off <= tol)
+    assert not bad.any(), (int(bad.sum()), float((off / tol).max()), float(np.linalg.norm(off) / np.linalg.norm(want)))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nats", [6, 12, 14, 18])
+@pytest.mark.parametrize("heads, kv, hd, block, context, mean, spread", [
+    (8, 2, 128, 32, 8000, 50, 1.0), (8, 2, 128, 64, 4000, 0, 1.0), (14, 2, 64, 16, 5000, 50, 1000.0), (16, 1, 128, 16, 700, 50, 1.0), (4, 4, 64, 128, 32, 50, 1.0)])
+def test_single_tokens_over_a_sink(cuda, dtype, nats, heads, kv, hd, block, context, mean, spread):
+    check_sink(make_sink(nats, heads, kv, hd, block, context, 1, dtype, nats, mean, spread), False)
