@@ -224,6 +224,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_rows_kernel(const Sa
         s.listed = 0u;
         s.overflow = 0;
     }
+    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");  // this block runs: the others may write to its shared memory
     pdl_wait();
     const T* const logits = static_cast<const T*>(a.logits) + (size_t)row * a.ld;
     auto each = [&](auto f) {
@@ -240,6 +241,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_rows_kernel(const Sa
     float top = -INFINITY;
     each([&](int, float l) { top = fmaxf(top, l); });
     top = block_max(top, s.scratch);
+    asm volatile("barrier.cluster.wait;" ::: "memory");  // every block of the cluster has started
     if (tid < blocks) cluster.map_shared_rank(&s, tid)->tops[rank] = top;
     cluster.sync();
     for (int b = 0; b < blocks; ++b) top = fmaxf(top, s.tops[b]);

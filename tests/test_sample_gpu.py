@@ -189,3 +189,16 @@ def test_both_borders_near_and_far(cuda, dtype, vocab, spread):
     p, u = np.tile([0.02, 0.5, 0.9, 0.999, 0.999999, 0.0], 4), np.repeat([0.0, 0.3, 0.97, 0.9999999], 6)
     check(logits, u, top_p=p, borders=10)
     check(logits, u, top_p=p, min_p=np.tile([0.9, 0.3, 0.02, 1e-4], 6), borders=10)
+
+
+@pytest.mark.parametrize("rows", [1, 15, 30, 60, 140])
+def test_many_launches_one_behind_the_other(cuda, rows):
+    """Rows enough for clusters of every size; every launch's blocks meet before they write to each other's shared memory, however late some of them start."""
+    x = torch.randn(rows, 40000, generator=torch.Generator("cuda").manual_seed(rows), device="cuda")
+    best = x.argmax(1).to(torch.int32)
+    u, cold = dev([0.5] * rows, torch.float64), dev([0.0] * rows, torch.float32)
+    k = dev([30] * rows, torch.int32)
+    first = ops.sample_rows(x, u, top_k=k)
+    outs = [(ops.sample_rows(x, u, temperature=cold)[0], ops.sample_rows(x, u, top_k=k)) for _ in range(60)]
+    for greedy, (tokens, logprobs) in outs:
+        assert torch.equal(greedy, best) and torch.equal(tokens, first[0]) and torch.equal(logprobs, first[1])
