@@ -296,67 +296,69 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                 page = next;
                 entry = entry_of(j + 2);
             }
-        } else if (warp == kPpIssue) {
+        } else if (warp >= kPpIssue) {  // (a warpgroup changes its registers with one instruction)
             asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
-            constexpr uint32_t idesc_s = gemm_idesc_f16(128, kPpKeys), idesc_o = gemm_idesc_f16(128, HD);
-            const uint64_t dq = gemm_smem_desc(base), dk = gemm_smem_desc(base + S::kOffK), dv = gemm_smem_desc(base + S::kOffV);
-            const uint32_t lead = elect_lead();
-            // scores of tile j for stream s; `last`: nobody else needs the keys
-            auto scores = [&](int j, int s, bool last) {
-                const int st = j % kStages;
-                if (!warp_wait(&k_full[st], (uint32_t)(j / kStages) & 1u)) return false;
+            if (warp == kPpIssue) {
+                constexpr uint32_t idesc_s = gemm_idesc_f16(128, kPpKeys), idesc_o = gemm_idesc_f16(128, HD);
+                const uint64_t dq = gemm_smem_desc(base), dk = gemm_smem_desc(base + S::kOffK), dv = gemm_smem_desc(base + S::kOffV);
+                const uint32_t lead = elect_lead();
+                // scores of tile j for stream s; `last`: nobody else needs the keys
+                auto scores = [&](int j, int s, bool last) {
+                    const int st = j % kStages;
+                    if (!warp_wait(&k_full[st], (uint32_t)(j / kStages) & 1u)) return false;
+                    tcgen05_fence_after();
+                    const uint64_t dkj = dk + (uint64_t)(st * (S::kK >> 4)), dqs = dq + (uint64_t)(two ? s * (S::kQTile >> 4) : 0);
+                    uint32_t acc = 0u;
+#pragma unroll
+                    for (int p = NP - 1; p >= 0; --p)  // the small products first
+#pragma unroll
+                        for (int ks = 0; ks < HD / 16; ++ks) {
+                            const int at = (ks >> 2) * kPpBox + (ks & 3) * 32;
+                            lead_mma_f16(lead, (uint32_t)s * 128u, dqs + (uint64_t)((p * S::kQPlane + at) >> 4), dkj + (uint64_t)(at >> 4), idesc_s, acc);
+                            acc = 1u;
+                        }
+                    lead_commit(lead, &s_full[s]);
+                    if (last) lead_commit(lead, &k_free[st]);
+                    return true;
+                };
+                // O of stream s takes its n-th tile, tile j
+                auto values = [&](int j, int s, int n, bool last) {
+                    const int st = j % kStages;
+                    if (!(warp_wait(&v_full[st], (uint32_t)(j / kStages) & 1u) && warp_wait(&p_ready[s], (uint32_t)n & 1u))) return false;
+                    tcgen05_fence_after();
+                    const uint64_t dvj = dv + (uint64_t)(st * (S::kV >> 4));
+                    uint32_t acc = (drains ? n % kPpDrain : n) > 0 ? 1u : 0u;
+#pragma unroll
+                    for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+                        for (int ks = 0; ks < kPpKeys / 16; ++ks) {  // weights of 32 keys: 16 columns of the first plane, 16 of the second
+                            lead_mma_f16_ts(lead, kPpTmemO + (uint32_t)s * 128u, (uint32_t)(s * 128 + (ks >> 1) * 32 + p * 16 + (ks & 1) * 8),
+                                            dvj + (uint64_t)(((ks >> 2) * S::kVBox + (ks & 3) * 32) >> 4), idesc_o, acc);
+                            acc = 1u;
+                        }
+                    lead_commit(lead, &pv_done[s]);
+                    if (last) lead_commit(lead, &v_free[st]);
+                    return true;
+                };
+                ok = warp_wait(q_full, 0u);
                 tcgen05_fence_after();
-                const uint64_t dkj = dk + (uint64_t)(st * (S::kK >> 4)), dqs = dq + (uint64_t)(two ? s * (S::kQTile >> 4) : 0);
-                uint32_t acc = 0u;
-#pragma unroll
-                for (int p = NP - 1; p >= 0; --p)  // the small products first
-#pragma unroll
-                    for (int ks = 0; ks < HD / 16; ++ks) {
-                        const int at = (ks >> 2) * kPpBox + (ks & 3) * 32;
-                        lead_mma_f16(lead, (uint32_t)s * 128u, dqs + (uint64_t)((p * S::kQPlane + at) >> 4), dkj + (uint64_t)(at >> 4), idesc_s, acc);
-                        acc = 1u;
+                if (!ok) {
+                } else if (two) {
+                    // (the second stream has every tile, the first the tiles up to its own rows' positions)
+                    if (tiles > 0) ok = (tiles0 < 1 || scores(0, 0, false)) && scores(0, 1, true);
+                    for (int j = 0; j < tiles && ok; ++j) {
+                        if (j < tiles0) ok = values(j, 0, j, false);
+                        if (ok && j + 1 < tiles0) ok = scores(j + 1, 0, false);
+                        if (ok) ok = values(j, 1, j, true);
+                        if (ok && j + 1 < tiles) ok = scores(j + 1, 1, true);
                     }
-                lead_commit(lead, &s_full[s]);
-                if (last) lead_commit(lead, &k_free[st]);
-                return true;
-            };
-            // O of stream s takes its n-th tile, tile j
-            auto values = [&](int j, int s, int n, bool last) {
-                const int st = j % kStages;
-                if (!(warp_wait(&v_full[st], (uint32_t)(j / kStages) & 1u) && warp_wait(&p_ready[s], (uint32_t)n & 1u))) return false;
-                tcgen05_fence_after();
-                const uint64_t dvj = dv + (uint64_t)(st * (S::kV >> 4));
-                uint32_t acc = (drains ? n % kPpDrain : n) > 0 ? 1u : 0u;
-#pragma unroll
-                for (int p = NP - 1; p >= 0; --p)
-#pragma unroll
-                    for (int ks = 0; ks < kPpKeys / 16; ++ks) {  // weights of 32 keys: 16 columns of the first plane, 16 of the second
-                        lead_mma_f16_ts(lead, kPpTmemO + (uint32_t)s * 128u, (uint32_t)(s * 128 + (ks >> 1) * 32 + p * 16 + (ks & 1) * 8),
-                                        dvj + (uint64_t)(((ks >> 2) * S::kVBox + (ks & 3) * 32) >> 4), idesc_o, acc);
-                        acc = 1u;
+                } else {
+                    if (tiles > 0) ok = scores(0, 0, true) && (kStages < 2 || tiles < 2 || scores(1, 1, true));
+                    for (int j = 0; j < tiles && ok; ++j) {
+                        if (kStages < 2 && j + 1 < tiles) ok = scores(j + 1, (j + 1) & 1, true);
+                        if (ok) ok = values(j, j & 1, j >> 1, true);
+                        if (ok && kStages >= 2 && j + 2 < tiles) ok = scores(j + 2, j & 1, true);
                     }
-                lead_commit(lead, &pv_done[s]);
-                if (last) lead_commit(lead, &v_free[st]);
-                return true;
-            };
-            ok = warp_wait(q_full, 0u);
-            tcgen05_fence_after();
-            if (!ok) {
-            } else if (two) {
-                // (the second stream has every tile, the first the tiles up to its own rows' positions)
-                if (tiles > 0) ok = (tiles0 < 1 || scores(0, 0, false)) && scores(0, 1, true);
-                for (int j = 0; j < tiles && ok; ++j) {
-                    if (j < tiles0) ok = values(j, 0, j, false);
-                    if (ok && j + 1 < tiles0) ok = scores(j + 1, 0, false);
-                    if (ok) ok = values(j, 1, j, true);
-                    if (ok && j + 1 < tiles) ok = scores(j + 1, 1, true);
-                }
-            } else {
-                if (tiles > 0) ok = scores(0, 0, true) && (kStages < 2 || tiles < 2 || scores(1, 1, true));
-                for (int j = 0; j < tiles && ok; ++j) {
-                    if (kStages < 2 && j + 1 < tiles) ok = scores(j + 1, (j + 1) & 1, true);
-                    if (ok) ok = values(j, j & 1, j >> 1, true);
-                    if (ok && kStages >= 2 && j + 2 < tiles) ok = scores(j + 2, j & 1, true);
                 }
             }
         } else if (warp < kPpConvert) {
@@ -676,7 +678,6 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
             }
         }
     }
-    if (warp > kPpIssue) asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
     if (!ok) atomicCAS(&g_paged_prompt_status, 0, 1);
     tcgen05_fence_before();
     __syncthreads();
