@@ -93,9 +93,10 @@ struct PagedOrder {
 // paged_decode.cu: requests of at most kPagedDecodeRows rows, heads of 64 or 128
 constexpr int kPagedDecodeRows = 16;
 // A workspace begins with what has to be zero between calls, at places that no size of a call moves: a counter per (request, kv head), a counter per part of the
-// prompt kernel.  Scratch follows.
+// prompt kernel, a bit per place for its sums.  Scratch follows.
 constexpr int kPagedCounters = 65536, kPpSplitBlocks = 296;  // parts: two for each multiprocessor
-constexpr size_t kPagedZeroBytes = (size_t)kPagedCounters * 4 + (kPpSplitBlocks * 4 + 255) / 256 * 256;
+constexpr int kPpSums = 160;  // places for sums: one for each block of the prompt kernel that runs, one on a multiprocessor
+constexpr size_t kPagedZeroBytes = (size_t)kPagedCounters * 4 + ((kPpSplitBlocks + kPpSums / 32) * 4 + 255) / 256 * 256;
 bool paged_decode_serves(int head_dim);
 size_t paged_decode_scratch_bytes(int head_dim, int max_rows);
 int paged_decode_launch(cudaStream_t stream, const PagedArgs& a, bool f32, int max_rows, int max_context, int* arrived, void* scratch, const PagedOrder& order);

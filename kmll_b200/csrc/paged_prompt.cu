@@ -136,13 +136,13 @@ __device__ inline uint64_t pp_add2(uint64_t a, uint64_t b) {
 
 struct PpWork {
     const int4* list;
-    int* arrived;      // [parts' places * kv heads], zero between calls
+    int* arrived;      // [kPpSplitBlocks]: parts' places * kv heads; zero between calls
+    uint32_t* taken;   // [kPpSums / 32]: places of sums that a block holds, a bit each; zero between calls
     float* partials;   // [parts' places * kv heads]: (maximum, sum) of 256 rows, then their O
-    float* sums;       // [multiprocessor][2][HD / 4][128 rows][4]: O of earlier tiles, one block at a time on each multiprocessor
+    float* sums;       // [place][2][HD / 4][128 rows][4]: O of earlier tiles, of one block at a time
 };
 template <int HD>
 __host__ __device__ constexpr size_t pp_partial_floats() { return (size_t)kPpUnit * (HD + 2); }
-constexpr int kPpSums = 160;         // multiprocessors that have a place for sums
 constexpr int kPpDrain = 6;
 
 template <int HD, typename T>
@@ -151,6 +151,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
     using S = PpShape<HD, NP>;
     constexpr int kStages = S::kStages;
     extern __shared__ unsigned char pp_smem_raw[];
+    __shared__ int s_place;  // this block's place for sums, -1: none
     unsigned char* const smem = pp_smem_raw + ((1024u - (smem_u32(pp_smem_raw) & 1023u)) & 1023u);
     uint64_t* const s_full = reinterpret_cast<uint64_t*>(smem + S::kOffBars);  // [2] the scores of a stream's tile are there
     uint64_t* const p_ready = s_full + 2;    // [2] its weights are there (and O is rescaled)
@@ -162,7 +163,8 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
     uint64_t* const sc_full = v_free + 2;    // [4] the scales of a tile are there
     uint64_t* const pair = sc_full + 4;      // [8] both threads of a row have left their maxima
     uint64_t* const q_full = pair + 8;       // the queries are there
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(q_full + 1);
+    uint64_t* const place_full = q_full + 1; // the block's place for sums is known
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(place_full + 1);
     int* const s_last = reinterpret_cast<int*>(tmem_slot + 1);  // all other parts of the unit have arrived
     PpScales* const scales = reinterpret_cast<PpScales*>(smem + S::kOffScales);
     float* const units = reinterpret_cast<float*>(smem + S::kOffUnit);
@@ -186,8 +188,10 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
         for (int b = 0; b < 4; ++b) mbar_init(&sc_full[b], 1);
         for (int b = 0; b < 8; ++b) mbar_init(&pair[b], 2);
         mbar_init(q_full, kPpConvert);
+        mbar_init(place_full, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (tid == 0) s_place = -1;
     if (warp == kPpIssue) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -196,10 +200,8 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
     __syncthreads();  // (columns first, then the dependents: tcgen05.cuh)
     tcgen05_fence_after();
     pdl_launch_dependents();
+    constexpr bool drains = NP == 2;
     bool ok = true;
-    uint32_t sm;
-    asm volatile("mov.u32 %0, %%smid;" : "=r"(sm));
-    const bool drains = NP == 2 && sm < (uint32_t)kPpSums;
     {
         const PagedRequest rq = PagedRequest::of(a, entry.x);
         const PagedUnit un = PagedUnit::of(a, rq, group, entry.y);
@@ -211,6 +213,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
         const int all_tiles = un.tiles(rq, group), size = (all_tiles + parts - 1) / parts, from_tile = min(all_tiles, part * size);
         const int tiles = min(size, all_tiles - from_tile), first = un.first + from_tile * kPpKeys;
         const int tiles0 = two ? min(tiles, max(0, un.tiles_to(rq, group, kPpRows - 1) - from_tile)) : tiles;  // of the first stream where the streams are tiles of rows
+        const bool keeps_sums = drains && (two ? tiles : (tiles + 1) / 2) > kPpDrain;  // a stream's O leaves tensor memory before its end
         const uint32_t base = smem_u32(smem);
 
         if (warp >= kPpConvert && warp < kPpIssue) {
@@ -298,6 +301,23 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
             }
         } else if (warp >= kPpIssue) {  // (a warpgroup changes its registers with one instruction)
             asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
+            if (warp == kPpIssue + 1 && keeps_sums) {
+                // a place for sums: the first free bit of a word from the block's number on (there are more places than blocks that run at once)
+                const uint32_t number = blockIdx.y * gridDim.x + blockIdx.x;
+                uint32_t word = number / 32 % (kPpSums / 32), bit = number % 32;
+                int place = -1;
+                for (int i = 0; i < 4 * kPpSums && place < 0 && lane == 0; ++i) {
+                    const uint32_t held = atomicOr(&work.taken[word], 1u << bit), free = __funnelshift_r(~held, ~held, bit);
+                    if ((free & 1u) != 0u) place = (int)(word * 32 + bit);
+                    else if (free != 0u) bit = (bit + __ffs(free) - 1) & 31u;
+                    else word = word + 1 == kPpSums / 32 ? 0 : word + 1;
+                }
+                if (lane == 0) {
+                    __threadfence();  // (what the block before did there is done)
+                    s_place = place;
+                    mbar_arrive(place_full);
+                }
+            }
             if (warp == kPpIssue) {
                 constexpr uint32_t idesc_s = gemm_idesc_f16(128, kPpKeys), idesc_o = gemm_idesc_f16(128, HD);
                 const uint64_t dq = gemm_smem_desc(base), dk = gemm_smem_desc(base + S::kOffK), dv = gemm_smem_desc(base + S::kOffV);
@@ -411,6 +431,12 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
             asm volatile("bar.sync 1, 512;" ::: "memory");  // (units and places of rows are there)
+            int place = -1;
+            if (keeps_sums) {
+                ok = warp_wait(place_full, 0u);
+                place = s_place;
+                ok = ok && place >= 0;  // (none: the workspace was not zero)
+            }
             // ---- softmax: the stream's tiles j = j0, j0 + step, ..
             const int stream = warp >> 3, half = (warp >> 2) & 1, r = (warp & 3) * 32 + lane, in_unit = two ? stream * kPpRows + r : r;
             uint64_t* const pair_bar = pair + stream * 4 + (warp & 3);  // of the two warps that have the same rows
@@ -424,9 +450,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
             float m_ref = -INFINITY, l = 0.0f;
             // O of the tiles so far leaves tensor memory: half of the columns each, relative to the maximum at that time
             float drained_ref = -INFINITY;
-            bool drained = false;
             // (four columns of 128 rows lie together, so that a warp writes whole runs)
-            auto sums_of = [&](int s, int column) { return reinterpret_cast<float4*>(work.sums) + ((size_t)sm * 2 + s) * (HD / 4) * kPpRows + (size_t)(column / 4) * kPpRows + r; };
+            auto sums_of = [&](int s, int column) { return reinterpret_cast<float4*>(work.sums) + ((size_t)place * 2 + s) * (HD / 4) * kPpRows + (size_t)(column / 4) * kPpRows + r; };
+            int n = 0;  // tiles of this stream so far
             auto drain = [&]() {
                 const float turn = drained_ref == -INFINITY ? 0.0f : ex2_approx(drained_ref - m_ref);
                 float4* const run = sums_of(stream, half * (HD / 2));
@@ -434,7 +460,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                 for (int i = 0; i < HD / 32; ++i) {
                     float4 x[4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) x[k] = drained ? run[(i * 4 + k) * kPpRows] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (int k = 0; k < 4; ++k) x[k] = n > kPpDrain ? run[(i * 4 + k) * kPpRows] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     uint32_t o[16];
                     tmem_load_x16(to + half * (HD / 2) + i * 16, o);
 #pragma unroll
@@ -444,11 +470,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                         run[(i * 4 + k) * kPpRows] = v;
                     }
                 }
-                drained = true;
                 drained_ref = m_ref;
             };
-            int n = 0;  // tiles of this stream so far
-            for (int j = two ? 0 : stream; j < end; j += step, ++n) {
+            for (int j = two ? 0 : stream; j < end && ok; j += step, ++n) {
                 const int t0 = first + j * kPpKeys;
                 ok = warp_wait(&sc_full[j & 3], (uint32_t)(j >> 2) & 1u) && warp_wait(&s_full[stream], (uint32_t)n & 1u);
                 if (!ok) break;
@@ -571,10 +595,10 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                 if (lane == 0) mbar_arrive(&p_ready[stream]);
             }
             if (ok && n > 0) ok = warp_wait(&pv_done[stream], (uint32_t)(n - 1) & 1u);
-            if (drained) __threadfence();
+            if (drains && n > kPpDrain) __threadfence();
             // ---- the sum of both threads of a row; where the streams are shares of the keys, maximum and sum over both
             float4* const stat = reinterpret_cast<float4*>(smem + S::kOffStat);  // [stream][half][row]
-            stat[(stream * 2 + half) * kPpRows + r] = make_float4(m_ref, l, drained ? ex2_approx(drained_ref == -INFINITY ? -INFINITY : drained_ref - m_ref) : 0.0f, 0.0f);
+            stat[(stream * 2 + half) * kPpRows + r] = make_float4(m_ref, l, drains && n > kPpDrain ? ex2_approx(drained_ref == -INFINITY ? -INFINITY : drained_ref - m_ref) : 0.0f, 0.0f);
             tcgen05_fence_before();
             asm volatile("bar.sync 1, 512;" ::: "memory");
             tcgen05_fence_after();
@@ -682,6 +706,10 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
+    if (drains && tid == 0 && s_place >= 0) {  // (all have written and read their sums)
+        __threadfence();
+        atomicAnd(&work.taken[s_place / 32], ~(1u << s_place % 32));
+    }
     if (warp == kPpIssue) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(512u) : "memory");
 }
 
@@ -718,7 +746,7 @@ PagedOrder paged_prompt_order(const PagedArgs& a, void* scratch) {
 int paged_prompt_launch(cudaStream_t stream, const PagedArgs& a, bool f32, int* arrived, void* scratch) {
     const int capacity = pp_capacity(a.heads, a.kv_heads, a.requests, a.tokens);
     unsigned char* const at = static_cast<unsigned char*>(scratch) + pp_list_bytes(capacity);
-    const PpWork work = {static_cast<const int4*>(scratch), arrived, reinterpret_cast<float*>(at), reinterpret_cast<float*>(at + pp_partial_bytes(a.head_dim))};
+    const PpWork work = {static_cast<const int4*>(scratch), arrived, reinterpret_cast<uint32_t*>(arrived + kPpSplitBlocks), reinterpret_cast<float*>(at), reinterpret_cast<float*>(at + pp_partial_bytes(a.head_dim))};
     auto go = [&](auto kern, int smem) {
         cudaFuncAttributes fa;
         cudaError_t e = cudaFuncGetAttributes(&fa, kern);

@@ -723,6 +723,21 @@ def test_value_scales_below_the_smallest_that_prompts_tell_apart(cuda):
     check_attention(s)
 
 
+def test_prompt_calls_leave_their_workspace_as_they_found_it(cuda):
+    """More blocks than run at once, keys of more tiles than stay in tensor memory: the counters and flags in front are zero behind every call, and
+    calls repeat themselves to the bit whichever places their blocks found."""
+    for s in (make_attention(91, 8, 8, 64, 64, [1500], [1100], torch.float32), make_attention(92, 8, 2, 128, 32, [3000, 900], [40, 70], torch.float32)):
+        args = (ints(s["start"]), ints(s["context"]), ints(s["table"]), s["cache"], s["most"], max(s["context"]), 0.09)
+        ws = ops.paged_attention_workspace(s["cache"], 8, len(s["context"]), s["q"].shape[0], s["most"], max(s["context"]))
+        front = ws[:4 * (65536 + 296 + 5)]
+        first = ops.paged_attention(s["q"], *args, workspace=ws)
+        assert not front.any()
+        for _ in range(20):
+            assert torch.equal(ops.paged_attention(s["q"], *args, workspace=ws), first)
+        assert not front.any()
+    check_attention(s, scale=0.09)
+
+
 # ---- rows with a sink: one key far above all others, whose value is nothing ---------------------------------------------------------
 def make_sink(seed, heads, kv, hd, block, context, new, dtype, nats, mean, spread=1.0):
     """Key 0 lies `nats` above the others, which score about alike; its value codes are 0, so that the row's result is what the others hold."""
