@@ -4,9 +4,11 @@
 // them, and short portions still fill the 128 rows of an MMA.  Codes are exact in binary16, which is what both contractions run on:
 //   S = Q K^T    Q as x * 2^sh = x0 + x1, two binary16 planes (f32 rows: 2^-22 of the row's largest entry) or one (bf16 rows: exact down to 2^-24 of
 //                it); times k_scale of the key's page and 2^-sh
-//   O += P V     the value scale of a key's page goes into the exponent, P = 2^(s + log2 v_scale - m): no multiplication, and the sum of the
-//                weights takes 1 / v_scale once per group of 16 keys.  P is two planes (f32 rows) or one (bf16 rows: 2^-12, below the rounding of
-//                the result).  A maximum is one of s + log2 v_scale; page scales of a head may differ by 2^100.
+//   O += P V     the value scale of a key's page goes into the exponent, P = 2^(s + log2 v_scale - m + 7): no multiplication, and the sum of the
+//                weights takes 1 / v_scale once per group of 16 keys.  P is two planes (f32 rows, 2^-22) or one (bf16 rows: 2^-11, and the weights of
+//                many keys are rounded either way, where the result is rounded to 2^-9).  A maximum is one of s + log2 v_scale; with the 2^7 and
+//                the 2^8 by which it may lag, P reaches 2^15 and ends at 2^-25, so that O loses what is 2^-32 of the row's largest weight times value scale;
+//                the sum of the weights has all of them.
 // Two streams of work share the keys that are brought in: two tiles of 128 rows, or (where there are 128 rows at most) the even and the odd
 // key tiles of one, each with a maximum, a sum and an O of its own, merged at the end.  Roles of the 28 warps:
 //   warps 0-7, 8-15  softmax of a stream, two threads per row with 64 keys of a tile each: scores by tcgen05.ld, their maximum (both threads'), then
@@ -144,6 +146,8 @@ struct PpWork {
 template <int HD>
 __host__ __device__ constexpr size_t pp_partial_floats() { return (size_t)kPpUnit * (HD + 2); }
 constexpr int kPpDrain = 6;
+// A weight is at most 2^(kPpLag + kPpRoom), half of what binary16 holds.
+constexpr float kPpLag = 8.0f, kPpRoom = 7.0f;
 
 template <int HD, typename T>
 __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const PagedArgs a, const PpWork work) {
@@ -562,7 +566,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                     ok = warp_wait(pair_bar, (uint32_t)n & 1u);
                     if (!ok) return;
                     top = fmaxf(top, at[(half ^ 1) * kPpRows]);
-                    const bool grow = top > m_ref + 8.0f;  // (a row with nothing attended so far has -inf)
+                    const bool grow = top > m_ref + kPpLag;  // (a row with nothing attended so far has -inf)
                     if (__any_sync(0xffffffffu, grow)) {
                         const float corr = grow ? ex2_approx(m_ref - top) : 1.0f;
                         if (grow) m_ref = top;
@@ -581,7 +585,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                             }
                         }
                     }
-                    const float m = m_ref == -INFINITY ? 0.0f : m_ref;
+                    const float m = (m_ref == -INFINITY ? 0.0f : m_ref) - kPpRoom;
                     weights(is_masked, 2 * half + 1, d, m);
                     tmem_load_x32(ts + half * 64, d);
                     weights(is_masked, 2 * half, d, m);

@@ -761,8 +761,8 @@ def sink_bound(s, want, prompt):
     """Elementwise, against what the weights hold: A = sum p_j |v_j| (p of sum 1).  Scores: q is held to 2^-23 of its row's largest entry (prompts: two planes of
     binary16, 2^-22; one of bf16 rows 2^-22 as well, q being bf16), their sums and the exponent are f32: d, a factor of exp(2 d) of each weight.  Weights: single
     tokens 2^-25 (bf16: 2^-17) of the largest weight times the largest value scale in a tile of 32 keys, where none is below 2^-14 (2^-10) of that, else 2^-41 (2^-33);
-    (twice that at the end of its 16 bits); prompts 2^-32 of the row's largest weight times value scale, and 2^-21
-    (bf16: 2^-12) of themselves.  ex2 and the sums of a few hundred f32 terms: 2^-18 A
+    (twice that at the end of its 16 bits); prompts 2^-32 of the row's largest weight times value scale, and 2^-22
+    (bf16: 2^-11) of themselves.  ex2 and the sums of a few hundred f32 terms: 2^-18 A
     (accumulators that cut: 2^-22 a tile of 128 keys)."""
     q, (k, v) = f64(s["q"]), s["values"]
     bf16, block, group = s["q"].dtype == torch.bfloat16, s["block"], q.shape[1] // k.shape[2]
@@ -778,7 +778,7 @@ def sink_bound(s, want, prompt):
             total, pa = p.sum(), p * vs
             d = scale * 2.0 ** (-22 if prompt else -23) * np.abs(q[i, h]).max() * np.abs(kk).sum(1).max() + 8 * 2.0 ** -24 * (np.abs(z).max() + 8)
             if prompt:
-                own = 2.0 ** -32 * pa.max() * np.abs(codes).sum(0) + 2.0 ** (-12 if bf16 else -21) * (p @ np.abs(vv))
+                own = 2.0 ** -32 * pa.max() * np.abs(codes).sum(0) + 2.0 ** (-11 if bf16 else -22) * (p @ np.abs(vv))
             else:
                 tile = np.arange(0, n, 32)
                 most = (np.maximum.reduceat(p, tile) * np.maximum.reduceat(vs, tile))[at[:n] // 32]
@@ -803,3 +803,10 @@ def check_sink(s, prompt):
     (8, 2, 128, 32, 8000, 50, 1.0), (8, 2, 128, 64, 4000, 0, 1.0), (14, 2, 64, 16, 5000, 50, 1000.0), (16, 1, 128, 16, 700, 50, 1.0), (4, 4, 64, 128, 32, 50, 1.0)])
 def test_single_tokens_over_a_sink(cuda, dtype, nats, heads, kv, hd, block, context, mean, spread):
     check_sink(make_sink(nats, heads, kv, hd, block, context, 1, dtype, nats, mean, spread), False)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nats", [6, 12, 14, 18])
+@pytest.mark.parametrize("heads, kv, hd, block, context, new, mean, spread", [(4, 1, 128, 32, 4000, 36, 50, 1.0), (4, 1, 64, 64, 6000, 10, 0, 1.0), (7, 1, 128, 16, 900, 20, 50, 1000.0)])
+def test_portions_over_a_sink(cuda, dtype, nats, heads, kv, hd, block, context, new, mean, spread):
+    check_sink(make_sink(nats + 100, heads, kv, hd, block, context, new, dtype, nats, mean, spread), True)
