@@ -45,6 +45,9 @@ __device__ inline uint32_t bf16_pair_of(float x, float y) {
 __device__ inline void store_row(float* p, float v) { *p = v; }
 __device__ inline void store_row(uint16_t* p, float v) { *p = bf16_of(v); }
 
+// The first position that a row at `pos` attends (its distance from rows in front of position 0 may not be a number of 32 bits).
+__device__ inline int window_start(int pos, int window) { return window > 0 ? max(0, max(pos, 0) - window + 1) : 0; }
+
 // A request's rows and the positions they attend together.
 struct PagedRequest {
     int first, rows;  // rows of the step, tokens
@@ -58,7 +61,7 @@ struct PagedRequest {
         const int context = a.context[r];
         q.pos0 = context - q.rows;
         q.hi = max(0, min(context, a.width * a.block));
-        q.lo = a.window > 0 ? min(q.hi, max(0, q.pos0 - a.window + 1)) : 0;
+        q.lo = min(q.hi, window_start(q.pos0, a.window));
         return q;
     }
 };
@@ -72,7 +75,7 @@ struct PagedUnit {
         PagedUnit u;
         u.row0 = unit * kPpUnit;
         u.live = min(kPpUnit, q.rows * group - u.row0);
-        u.low = a.window > 0 ? max(0, q.pos0 + u.row0 / group - a.window + 1) : 0;
+        u.low = window_start(q.pos0 + u.row0 / group, a.window);
         u.first = u.low & ~15;
         return u;
     }

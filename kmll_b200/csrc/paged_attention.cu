@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(128) paged_rows_kernel(const PagedArgs a) {
     }
     const PagedRequest rq = PagedRequest::of(a, lo);
     if (t < rq.first || t >= rq.first + rq.rows || (long long)rq.rows * group <= a.skip_rows) return;
-    const int pos = min(rq.pos0 + (t - rq.first), rq.hi - 1), start = a.window > 0 ? max(0, rq.pos0 + (t - rq.first) - a.window + 1) : 0;
+    const int pos = min(rq.pos0 + (t - rq.first), rq.hi - 1), start = window_start(rq.pos0 + (t - rq.first), a.window);
     const int32_t* const table = a.table + (size_t)lo * a.width;
     for (int g = warp; g < group; g += 4) {
         const size_t row = ((size_t)t * a.heads + (size_t)h * group + g) * hd;

@@ -422,10 +422,10 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
                 q_unit[nc][e] = __shfl_sync(0xffffffffu, unit, 8 * t + 4 * e);
                 const int col = nc * 8 + 2 * t + e;
                 last[nc][e] = col < n_rows ? min(rq.pos0 + col / group, rq.hi - 1) : -1;
-                first_key[nc][e] = a.window > 0 ? last[nc][e] < 0 ? 0 : rq.pos0 + col / group - a.window + 1 : 0;
+                first_key[nc][e] = window_start(rq.pos0 + col / group, a.window);
             }
         }
-        const int sure_end = min(rq.pos0 + 1, rq.hi), sure_from = a.window > 0 ? rq.pos0 + rq.rows - a.window : 0;  // keys that every row attends
+        const int sure_end = min(rq.pos0 + 1, rq.hi), sure_from = window_start(rq.pos0 + rq.rows - 1, a.window);  // keys that every row attends
 
         float m[NC][2], l[NC][2], acc[NC][DT][4];
 #pragma unroll

@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
         const PagedRequest rq = PagedRequest::of(a, entry.x);
         const PagedUnit un = PagedUnit::of(a, rq, group, entry.y);
         const int parts = entry.z >> 16, part = entry.z & 0xffff;
-        const int row0 = un.row0, live = un.live, low = un.low;
+        const int row0 = un.row0, live = un.live;
         const bool two = live > kPpRows;  // two tiles of rows; else two shares of the keys
         auto own_pos = [&](int r) { return rq.pos0 + (row0 + r) / group; };  // (a context longer than its table row is cut at the table's end)
         // this part's tiles, counted from its first one
@@ -446,8 +446,8 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
             uint64_t* const pair_bar = pair + stream * 4 + (warp & 3);  // of the two warps that have the same rows
             float* const tops = reinterpret_cast<float*>(smem + S::kOffTop) + stream * 2 * kPpRows + r;  // [tile parity][stream][half][row]
             const int step = two ? 1 : 2, end = two && stream == 0 ? tiles0 : tiles;
-            const int own = own_pos(in_unit), pos = min(own, rq.hi - 1), lo = a.window > 0 ? own - a.window + 1 : 0;
-            const int row_a = two ? stream * kPpRows : 0, row_b = min(live, row_a + kPpRows) - 1, first_pos = own_pos(row_a), last_own = own_pos(max(row_b, row_a));
+            const int own = own_pos(in_unit), pos = min(own, rq.hi - 1), lo = window_start(own, a.window);
+            const int row_a = two ? stream * kPpRows : 0, row_b = min(live, row_a + kPpRows) - 1, first_pos = own_pos(row_a), last_own = max(own_pos(max(row_b, row_a)), 0);
             const float unit = a.scale2 / units[in_unit];  // (a row with an infinity or NaN has no scores)
             const uint32_t rows = (uint32_t)((warp & 3) * 32) << 16;
             const uint32_t ts = rows + (uint32_t)stream * 128u, to = rows + kPpTmemO + (uint32_t)stream * 128u;
@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prompt_kernel(const Paged
                 tcgen05_fence_after();
                 const PpScales& sc = scales[j & 3];
                 const uint32_t there_bits = sc.there;
-                const bool masked = t0 + kPpKeys - 1 > first_pos || t0 < low || (a.window > 0 && t0 < last_own - a.window + 1) || there_bits != 0xffu;
+                const bool masked = t0 + kPpKeys - 1 > first_pos || (a.window > 0 && t0 < last_own - a.window + 1) || there_bits != 0xffu;
                 // keys of chunk c that the row attends, a bit each
                 auto seen_of = [&](int c) {
                     const int k0 = t0 + c * 32, from = max(lo - k0, 0), to_key = min(pos - k0, 31);

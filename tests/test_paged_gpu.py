@@ -810,3 +810,13 @@ def test_single_tokens_over_a_sink(cuda, dtype, nats, heads, kv, hd, block, cont
 @pytest.mark.parametrize("heads, kv, hd, block, context, new, mean, spread", [(4, 1, 128, 32, 4000, 36, 50, 1.0), (4, 1, 64, 64, 6000, 10, 0, 1.0), (7, 1, 128, 16, 900, 20, 50, 1000.0)])
 def test_portions_over_a_sink(cuda, dtype, nats, heads, kv, hd, block, context, new, mean, spread):
     check_sink(make_sink(nats + 100, heads, kv, hd, block, context, new, dtype, nats, mean, spread), True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads, kv, hd, new", [(4, 4, 128, 6), (8, 2, 64, 40), (2, 1, 80, 9)])
+def test_windows_as_long_as_32_bits_hold(cuda, dtype, heads, kv, hd, new):
+    """Rows in front of position 0 attend nothing; the distance from them to a window's first position is no 32-bit number."""
+    s = make_attention(87, heads, kv, hd, 16, [30, 0, 7], [new] * 3, dtype)
+    s["context"] = [new - 4, new, new + 7]  # of the first request, four rows are in front of position 0
+    outs = [check_attention(s, window=w) for w in (0, 2 ** 31 - 1, 2 ** 31 - 5, 2 ** 30)]
+    assert all(torch.equal(o, outs[0]) for o in outs)
