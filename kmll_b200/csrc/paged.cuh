@@ -21,6 +21,7 @@ struct PagedArgs {
     float scale2;  // log2(e) times the score scale
     int window;
     void* out;
+    int max_query;  // requests with more rows are left out
     int skip_rows;  // requests with at most this many rows (tokens times query heads of a kv head) belong to another kernel
 };
 
@@ -57,7 +58,7 @@ struct PagedRequest {
         PagedRequest q;
         q.first = a.query_start[r];
         q.rows = min(a.query_start[r + 1], a.tokens) - q.first;
-        if (q.first < 0 || q.rows < 0) q.rows = 0;
+        if (q.first < 0 || q.rows < 0 || q.rows > a.max_query) q.rows = 0;
         const int context = a.context[r];
         q.pos0 = context - q.rows;
         q.hi = max(0, min(context, a.width * a.block));

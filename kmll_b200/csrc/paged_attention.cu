@@ -117,7 +117,7 @@ extern "C" int kmll_paged_attention(kmll_stream_t stream, const void* query, int
     KMLL_REQUIRE_PTR(block_table);
     KMLL_REQUIRE_PTR(out);
     PagedArgs a = {query, query_start, context, block_table, table_width, requests, tokens, heads, kv_heads, head_dim, block, pages, k_codes, v_codes,
-                   k_scales, v_scales, scale * 1.4426950408889634f, window, out, 0};
+                   k_scales, v_scales, scale * 1.4426950408889634f, window, out, max_query, 0};
     const long long max_rows = (long long)max_query * (heads / kv_heads);
     if (paged_decode_serves(head_dim) && (reinterpret_cast<uintptr_t>(query) & 15u) == 0) {
         KMLL_REQUIRE_PTR(workspace);

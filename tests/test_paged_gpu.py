@@ -820,3 +820,15 @@ def test_windows_as_long_as_32_bits_hold(cuda, dtype, heads, kv, hd, new):
     s["context"] = [new - 4, new, new + 7]  # of the first request, four rows are in front of position 0
     outs = [check_attention(s, window=w) for w in (0, 2 ** 31 - 1, 2 ** 31 - 5, 2 ** 30)]
     assert all(torch.equal(o, outs[0]) for o in outs)
+
+
+@pytest.mark.parametrize("heads, kv, hd, new, most", [(4, 2, 128, [1, 3, 1], 1), (8, 2, 64, [3, 40, 20], 20), (8, 2, 128, [5, 200, 1], 100), (2, 1, 80, [1, 4, 3], 3)])
+def test_requests_of_more_rows_than_announced_are_left_as_they_were(cuda, heads, kv, hd, new, most):
+    s = make_attention(88, heads, kv, hd, 32, [50, 90, 400], new, torch.float32)
+    out = check_attention(s, fill=9.0)
+    short = torch.full_like(out, 9.0)
+    ops.paged_attention(s["q"], ints(s["start"]), ints(s["context"]), ints(s["table"]), s["cache"], most, 500, 1 / math.sqrt(hd), out=short)
+    a, b = s["start"][1], s["start"][2]
+    assert (short[a:b] == 9.0).all()
+    tol = torch.from_numpy(attention_bound(s, f64(out).reshape(s["q"].shape), 1 / math.sqrt(hd), 0)).cuda().view_as(out)
+    assert ((short - out).abs() <= 2 * tol)[:a].all() and ((short - out).abs() <= 2 * tol)[b:].all()
