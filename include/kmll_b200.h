@@ -392,7 +392,9 @@ int kmll_paged_plan(kmll_stream_t stream, const int32_t* lengths, const int32_t*
                     const int32_t* free_blocks, int free_capacity, const int32_t* free_count, int token_capacity, int32_t* context, int32_t* query_start,
                     int32_t* positions, int32_t* slots, int32_t* free_count_out, int32_t* status);
 /* Pages of the requests with ended[r] != 0 go back on the stack (request after request, their table entries become -1) and their context becomes
- * 0; context_out and free_count_out may be the inputs.  *status: 0, or nothing is changed because 1 = the stack is too small, 3 = a context that is
+ * 0; context_out and free_count_out may be the inputs.  A row of the table owns its pages: a page that stands in the rows of other requests too (a common
+ * beginning) must not go back while they use it, and only once.  Entries that are negative are passed over, so the caller sets those of shared pages to -1
+ * in front of the release of every request but the last that holds them.  *status: 0, or nothing is changed because 1 = the stack is too small, 3 = a context that is
  * negative or longer than its table row. */
 int kmll_paged_release(kmll_stream_t stream, const int32_t* context, const int32_t* ended, int requests, int block, int32_t* block_table, int table_width,
                        int32_t* free_blocks, int free_capacity, const int32_t* free_count, int32_t* context_out, int32_t* free_count_out, int32_t* status);

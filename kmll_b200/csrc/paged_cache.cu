@@ -132,13 +132,14 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanArgs
     }
 }
 
-// Pages of the requests that have ended go back on the stack, request after request, first page first.
+// Pages of the requests that have ended go back on the stack, request after request, first page first; negative entries of the table are no pages.
 __global__ void __launch_bounds__(kPlanThreads) paged_release_kernel(const int32_t* context, const int32_t* ended, int requests, int block, int32_t* table, int width,
                                                                      int32_t* free_blocks, int free_capacity, const int32_t* free_count, int32_t* context_out,
                                                                      int32_t* free_count_out, int32_t* status) {
     extern __shared__ int32_t plan_smem[];
     __shared__ longlong2 scratch[kPlanThreads / 32];
-    int32_t* const s_pages = plan_smem;
+    int32_t* const s_entries = plan_smem;           // of the table, of a request that has ended
+    int32_t* const s_pages = s_entries + requests;  // those that are pages
     int32_t* const s_at = s_pages + requests;
     const int tid = threadIdx.x, per = (requests + kPlanThreads - 1) / kPlanThreads;
     pdl_wait();
@@ -150,9 +151,17 @@ __global__ void __launch_bounds__(kPlanThreads) paged_release_kernel(const int32
         if (r >= requests) break;
         const long long c = context[r], n = (c + block - 1) / block;
         if (c < 0 || n > width) bad = 1;
-        s_pages[r] = ended[r] != 0 && c >= 0 && n <= width ? (int)n : 0;
-        mine.x += s_pages[r];
+        s_entries[r] = ended[r] != 0 && c >= 0 && n <= width ? (int)n : 0;
     }
+    __syncthreads();
+    for (int r = tid >> 5; r < requests; r += kPlanThreads / 32) {
+        int pages = 0;
+        for (int i = tid & 31; i < s_entries[r]; i += 32) pages += table[(size_t)r * width + i] >= 0 ? 1 : 0;
+        pages = __reduce_add_sync(0xffffffffu, pages);
+        if ((tid & 31) == 0) s_pages[r] = pages;
+    }
+    __syncthreads();
+    for (int i = 0; i < per && tid * per + i < requests; ++i) mine.x += s_pages[tid * per + i];
     longlong2 whole;
     long long at = plan_scan(mine, whole, scratch).x;
     bad = __syncthreads_or(bad) ? 3 : count < 0 || count + whole.x > free_capacity ? 1 : 0;
@@ -169,12 +178,20 @@ __global__ void __launch_bounds__(kPlanThreads) paged_release_kernel(const int32
         *status = bad;
     }
     if (bad) return;
-    for (int r = tid >> 5; r < requests; r += kPlanThreads / 32)
-        for (int i = tid & 31; i < s_pages[r]; i += 32) {
+    for (int r = tid >> 5; r < requests; r += kPlanThreads / 32) {
+        int at = s_at[r];
+        for (int i0 = 0; i0 < s_entries[r]; i0 += 32) {
+            const int i = i0 + (tid & 31);
             int32_t* const entry = table + (size_t)r * width + i;
-            free_blocks[s_at[r] + i] = *entry;
-            *entry = -1;
+            const int page = i < s_entries[r] ? *entry : -1;
+            const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+            if (page >= 0) {
+                free_blocks[at + __popc(there & ((1u << (tid & 31)) - 1u))] = page;
+                *entry = -1;
+            }
+            at += __popc(there);
         }
+    }
 }
 
 // ---- rotation and storage -------------------------------------------------------------------------------------------------
@@ -763,9 +780,9 @@ extern "C" int kmll_paged_release(kmll_stream_t stream, const int32_t* context, 
         KMLL_REQUIRE_PTR(context_out);
     }
     if (free_capacity > 0) KMLL_REQUIRE_PTR(free_blocks);
-    cudaError_t e = allow_dynamic_smem(paged_release_kernel, 2 * (size_t)requests * 4);
+    cudaError_t e = allow_dynamic_smem(paged_release_kernel, 3 * (size_t)requests * 4);
     if (e == cudaSuccess)
-        e = launch(paged_release_kernel, dim3(1), dim3(kPlanThreads), 2 * (size_t)requests * 4, as_stream(stream), true, context, ended, requests, block, block_table,
+        e = launch(paged_release_kernel, dim3(1), dim3(kPlanThreads), 3 * (size_t)requests * 4, as_stream(stream), true, context, ended, requests, block, block_table,
                    table_width, free_blocks, free_capacity, free_count, context_out, free_count_out, status);
     if (e != cudaSuccess) return fail(KMLL_ERR_CUDA, "paged release: %s", cudaGetErrorString(e));
     return check_launch("paged release");

@@ -674,7 +674,7 @@ def paged_plan(lengths, new_tokens, block: int, block_table, free_blocks, free_c
 
 
 def paged_release(context, ended, block: int, block_table, free_blocks, free_count, context_out, free_count_out, status):
-    """Pages of the requests with ended != 0 go back on the stack: kmll_paged_release."""
+    """Pages of the requests with ended != 0 go back on the stack: kmll_paged_release.  Set the entries of pages that another request still uses to -1 before."""
     requests, width = block_table.shape
     i32, gpu = torch.int32, _here(block_table)
     check(load().kmll_paged_release(_stream(), _array(context, i32, requests, "context", gpu), _array(ended, i32, requests, "ended", gpu), requests, block,

@@ -832,3 +832,28 @@ def test_requests_of_more_rows_than_announced_are_left_as_they_were(cuda, heads,
     assert (short[a:b] == 9.0).all()
     tol = torch.from_numpy(attention_bound(s, f64(out).reshape(s["q"].shape), 1 / math.sqrt(hd), 0)).cuda().view_as(out)
     assert ((short - out).abs() <= 2 * tol)[:a].all() and ((short - out).abs() <= 2 * tol)[b:].all()
+
+
+def test_release_passes_over_entries_that_are_no_pages(cuda):
+    """Two requests with a common beginning end one after the other: the shared entries of the first one to end are set to -1, and every page comes back
+    once; long rows with holes anywhere come back without them."""
+    table = np.full((2, 90), -1)
+    table[0, :5], table[1, :6] = [10, 11, 12, 13, 14], [10, 11, 12, 15, 16, 17]
+    t, c, stack, left, status = ints(table), ints([70, 96]), ints([-5] * 20), ints([0]), ints([-7])
+    t[0, :3] = -1
+    ops.paged_release(c, ints([1, 0]), 16, t, stack, left, c, left, status)
+    assert status.item() == 0 and left.item() == 2 and stack.tolist()[:3] == [13, 14, -5] and c.tolist() == [0, 96] and t[1].tolist() == table[1].tolist()
+    ops.paged_release(c, ints([1, 1]), 16, t, stack, left, c, left, status)
+    assert status.item() == 0 and left.item() == 8 and sorted(stack.tolist()[:8]) == list(range(10, 18)) and (t == -1).all()
+    rng = np.random.default_rng(0)
+    table = rng.permutation(40 * 90).reshape(40, 90)
+    table[rng.random(table.shape) < 0.3] = -1
+    context, ended = rng.integers(0, 90 * 16 + 1, 40), rng.integers(0, 2, 40)
+    t, c, out, left, status = ints(table), ints(context), ints([-7] * 40), ints([3]), ints([-7])
+    stack = ints(np.full(4000, -9))
+    ops.paged_release(c, ints(ended), 16, t, stack, left, out, left, status)
+    back = [int(p) for r in range(40) if ended[r] for p in table[r, :-(-context[r] // 16)] if p >= 0]
+    assert status.item() == 0 and left.item() == 3 + len(back) and stack.tolist()[:4 + len(back)] == [-9] * 3 + back + [-9]
+    kept = np.where((ended[:, None] != 0) & (np.arange(90) < -(-context // 16)[:, None]), -1, table)
+    np.testing.assert_array_equal(t.cpu().numpy(), kept)
+    assert out.tolist() == [0 if e else x for e, x in zip(ended, context.tolist())]
