@@ -19,6 +19,7 @@
 
 #include <atomic>
 #include <cfloat>
+#include <type_traits>
 
 #include "internal.cuh"
 
@@ -533,11 +534,12 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_rows_kernel(const Sa
     cluster.sync();
 }
 
-// Clusters of `c` blocks that the GPU runs at once: asked for once per kernel and size (an occupancy query, no allocation).
-template <typename K>
-int clusters_at_once(K kernel, int c) {
-    static std::atomic<int> known[9];
-    int n = known[c].load(std::memory_order_relaxed);
+// Clusters of `c` blocks that the current GPU runs at once: asked for once per kernel, GPU and size (an occupancy query, no allocation).
+constexpr int kKnownDevices = 64;
+template <auto kernel>
+cudaError_t clusters_at_once(int device, int c, int& n) {
+    static std::atomic<int> known[kKnownDevices][9];
+    n = device < kKnownDevices ? known[device][c].load(std::memory_order_relaxed) : 0;
     if (n == 0) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(c * 16);
@@ -550,13 +552,12 @@ int clusters_at_once(K kernel, int c) {
         attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
-            cudaGetLastError();
-            n = 1;
-        }
-        known[c].store(n, std::memory_order_relaxed);
+        const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+        if (e != cudaSuccess) return e;
+        n = n < 1 ? 1 : n;
+        if (device < kKnownDevices) known[device][c].store(n, std::memory_order_relaxed);
     }
-    return n;
+    return cudaSuccess;
 }
 
 }  // namespace
@@ -577,19 +578,20 @@ extern "C" int kmll_sample_rows(kmll_stream_t stream, const void* logits, int is
     const SampleArgs a = {logits, vocab, (size_t)ld, u, temperature, top_k, top_p, min_p, tokens, logprobs};
     // The most blocks per row that still let all rows run at once: a row's steps are short, a second round of clusters costs as much as the first
     // (16 rows of 151936, greedy: clusters of 8, of which fewer than 16 fit, 29 us, of 4 19, of 2 29; 64 rows of 152064: of 4 41, of 2 30, of 1 51).
-    auto go = [&](auto kern) {
+    auto go = [&](auto which) {
+        constexpr auto kern = decltype(which)::value;
+        int cluster = 1, device = 0, at_once = 0;
         cudaError_t e = allow_all_dynamic_smem(kern);
-        int cluster = 1;
-        for (int c = 8; c > 1 && e == cudaSuccess; c >>= 1) {
+        if (e == cudaSuccess) e = cudaGetDevice(&device);
+        for (int c = 8; c > 1 && cluster == 1 && e == cudaSuccess; c >>= 1) {
             if (rows > 148 / c) continue;
-            if (rows > clusters_at_once(kern, c)) continue;
-            cluster = c;
-            break;
+            e = clusters_at_once<kern>(device, c, at_once);
+            if (rows <= at_once) cluster = c;
         }
         if (e != cudaSuccess) return e;
         return launch_cluster(kern, dim3((unsigned)rows * cluster), cluster, dim3(kSampleThreads), sizeof(SampleShared), as_stream(stream), true, a);
     };
-    const cudaError_t e = is_f32 ? go(sample_rows_kernel<float>) : go(sample_rows_kernel<uint16_t>);
+    const cudaError_t e = is_f32 ? go(std::integral_constant<void (*)(SampleArgs), sample_rows_kernel<float>>()) : go(std::integral_constant<void (*)(SampleArgs), sample_rows_kernel<uint16_t>>());
     if (e != cudaSuccess) return fail(KMLL_ERR_CUDA, "sample rows: %s", cudaGetErrorString(e));
     return check_launch("sample rows");
 }
