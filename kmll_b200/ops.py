@@ -580,7 +580,7 @@ def sample_rows(logits, u, temperature=None, top_k=None, top_p=None, min_p=None,
     f32, i32 = torch.float32, torch.int32
     tokens = torch.empty(rows, dtype=i32, device=logits.device) if tokens is None else tokens
     logprobs = torch.empty(rows, dtype=f32, device=logits.device) if logprobs is None else logprobs
-    check(load().kmll_sample_rows(_stream(), logits.data_ptr(), 1 if logits.dtype is f32 else 0, logits.stride(0) if rows > 1 else vocab, rows, vocab,
+    check(load().kmll_sample_rows(_stream(), logits.data_ptr(), 1 if logits.dtype is f32 else 0, _row_pitch(logits, "logits") if rows > 1 else vocab, rows, vocab,
                                   _array(u, torch.float64, rows, "u", gpu), _array(temperature, f32, rows, "temperature", gpu), _array(top_k, i32, rows, "top_k", gpu),
                                   _array(top_p, f32, rows, "top_p", gpu), _array(min_p, f32, rows, "min_p", gpu), _array(tokens, i32, rows, "tokens", gpu),
                                   _array(logprobs, f32, rows, "logprobs", gpu)))
@@ -596,6 +596,14 @@ def _here(t: torch.Tensor) -> int:
     if at != torch._C._cuda_getDevice():
         raise KmllError(-2, f"operand lies on GPU {at}, the current one is {torch._C._cuda_getDevice()}")
     return at
+
+
+def _row_pitch(t: torch.Tensor, name: str) -> int:
+    """Elements from row to row; ctypes would cut what does not fit into the entry points' int."""
+    pitch = t.stride(0)
+    if pitch >= 1 << 31:
+        raise KmllError(-2, f"rows of {name} lie {pitch} elements apart, a pitch is 32 bits")
+    return pitch
 
 
 def _array(t, dtype, least: int, name: str, gpu: int) -> int | None:
@@ -691,7 +699,7 @@ def _head_rows(t, tokens, heads, head_dim, dtype, name, gpu):
         return t.data_ptr(), heads * head_dim
     if t.dim() not in (2, 3) or t.stride(-1) != 1 or (t.dim() == 3 and t.shape[1] > 1 and (t.stride(1) != t.shape[2] or t.shape[2] != head_dim)):
         raise KmllError(-2, f"the heads of a row of {name} must lie together")
-    return t.data_ptr(), t.stride(0) if tokens > 1 else heads * head_dim
+    return t.data_ptr(), _row_pitch(t, name) if tokens > 1 else heads * head_dim
 
 
 def prepare_paged_attention(query, key, value, freqs, positions, slots, cache: DevicePagedI8Cache, query_rot=None):

@@ -162,3 +162,16 @@ def test_pointer_types_of_the_new_entry_points():
     protos = lib.parse_prototypes(lib.HEADERS[0])
     assert len(protos["kmll_paged_attention"][1]) == 24 and protos["kmll_paged_attention_workspace_bytes"][0] is C.c_size_t
     assert len(protos["kmll_prepare_paged_attention"][1]) == 23 and len(protos["kmll_paged_plan"][1]) == 17 and len(protos["kmll_sample_rows"][1]) == 13
+
+
+def test_pitches_beyond_32_bits_are_refused():
+    """A pitch of 2^32 + 64 must not become one of 64 (tensors without memory: only their strides are looked at)."""
+    import torch
+
+    from kmll_b200 import ops
+    rows = torch.empty_strided((3, 1, 64), (2 ** 32 + 64, 64, 1), dtype=torch.bfloat16, device="meta")
+    with pytest.raises(lib.KmllError, match="32 bits"):
+        ops._head_rows(rows, 3, 1, 64, torch.bfloat16, "key", rows.get_device())
+    assert ops._head_rows(rows[:1], 1, 1, 64, torch.bfloat16, "key", rows.get_device())[1] == 64  # (one row has no pitch)
+    near = torch.empty_strided((2, 64), (2 ** 31 - 1, 1), dtype=torch.float32, device="meta")
+    assert ops._row_pitch(near, "logits") == 2 ** 31 - 1

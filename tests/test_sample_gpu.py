@@ -202,3 +202,10 @@ def test_many_launches_one_behind_the_other(cuda, rows):
     outs = [(ops.sample_rows(x, u, temperature=cold)[0], ops.sample_rows(x, u, top_k=k)) for _ in range(60)]
     for greedy, (tokens, logprobs) in outs:
         assert torch.equal(greedy, best) and torch.equal(tokens, first[0]) and torch.equal(logprobs, first[1])
+
+
+def test_rows_too_far_apart_are_refused(cuda):
+    from kmll_b200.lib import KmllError
+    far = torch.empty(2 ** 32 + 256, dtype=torch.bfloat16, device="cuda").as_strided((2, 64), (2 ** 32 + 64, 1))
+    with pytest.raises(KmllError, match="32 bits"):
+        ops.sample_rows(far, dev([0.5, 0.5], torch.float64))
