@@ -402,8 +402,9 @@ int kmll_paged_release(kmll_stream_t stream, const int32_t* context, const int32
  * = 0) bf16, [tokens] at a pitch of ld_* elements; query_rot is [tokens, heads, head_dim] of the same type and may be `query` where its rows lie together.
  * Entries d and d + n_freqs turn by positions[t] * freqs[d] (computed in 64 bits, so far positions keep their angles), entries from 2 * n_freqs on pass
  * through; n_freqs = 0: no rotation, positions and freqs may be null.  Codes are those of the 64-bit rotated keys.  heads = 0: keys and values only.
- * Rows whose slot is outside the cache are left out, their query_rot as it was.  The rows of one page must follow one another in ascending
- * order, and no two rows may have the same slot. */
+ * Rows whose slot is outside the cache are left out, their query_rot as it was.  The rows of one page must follow one another directly, each in the slot
+ * behind the one before (as kmll_paged_plan gives them): rows of a page with a gap between their slots, or with other rows in between, are taken by
+ * different blocks, which would both set the page's scale. */
 int kmll_prepare_paged_attention(kmll_stream_t stream, const void* query, int ld_query, const void* key, int ld_key, const void* value, int ld_value, int is_f32,
                                  const float* freqs, int n_freqs, const int32_t* positions, const int32_t* slots, int tokens, int heads, int kv_heads,
                                  int head_dim, void* query_rot, int8_t* k_codes, float* k_scales, int8_t* v_codes, float* v_scales, int pages, int block);

@@ -606,7 +606,7 @@ __global__ void __launch_bounds__(kPrepareThreads) prepare_paged_kernel(const Pr
             const float mine = warp_max((float)(largest / 127.0));
             if ((tid & 31) == 0) s_top[tid >> 5] = mine;
             float* const scale_at = (keys ? a.k_scales : a.v_scales) + (size_t)page * a.kv_heads + (live ? h : 0);
-            const float before = at == 0 ? 0.0f : *scale_at;
+            const float before = at == 0 || !live ? 0.0f : *scale_at;
             __syncthreads();  // (all have read the scale)
             float scale = before;
     #pragma unroll

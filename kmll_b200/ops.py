@@ -705,7 +705,7 @@ def _head_rows(t, tokens, heads, head_dim, dtype, name, gpu):
 def prepare_paged_attention(query, key, value, freqs, positions, slots, cache: DevicePagedI8Cache, query_rot=None):
     """Rotation of a step's queries and keys, keys and values into the cache: prepare_incremental_attention (ops/inference.rs:1291-1362) for rows
     of many requests.  query [tokens, heads, head_dim], key and value [tokens, kv_heads, head_dim], f32 or bf16; freqs None: no
-    rotation.  Returns the turned queries."""
+    rotation.  The rows of a page follow one another directly, each in the slot behind the one before.  Returns the turned queries."""
     dtype, tokens, kv_heads, head_dim = key.dtype, key.shape[0], cache.kv_heads, cache.head_dim
     if dtype is not torch.float32 and dtype is not torch.bfloat16:
         raise KmllError(-2, "query, key and value must be rows in float32 or bfloat16")
