@@ -506,10 +506,9 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
                     const float base = top == -INFINITY ? 0.0f : top;
                     turn[e] = ex2_approx(m[nc][e] - base);
                     m[nc][e] = top;
-                    const float largest = ex2_approx(own - base);
-                    const bool any = largest > 0x1p-80f;  // (what is less counts in the sum alone)
-                    const float up = any ? __fdividef(kWhole, largest) : 0.0f;
-                    v_unit[nc][e] = any ? largest * (vmax / kWhole) : 0.0f;
+                    // (the tile's largest weight is kWhole after `up`; where that overflows, or nothing is attended, v_unit makes nothing of what comes out)
+                    const float up = ex2_approx(base - own) * kWhole;
+                    v_unit[nc][e] = ex2_approx(own - base) * (vmax / kWhole);
                     float sum = 0.0f;
 #pragma unroll
                     for (int half16 = 0; half16 < 2; ++half16)
