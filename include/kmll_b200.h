@@ -420,7 +420,7 @@ int kmll_paged_cache_rows(kmll_stream_t stream, const int8_t* k_codes, const flo
  * workspace serves calls of any sizes that need no more bytes, one after another; calls that overlap need workspaces of their own, and two
  * graphs that may run at the same time are captured with two.  May be null where that function says 0.  requests * kv_heads <= 65536 for heads of
  * 64 and 128.  After a time-out (kmll_device_status) the workspace has to be zeroed.
- * Rounding, heads of 64 and 128 (others: f32).  q: to 2^-24 of its row's largest entry (bf16 rows 2^-16; requests of more than 8 to 16 rows of a kv head 2^-22).  A
+ * Rounding, heads of 64 and 128 (others: f32).  q: to 2^-24 of its row's largest entry (requests of more than 8 to 16 rows of a kv head 2^-22).  A
  * key's weight times its page's value scale, where the output takes it (their sum takes all of it): requests of few rows to 2^-25 (bf16 rows 2^-17) of the largest
  * weight times the largest value scale in its tile of 32 keys, in a tile with one below 2^-14 (2^-10) of that to 2^-41 (2^-33); requests of more rows to 2^-22
  * (2^-11) of itself and 2^-32 of the row's largest, and value scales below 2^-80 count as 2^-80.  That is about 1e-6 (f32 rows) of the largest weighted |value| of

@@ -1,11 +1,11 @@
 // Attention of single tokens (and of a few rows) over the paged 8-bit cache: the codes go to the tensor cores as they lie.
 //
-//   S^T[key][row] = K[key] . q[row]: A = 16 keys x 32 codes by ldmatrix, B = q as a 24-bit integer (bf16 rows: 16 bits) below the largest
+//   S^T[key][row] = K[key] . q[row]: A = 16 keys x 32 codes by ldmatrix, B = q as a 24-bit integer below the largest
 //   entry of its row, in bytes; mma.m16n8k32 s8 x u8 / s8 -> s32, one MMA per byte, exact; S = k_scale * q_scale * (D0 + 2^8 D1 + 2^16 D2)
 //   O^T[dim][row] += V^T[dim][key] P^T[key][row]: A = 16 columns x 32 keys (values lie with the keys of a column together), B =
 //   softmax weights times the page's value scale, as 24-bit (bf16 rows: 16-bit) fractions of the largest of them in the tile of 32 keys, in bytes
-// Nothing is converted on the way from memory to the tensor cores, and both contractions are exact.  What is rounded are q, to 2^-24 (bf16 rows, whose
-// entries have eight bits: 2^-16) of its row's largest entry, and the weights, to 2^-25 (2^-17) of the tile's largest: of the tile's, not of the row's, because
+// Nothing is converted on the way from memory to the tensor cores, and both contractions are exact.  What is rounded are q, to 2^-24 of its row's largest
+// entry (of bf16 rows too: a strong channel would leave the others of 16 bits fewer than they have), and the weights, to 2^-25 (bf16 rows 2^-17) of the tile's largest: of the tile's, not of the row's, because
 // the sum of the weights has all of them, and what lies far below one key that dominates a row is most of the result where that key's value is small.
 // For the same reason a tile with weights below 2^-14 (2^-10) of its largest goes twice, the second time with 16 bits of what rounding left.  (64 requests of 8192, 32
 // query heads over 8 of size 128, f32: 186 us either way where scores spread by 1; 208 where they spread by 3 and many tiles go twice, 186 without.)
@@ -218,7 +218,7 @@ __device__ inline void paged_order(const PagedArgs& a, const PagedOrder& o, int 
     }
 }
 
-// NB: bytes of q and of the weights; NC: columns of eight rows.
+// NB: bytes of the weights; NC: columns of eight rows.
 template <int HD, typename T, int NB, int NC>
 __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kernel(const PagedArgs a, const PdWork work, const PagedOrder order) {
     using S = PdShape<HD>;
@@ -372,8 +372,8 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
         }
         int next_page = page_of(kPdStages);
 
-        // ---- q of eight rows a column: bytes of round(q * 2^sh), the largest entry of a row between 2^(8 NB - 2) and 2^(8 NB - 1)
-        uint32_t qb[NC][NB][KS][2];
+        // ---- q of eight rows a column: bytes of round(q * 2^sh), the largest entry of a row between 2^22 and 2^23
+        uint32_t qb[NC][3][KS][2];
         float q_unit[NC][2];   // of this lane's two score columns: 2^-sh * scale
         int last[NC][2], first_key[NC][2];
 #pragma unroll
@@ -399,9 +399,9 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
             finite = ((finite ? 1 : 0) & __shfl_xor_sync(0xffffffffu, finite ? 1 : 0, 2)) != 0;
             int e2 = 0;
             if (top > 0.0f && top < INFINITY) frexpf(top, &e2);  // top in [2^(e2 - 1), 2^e2)
-            const int sh = max(-120, min(120, 8 * NB - 1 - e2));
+            const int sh = max(-120, min(120, 23 - e2));
             const float up = ldexpf(1.0f, sh);
-            const int most = (1 << (8 * NB - 1)) - 1;
+            const int most = (1 << 23) - 1;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[i] = live ? (uint32_t)max(-most, min(most, __float2int_rn(q[nc][ks][e][i] * up))) : 0u;
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) {
+                    for (int b = 0; b < 3; ++b) {
                         const uint32_t pick = (uint32_t)(b | ((b + 4) << 4));
                         qb[nc][b][ks][e] = __byte_perm(__byte_perm(x[0], x[1], pick), __byte_perm(x[2], x[3], pick), 0x5410);
                     }
@@ -446,11 +446,11 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
             float s[NC][2][4];
 #pragma unroll
             for (int half16 = 0; half16 < 2; ++half16) {
-                int d[NC][NB][4];
+                int d[NC][3][4];
 #pragma unroll
                 for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) d[nc][b][0] = d[nc][b][1] = d[nc][b][2] = d[nc][b][3] = 0;
+                    for (int b = 0; b < 3; ++b) d[nc][b][0] = d[nc][b][1] = d[nc][b][2] = d[nc][b][3] = 0;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
                     uint32_t f[4];
@@ -458,16 +458,15 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
 #pragma unroll
                     for (int nc = 0; nc < NC; ++nc) {
 #pragma unroll
-                        for (int b = 0; b < NB - 1; ++b) mma_s8u8(d[nc][b], f, qb[nc][b][ks][0], qb[nc][b][ks][1]);
-                        mma_s8s8(d[nc][NB - 1], f, qb[nc][NB - 1][ks][0], qb[nc][NB - 1][ks][1]);
+                        for (int b = 0; b < 2; ++b) mma_s8u8(d[nc][b], f, qb[nc][b][ks][0], qb[nc][b][ks][1]);
+                        mma_s8s8(d[nc][2], f, qb[nc][2][ks][0], qb[nc][2][ks][1]);
                     }
                 }
 #pragma unroll
                 for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float v = (float)(d[nc][0][e] + (d[nc][1][e] << 8));
-                        if (NB == 3) v = fmaf((float)d[nc][NB - 1][e], 65536.0f, v);
+                        const float v = fmaf((float)d[nc][2][e], 65536.0f, (float)(d[nc][0][e] + (d[nc][1][e] << 8)));
                         s[nc][half16][e] = v * (mt.k_scale[half16] * q_unit[nc][e & 1]);
                     }
             }

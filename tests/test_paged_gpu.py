@@ -857,3 +857,15 @@ def test_release_passes_over_entries_that_are_no_pages(cuda):
     kept = np.where((ended[:, None] != 0) & (np.arange(90) < -(-context // 16)[:, None]), -1, table)
     np.testing.assert_array_equal(t.cpu().numpy(), kept)
     assert out.tolist() == [0 if e else x for e, x in zip(ended, context.tolist())]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads, kv, hd, new", [(8, 2, 128, 1), (14, 1, 64, 1), (8, 1, 128, 3), (4, 1, 128, 20)])
+def test_queries_with_a_strong_channel(cuda, dtype, heads, kv, hd, new):
+    """One entry of 5000 beside entries of about 1, over few keys that have nothing there: what is left of the others decides.  The bound is that of the rows with a
+    sink, whose first term is the rounding of q below its largest entry."""
+    s = make_sink(93, heads, kv, hd, 32, 11 + new, new, dtype, 0.0, 0)
+    s["cache"].k_codes[:, :, 0, :, 0] = 0
+    s["values"][0][..., 0] = 0.0
+    s["q"][..., 0] = 5000.0
+    check_sink(s, new > 3)
