@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
             }
             // ---- running maximum and sum of this lane's two columns; weights times value scale, the tile's largest weight times its largest scale as kWhole
             const float vmax = fmaxf(mt.v_scale[0], mt.v_scale[1]);
-            const float v_rel[2] = {vmax > 0.0f ? mt.v_scale[0] / vmax : 0.0f, vmax > 0.0f ? mt.v_scale[1] / vmax : 0.0f};
+            const float whole[2] = {vmax > 0.0f ? kWhole * __fdividef(mt.v_scale[0], vmax) : 0.0f, vmax > 0.0f ? kWhole * __fdividef(mt.v_scale[1], vmax) : 0.0f};
             float v_unit[NC][2];
             bool wide = false;
 #pragma unroll
@@ -502,24 +502,23 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) own = fmaxf(own, __shfl_xor_sync(0xffffffffu, own, o));
                     const float top = fmaxf(own, m[nc][e]);
-                    const float base = top == -INFINITY ? 0.0f : top;
+                    const float base = top == -INFINITY ? 0.0f : top, own_base = own == -INFINITY ? 0.0f : own;
+                    const float down = ex2_approx(own - base);  // weights are 2^(score - own), and 2^own of the row's
                     turn[e] = ex2_approx(m[nc][e] - base);
                     m[nc][e] = top;
-                    // (the tile's largest weight is kWhole after `up`; where that overflows, or nothing is attended, v_unit makes nothing of what comes out)
-                    const float up = ex2_approx(base - own) * kWhole;
-                    v_unit[nc][e] = ex2_approx(own - base) * (vmax / kWhole);
+                    v_unit[nc][e] = down * (vmax * (1.0f / kWhole));
                     float sum = 0.0f;
 #pragma unroll
                     for (int half16 = 0; half16 < 2; ++half16)
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
                             float& x = s[nc][half16][e + 2 * k];
-                            x = ex2_approx(x - base);
+                            x = ex2_approx(x - own_base);
                             sum += x;
-                            x *= up * v_rel[half16];
+                            x *= whole[half16];
                             wide = wide || __float_as_uint(x) - __float_as_uint(kNothing) < __float_as_uint(kNarrow) - __float_as_uint(kNothing);
                         }
-                    l[nc][e] = fmaf(l[nc][e], turn[e], sum);
+                    l[nc][e] = fmaf(l[nc][e], turn[e], sum * down);
                 }
                 if (__any_sync(0xffffffffu, turn[0] != 1.0f || turn[1] != 1.0f)) {
 #pragma unroll
