@@ -423,8 +423,9 @@ int kmll_paged_cache_rows(kmll_stream_t stream, const int8_t* k_codes, const flo
  * Rounding, heads of 64 and 128 (others: f32).  q: to 2^-24 of its row's largest entry (requests of more than 8 to 16 rows of a kv head 2^-22).  A
  * key's weight times its page's value scale, where the output takes it (their sum takes all of it): requests of few rows to 2^-25 (bf16 rows 2^-17) of the largest
  * weight times the largest value scale in its tile of 32 keys, in a tile with one below 2^-14 (2^-10) of that to 2^-41 (2^-33); requests of more rows to 2^-22
- * (2^-11) of itself and 2^-32 of the row's largest, and value scales below 2^-80 count as 2^-80.  That is about 1e-6 (f32 rows) of the largest weighted |value| of
- * a row, and of the result itself wherever that is not what keys 2^-10 and more below a key of no value hold. */
+ * (2^-11) of itself and 2^-32 of the row's largest, and value scales below 2^-80 count as 2^-80.  f32 rows come out to about
+ * 1e-6 of their norm.  A row whose norm is what 4000 keys hold behind one key of no value 12, 14 or 18 nats above them: 4e-6 in requests of few rows, 6e-6, 1e-4 or
+ * 4e-3 in those of more; bf16 rows are at the rounding of the result (2e-3), 5e-3 in the last case. */
 size_t kmll_paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim, int requests, int tokens, int max_query, int max_context);
 int kmll_paged_attention(kmll_stream_t stream, const void* query, int is_f32, const int32_t* query_start, const int32_t* context, const int32_t* block_table,
                          int table_width, int requests, int tokens, int max_query, int max_context, int heads, const int8_t* k_codes, const float* k_scales,

@@ -4,20 +4,22 @@
 //   entry of its row, in bytes; mma.m16n8k32 s8 x u8 / s8 -> s32, one MMA per byte, exact; S = k_scale * q_scale * (D0 + 2^8 D1 + 2^16 D2)
 //   O^T[dim][row] += V^T[dim][key] P^T[key][row]: A = 16 columns x 32 keys (values lie with the keys of a column together), B =
 //   softmax weights times the page's value scale, as 24-bit (bf16 rows: 16-bit) fractions of the largest of them in the tile of 32 keys, in bytes
-// Nothing is converted on the way from memory to the tensor cores, and both contractions are exact.  What is rounded are q, to 2^-24 of its row's largest
-// entry (of bf16 rows too: a strong channel would leave the others of 16 bits fewer than they have), and the weights, to 2^-25 (bf16 rows 2^-17) of the tile's largest: of the tile's, not of the row's, because
-// the sum of the weights has all of them, and what lies far below one key that dominates a row is most of the result where that key's value is small.
-// For the same reason a tile with weights below 2^-14 (2^-10) of its largest goes twice, the second time with 16 bits of what rounding left.  (64 requests of 8192, 32
-// query heads over 8 of size 128, f32: 186 us either way where scores spread by 1; 208 where they spread by 3 and many tiles go twice, 186 without.)
+// Nothing is converted on the way from memory to the tensor cores, and both contractions are exact.  What is rounded:
+//   q, to 2^-24 of its row's largest entry (of bf16 rows too: 16 bits below a strong channel leave the other entries fewer than the eight they have;
+//   64 requests of 100 to 8000 tokens 75.5 us, with 16 bits 74.2);
+//   the weights, to 2^-25 (bf16 rows 2^-17) of the largest of the tile.  Not of the row's largest: the sum of the weights has all of them, and what lies far below one
+//   key that dominates a row is most of the result where that key's value is small.  For the same reason a tile with weights below 2^-14 (2^-10) of its
+//   largest goes twice, the second time with 16 bits of what rounding left (64 requests of 8192, 32 query heads over 8 of size 128, f32: 183 us where scores
+//   spread by 1, 201 where they spread by 3 and many tiles go twice; 185 without a second time).
 // (f32 rows cost three MMAs where bf16 heads and remainders would cost two of twice the size, behind a conversion of every code.)
 //
 // A warp is a pipeline of its own over tiles of 32 keys (two stages of keys and values, cp.async in 16-byte groups), with its own running
 // maximum and sum; four warps take the tiles of a stretch in turn and meet at its end.  The work of a call is one axis, requests x kv heads x
 // tiles, cut into equal shares for the blocks, whatever the contexts; where a share ends within a head, the blocks that have parts of it leave
 // maximum, sum and O in the workspace and the last to arrive joins them in the order of the blocks: results do not change from call to call.
-// Bound: HBM (2 * head_dim bytes per key and kv head): 64 requests of 8192 tokens, 32 query heads over 8 of size 128, 203 us for 1074 MB, 5.3
-// TB/s with f32 or bf16 rows; 64 of 100 to 8000 tokens 72 us for 369 MB, 10 us of which are fixed (share, queries, first tiles, join).  Few short
-// requests are that latency alone: one of 2048 tokens 10 us.  Sixteen rows (16 query heads over one): 64 of 8192, 134 MB, 51 us.
+// Bound: HBM (2 * head_dim bytes per key and kv head): 64 requests of 8192 tokens, 32 query heads over 8 of size 128, 184 us for 1074 MB, 5.8
+// TB/s with f32 or bf16 rows (in a graph, one call behind the other); 64 of 100 to 8000 tokens 75 us for 369 MB, 10 us of which are fixed (share, queries, first
+// tiles, join).  Few short requests are that latency alone: one of 2048 tokens 10.6 us.  Sixteen rows (16 query heads over one): 64 of 8192, 134 MB, 58 us.
 #include <climits>
 #include <type_traits>
 

@@ -18,15 +18,15 @@
 //   warp 24          issues S = Q K^T and O += P V
 // O is rescaled only when a row's maximum has grown by more than 2^8.  The accumulators cut what does not fit into 24 bits, so an O of many tiles
 // comes out short, by 2.4e-7 a tile where every tile adds two planes: of f32 rows it leaves tensor memory every six tiles and is summed in f32,
-// rounded, in the workspace (relative error of a prompt of 2048: 1.4e-6 without, 8.7e-7 so; of 8192 5.4e-6 and 1.1e-6; every four tiles 6.6e-7
-// and 8.0e-7; 32 query heads over 8, 2048 tokens: 73, 84 and 87 us).  bf16 results are rounded to 2^-9 in any case.
+// rounded, in the workspace (relative error of a prompt of 2048: 1.4e-6 without, 8.9e-7 so; of 8192 5.4e-6 and 1.1e-6; every four tiles 6.6e-7
+// and 8.0e-7; 32 query heads over 8, 2048 tokens: 73, 85 and 88 us).  Where in the workspace is a block's for as long as it runs: a bit that it claims.  bf16 results are rounded to 2^-9 in any case.
 // Which rows a block takes, and which part of their keys, stands in a list that a block of the kernel for few rows has made (paged_decode.cu):
 // parts leave maximum, sum and O in the workspace, and the last to arrive joins them in order.
 // Every wait is bounded; a time-out raises the status word, and the block frees its tensor memory and returns (no copies are under way: the
 // fetches are loads).
 // Bound: the softmax between the two MMAs of a tile (one thread a row took 3400 cycles a tile, all of it latency), beside the MMAs of f32 rows' two
-// planes.  32 query heads over 8, head size 128, random codes: 2048 tokens 72 us (bf16), 84 to 99 us (f32: more where maxima keep growing), 8192
-// tokens 594 us (bf16, 0.93 PFLOP/s of the causal half) and 965 us (f32); 512 tokens behind 32256 370 us (bf16, 0.74).
+// planes.  32 query heads over 8, head size 128, random codes: 2048 tokens 61 us (bf16), 85 us (f32), 8192
+// tokens 583 us (bf16, 0.94 PFLOP/s of the causal half) and 914 us (f32); 512 tokens behind 32256 328 us (bf16, 0.83).
 #include <climits>
 #include <type_traits>
 
