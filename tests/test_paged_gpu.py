@@ -869,3 +869,46 @@ def test_queries_with_a_strong_channel(cuda, dtype, heads, kv, hd, new):
     s["values"][0][..., 0] = 0.0
     s["q"][..., 0] = 5000.0
     check_sink(s, new > 3)
+
+
+def test_two_long_prompts_at_once(cuda):
+    """Two streams, each with a workspace of its own, whose blocks claim their places for sums side by side; a captured call among them."""
+    sets = [make_attention(94 + i, 8, 4, 128, 64, [1200], [700 + 100 * i], torch.float32) for i in range(2)]
+    args = [(ints(s["start"]), ints(s["context"]), ints(s["table"]), s["cache"], s["most"], max(s["context"]), 0.09) for s in sets]
+    works = [ops.paged_attention_workspace(s["cache"], 8, 1, s["q"].shape[0], s["most"], max(s["context"])) for s in sets]
+    alone = [ops.paged_attention(s["q"], *x).clone() for s, x in zip(sets, args)]
+    outs = [[torch.zeros_like(alone[i]) for _ in range(6)] for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=streams[1]):
+        for out in outs[1]:
+            ops.paged_attention(sets[1]["q"], *args[1], workspace=works[1], out=out)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(streams[1]):
+        graph.replay()
+    with torch.cuda.stream(streams[0]):
+        for out in outs[0]:
+            ops.paged_attention(sets[0]["q"], *args[0], workspace=works[0], out=out)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, alone[i]) for i in range(2) for o in outs[i])
+    assert not any(w[:4 * (65536 + 296 + 5)].any() for w in works)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_sinks_of_many_requests_in_a_window(cuda, dtype):
+    """Requests of unequal length whose first visible key lies far above the rest, under a window that begins at it or behind it."""
+    s = make_attention(96, 8, 2, 128, 32, [300, 64, 999, 31], [1] * 4, dtype)
+    k, v = s["values"]
+    for r, c in enumerate(s["context"]):
+        at = max(0, c - 200) if r != 1 else 0
+        page, place = int(s["table"][r, at // 32]), at % 32
+        s["cache"].k_codes[page, :, :, place] = 0
+        s["cache"].k_codes[page, :, 0, place, 0] = 127
+        s["cache"].v_codes[page, :, place // 16, :, place % 16] = 0
+        k[page, place], v[page, place] = 0.0, 0.0
+        k[page, place, :, 0] = 127.0 * s["cache"].k_scales[page].cpu().numpy()
+    s["q"][..., 0] = 60.0
+    s["q"][..., 1:] *= 0.25
+    for window in (0, 200, 199, 50):
+        check_attention(s, window)
