@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(kPdThreads, NC == 1 ? 3 : 2) paged_decode_kern
                     for (int o = 4; o < 32; o <<= 1) own = fmaxf(own, __shfl_xor_sync(0xffffffffu, own, o));
                     const float top = fmaxf(own, m[nc][e]);
                     const float base = top == -INFINITY ? 0.0f : top, own_base = own == -INFINITY ? 0.0f : own;
-                    const float down = ex2_approx(own - base);  // weights are 2^(score - own), and 2^own of the row's
+                    const float down = ex2_approx(own - base);  // (weights below are 2^(score - own): `down` times as much of the row's)
                     turn[e] = ex2_approx(m[nc][e] - base);
                     m[nc][e] = top;
                     v_unit[nc][e] = down * (vmax * (1.0f / kWhole));
